@@ -18,7 +18,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD_DIR = os.path.join(CSRC, "build")
 
-SOURCES = ["bindings.cpp", "gemm_host.cu", "gemm_inst_a.cu", "gemm_inst_b.cu", "gemm_inst_c.cu", "gemm_inst_d.cu", "gemm_inst_e.cu", "rowwise.cu", "noalloc_decoder.cu", "decode.cu", "scaffold.cu", "comm.cu", "gdpo.cu", "ssd_chunk.cu"]
+SOURCES = ["bindings.cpp", "gemm_host.cu", "gemm_inst_a.cu", "gemm_inst_b.cu", "gemm_inst_c.cu", "gemm_inst_d.cu", "gemm_inst_e.cu", "rowwise.cu", "noalloc_decoder.cu", "decode.cu", "scaffold.cu", "comm.cu", "gdpo.cu", "ssd_chunk.cu",
+           "adapters.cu", "sampling.cu", "adamw_many.cu"]
 
 NVCC_FLAGS = [
     "-gencode=arch=compute_100a,code=sm_100a",
@@ -32,7 +33,7 @@ if os.environ.get("BDH_PTXAS_VERBOSE"):
 
 
 # Kernels launched by one call of each binding (for the bench's launch count).
-_LAUNCHES_PER_CALL = {"grad_clip_coef": 2}
+_LAUNCHES_PER_CALL = {"grad_clip_coef": 2, "adapter_forward": 2, "adapter_backward": 4}
 
 
 class _Counted:

@@ -1,0 +1,861 @@
+// adapters.cu — low-rank adapters of many requests at once beside a shared, frozen projection.
+//
+//   t[m,h,:]  = x[m(,h),:] a[g(m),h]^T                     (a [G, H, r, K], g(m) the row's adapter)
+//   y[m,h,:]  = x[m(,h),:] W[h] + s[g(m)] t[m,h,:] b[g(m),h]        (W [H, K, N], b [G, H, r, N])
+// and its gradients, which are the same three operations with the roles of a and b exchanged:
+//   u = dy b^T,  dx = dy W^T + s u a  (summed over the heads where they share x),
+//   da[g] = s u_g^T x_g,  db[g] = s t_g^T dy_g            (the rows of adapter g)
+//
+// Three kernels:
+//  * adapter_shrink: t (or u), one CTA per run of up to 32 rows of one adapter, per head and
+//    per part of the reduction. Bound by the bytes of x and a; both are K-contiguous, so the
+//    mma.sync operands are loaded straight from memory, 16 bytes a lane.
+//  * adapter_gemm: the projection on tcgen05 (TMA, TMEM, warp roles as in the GEMM engine),
+//    with the adapters as an extension of its reduction: after the K-blocks of x and W
+//    come blocks of 64 / rp adapter slots. A 128-row tile lists the distinct adapters of its rows
+//    ("slots"); four builder warps write t s into the columns of each row's slot and zeros
+//    elsewhere, and TMA loads the slots' b rows beside each other. So one accumulator takes both
+//    products, rows of any adapters can share a tile, and W and every b are read once per
+//    row tile. The projection's blocks need no t, so with programmatic launch they run
+//    while adapter_shrink still does; only the builders wait for it.
+//  * adapter_wgrad: da / db, one CTA per adapter, head and 128 columns.
+// t and u are kept in fp32 (partial sums over the parts of the reduction) and rounded to bf16
+// once, as an operand of the next product, like every activation of the bf16 path. All sums are
+// fp32 and in a fixed order: no atomics.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include "gemm_table.h"
+#include "sm100_ptx.cuh"
+#include "tensor_map.h"
+
+namespace bd {
+namespace {
+
+using bf16 = __nv_bfloat16;
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// ------------------------------------------------------------------------------- shrink
+
+constexpr int kShrinkThreads = 256;
+
+struct ShrinkArgs {
+  const bf16* x;
+  long long x_row, x_head;
+  const bf16* a;  // [G, H, r, K]
+  float* t;       // [parts, H, M, rp]
+  const int* order;
+  const int* chunks;  // (start in order, rows, adapter) each
+  int M, H, K, r, part_k;
+};
+
+// Rank rows are the m of the product, the run's x rows its n (MT 16-row and NT 8-row tiles).
+// The k order inside 32 values is permuted alike for both operands so that a lane's 16-byte
+// load holds the fragments of two products.
+template <int MT, int NT>
+__global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const __grid_constant__ ShrinkArgs p) {
+  constexpr int RP = 16 * MT;
+  __shared__ float red[4][RP][NT * 8];
+  grid_dependents_launch();
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int start = p.chunks[3 * blockIdx.x], rows = p.chunks[3 * blockIdx.x + 1], g = p.chunks[3 * blockIdx.x + 2];
+  const int h = blockIdx.y;
+  const int k1 = min((int)(blockIdx.z + 1) * p.part_k, p.K);
+  const bf16* a = p.a + ((long long)g * p.H + h) * p.r * p.K;
+  const bf16* xr[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int i = nt * 8 + lane / 4;
+    xr[nt] = i < rows ? p.x + (long long)p.order[start + i] * p.x_row + (long long)h * p.x_head : nullptr;
+  }
+  float acc[MT][NT][4];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[mt][nt][i] = 0.f;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 2
+  for (int k = (int)blockIdx.z * p.part_k + warp * 32 + 8 * (lane % 4); k < k1 + 8 * (lane % 4); k += 32 * (kShrinkThreads / 32)) {
+    const bool in = k < k1;
+    uint4 xv[NT], av[MT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) xv[nt] = in && xr[nt] ? *reinterpret_cast<const uint4*>(xr[nt] + k) : zero;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = mt * 16 + i * 8 + lane / 4;
+        av[mt][i] = in && row < p.r ? *reinterpret_cast<const uint4*>(a + (long long)row * p.K + k) : zero;
+      }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        mma_bf16(acc[mt][nt], av[mt][0].x, av[mt][1].x, av[mt][0].y, av[mt][1].y, xv[nt].x, xv[nt].y);
+        mma_bf16(acc[mt][nt], av[mt][0].z, av[mt][1].z, av[mt][0].w, av[mt][1].w, xv[nt].z, xv[nt].w);
+      }
+  }
+  // the warps' sums, folded in halves (a fixed order)
+#pragma unroll
+  for (int half = 4; half > 0; half /= 2) {
+    if (warp >= half && warp < 2 * half) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            red[warp - half][mt * 16 + lane / 4 + (i / 2) * 8][nt * 8 + 2 * (lane % 4) + i % 2] = acc[mt][nt][i];
+    }
+    __syncthreads();
+    if (warp < half) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            acc[mt][nt][i] += red[warp][mt * 16 + lane / 4 + (i / 2) * 8][nt * 8 + 2 * (lane % 4) + i % 2];
+    }
+    __syncthreads();
+  }
+  if (warp == 0) {
+    float* t = p.t + ((long long)blockIdx.z * p.H + h) * p.M * RP;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = nt * 8 + 2 * (lane % 4) + i % 2;
+        if (n >= rows) continue;
+        float* o = t + (long long)p.order[start + n] * RP + lane / 4 + (i / 2) * 8;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) o[mt * 16] = acc[mt][nt][i];
+      }
+  }
+}
+
+// ------------------------------------------------------------------------------- projection
+
+struct AdapterGemm {
+  CUtensorMap tx, tw, tb, ty;
+  int M, N, KB;      // rows, output columns, 64-wide blocks of one head's reduction
+  int HR, Z;         // heads summed in the reduction, heads of the output
+  int x_heads;       // x has a head coordinate
+  int H;             // heads of b and t
+  int tiles_m, tiles_n, splits;
+  int rp, per_block;  // padded rank, slots per 64-wide block
+  int parts;          // partial sums of t
+  long long t_part;
+  const float* t;     // [parts, H, M, rp]; null without adapters
+  const int* row_slot;
+  const int* row_adapter;
+  const int* tile_ptr;
+  const int* slots;
+  const float* scale;  // per adapter, or null
+  float scale0;
+  float* partial;     // [splits, Z, M, N] where the reduction is split
+  int* err;
+};
+
+struct AdapterTile {
+  int m0, n0, z, slot0, nslots, ext, kb0, kb1, split;
+};
+
+__device__ __forceinline__ AdapterTile adapter_tile(const AdapterGemm& p, int t, int BN) {
+  AdapterTile c;
+  c.n0 = (t % p.tiles_n) * BN;
+  t /= p.tiles_n;
+  const int mb = t % p.tiles_m;
+  c.m0 = mb * 128;
+  t /= p.tiles_m;
+  c.split = t % p.splits;
+  c.z = t / p.splits;
+  c.slot0 = p.t ? p.tile_ptr[mb] : 0;
+  c.nslots = p.t ? p.tile_ptr[mb + 1] - c.slot0 : 0;
+  c.ext = (c.nslots + p.per_block - 1) / p.per_block;
+  const long long total = (long long)p.HR * (p.KB + c.ext);
+  c.kb0 = (int)(total * c.split / p.splits);
+  c.kb1 = (int)(total * (c.split + 1) / p.splits);
+  return c;
+}
+
+constexpr int kEpiWarps = 8, kBuildWarps = 4;
+constexpr int kAdapterThreads = 32 * (2 + kEpiWarps + kBuildWarps);
+
+template <int BN>
+struct AdapterCfg {
+  static constexpr int A_BYTES = 128 * 64 * 2;
+  static constexpr int B_BYTES = BN * 64 * 2;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;  // 192 KB of operands
+  static constexpr int EPI_BYTES = kEpiWarps * 4096;                // a 32 x 64 bf16 tile per epilogue warp
+  static constexpr int SMEM = STAGES * STAGE_BYTES + EPI_BYTES + 1024;
+  static constexpr int TMEM_COLS = 2 * BN;
+};
+
+// Byte offset of 16-byte chunk `chunk` of row `row` in a 128-byte-row, 128B-swizzled tile.
+__device__ __forceinline__ uint32_t sw128(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
+
+__device__ __forceinline__ uint4 to_bf16x8(const float* v) {
+  __nv_bfloat162 h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+  return *reinterpret_cast<uint4*>(h);
+}
+
+// W_MN: W's rows are the reduction (y = x W); else its columns are (dx = dy W^T).
+template <int BN, bool W_MN>
+__global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const __grid_constant__ AdapterGemm p) {
+  using Cfg = AdapterCfg<BN>;
+  constexpr int STAGES = Cfg::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES];
+  // an adapter block's stage passes from the producer (granted) over the builders (built) to the MMA warp
+  __shared__ uint64_t granted_bar[STAGES], built_bar[STAGES];
+  __shared__ uint64_t tfull_bar[2], tempty_bar[2], drain_bar;
+  __shared__ uint32_t tmem_base_s;
+  __shared__ volatile int abort_flag;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + STAGES * Cfg::A_BYTES;
+  uint8_t* sEpi = smem + STAGES * Cfg::STAGE_BYTES;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+      mbar_init(&granted_bar[s], 1);
+      mbar_init(&built_bar[s], kBuildWarps);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull_bar[a], 1);
+      mbar_init(&tempty_bar[a], kEpiWarps);
+    }
+    mbar_init(&drain_bar, 1);
+    fence_barrier_init();
+    tma_prefetch_desc(&p.tx);
+    tma_prefetch_desc(&p.tw);
+  }
+  if (warp == 1) tmem_alloc(&tmem_base_s, Cfg::TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_base_s;
+  const int total = p.tiles_m * p.tiles_n * p.splits * p.Z;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ------------------------------------------------ TMA producer
+      int stage = 0;
+      uint32_t phase = 0;
+      long long issued = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+        const AdapterTile c = adapter_tile(p, t, BN);
+        for (int kb = c.kb0; kb < c.kb1; ++kb) {
+          if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutProducer)) {
+            ok = false;
+            break;
+          }
+          uint8_t* a_dst = sA + stage * Cfg::A_BYTES;
+          uint8_t* b_dst = sB + stage * Cfg::B_BYTES;
+          if (kb < p.HR * p.KB) {
+            const int h = p.HR > 1 ? kb / p.KB : c.z;
+            const int k0 = (p.HR > 1 ? kb % p.KB : kb) * 64;
+            mbar_arrive_expect_tx(&full_bar[stage], Cfg::STAGE_BYTES);
+            tma_load_4d(a_dst, &p.tx, &full_bar[stage], k0, c.m0, p.x_heads ? h : 0, 0);
+            if constexpr (W_MN) {
+#pragma unroll
+              for (int i = 0; i < BN / 64; ++i)
+                tma_load_4d(b_dst + i * 8192, &p.tw, &full_bar[stage], c.n0 + 64 * i, k0, h, 0);
+            } else {
+              tma_load_4d(b_dst, &p.tw, &full_bar[stage], k0, c.n0, h, 0);
+            }
+          } else {
+            const int e = kb - p.HR * p.KB;
+            const int h = p.HR > 1 ? e / c.ext : c.z;
+            const int j0 = (e % c.ext) * p.per_block;
+            const int n = min(p.per_block, c.nslots - j0);
+            mbar_arrive(&granted_bar[stage]);
+            mbar_arrive_expect_tx(&full_bar[stage], n * p.rp * 2 * BN);
+            for (int j = 0; j < n; ++j) {
+              const int gh = p.slots[c.slot0 + j0 + j] * p.H + h;
+#pragma unroll
+              for (int i = 0; i < BN / 64; ++i)
+                tma_load_4d(b_dst + i * 8192 + j * p.rp * 128, &p.tb, &full_bar[stage], c.n0 + 64 * i, 0, gh, 0);
+            }
+          }
+          ++issued;
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!ok) {
+        // wait (bounded, ignoring the abort flag) for the loads still in flight
+        int dummy_abort = 0;
+        const long long inflight = issued < STAGES ? issued : STAGES;
+        int s = stage;
+        uint32_t ph = phase;
+        for (long long i = 0; i < inflight; ++i) {
+          if (--s < 0) {
+            s = STAGES - 1;
+            ph ^= 1;
+          }
+          mbar_wait_bounded(&full_bar[s], ph, (volatile int*)&dummy_abort, p.err, kErrTimeoutDrain);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // ------------------------------------------------ MMA issuer
+      constexpr uint32_t idesc_w = make_idesc_bf16(128, BN, false, W_MN);
+      constexpr uint32_t idesc_b = make_idesc_bf16(128, BN, false, true);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0, built_phase = 0;  // built_phase: one bit per stage
+      bool ok = true;
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+        const AdapterTile c = adapter_tile(p, t, BN);
+        if (!mbar_wait_bounded(&tempty_bar[acc], acc_phase ^ 1, &abort_flag, p.err, kErrTimeoutMma)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * BN;
+        for (int kb = c.kb0; kb < c.kb1; ++kb) {
+          const bool ext = kb >= p.HR * p.KB;
+          if (!mbar_wait_bounded(&full_bar[stage], phase, &abort_flag, p.err, kErrTimeoutMma) ||
+              (ext && !mbar_wait_bounded(&built_bar[stage], (built_phase >> stage) & 1, &abort_flag, p.err,
+                                         kErrTimeoutMma))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a_base = smem_u32(sA + stage * Cfg::A_BYTES);
+          const uint32_t b_base = smem_u32(sB + stage * Cfg::B_BYTES);
+          if (!ext) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_bf16(d_tmem, make_sdesc_sw128(a_base + kk * 32, 16, 1024),
+                        W_MN ? make_sdesc_sw128(b_base + kk * 2048, 8192, 1024)
+                             : make_sdesc_sw128(b_base + kk * 32, 16, 1024),
+                        idesc_w, (kb > c.kb0 || kk > 0) ? 1u : 0u);
+          } else {
+            built_phase ^= 1u << stage;
+            const int j0 = ((kb - p.HR * p.KB) % c.ext) * p.per_block;
+            const int steps = min(p.per_block, c.nslots - j0) * p.rp / 16;
+            for (int kk = 0; kk < steps; ++kk)
+              umma_bf16(d_tmem, make_sdesc_sw128(a_base + kk * 32, 16, 1024),
+                        make_sdesc_sw128(b_base + kk * 2048, 8192, 1024), idesc_b, (kb > c.kb0 || kk > 0) ? 1u : 0u);
+          }
+          umma_commit(&empty_bar[stage]);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        umma_commit(&tfull_bar[acc]);
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
+      }
+      // every MMA of this thread is done before TMEM is released
+      umma_commit(&drain_bar);
+      int dummy_abort = 0;
+      mbar_wait_bounded(&drain_bar, 0, (volatile int*)&dummy_abort, p.err, kErrTimeoutDrain);
+    }
+  } else if (warp < 2 + kEpiWarps) {
+    // ------------------------------------------------ epilogue: bf16 tiles by TMA, or fp32 parts
+    const int quad = warp & 3;         // TMEM lane quadrant of this warp
+    const int half = (warp - 2) >> 2;  // half of the tile's columns
+    uint8_t* buf = sEpi + (warp - 2) * 4096;
+    constexpr int COLS = BN >= 128 ? BN / 2 : 64;
+    const int col0 = half * COLS;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int t = blockIdx.x; t < total; t += gridDim.x) {
+      const AdapterTile c = adapter_tile(p, t, BN);
+      if (!mbar_wait_bounded(&tfull_bar[acc], acc_phase, &abort_flag, p.err, kErrTimeoutEpilogue)) break;
+      tc_fence_after();
+      const int row0 = c.m0 + quad * 32;
+#pragma unroll 1
+      for (int cc = 0; cc < COLS; cc += 64) {
+        const int col = c.n0 + col0 + cc;
+        if (col0 >= BN || row0 >= p.M || col >= p.N) continue;
+        float v[64];
+        tmem_ld64(tmem_base + ((uint32_t)(quad * 32) << 16) + acc * BN + col0 + cc, v);
+        if (p.splits == 1) {
+          if (lane == 0) bulk_wait_group_read0();  // the previous tile has left the buffer
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(buf + sw128(lane, q)) = to_bf16x8(v + 8 * q);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_4d(&p.ty, buf, col, row0, c.z, 0);
+            bulk_commit_group();
+          }
+        } else if (row0 + lane < p.M) {
+          float* o = p.partial + (((long long)c.split * p.Z + c.z) * p.M + row0 + lane) * p.N + col;
+#pragma unroll
+          for (int q = 0; q < 16; ++q)
+            if (col + 4 * q < p.N)
+              reinterpret_cast<float4*>(o)[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty_bar[acc]);
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1;
+      }
+    }
+    if (lane == 0) bulk_wait_group0();
+  } else {
+    // ------------------------------------------------ builders: one row of the tile per thread
+    grid_dependency_wait();  // t is complete (and this grid does not end before the one that wrote it)
+    const int r = threadIdx.x - 32 * (2 + kEpiWarps);
+    int stage = 0;
+    uint32_t granted_phase = 0;  // one bit per stage: a stage is granted again only after it was built and used
+    bool ok = true;
+    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+      const AdapterTile c = adapter_tile(p, t, BN);
+      const int m = c.m0 + r;
+      const int slot = p.t && m < p.M ? p.row_slot[m] : -1;
+      const float s = slot < 0 ? 0.f : p.scale ? p.scale[p.row_adapter[m]] : p.scale0;
+      for (int kb = c.kb0; kb < c.kb1; ++kb) {
+        if (kb >= p.HR * p.KB) {
+          const int e = kb - p.HR * p.KB;
+          const int h = p.HR > 1 ? e / c.ext : c.z;
+          const int j = slot - (e % c.ext) * p.per_block;  // my slot's place in this block
+          const bool here = slot >= 0 && j >= 0 && j < p.per_block;
+          const float* src = p.t + ((long long)h * p.M + m) * p.rp;
+          if (!mbar_wait_bounded(&granted_bar[stage], (granted_phase >> stage) & 1, &abort_flag, p.err,
+                                 kErrTimeoutProducer)) {
+            ok = false;
+            break;
+          }
+          granted_phase ^= 1u << stage;
+          uint8_t* dst = sA + stage * Cfg::A_BYTES;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            const int at = 8 * q - j * p.rp;  // of my t values
+            if (here && at >= 0 && at < p.rp) {
+              float f[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) f[i] = 0.f;
+              for (int part = 0; part < p.parts; ++part) {
+                const float4 lo = *reinterpret_cast<const float4*>(src + part * p.t_part + at);
+                const float4 hi = *reinterpret_cast<const float4*>(src + part * p.t_part + at + 4);
+                f[0] += lo.x, f[1] += lo.y, f[2] += lo.z, f[3] += lo.w;
+                f[4] += hi.x, f[5] += hi.y, f[6] += hi.z, f[7] += hi.w;
+              }
+#pragma unroll
+              for (int i = 0; i < 8; ++i) f[i] *= s;
+              v = to_bf16x8(f);
+            }
+            *reinterpret_cast<uint4*>(dst + sw128(r, q)) = v;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&built_bar[stage]);
+        }
+        if (++stage == STAGES) stage = 0;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
+// y [M, Z, N] bf16 = the sum of the parts [splits, Z, M, N], in their order.
+__global__ void __launch_bounds__(256) adapter_sum_kernel(const float* __restrict__ partial, int splits, int Z, int M,
+                                                          int N, bf16* __restrict__ y) {
+  const long long n = (long long)Z * M * N;
+  for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long long)gridDim.x * 1024) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int q = 0; q < splits; ++q) {
+      const float4 v = *reinterpret_cast<const float4*>(partial + q * n + i);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    const int col = (int)(i % N);
+    const long long zm = i / N;
+    __nv_bfloat162 lo = __floats2bfloat162_rn(s.x, s.y), hi = __floats2bfloat162_rn(s.z, s.w);
+    *reinterpret_cast<uint2*>(y + ((zm % M) * Z + zm / M) * N + col) =
+        make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
+  }
+}
+
+// ------------------------------------------------------------------------------- weight gradients
+
+struct WgradArgs {
+  const bf16* x;  // x or dy
+  long long x_row, x_head;
+  const float* t;  // [parts, H, M, rp]
+  long long t_part;
+  int parts;
+  const int* order;
+  const int* group;  // [G + 1]: the rows of adapter g in `order`
+  const float* scale;
+  float scale0;
+  bf16* out;  // [G, H, r, C]
+  int M, H, r, C;
+};
+
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&v)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(addr));
+}
+
+constexpr int kWgradRows = 32, kWgradCols = 128;
+
+// out[g,h] = s t_g^T x_g: rank rows (16 MT) by 128 columns a CTA, the adapter's rows in steps of 32.
+template <int MT>
+__global__ void __launch_bounds__(256) adapter_wgrad_kernel(const __grid_constant__ WgradArgs p) {
+  constexpr int RP = 16 * MT;
+  constexpr int XP = kWgradCols + 8, TP = RP + 8;  // padded rows: ldmatrix reads without bank conflicts
+  __shared__ __align__(16) bf16 xs[2][kWgradRows][XP];
+  __shared__ __align__(16) bf16 ts[2][kWgradRows][TP];
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int c0 = blockIdx.x * kWgradCols, h = blockIdx.y, g = blockIdx.z;
+  const int r0 = p.group[g], rows = p.group[g + 1] - r0;
+  const int steps = (rows + kWgradRows - 1) / kWgradRows;
+  auto load = [&](int step, int buf) {
+    for (int i = tid; i < kWgradRows * (kWgradCols / 8); i += 256) {
+      const int row = i / (kWgradCols / 8), c = (i % (kWgradCols / 8)) * 8;
+      const int at = step * kWgradRows + row;
+      const bool in = at < rows && c0 + c < p.C;
+      const bf16* src = in ? p.x + (long long)p.order[r0 + at] * p.x_row + (long long)h * p.x_head + c0 + c : p.x;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(&xs[buf][row][c])), "l"(src),
+                   "r"(in ? 16 : 0)
+                   : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    for (int i = tid; i < kWgradRows * RP; i += 256) {
+      const int row = i / RP, c = i % RP;
+      const int at = step * kWgradRows + row;
+      float f = 0.f;
+      if (at < rows) {
+        const float* src = p.t + ((long long)h * p.M + p.order[r0 + at]) * RP + c;
+        for (int part = 0; part < p.parts; ++part) f += src[part * p.t_part];
+      }
+      ts[buf][row][c] = __float2bfloat16_rn(f);
+    }
+  };
+  float acc[MT][2][4];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[mt][nt][i] = 0.f;
+  if (steps > 0) load(0, 0);
+  for (int step = 0; step < steps; ++step) {
+    const int buf = step & 1;
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    if (step + 1 < steps) load(step + 1, buf ^ 1);
+#pragma unroll
+    for (int kk = 0; kk < kWgradRows / 16; ++kk) {
+      uint32_t b[4];
+      ldmatrix_x4_trans(b, smem_u32(&xs[buf][kk * 16 + (lane & 15)][warp * 16 + (lane >> 4) * 8]));
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        uint32_t a[4];
+        ldmatrix_x4_trans(a, smem_u32(&ts[buf][kk * 16 + (lane & 7) + (lane >> 4) * 8][mt * 16 + ((lane >> 3) & 1) * 8]));
+        mma_bf16(acc[mt][0], a[0], a[1], a[2], a[3], b[0], b[1]);
+        mma_bf16(acc[mt][1], a[0], a[1], a[2], a[3], b[2], b[3]);
+      }
+    }
+    __syncthreads();
+  }
+  const float s = p.scale ? p.scale[g] : p.scale0;
+  bf16* out = p.out + ((long long)g * p.H + h) * p.r * p.C;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = mt * 16 + lane / 4 + 8 * i, col = c0 + warp * 16 + nt * 8 + 2 * (lane % 4);
+        if (row < p.r && col < p.C)
+          *reinterpret_cast<__nv_bfloat162*>(out + (long long)row * p.C + col) =
+              __floats2bfloat162_rn(acc[mt][nt][2 * i] * s, acc[mt][nt][2 * i + 1] * s);
+      }
+}
+
+// ------------------------------------------------------------------------------- host
+
+// The batch's plan: one int32 buffer, and where its parts lie.
+struct Plan {
+  int M, G, tiles, chunks, rows_per_chunk, rows;  // rows: those with an adapter
+  const int *row_adapter, *row_slot, *tile_ptr, *slots, *order, *chunk, *group;
+};
+
+Plan read_plan(const at::Tensor& buf, const std::vector<int64_t>& d) {
+  TORCH_CHECK(buf.is_cuda() && buf.scalar_type() == at::kInt && buf.is_contiguous() && d.size() == 7,
+              "adapter_linear: bad batch plan");
+  Plan p;
+  p.M = (int)d[0], p.G = (int)d[1], p.tiles = (int)d[2], p.rows = (int)d[4], p.chunks = (int)d[5], p.rows_per_chunk = (int)d[6];
+  const int* b = buf.data_ptr<int>();
+  p.row_adapter = b, b += p.M;
+  p.row_slot = b, b += p.M;
+  p.tile_ptr = b, b += p.tiles + 1;
+  p.slots = b, b += d[3];
+  p.order = b, b += p.rows;
+  p.chunk = b, b += 3 * p.chunks;
+  p.group = b;
+  TORCH_CHECK(buf.numel() == 2 * d[0] + d[2] + 1 + d[3] + d[4] + 3 * d[5] + d[1] + 1, "adapter_linear: bad batch plan");
+  return p;
+}
+
+int padded_rank(int64_t r) { return r <= 16 ? 16 : r <= 32 ? 32 : 64; }
+
+struct Rows {  // [M, C] shared by the heads, or [M, H, C]
+  const bf16* p;
+  long long row, head;
+  int C;
+};
+
+Rows rows_of(const at::Tensor& t, bool per_head) {
+  Rows r;
+  r.p = reinterpret_cast<const bf16*>(t.data_ptr());
+  r.row = t.stride(0);
+  r.head = per_head ? t.stride(1) : 0;
+  r.C = (int)t.size(-1);
+  return r;
+}
+
+at::Tensor shrink(const Rows& x, const at::Tensor& a, const Plan& p, int H, int r, cudaStream_t st) {
+  const int rp = padded_rank(r);
+  const long long ctas = (long long)p.chunks * H;
+  // parts of the reduction: enough CTAs for two a SM, at least 512 values each, 16 at most
+  const int parts = (int)std::max<long long>(1, std::min<long long>({16, (x.C + 511) / 512, (296 + ctas - 1) / ctas}));
+  const int part_k = ((x.C + parts - 1) / parts + 31) / 32 * 32;
+  const int used = (x.C + part_k - 1) / part_k;
+  at::Tensor t = at::empty({used, H, p.M, rp}, a.options().dtype(at::kFloat));
+  ShrinkArgs s{x.p, x.row, x.head, reinterpret_cast<const bf16*>(a.data_ptr()), t.data_ptr<float>(), p.order, p.chunk,
+               p.M, H, x.C, r, part_k};
+  const dim3 grid((unsigned)p.chunks, (unsigned)H, (unsigned)used);
+  auto go = [&](auto mt) {
+    if (p.rows_per_chunk <= 8)
+      adapter_shrink_kernel<decltype(mt)::value, 1><<<grid, kShrinkThreads, 0, st>>>(s);
+    else
+      adapter_shrink_kernel<decltype(mt)::value, 4><<<grid, kShrinkThreads, 0, st>>>(s);
+  };
+  if (rp == 16)
+    go(std::integral_constant<int, 1>());
+  else if (rp == 32)
+    go(std::integral_constant<int, 2>());
+  else
+    go(std::integral_constant<int, 4>());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return t;
+}
+
+template <int BN, bool W_MN>
+void launch_gemm(const AdapterGemm& p, cudaStream_t st, int dev, bool after_shrink) {
+  using Cfg = AdapterCfg<BN>;
+  auto kern = adapter_gemm_kernel<BN, W_MN>;
+  static bool attr_set[64] = {false};
+  if (!attr_set[dev]) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
+    attr_set[dev] = true;
+  }
+  const long long total = (long long)p.tiles_m * p.tiles_n * p.splits * p.Z;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)std::min<long long>(total, num_sms_of(dev)));
+  cfg.blockDim = dim3(kAdapterThreads);
+  cfg.dynamicSmemBytes = Cfg::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = after_shrink ? 1 : 0;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, p));
+}
+
+// out [M, Z, N] = sum over the reduction's heads of x w (+ s t b).
+at::Tensor project(const Rows& x, const at::Tensor& w, bool w_mn, bool sum_heads, const at::Tensor& b,
+                   const at::Tensor& t, const Plan& plan, int r, const c10::optional<at::Tensor>& scale, double scale0,
+                   const at::Tensor& err, cudaStream_t st, int dev) {
+  const int H = (int)w.size(0), K = (int)w.size(w_mn ? 1 : 2), N = (int)w.size(w_mn ? 2 : 1), M = plan.M;
+  AdapterGemm p;
+  memset(&p, 0, sizeof(p));
+  p.M = M, p.N = N, p.KB = (K + 63) / 64, p.H = H;
+  p.HR = sum_heads ? H : 1;
+  p.Z = sum_heads ? 1 : H;
+  p.x_heads = x.head != 0;
+  p.rp = padded_rank(r), p.per_block = 64 / p.rp;
+  const bool adapters = plan.rows > 0;
+  if (adapters) {
+    p.t = t.data_ptr<float>(), p.parts = (int)t.size(0), p.t_part = t.stride(0);
+    p.row_slot = plan.row_slot, p.row_adapter = plan.row_adapter, p.tile_ptr = plan.tile_ptr, p.slots = plan.slots;
+    p.scale = scale ? scale->data_ptr<float>() : nullptr, p.scale0 = (float)scale0;
+  }
+  p.err = err.data_ptr<int>();
+  p.tiles_m = (M + 127) / 128;
+  auto tiles = [&](int bn) { return (long long)p.tiles_m * ((N + bn - 1) / bn) * p.Z; };
+  const int bn = tiles(256) >= 148 ? 256 : tiles(128) >= 148 ? 128 : 64;
+  p.tiles_n = (N + bn - 1) / bn;
+  // parts of a long reduction where there are few tiles, at least four blocks each
+  p.splits = (int)std::max<long long>(1, std::min<long long>(148 / tiles(bn), (long long)p.HR * p.KB / 4));
+  at::Tensor y = at::empty({M, p.Z, N}, w.options());
+  at::Tensor partial;
+  if (p.splits > 1) {
+    partial = at::empty({p.splits, p.Z, M, N}, w.options().dtype(at::kFloat));
+    p.partial = partial.data_ptr<float>();
+  }
+  const int64_t xh = p.x_heads ? H : 1;
+  p.tx = tensor_map_bf16(x.p, {K, M, xh}, {x.row, p.x_heads ? x.head : (int64_t)M * x.row}, 64, 128);
+  if (w_mn)
+    p.tw = tensor_map_bf16(w.data_ptr(), {N, K, H}, {w.stride(1), w.stride(0)}, 64, 64);
+  else
+    p.tw = tensor_map_bf16(w.data_ptr(), {K, N, H}, {w.stride(1), w.stride(0)}, 64, (uint32_t)bn);
+  if (adapters)
+    p.tb = tensor_map_bf16(b.data_ptr(), {N, r, b.size(0) * H}, {N, (int64_t)r * N}, 64, (uint32_t)p.rp);
+  p.ty = tensor_map_bf16(y.data_ptr(), {N, M, p.Z}, {(int64_t)p.Z * N, N}, 64, 32);
+#define BD_ADAPTER(BN)                                 \
+  if (bn == BN) {                                      \
+    if (w_mn)                                          \
+      launch_gemm<BN, true>(p, st, dev, adapters);     \
+    else                                               \
+      launch_gemm<BN, false>(p, st, dev, adapters);    \
+  }
+  BD_ADAPTER(64)
+  BD_ADAPTER(128)
+  BD_ADAPTER(256)
+#undef BD_ADAPTER
+  if (p.splits > 1) {
+    const long long n = (long long)p.Z * M * N;
+    adapter_sum_kernel<<<(unsigned)std::min<long long>((n + 1023) / 1024, 148 * 8), 256, 0, st>>>(
+        p.partial, p.splits, p.Z, M, N, reinterpret_cast<bf16*>(y.data_ptr()));
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  return y;
+}
+
+at::Tensor wgrad(const Rows& x, const at::Tensor& t, const Plan& p, const at::Tensor& like, int H, int r,
+                 const c10::optional<at::Tensor>& scale, double scale0, cudaStream_t st) {
+  at::Tensor out = at::empty_like(like);
+  WgradArgs w{x.p, x.row, x.head, t.data_ptr<float>(), t.stride(0), (int)t.size(0), p.order, p.group,
+              scale ? scale->data_ptr<float>() : nullptr, (float)scale0, reinterpret_cast<bf16*>(out.data_ptr()), p.M, H,
+              r, x.C};
+  const dim3 grid((unsigned)((x.C + kWgradCols - 1) / kWgradCols), (unsigned)H, (unsigned)p.G);
+  const int rp = padded_rank(r);
+  if (rp == 16)
+    adapter_wgrad_kernel<1><<<grid, 256, 0, st>>>(w);
+  else if (rp == 32)
+    adapter_wgrad_kernel<2><<<grid, 256, 0, st>>>(w);
+  else
+    adapter_wgrad_kernel<4><<<grid, 256, 0, st>>>(w);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return out;
+}
+
+void check_operand(const at::Tensor& t, int dev, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.get_device() == dev && t.scalar_type() == at::kBFloat16, "adapter_linear: ", what,
+              " must be bf16 on one GPU");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "adapter_linear: ", what, " must be 16-byte aligned");
+  TORCH_CHECK(t.stride(-1) == 1, "adapter_linear: ", what, " must be contiguous in its last dimension");
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    TORCH_CHECK(t.stride(i) % 8 == 0, "adapter_linear: ", what, ": strides must be multiples of 8 values");
+}
+
+struct Checked {
+  int H, K, N, r, dev;
+};
+
+Checked check_all(const at::Tensor& x, const at::Tensor& w, const at::Tensor& a, const at::Tensor& b, const Plan& p,
+                  const c10::optional<at::Tensor>& scale) {
+  const int dev = w.get_device();
+  check_operand(x, dev, "x");
+  check_operand(w, dev, "weight");
+  check_operand(a, dev, "a");
+  check_operand(b, dev, "b");
+  TORCH_CHECK(w.dim() == 3 && a.dim() == 4 && b.dim() == 4 && a.is_contiguous() && b.is_contiguous(),
+              "adapter_linear: weight [H, K, N]; a [G, H, r, K] and b [G, H, r, N] contiguous");
+  const int64_t H = w.size(0), K = w.size(1), N = w.size(2), G = a.size(0), r = a.size(2);
+  TORCH_CHECK(K % 8 == 0 && N % 8 == 0 && K > 0 && N > 0, "adapter_linear: K and N must be multiples of 8");
+  TORCH_CHECK(r >= 1 && r <= 64, "adapter_linear: rank of 1 to 64");
+  TORCH_CHECK(H <= 65535 && G <= 65535, "adapter_linear: at most 65535 heads and adapters");
+  TORCH_CHECK(a.size(1) == H && a.size(3) == K && b.size(0) == G && b.size(1) == H && b.size(2) == r && b.size(3) == N,
+              "adapter_linear: a and b do not fit the weight");
+  TORCH_CHECK(G == p.G, "adapter_linear: the batch was planned for ", p.G, " adapters, not ", G);
+  TORCH_CHECK((x.dim() == 2 || (x.dim() == 3 && x.size(1) == H)) && x.size(0) == p.M && x.size(-1) == K,
+              "adapter_linear: x must be [M, K] or [M, H, K] with the batch's ", p.M, " rows");
+  if (scale)
+    TORCH_CHECK(scale->is_cuda() && scale->get_device() == dev && scale->scalar_type() == at::kFloat && scale->dim() == 1 &&
+                    scale->size(0) == G && scale->is_contiguous(),
+                "adapter_linear: scale must be fp32 [adapters]");
+  return Checked{(int)H, (int)K, (int)N, (int)r, dev};
+}
+
+}  // namespace
+
+// y [M, H, N], and t [parts, H, M, rp] fp32 (empty without adapters) for the backward pass.
+std::vector<at::Tensor> adapter_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor& a, const at::Tensor& b,
+                                        const at::Tensor& plan, const std::vector<int64_t>& dims,
+                                        const c10::optional<at::Tensor>& scale, double scale0, const at::Tensor& err) {
+  const Plan p = read_plan(plan, dims);
+  const Checked c = check_all(x, w, a, b, p, scale);
+  c10::cuda::CUDAGuard guard(c.dev);
+  auto st = at::cuda::getCurrentCUDAStream(c.dev).stream();
+  const Rows rows = rows_of(x, x.dim() == 3);
+  at::Tensor t;
+  if (p.rows > 0)
+    t = shrink(rows, a, p, c.H, c.r, st);
+  else
+    t = at::empty({0}, a.options().dtype(at::kFloat));
+  return {project(rows, w, true, false, b, t, p, c.r, scale, scale0, err, st, c.dev), t};
+}
+
+// dx (like x), da, db from dy [M, H, N]; an output that is not asked for is an empty tensor.
+std::vector<at::Tensor> adapter_backward(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& w,
+                                         const at::Tensor& a, const at::Tensor& b, const at::Tensor& t,
+                                         const at::Tensor& plan, const std::vector<int64_t>& dims,
+                                         const c10::optional<at::Tensor>& scale, double scale0, const at::Tensor& err,
+                                         bool want_dx, bool want_da, bool want_db) {
+  const Plan p = read_plan(plan, dims);
+  const Checked c = check_all(x, w, a, b, p, scale);
+  check_operand(dy, c.dev, "dy");
+  TORCH_CHECK(dy.dim() == 3 && dy.size(0) == p.M && dy.size(1) == c.H && dy.size(2) == c.N, "adapter_linear: dy [M, H, N]");
+  c10::cuda::CUDAGuard guard(c.dev);
+  auto st = at::cuda::getCurrentCUDAStream(c.dev).stream();
+  const bool shared = x.dim() == 2;
+  const Rows rx = rows_of(x, !shared), ry = rows_of(dy, true);
+  at::Tensor none = at::empty({0}, w.options()), u, dx = none, da = none, db = none;
+  if (p.rows > 0 && (want_dx || want_da)) u = shrink(ry, b, p, c.H, c.r, st);
+  if (want_dx) dx = project(ry, w, false, shared, a, u, p, c.r, scale, scale0, err, st, c.dev);
+  if (want_da) da = p.rows > 0 ? wgrad(rx, u, p, a, c.H, c.r, scale, scale0, st) : at::zeros_like(a);
+  if (want_db) db = p.rows > 0 ? wgrad(ry, t, p, b, c.H, c.r, scale, scale0, st) : at::zeros_like(b);
+  return {dx, da, db};
+}
+
+}  // namespace bd

@@ -114,6 +114,23 @@ void ddp_apply_nvls(int64_t mc_shadow, int64_t mc_master, int64_t lo, int64_t hi
                     double eps, double wd, const at::Tensor& hyper, const at::Tensor& coef);
 void set_debug_bounds(int64_t device, const c10::optional<at::Tensor>& word);
 void percentile_thresholds(const at::Tensor& values, double q, const at::Tensor& out);
+std::vector<at::Tensor> adapter_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor& a, const at::Tensor& b,
+                                        const at::Tensor& plan, const std::vector<int64_t>& dims,
+                                        const c10::optional<at::Tensor>& scale, double scale0, const at::Tensor& err);
+std::vector<at::Tensor> adapter_backward(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& w,
+                                         const at::Tensor& a, const at::Tensor& b, const at::Tensor& t,
+                                         const at::Tensor& plan, const std::vector<int64_t>& dims,
+                                         const c10::optional<at::Tensor>& scale, double scale0, const at::Tensor& err,
+                                         bool want_dx, bool want_da, bool want_db);
+void sample_tokens(const at::Tensor& logits, const at::Tensor& u, const c10::optional<at::Tensor>& temperature,
+                   double temperature0, const c10::optional<at::Tensor>& top_k, int64_t top_k0,
+                   const c10::optional<at::Tensor>& top_p, double top_p0, const c10::optional<at::Tensor>& min_p,
+                   double min_p0, const at::Tensor& tokens, const at::Tensor& logprobs);
+void adamw_many(const std::vector<at::Tensor>& params, const std::vector<c10::optional<at::Tensor>>& grads,
+                const std::vector<at::Tensor>& shadows, const std::vector<int64_t>& block0, const at::Tensor& owner,
+                const at::Tensor& m, const at::Tensor& v, const c10::optional<at::Tensor>& m_scale,
+                const c10::optional<at::Tensor>& v_scale, double lr, double b1, double b2, double eps, double wd,
+                double bc1, double bc2, int64_t key, const c10::optional<at::Tensor>& gscale);
 }  // namespace bd
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -171,4 +188,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("tp_sum_slots", &bd::tp_sum_slots);
   m.def("tp_gather_bytes", &bd::tp_gather_bytes);
   m.def("percentile_thresholds", &bd::percentile_thresholds);
+  m.def("adapter_forward", &bd::adapter_forward);
+  m.def("adapter_backward", &bd::adapter_backward);
+  m.def("sample_tokens", &bd::sample_tokens);
+  m.def("adamw_many", &bd::adamw_many);
 }

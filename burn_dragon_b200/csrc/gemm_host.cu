@@ -13,6 +13,7 @@
 
 #include "gemm_sm100.cuh"
 #include "gemm_table.h"
+#include "tensor_map.h"
 
 namespace bd {
 
@@ -124,6 +125,22 @@ int num_sms(int dev) {
 }  // namespace
 
 int num_sms_of(int dev) { return num_sms(dev); }
+
+CUtensorMap tensor_map_bf16(const void* base, std::array<int64_t, 3> dims, std::array<int64_t, 2> strides,
+                            uint32_t box_inner, uint32_t box_rows) {
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(base) % 16 == 0 && strides[0] % 8 == 0 && strides[1] % 8 == 0,
+              "TMA operands: 16-byte aligned base and strides");
+  cuuint64_t d[4] = {(cuuint64_t)dims[0], (cuuint64_t)dims[1], (cuuint64_t)dims[2], 1};
+  cuuint64_t s[3] = {(cuuint64_t)strides[0] * 2, (cuuint64_t)strides[1] * 2, (cuuint64_t)strides[1] * 2};
+  cuuint32_t box[4] = {box_inner, box_rows, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUtensorMap m;
+  CUresult r = get_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, s, box, estr,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", (int)r);
+  return m;
+}
 
 namespace {
 const Entry* find_entry(int bn, bool a_mn, bool b_mn, int epi, bool pair) {

@@ -118,3 +118,140 @@ class FusedAdamW:
     def step(self, lr: float | None = None) -> None:
         self.prepare(lr)
         self.apply()
+
+
+BLOCK = 256  # values of a state that share one 8-bit scale
+
+
+def _e4m3_stochastic(x: torch.Tensor, bits16: torch.Tensor, floor: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """[n * 256] values -> (e4m3 codes, one scale per 256), as csrc/adamw_many.cu rounds them."""
+    b = x.view(-1, BLOCK)
+    amax = b.abs().amax(1, keepdim=True)
+    fine = (amax >= 2.0 ** -110) & (amax < math.inf)
+    scale = torch.where(fine, amax * 2.0 ** -8, torch.where(amax < 2.0 ** -110, torch.zeros_like(amax), amax))
+    inverse = torch.where(fine, 256.0 / amax, torch.zeros_like(amax))
+    # multiplied by 2^-120 the e4m3 grid is bits 20 and up of the fp32 pattern, denormals included
+    y = (b.abs() * inverse) * 2.0 ** -120
+    code = (y.view(torch.int32) + (bits16.view(-1, BLOCK) << 4).to(torch.int32)) >> 20
+    if floor:
+        code = torch.where(b > 0, code.clamp_min(1), code)
+    code = torch.where(b < 0, code + 128, code) * fine
+    return code.to(torch.uint8).view(torch.float8_e4m3fn).reshape(-1), scale[:, 0]
+
+
+class AdamWMany:
+    """AdamW over many tensors in one launch, e.g. the adapters of an ``AdapterBank``.
+
+    ``params``: contiguous fp32 or bf16 tensors of one device; ``shadows``: none, or a bf16
+    working copy of each that the step writes too. ``state_bits`` 32 keeps both moments in fp32, 8
+    keeps them as e4m3 codes with one fp32 scale per 256 values (a quarter of the state and
+    of its traffic), rounded stochastically from ``seed``, the step and the index, so that a
+    step of v by a thousandth of itself is kept on average and a run repeats bit for bit.
+
+    ``state``: ``m`` and ``v`` (and ``m_scale`` / ``v_scale``), every tensor padded to blocks of 256
+    values in the order of ``params``. A tensor whose gradient is None is left alone. The step
+    count and the learning rate are arguments of the launch, so a captured CUDA graph would
+    repeat one step; ``FusedAdamW`` keeps them on the device for that."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.1,
+                 state_bits: int = 32, shadows=None, seed: int = 0):
+        self.params = [p.detach() for p in params]
+        if not self.params:
+            raise ValueError("AdamWMany needs at least one tensor")
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        dev = self.params[0].device
+        self.shadows = [] if shadows is None else list(shadows)
+        if self.shadows and len(self.shadows) != len(self.params):
+            raise ValueError("no shadows, or one per tensor")
+        for p in self.params:
+            if p.device != dev or not p.is_contiguous() or p.dtype not in (torch.float32, torch.bfloat16):
+                raise ValueError("AdamWMany takes contiguous fp32 or bf16 tensors on one device")
+        for p, s in zip(self.params, self.shadows):
+            if s.device != dev or not s.is_contiguous() or s.dtype != torch.bfloat16 or s.numel() != p.numel():
+                raise ValueError("a shadow is a contiguous bf16 tensor of its tensor's size")
+        self.lr, (self.b1, self.b2), self.eps, self.wd = lr, betas, eps, weight_decay
+        self.state_bits, self.seed, self.t = state_bits, int(seed), 0
+        sizes = [-(-p.numel() // BLOCK) for p in self.params]
+        self.block0 = [0]
+        for n in sizes:
+            self.block0.append(self.block0[-1] + n)
+        total = self.block0[-1]
+        self.owner = torch.repeat_interleave(torch.arange(len(sizes), dtype=torch.int32),
+                                             torch.tensor(sizes)).to(dev)
+        kind = torch.float8_e4m3fn if state_bits == 8 else torch.float32
+        self.state = {k: torch.zeros(total * BLOCK, dtype=kind, device=dev) for k in ("m", "v")}
+        if state_bits == 8:
+            self.state |= {k: torch.zeros(total, device=dev) for k in ("m_scale", "v_scale")}
+
+    def state_dict(self) -> dict:
+        return {**self.state, "t": self.t, "lr": self.lr, "seed": self.seed}
+
+    def load_state_dict(self, sd: dict) -> None:
+        for k, t in self.state.items():
+            if sd[k].dtype != t.dtype or sd[k].shape != t.shape:
+                raise ValueError(f"state {k!r} is {tuple(sd[k].shape)} {sd[k].dtype}, not {tuple(t.shape)} {t.dtype}")
+            t.copy_(sd[k])
+        self.t = int(sd["t"])
+        self.seed = int(sd.get("seed", self.seed))
+
+    def moments(self, i: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """The first and second moment of tensor ``i`` in fp32, in its shape."""
+        lo, hi = self.block0[i], self.block0[i + 1]
+        p, out = self.params[i], []
+        for k in ("m", "v"):
+            x = self.state[k][lo * BLOCK:hi * BLOCK].float().view(-1, BLOCK)
+            if self.state_bits == 8:
+                x = x * self.state[k + "_scale"][lo:hi, None]
+            out.append(x.reshape(-1)[:p.numel()].view(p.shape))
+        return out[0], out[1]
+
+    @torch.no_grad()
+    def step(self, grads, lr: float | None = None, grad_scale: torch.Tensor | None = None) -> None:
+        """One step. ``grads``: a gradient (fp32 or bf16) or None per tensor; ``grad_scale``: an
+        fp32 device scalar that multiplies them all (a clipping coefficient)."""
+        grads = list(grads)
+        if len(grads) != len(self.params):
+            raise ValueError(f"{len(grads)} gradients for {len(self.params)} tensors")
+        t = self.t + 1
+        lr = self.lr if lr is None else lr
+        bc1, bc2 = 1.0 - self.b1 ** t, 1.0 - self.b2 ** t
+        key = (self.seed * 0x9E3779B1 + t * 0x85EBCA77) & 0xFFFFFFFF
+        if self.state["m"].is_cuda:
+            grads = [g if g is None or g.is_contiguous() else g.contiguous() for g in grads]
+            _ext.load().adamw_many(self.params, grads, self.shadows, self.block0, self.owner, self.state["m"],
+                                   self.state["v"], self.state.get("m_scale"), self.state.get("v_scale"), lr, self.b1,
+                                   self.b2, self.eps, self.wd, bc1, bc2, key, grad_scale)
+        else:
+            for p, g in zip(self.params, grads):
+                if g is not None and g.numel() != p.numel():
+                    raise ValueError("a gradient has its tensor's size")
+            for i, (p, g) in enumerate(zip(self.params, grads)):
+                if g is not None:
+                    self._step_cpu(i, p, g, lr, bc1, bc2, key, grad_scale)
+        self.t = t
+
+    def _step_cpu(self, i, p, g, lr, bc1, bc2, key, grad_scale) -> None:
+        blocks = slice(self.block0[i], self.block0[i + 1])
+        values = slice(blocks.start * BLOCK, blocks.stop * BLOCK)
+        n = p.numel()
+        g = torch.nn.functional.pad(g.reshape(-1).float(), (0, -n % BLOCK))
+        g = g if grad_scale is None else g * grad_scale
+        m, v = (self.state[k][values].float() for k in ("m", "v"))
+        if self.state_bits == 8:
+            m, v = ((x.view(-1, BLOCK) * self.state[k][blocks, None]).view(-1)
+                    for x, k in ((m, "m_scale"), (v, "v_scale")))
+        m = m * self.b1 + g * (1 - self.b1)
+        v = v * self.b2 + (g * g) * (1 - self.b2)
+        q = p.reshape(-1).float() * (1 - lr * self.wd) - lr * ((m / bc1) / ((v / bc2).sqrt() + self.eps))[:n]
+        p.view(-1).copy_(q)
+        if self.shadows:
+            self.shadows[i].view(-1).copy_(q)
+        if self.state_bits == 8:
+            h = (torch.arange(values.start, values.stop) * 0x9E3779B1 + key) & 0xFFFFFFFF
+            h = ((h ^ (h >> 16)) * 0x85EBCA6B) & 0xFFFFFFFF
+            h = ((h ^ (h >> 13)) * 0xC2B2AE35) & 0xFFFFFFFF
+            h = h ^ (h >> 16)
+            m, self.state["m_scale"][blocks] = _e4m3_stochastic(m, h & 0xFFFF, False)
+            v, self.state["v_scale"][blocks] = _e4m3_stochastic(v, h >> 16, True)
+        self.state["m"][values], self.state["v"][values] = m, v
