@@ -11,11 +11,16 @@
 //   min-p   w_i >= min_p;
 //   token   the first index whose running sum over the kept (in index order) exceeds
 //           floor(u * sum of the kept);  logprob = (l - m) / T - log(sum 2^-40).
-// What is kept is a prefix of the order, i.e. one bound (value, index). It is found by
-// histograms of counts and weights, not by sorting: 1024 linear buckets of (m - l) / T first
-// (1/32 wide; a weight below 2^-40 is zero and needs no bucket), then, among the bucket
-// that holds the bound, the bits of the value and of the index, until at most kList
-// candidates are left, which are ranked against each other.
+// What is kept is a prefix of the order, i.e. one bound (value, index), found without sorting
+// the row:
+//   top-k   a histogram of 1024 linear buckets of (m - l) / T (1/32 wide) names the bucket of the
+//           k-th value; it and all above it, few, are sorted;
+//   top-p   the weights replace the logits in shared memory; a histogram of counts over their
+//           bits (16 buckets an octave) names a window of three buckets around the border; the sum above
+//           it and a histogram of its weights are exact and name one of 768 parts of the
+//           window, which is sorted.
+// Where more than kList values are left (many equal ones), or the border is not in the window,
+// find_bound refines exact histograms over the row's bits, read again from memory.
 //
 // A row is split over a cluster of C CTAs that keep their slice of it in shared memory (the
 // logits are read from memory once) and merge maxima, histograms and sums through
@@ -34,10 +39,11 @@ using u64 = unsigned long long;
 
 constexpr int kThreads = 512;
 constexpr int kWarpsS = kThreads / 32;
-constexpr int kBuckets = 1024;
-constexpr int kList = 512;
+constexpr int kBuckets = 1024;  // two a thread
+constexpr int kList = 1024;     // values that are sorted
 constexpr int kMaxCluster = 8;
-constexpr int kMaxSlice = 40960;  // logits a CTA can hold
+constexpr int kMaxSlice = 32768;  // logits a CTA can hold
+constexpr float kMinusInf = -INFINITY;
 
 struct SampleArgs {
   const void* logits;
@@ -51,55 +57,55 @@ struct SampleArgs {
   float* logprobs;
 };
 
+// With a slice of 64,000 bytes (128,000 tokens over 8 CTAs) three CTAs share an SM.
 struct Shared {
-  unsigned count[kBuckets];
-  unsigned lo[kBuckets], hi[kBuckets];  // a bucket's weight as two words
-  u64 list_order[kList];                // ~value bits : index, ascending = the order of the row
-  u64 list_weight[kList];
+  union {
+    struct {
+      unsigned count[kBuckets];
+      unsigned lo[kBuckets], hi[kBuckets];  // a bucket's weight as two words
+    };
+    u64 list[kList];  // order bits : index, ascending = the order of the row
+  };
   u64 warp_sum[kWarpsS];
-  u64 warp_count[kWarpsS];
-  u64 slot[kMaxCluster];  // one value per CTA of the cluster
+  unsigned warp_count[kWarpsS];
+  u64 slot[3][kMaxCluster];  // one value per CTA of the cluster; the next exchange uses another row
   float slot_max[kMaxCluster];
-  int slot_first[kMaxCluster];
-  unsigned list_n;
-  // result of a bucket search / of a ranking
+  u64 before_count, before_weight, bound;
+  unsigned list_n, digit_count;
   int digit;
-  unsigned digit_count;
-  u64 before_count, before_weight;
-  u64 bound, list_kept_weight;
 };
 
 __device__ __forceinline__ unsigned order_bits(float l) {  // ascending in descending l
   const unsigned b = __float_as_uint(l);
   return (b & 0x80000000u) ? b : ~(b | 0x80000000u);
 }
+__device__ __forceinline__ float order_value(unsigned o) {
+  return __uint_as_float((o & 0x80000000u) ? o : (~o & 0x7fffffffu));
+}
+__device__ __forceinline__ u64 order_of(float l, int index) { return (u64)order_bits(l) << 32 | (unsigned)index; }
 
 __device__ __forceinline__ u64 fixed40(float w) {  // floor(w 2^40) for 0 <= w <= 1
   const unsigned b = __float_as_uint(w);
   const int s = (int)(b >> 23) - (127 + 23 - 40);
   const u64 m = (b & 0x7fffffu) | 0x800000u;
-  return s >= 0 ? m << s : (s > -24 ? m >> -s : 0ull);
+  return s >= 0 ? (s <= 17 ? m << s : 0ull) : (s > -24 ? m >> -s : 0ull);
 }
 
 struct Row {
-  float top, inv_t;
+  float top, inv_t, per_bucket;
   __device__ __forceinline__ float z(float l) const { return l == top ? 0.f : __fmul_rn(__fsub_rn(l, top), inv_t); }
   __device__ __forceinline__ float w(float l) const { return expf(z(l)); }
-  __device__ __forceinline__ int bucket(float l) const {
-    return l == top ? 0 : min(kBuckets - 1, (int)(__fmul_rn(__fsub_rn(top, l), inv_t) * 32.f));
-  }
+  __device__ __forceinline__ u64 weight(float l) const { return l == kMinusInf ? 0ull : fixed40(w(l)); }
+  // linear in (top - l) / T; a NaN product (0 * inf: l is the top) is bucket 0
+  __device__ __forceinline__ int bucket(float l) const { return min(kBuckets - 1, (int)((top - l) * per_bucket)); }
 };
 
-template <typename T>
-__device__ __forceinline__ float logit(T x);
-template <>
-__device__ __forceinline__ float logit<float>(float x) {
-  return isnan(x) ? -INFINITY : x + 0.f;  // -0 counts as 0
-}
-template <>
-__device__ __forceinline__ float logit<__nv_bfloat16>(__nv_bfloat16 x) {
-  return logit<float>(__bfloat162float(x));
-}
+// 16 buckets an octave of a weight in (2^-40, 1]
+__device__ __forceinline__ int weight_bucket(float w) { return (int)((0x3f800000u - __float_as_uint(w)) >> 19); }
+constexpr unsigned kWindowBits = 3u << 19;
+
+__device__ __forceinline__ float logit(float x) { return fmaxf(x, kMinusInf) + 0.f; }  // NaN counts as -inf, -0 as 0
+__device__ __forceinline__ float logit(__nv_bfloat16 x) { return logit(__bfloat162float(x)); }
 
 __device__ __forceinline__ u64 warp_total(u64 v) {
 #pragma unroll
@@ -116,159 +122,371 @@ __device__ __forceinline__ u64 warp_inclusive(u64 v, int lane) {
   return v;
 }
 
-// Candidate digits after the linear bucket: three digits of the value's order bits, its
-// last two bits, two digits of the index.
+struct Sums {
+  u64 count, weight;
+};
+
+// Exclusive running sums over the block's threads; `all` gets the totals.
+__device__ __forceinline__ Sums block_exclusive(Shared& s, Sums mine, bool weigh, Sums& all) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const u64 ic = warp_inclusive(mine.count, lane), iw = weigh ? warp_inclusive(mine.weight, lane) : 0;
+  __syncthreads();
+  if (lane == 31) s.warp_count[warp] = (unsigned)ic, s.warp_sum[warp] = iw;
+  __syncthreads();
+  Sums e{ic - mine.count, iw - mine.weight};
+  all = Sums{0, 0};
+#pragma unroll
+  for (int q = 0; q < kWarpsS; ++q) {
+    if (q < warp) e.count += s.warp_count[q], e.weight += s.warp_sum[q];
+    all.count += s.warp_count[q], all.weight += s.warp_sum[q];
+  }
+  return e;
+}
+
+// The sum of one value per thread over the cluster; also a barrier of the cluster. `row`: of slot, another
+// one than the last exchange's unless a barrier lies between.
+__device__ __forceinline__ u64 cluster_total(Shared& s, int row, u64 mine, u64* before = nullptr) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const u64 w = warp_total(mine);
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) s.warp_sum[threadIdx.x / 32] = w;
+  __syncthreads();
+  u64 block = 0;
+#pragma unroll
+  for (int q = 0; q < kWarpsS; ++q) block += s.warp_sum[q];
+  if ((int)threadIdx.x < C) cluster.map_shared_rank(&s, threadIdx.x)->slot[row][rank] = block;
+  cluster.sync();
+  u64 total = 0;
+  for (int q = 0; q < C; ++q) {
+    if (before && q < rank) *before += s.slot[row][q];
+    total += s.slot[row][q];
+  }
+  return total;
+}
+
+__device__ __forceinline__ void add_weight(Shared& s, int d, u64 w) {
+  const unsigned lo = (unsigned)w, old = atomicAdd(&s.lo[d], lo);
+  const unsigned hi = (unsigned)(w >> 32) + (old + lo < old ? 1u : 0u);
+  if (hi) atomicAdd(&s.hi[d], hi);
+}
+
+__device__ __forceinline__ void clear_histogram(Shared& s, bool weigh) {
+  for (int b = threadIdx.x; b < kBuckets; b += kThreads) {
+    s.count[b] = 0;
+    if (weigh) s.lo[b] = s.hi[b] = 0;
+  }
+  __syncthreads();
+}
+
+// This thread's two buckets of the cluster's histogram.
+__device__ __forceinline__ void merged(Shared& s, bool weigh, Sums (&b)[2]) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks();
+  b[0] = b[1] = Sums{0, 0};
+  const int at = 2 * threadIdx.x;
+  for (int q = 0; q < C; ++q) {
+    const Shared* o = cluster.map_shared_rank(&s, q);
+    const uint2 c = *reinterpret_cast<const uint2*>(&o->count[at]);
+    b[0].count += c.x, b[1].count += c.y;
+    if (weigh) {
+      const uint2 lo = *reinterpret_cast<const uint2*>(&o->lo[at]), hi = *reinterpret_cast<const uint2*>(&o->hi[at]);
+      b[0].weight += (u64)hi.x << 32 | lo.x, b[1].weight += (u64)hi.y << 32 | lo.y;
+    }
+  }
+}
+
+// The first bucket after which `most` values or `reach` weight is there, from running sums `at`.
+// Written to s by the one thread that has it; s.digit stays -1 if there is none.
+__device__ __forceinline__ void pick(Shared& s, const Sums (&b)[2], Sums at, u64 most, u64 reach) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (b[k].count > 0 && at.count < most && at.weight < reach &&
+        (at.count + b[k].count >= most || at.weight + b[k].weight >= reach)) {
+      s.digit = 2 * threadIdx.x + k;
+      s.digit_count = (unsigned)min(b[k].count, 0xffffffffull);
+      s.before_count = at.count;
+      s.before_weight = at.weight;
+    }
+    at.count += b[k].count;
+    at.weight += b[k].weight;
+  }
+}
+
+__device__ __forceinline__ void push(Shared* first, u64 order) {
+  const unsigned at = atomicAdd(&first->list_n, 1u);
+  if (at < kList) first->list[at] = order;
+}
+
+// Ascending bitonic sort of the first CTA's list.
+__device__ void sort_list(Shared& s, int n) {
+  int size = 2;
+  while (size < n) size <<= 1;
+  for (int i = n + threadIdx.x; i < size; i += kThreads) s.list[i] = ~0ull;
+  __syncthreads();
+  for (int k = 2; k <= size; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int t = threadIdx.x; t < size / 2; t += kThreads) {
+        const int i = 2 * t - (t & (j - 1)), l = i + j;
+        const u64 a = s.list[i], b = s.list[l];
+        if ((a > b) == ((i & k) == 0)) s.list[i] = b, s.list[l] = a;
+      }
+      __syncthreads();
+    }
+}
+
+// After the gather's barrier: the first CTA sorts the list and finds the last value that is kept: fewer
+// than `most` values and less than `reach` weight before it, counted from `before`. Where `share` is
+// given, reach is that share of the first `most` values' weight. Every CTA gets the bound.
+__device__ u64 list_bound(Shared& s, const Row& r, Sums before, u64 most, u64 reach, const float* share) {
+  cg::cluster_group cluster = cg::this_cluster();
+  if (cluster.block_rank() == 0) {
+    const int n = (int)min(s.list_n, (unsigned)kList);
+    sort_list(s, n);
+    Sums v[2], all;
+    u64 order[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int i = 2 * threadIdx.x + k;
+      order[k] = i < n ? s.list[i] : ~0ull;
+      v[k] = Sums{i < n ? 1ull : 0ull, 0};
+      if (i < n && (share || reach != ~0ull) && before.count + i < most) v[k].weight = r.weight(order_value((unsigned)(order[k] >> 32)));
+    }
+    Sums at = block_exclusive(s, Sums{v[0].count + v[1].count, v[0].weight + v[1].weight}, true, all);
+    if (share) {
+      const double want = ceil(__dmul_rn(__ull2double_rn(all.weight), (double)*share));
+      reach = want > 1.0 ? (u64)want : 1ull;
+    }
+    at.count += before.count;
+    at.weight += before.weight;
+    const u64 end = min(most, before.count + n);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (v[k].count && at.count < most && at.weight < reach &&
+          (at.count + 1 >= end || at.weight + v[k].weight >= reach)) {
+        for (int q = 0; q < (int)cluster.num_blocks(); ++q) cluster.map_shared_rank(&s, q)->bound = order[k];
+      }
+      at.count += v[k].count;
+      at.weight += v[k].weight;
+    }
+  }
+  cluster.sync();
+  return s.bound;
+}
+
+// Digits of a value after its linear bucket: ten bits of its order thrice, the last two, its index's ten and ten.
 constexpr int kLevels = 7;
-__device__ __forceinline__ int digit_of(int level, const Row& r, float l, unsigned ob, int index) {
+__device__ __forceinline__ int digit_of(int level, const Row& r, float l, int index) {
   switch (level) {
     case 0: return r.bucket(l);
-    case 1: return (int)(ob >> 22);
-    case 2: return (int)(ob >> 12) & 1023;
-    case 3: return (int)(ob >> 2) & 1023;
-    case 4: return (int)ob & 3;
+    case 1: return (int)(order_bits(l) >> 22);
+    case 2: return (int)(order_bits(l) >> 12) & 1023;
+    case 3: return (int)(order_bits(l) >> 2) & 1023;
+    case 4: return (int)order_bits(l) & 3;
     case 5: return index >> 10;
     default: return index & 1023;
   }
 }
 
-struct Path {  // digits chosen so far
-  int n;
-  int digit[kLevels];
-};
-
-__device__ __forceinline__ bool on_path(const Path& p, const Row& r, float l, int index) {
-  const unsigned ob = order_bits(l);
-  for (int i = 0; i < p.n; ++i)
-    if (digit_of(i, r, l, ob, index) != p.digit[i]) return false;
-  return true;
-}
-
-// Finds the last kept candidate of the row's order, where a candidate is kept while its count of
-// predecessors is below `most` and the weight of its predecessors below `reach`, or 2^64-1 if every
-// candidate is kept. Candidates: weight above zero and order <= `bound`. Also the weight of all kept.
-// Every CTA of the cluster calls it with the same arguments and gets the same answer.
-__device__ u64 find_bound(Shared& s, const float* x, int base, int n, const Row& r, u64 bound, u64 most, u64 reach,
-                          bool weigh, u64& kept_weight) {
+// The same bound for any row: exact histograms digit by digit, until at most kList values share all of
+// them. Reads the logits from memory. Values after `bound` and of weight zero are not there. Returns
+// `bound` if all are kept; `kept_weight` gets the weight of the kept.
+template <typename T>
+__device__ __noinline__ u64 find_bound(Shared& s, const T* src, int base, int n, const Row& r, u64 bound, u64 most,
+                                       u64 reach, u64& kept_weight) {
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks();
-  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  Path path;
-  path.n = 0;
-  u64 count0 = 0, weight0 = 0;  // before the candidates on the path
-  for (int level = 0; level < kLevels; ++level) {
-    for (int b = tid; b < kBuckets; b += kThreads) s.count[b] = s.lo[b] = s.hi[b] = 0;
-    if (tid == 0) s.list_n = 0, s.digit = -1;
-    __syncthreads();
-    for (int i = tid; i < n; i += kThreads) {
-      const float l = x[i];
-      if (l == -INFINITY || !on_path(path, r, l, base + i)) continue;
-      const unsigned ob = order_bits(l);
-      if (((u64)ob << 32 | (unsigned)(base + i)) > bound) continue;
-      const u64 w = fixed40(r.w(l));
-      if (w == 0) continue;
-      const int d = digit_of(level, r, l, ob, base + i);
-      atomicAdd(&s.count[d], 1u);
-      if (weigh) {
-        const unsigned lo = (unsigned)w, old = atomicAdd(&s.lo[d], lo);
-        const unsigned hi = (unsigned)(w >> 32) + (old + lo < old ? 1u : 0u);
-        if (hi) atomicAdd(&s.hi[d], hi);
+  int path[kLevels];
+  Sums before{0, 0};
+  int level = 0;
+  for (;; ++level) {
+    cluster.sync();  // what the shared memory held is read
+    clear_histogram(s, true);
+    if (threadIdx.x == 0) s.list_n = 0, s.digit = -1;
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const float l = logit(src[i]);
+      bool on = order_of(l, base + i) <= bound;
+      for (int q = 0; q < level; ++q) on = on && digit_of(q, r, l, base + i) == path[q];
+      const u64 w = on ? r.weight(l) : 0ull;
+      if (w) {
+        const int d = digit_of(level, r, l, base + i);
+        atomicAdd(&s.count[d], 1u);
+        add_weight(s, d, w);
       }
     }
     cluster.sync();
-    // merged histogram: two buckets a thread, then the block's running sums
-    u64 c[2], w[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      c[k] = w[k] = 0;
-      const int b = 2 * tid + k;
-      for (int q = 0; q < C; ++q) {
-        const Shared* o = cluster.map_shared_rank(&s, q);
-        c[k] += o->count[b];
-        if (weigh) w[k] += (u64)o->hi[b] << 32 | o->lo[b];
-      }
-    }
-    u64 ic = warp_inclusive(c[0] + c[1], lane), iw = weigh ? warp_inclusive(w[0] + w[1], lane) : 0;
-    if (lane == 31) s.warp_count[warp] = ic, s.warp_sum[warp] = iw;
-    __syncthreads();
-    u64 bc = count0 + ic - c[0] - c[1], bw = weight0 + iw - w[0] - w[1];
-    u64 all_c = count0, all_w = weight0;
-    for (int q = 0; q < kWarpsS; ++q) {
-      if (q < warp) bc += s.warp_count[q], bw += s.warp_sum[q];
-      all_c += s.warp_count[q], all_w += s.warp_sum[q];
-    }
-    // the bound lies in the first bucket after which the count or the weight is reached
-    if (level == 0 && all_c <= most && all_w <= reach) {
-      kept_weight = all_w;
-      cluster.sync();  // the histograms are read
+    Sums b[2], all;
+    merged(s, true, b);
+    Sums at = block_exclusive(s, Sums{b[0].count + b[1].count, b[0].weight + b[1].weight}, true, all);
+    if (level == 0 && all.count <= most && all.weight <= reach) {
+      kept_weight = all.weight;
       return bound;
     }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (c[k] > 0 && bc < most && bw < reach && (bc + c[k] >= most || bw + w[k] >= reach)) {
-        s.digit = 2 * tid + k;
-        s.digit_count = (unsigned)c[k];
-        s.before_count = bc;
-        s.before_weight = bw;
-      }
-      bc += c[k];
-      bw += w[k];
-    }
-    cluster.sync();  // the search is written, the histograms are read
-    if (s.digit < 0) {  // neither is reached: everything is kept
-      kept_weight = all_w;
-      return bound;
-    }
-    path.digit[path.n++] = s.digit;
-    count0 = s.before_count;
-    weight0 = s.before_weight;
-    if (s.digit_count <= kList || level == kLevels - 1) break;
-    __syncthreads();
+    pick(s, b, Sums{at.count + before.count, at.weight + before.weight}, most, reach);
+    cluster.sync();
+    path[level] = s.digit;
+    before = Sums{s.before_count, s.before_weight};
+    if (s.digit_count <= kList || level + 1 == kLevels) break;
   }
-  // gather the candidates in the first CTA, rank them there
   Shared* first = cluster.map_shared_rank(&s, 0);
-  for (int i = tid; i < n; i += kThreads) {
-    const float l = x[i];
-    if (l == -INFINITY || !on_path(path, r, l, base + i)) continue;
-    const u64 order = (u64)order_bits(l) << 32 | (unsigned)(base + i);
-    if (order > bound) continue;
-    const u64 w = fixed40(r.w(l));
-    if (w == 0) continue;
-    const unsigned at = atomicAdd(&first->list_n, 1u);
-    if (at < kList) {
-      first->list_order[at] = order;
-      first->list_weight[at] = w;
-    }
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const float l = logit(src[i]);
+    bool on = order_of(l, base + i) <= bound;
+    for (int q = 0; q <= level; ++q) on = on && digit_of(q, r, l, base + i) == path[q];
+    if (on && r.weight(l)) push(first, order_of(l, base + i));
   }
   cluster.sync();
-  if (cluster.block_rank() == 0) {
-    const int m = (int)min(s.list_n, (unsigned)kList);
-    for (int i = tid; i < m; i += kThreads) {
-      const u64 me = s.list_order[i];
-      u64 bc = count0, bw = weight0;
-      for (int j = 0; j < m; ++j) {
-        const bool before = s.list_order[j] < me;
-        bc += before ? 1 : 0;
-        bw += before ? s.list_weight[j] : 0;
-      }
-      const u64 ac = bc + 1, aw = bw + s.list_weight[i];
-      // exactly one candidate is kept and its successor is not
-      if (bc < most && bw < reach && (ac >= most || aw >= reach)) {
-        for (int q = 0; q < C; ++q) {
-          Shared* o = cluster.map_shared_rank(&s, q);
-          o->bound = me;
-          o->list_kept_weight = aw;
+  bound = list_bound(s, r, before, most, reach, nullptr);
+  // the weight of the kept: of what lies before the bound and of itself
+  u64 mine = 0;
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const float l = logit(src[i]);
+    if (order_of(l, base + i) <= bound) mine += r.weight(l);
+  }
+  kept_weight = cluster_total(s, 1, mine);
+  return bound;
+}
+
+__device__ __forceinline__ u64 share_of(u64 total, float p) {
+  const double want = ceil(__dmul_rn(__ull2double_rn(total), (double)p));
+  return want > 1.0 ? (u64)want : 1ull;
+}
+
+// top-k (and, inside it, top-p)
+template <typename T>
+__device__ __forceinline__ u64 bound_of_k(Shared& s, const float* x, const T* src, int base, int n, const Row& r, int k,
+                                          const float* p) {
+  cg::cluster_group cluster = cg::this_cluster();
+  clear_histogram(s, false);
+  if (threadIdx.x == 0) s.list_n = 0, s.digit = -1;
+  const float4* x4 = reinterpret_cast<const float4*>(x);
+  const int n4 = (n + 3) / 4;
+  for (int i = threadIdx.x; i < n4; i += kThreads) {
+    const float4 l = x4[i];
+    // the last bucket holds weights of zero only: 2^-40 is (top - l) / T = 27.7 of 32
+    const int b[4] = {r.bucket(l.x), r.bucket(l.y), r.bucket(l.z), r.bucket(l.w)};
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (b[q] < kBuckets - 1) atomicAdd(&s.count[b[q]], 1u);
+  }
+  cluster.sync();
+  Sums b[2], all;
+  merged(s, false, b);
+  const Sums at = block_exclusive(s, Sums{b[0].count + b[1].count, 0}, false, all);
+  pick(s, b, at, (u64)k, ~0ull);
+  cluster.sync();
+  u64 kept = 0;
+  const int last = s.digit < 0 ? kBuckets - 2 : s.digit;
+  const u64 listed = s.digit < 0 ? all.count : s.before_count + s.digit_count;
+  if (listed > kList) {
+    u64 bound = find_bound(s, src, base, n, r, ~0ull, (u64)k, ~0ull, kept);
+    if (p) {
+      const u64 reach = share_of(kept, *p);
+      if (reach < kept) bound = find_bound(s, src, base, n, r, bound, ~0ull, reach, kept);
+    }
+    return bound;
+  }
+  Shared* first = cluster.map_shared_rank(&s, 0);
+  for (int i = threadIdx.x; i < n4; i += kThreads) {
+    const float4 l = x4[i];
+    const float v[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (r.bucket(v[q]) <= last) push(first, order_of(v[q], base + 4 * i + q));
+  }
+  cluster.sync();
+  return list_bound(s, r, Sums{0, 0}, (u64)k, ~0ull, p);
+}
+
+// top-p alone; replaces the logits in x by their weights w
+template <typename T>
+__device__ __forceinline__ u64 bound_of_p(Shared& s, float* x, const T* src, int base, int n, const Row& r, float p) {
+  cg::cluster_group cluster = cg::this_cluster();
+  clear_histogram(s, false);
+  float4* x4 = reinterpret_cast<float4*>(x);
+  const int n4 = (n + 3) / 4;
+  u64 mine = 0;
+  for (int i = threadIdx.x; i < n4; i += kThreads) {
+    const float4 l = x4[i];
+    const float4 w = make_float4(r.w(l.x), r.w(l.y), r.w(l.z), r.w(l.w));
+    x4[i] = w;
+    const float v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const u64 f = fixed40(v[q]);
+      mine += f;
+      if (f) atomicAdd(&s.count[weight_bucket(v[q])], 1u);
+    }
+  }
+  const u64 total = cluster_total(s, 1, mine);
+  const u64 reach = share_of(total, p);
+  if (reach >= total) return ~0ull;
+  // a bucket's weight is near its count times its middle; scaled to the exact total that names the window
+  Sums b[2], all;
+  merged(s, false, b);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const unsigned below = ((unsigned)(2 * threadIdx.x + k) << 19) + (1u << 18);
+    b[k].weight = below < 0x3f800000u ? b[k].count * fixed40(__uint_as_float(0x3f800000u - below)) : 0ull;
+  }
+  Sums at = block_exclusive(s, Sums{b[0].count + b[1].count, b[0].weight + b[1].weight}, true, all);
+  if (threadIdx.x == 0) s.digit = kBuckets;  // where rounding leaves no crossing
+  __syncthreads();
+  const u64 near = (u64)(__ull2double_rn(reach) * (__ull2double_rn(all.weight) / __ull2double_rn(total)));
+  pick(s, b, at, ~0ull, near > 0 ? near : 1ull);
+  cluster.sync();
+  const int window = max(min(s.digit, weight_bucket(9.094947017729282e-13f)) - 1, 0);  // its first bucket
+  const unsigned head = 0x3f800000u - ((unsigned)window << 19);  // bits of the largest weight in it
+  __syncthreads();
+  clear_histogram(s, true);
+  if (threadIdx.x == 0) s.list_n = 0, s.digit = -1;
+  mine = 0;
+  for (int i = threadIdx.x; i < n4; i += kThreads) {
+    const float4 w = x4[i];
+    const float v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const unsigned bits = __float_as_uint(v[q]);
+      if (bits > head) {
+        mine += fixed40(v[q]);
+      } else if (head - bits < kWindowBits) {
+        const int d = (int)((head - bits) >> 11);
+        const u64 f = fixed40(v[q]);
+        if (f) {
+          atomicAdd(&s.count[d], 1u);
+          add_weight(s, d, f);
         }
       }
     }
   }
+  const u64 above = cluster_total(s, 2, mine);
+  merged(s, true, b);
+  at = block_exclusive(s, Sums{b[0].count + b[1].count, b[0].weight + b[1].weight}, true, all);
+  pick(s, b, Sums{at.count, at.weight + above}, ~0ull, reach);
   cluster.sync();
-  kept_weight = s.list_kept_weight;
-  return s.bound;
+  if (above >= reach || s.digit < 0 || s.digit_count > kList) {
+    u64 kept;
+    return find_bound(s, src, base, n, r, ~0ull, ~0ull, reach, kept);
+  }
+  const unsigned part = (unsigned)s.digit;
+  const Sums before{0, s.before_weight};
+  Shared* first = cluster.map_shared_rank(&s, 0);
+  for (int i = threadIdx.x; i < n4; i += kThreads) {
+    const float4 w = x4[i];
+    const float v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const unsigned bits = __float_as_uint(v[q]);
+      if (bits <= head && (head - bits) >> 11 == part && fixed40(v[q]))
+        push(first, order_of(logit(src[4 * i + q]), base + 4 * i + q));
+    }
+  }
+  cluster.sync();
+  return list_bound(s, r, before, ~0ull, reach, nullptr);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ SampleArgs a) {
-  extern __shared__ float x[];
+__global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_constant__ SampleArgs a) {
+  extern __shared__ __align__(16) float x[];
   __shared__ Shared s;
   cg::cluster_group cluster = cg::this_cluster();
   cluster.barrier_arrive();  // waited for before the first access to another CTA's memory
@@ -277,122 +495,151 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int base = min(rank * a.slice, a.V), n = min(a.slice, a.V - base);
   const T* src = static_cast<const T*>(a.logits) + (long long)row * a.row_stride + base;
+  const float temperature = a.temperature ? a.temperature[row] : a.temperature0;
+  const int k = a.top_k ? a.top_k[row] : a.top_k0;
+  const float p = a.top_p ? a.top_p[row] : a.top_p0;
+  const float least = fminf(a.min_p ? a.min_p[row] : a.min_p0, 1.f);
+  const float u = a.u[row];
 
-  // ---- the slice, and the row's maximum with its first index
-  float top = -INFINITY;
-  int first = 0x7fffffff;
-  for (int i = tid; i < n; i += kThreads) {
-    const float l = logit<T>(src[i]);
-    x[i] = l;
-    if (l > top) top = l, first = base + i;
-  }
+  // ---- the slice, and the row's maximum
+  float top = kMinusInf;
+  constexpr int VEC = 16 / sizeof(T);
+  const int nv = reinterpret_cast<uintptr_t>(src) % 16 == 0 ? n / VEC : 0;
+  for (int v0 = tid; v0 < nv; v0 += 4 * kThreads) {
+    uint4 raw[4];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float t = __shfl_xor_sync(0xffffffffu, top, o);
-    const int f = __shfl_xor_sync(0xffffffffu, first, o);
-    if (t > top || (t == top && f < first)) top = t, first = f;
+    for (int q = 0; q < 4; ++q)
+      if (v0 + q * kThreads < nv) raw[q] = __ldcs(reinterpret_cast<const uint4*>(src) + v0 + q * kThreads);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int v = v0 + q * kThreads;
+      if (v >= nv) break;
+      const T* t = reinterpret_cast<const T*>(&raw[q]);
+#pragma unroll
+      for (int e = 0; e < VEC; e += 4) {
+        const float4 l = make_float4(logit(t[e]), logit(t[e + 1]), logit(t[e + 2]), logit(t[e + 3]));
+        top = fmaxf(fmaxf(fmaxf(top, l.x), fmaxf(l.y, l.z)), l.w);
+        *reinterpret_cast<float4*>(x + v * VEC + e) = l;
+      }
+    }
   }
-  if (lane == 0) {
-    s.warp_sum[warp] = __float_as_uint(top);
-    s.warp_count[warp] = (unsigned)first;
+#pragma unroll 4
+  for (int i = nv * VEC + tid; i < n; i += kThreads) {
+    const float l = logit(src[i]);
+    x[i] = l;
+    top = fmaxf(top, l);
   }
+  if (tid < 3 && n + tid < (n + 3) / 4 * 4) x[n + tid] = kMinusInf;  // the passes read whole float4
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) s.warp_sum[warp] = __float_as_uint(top);
   __syncthreads();
   cluster.barrier_wait();
   if (tid < C) {
-    for (int q = 0; q < kWarpsS; ++q) {
-      const float t = __uint_as_float((unsigned)s.warp_sum[q]);
-      const int f = (int)s.warp_count[q];
-      if (q == 0 || t > top || (t == top && f < first)) top = t, first = f;
-    }
-    Shared* o = cluster.map_shared_rank(&s, tid);
-    o->slot_max[rank] = top;
-    o->slot_first[rank] = first;
+    top = kMinusInf;
+    for (int q = 0; q < kWarpsS; ++q) top = fmaxf(top, __uint_as_float((unsigned)s.warp_sum[q]));
+    cluster.map_shared_rank(&s, tid)->slot_max[rank] = top;
   }
   cluster.sync();
   top = s.slot_max[0];
-  first = s.slot_first[0];
-  for (int q = 1; q < C; ++q)
-    if (s.slot_max[q] > top) top = s.slot_max[q], first = s.slot_first[q];
+  for (int q = 1; q < C; ++q) top = fmaxf(top, s.slot_max[q]);
 
-  const float temperature = a.temperature ? a.temperature[row] : a.temperature0;
-  if (top == -INFINITY || !(temperature > 0.f)) {  // nothing to draw from, or the first maximum
-    if (rank == 0 && tid == 0) {
-      a.tokens[row] = top == -INFINITY ? -1 : first;
-      a.logprobs[row] = top == -INFINITY ? -INFINITY : 0.f;
+  if (top == kMinusInf) {  // nothing to draw from
+    if (rank == 0 && tid == 0) a.tokens[row] = -1, a.logprobs[row] = kMinusInf;
+    return;
+  }
+  if (!(temperature > 0.f)) {  // the first maximum
+    int first = 0x7fffffff;
+    for (int i = tid; i < n; i += kThreads)
+      if (x[i] == top) first = min(first, base + i);
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) s.warp_count[warp] = (unsigned)first;
+    __syncthreads();
+    if (tid == 0) {
+      for (int q = 0; q < kWarpsS; ++q) first = min(first, (int)s.warp_count[q]);
+      cluster.map_shared_rank(&s, 0)->slot[2][rank] = (unsigned)first;
     }
     cluster.sync();
+    if (rank == 0 && tid == 0) {
+      for (int q = 0; q < C; ++q) first = min(first, (int)s.slot[2][q]);
+      a.tokens[row] = first;
+      a.logprobs[row] = 0.f;
+    }
     return;
   }
   Row r;
   r.top = top;
   r.inv_t = __fdiv_rn(1.f, temperature);
-  const int k = a.top_k ? a.top_k[row] : a.top_k0;
-  const float p = a.top_p ? a.top_p[row] : a.top_p0;
-  const float least = fminf(a.min_p ? a.min_p[row] : a.min_p0, 1.f);
+  r.per_bucket = r.inv_t * 32.f;
   const bool use_k = k > 0 && k < a.V, use_p = p < 1.f;
 
-  // ---- the bound of the kept prefix
-  u64 bound = ~0ull, kept = 0;
-  if (use_k || use_p) {
-    bound = find_bound(s, x, base, n, r, bound, use_k ? (u64)k : ~0ull, ~0ull, use_p, kept);
-    if (use_p) {
-      const double want = ceil(__dmul_rn(__ull2double_rn(kept), (double)p));
-      const u64 reach = want > 1.0 ? (u64)want : 1ull;
-      if (reach < kept) bound = find_bound(s, x, base, n, r, bound, ~0ull, reach, true, kept);
-    }
-  }
+  u64 bound = ~0ull;
+  if (use_k)
+    bound = bound_of_k(s, x, src, base, n, r, k, use_p ? &p : nullptr);
+  else if (use_p)
+    bound = bound_of_p(s, x, src, base, n, r, p);
+  const bool weights = !use_k && use_p;  // x holds weights
+  const float border = weights && bound != ~0ull ? r.w(order_value((unsigned)(bound >> 32))) : 0.f;
 
-  // ---- sums of the kept weights: warp w owns a run of 32-value steps of the slice
-  const int per_warp = ((n + kWarpsS * 32 - 1) / (kWarpsS * 32)) * 32;
-  const int w0 = min(warp * per_warp, n), w1 = min(w0 + per_warp, n);
+  // ---- sums of the kept weights: warp w owns a run of 256-value steps of the slice
   auto weight = [&](int i) -> u64 {
-    const float l = x[i];
-    if (l == -INFINITY || ((u64)order_bits(l) << 32 | (unsigned)(base + i)) > bound) return 0ull;
-    const float w = r.w(l);
+    float w = x[i];
+    if (weights) {  // equal weights may come of different logits: those are looked up
+      if (w < border || (w == border && bound != ~0ull && order_of(logit(src[i]), base + i) > bound)) return 0ull;
+    } else {
+      if (w == kMinusInf || order_of(w, base + i) > bound) return 0ull;
+      w = r.w(w);
+    }
     return w >= least ? fixed40(w) : 0ull;
   };
+  const int per_warp = ((n + kWarpsS * 256 - 1) / (kWarpsS * 256)) * 256;
+  const int w0 = min(warp * per_warp, n), w1 = min(w0 + per_warp, n);
   u64 sum = 0;
+#pragma unroll 4
   for (int i = w0 + lane; i < w1; i += 32) sum += weight(i);
-  sum = warp_total(sum);
-  if (lane == 0) s.warp_sum[warp] = sum;
-  __syncthreads();
-  u64 mine = 0;
-  for (int q = 0; q < kWarpsS; ++q) mine += s.warp_sum[q];
-  if (tid < C) cluster.map_shared_rank(&s, tid)->slot[rank] = mine;
-  cluster.sync();
-  u64 total = 0, before = 0;
-  for (int q = 0; q < C; ++q) {
-    if (q < rank) before += s.slot[q];
-    total += s.slot[q];
-  }
-  u64 target = (u64)__dmul_rn((double)a.u[row], __ull2double_rn(total));
+  u64 before = 0;
+  const u64 total = cluster_total(s, 0, sum, &before);
+  u64 target = (u64)__dmul_rn((double)u, __ull2double_rn(total));
   target = min(target, total - 1);
-  if (target < before || target >= before + mine) return;
-  // ---- this CTA holds the token: the warp whose run crosses the target walks it
+  sum = s.warp_sum[warp];
   u64 at = before;
   for (int q = 0; q < warp; ++q) at += s.warp_sum[q];
   if (target < at || target >= at + sum) return;
-  for (int i0 = w0; i0 < w1; i0 += 32) {
-    const int i = i0 + lane;
-    const u64 w = i < w1 ? weight(i) : 0ull;
-    const u64 run = at + warp_inclusive(w, lane);
-    const unsigned hit = __ballot_sync(0xffffffffu, run > target);
-    if (hit) {
-      if (lane == __ffs(hit) - 1) {
-        a.tokens[row] = base + i;
-        a.logprobs[row] = r.z(x[i]) - logf(__fmul_rn(__ull2float_rn(total), 9.094947017729282e-13f));
-      }
-      return;
+  // ---- this warp's run crosses the target: 256 values at a time, then 32
+  for (int j0 = w0; j0 < w1; j0 += 256) {
+    u64 part = 0;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) part += j0 + 32 * q + lane < w1 ? weight(j0 + 32 * q + lane) : 0ull;
+    part = warp_total(part);
+    if (target >= at + part) {
+      at += part;
+      continue;
     }
-    at = __shfl_sync(0xffffffffu, run, 31);
+    for (int i0 = j0;; i0 += 32) {
+      const int i = i0 + lane;
+      const u64 run = at + warp_inclusive(i < w1 ? weight(i) : 0ull, lane);
+      const unsigned hit = __ballot_sync(0xffffffffu, run > target);
+      if (hit) {
+        if (lane == __ffs(hit) - 1) {
+          a.tokens[row] = base + i;
+          a.logprobs[row] = r.z(logit(src[i])) - logf(__fmul_rn(__ull2float_rn(total), 9.094947017729282e-13f));
+        }
+        return;
+      }
+      at = __shfl_sync(0xffffffffu, run, 31);
+    }
   }
 }
 
 template <typename T>
-void launch(const SampleArgs& a, int rows, int C, cudaStream_t st) {
+void launch(const SampleArgs& a, int rows, int C, cudaStream_t st, int dev) {
   auto kern = sample_kernel<T>;
   const size_t bytes = (size_t)a.slice * sizeof(float);
-  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSlice * (int)sizeof(float)));
+  static bool attr_set[64] = {false};
+  if (!attr_set[dev]) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSlice * (int)sizeof(float)));
+    attr_set[dev] = true;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * C));
   cfg.blockDim = dim3(kThreads);
@@ -429,7 +676,7 @@ void sample_tokens(const at::Tensor& logits, const at::Tensor& u, const c10::opt
   const bool bf16 = logits.scalar_type() == at::kBFloat16;
   TORCH_CHECK(bf16 || logits.scalar_type() == at::kFloat, "sample_tokens: fp32 or bf16 logits");
   const int64_t B = logits.size(0), V = logits.size(1);
-  TORCH_CHECK(V >= 1 && V <= (int64_t)kMaxCluster * 32768, "sample_tokens: vocabulary of 1 to 262144 tokens");
+  TORCH_CHECK(V >= 1 && V <= (int64_t)kMaxCluster * kMaxSlice, "sample_tokens: vocabulary of 1 to 262144 tokens");
   const int dev = logits.get_device();
   c10::cuda::CUDAGuard guard(dev);
   if (B == 0) return;
@@ -455,9 +702,9 @@ void sample_tokens(const at::Tensor& logits, const at::Tensor& u, const c10::opt
   a.slice = (int)(((V + C - 1) / C + 7) / 8 * 8);
   auto st = at::cuda::getCurrentCUDAStream(dev).stream();
   if (bf16)
-    launch<__nv_bfloat16>(a, (int)B, C, st);
+    launch<__nv_bfloat16>(a, (int)B, C, st, dev);
   else
-    launch<float>(a, (int)B, C, st);
+    launch<float>(a, (int)B, C, st, dev);
 }
 
 }  // namespace bd
