@@ -13,12 +13,12 @@
 //           floor(u * sum of the kept);  logprob = (l - m) / T - log(sum 2^-40).
 // What is kept is a prefix of the order, i.e. one bound (value, index), found without sorting
 // the row:
-//   top-k   a histogram of 1024 linear buckets of (m - l) / T (1/32 wide) names the bucket of the
-//           k-th value; it and all above it, few, are sorted;
-//   top-p   the weights replace the logits in shared memory; a histogram of counts over their
-//           bits (16 buckets an octave) names a window of three buckets around the border; the sum above
-//           it and a histogram of its weights are exact and name one of 768 parts of the
-//           window, which is sorted.
+//   top-k   a histogram of the threads' largest logits, in 1024 linear buckets of (m - l) / T (1/32
+//           wide), names a bucket that k of them reach: all values up to it, few more than k, are sorted;
+//   top-p   the weights replace the logits in shared memory; a sample of them (an eighth, and all
+//           heavy ones), in 16 buckets an octave, names a window around the border that holds
+//           5 % of the weight; the sum above it and a histogram of the window's weights are exact and
+//           name one of up to 1024 parts of it, which is sorted.
 // Where more than kList values are left (many equal ones), or the border is not in the window,
 // find_bound refines exact histograms over the row's bits, read again from memory.
 //
@@ -72,7 +72,7 @@ struct Shared {
   float slot_max[kMaxCluster];
   u64 before_count, before_weight, bound;
   unsigned list_n, digit_count;
-  int digit;
+  int digit, window[2];
 };
 
 __device__ __forceinline__ unsigned order_bits(float l) {  // ascending in descending l
@@ -91,6 +91,22 @@ __device__ __forceinline__ u64 fixed40(float w) {  // floor(w 2^40) for 0 <= w <
   return s >= 0 ? (s <= 17 ? m << s : 0ull) : (s > -24 ? m >> -s : 0ull);
 }
 
+// Sums of fixed40(w) in 32-bit halves: w is split at 2^-17 by adding and taking away 1.5 * 2^6, the rest is
+// floored at 2^-40 by adding 1.5 * 2^-17 rounded down; both sums leave their bits in the low mantissa. Six
+// single-rate instructions a value against about twenty for 64-bit shifts and adds.
+struct WeightSum {
+  unsigned high = 0, low = 0, n = 0;  // at most 2^14 values
+  __device__ __forceinline__ void add(float w) {
+    const float t = __fadd_rn(w, 96.f);
+    const float rest = __fsub_rn(w, __fsub_rn(t, 96.f));
+    high += __float_as_uint(t);
+    low += __float_as_uint(__fadd_rd(rest, 1.1444091796875e-05f));
+  }
+  __device__ __forceinline__ u64 total() const {
+    return ((u64)(high - n * 0x42c00000u) << 23) + (u64)(long long)(int)(low - n * 0x37400000u);
+  }
+};
+
 struct Row {
   float top, inv_t, per_bucket;
   __device__ __forceinline__ float z(float l) const { return l == top ? 0.f : __fmul_rn(__fsub_rn(l, top), inv_t); }
@@ -102,7 +118,7 @@ struct Row {
 
 // 16 buckets an octave of a weight in (2^-40, 1]
 __device__ __forceinline__ int weight_bucket(float w) { return (int)((0x3f800000u - __float_as_uint(w)) >> 19); }
-constexpr unsigned kWindowBits = 3u << 19;
+constexpr float kOne40 = 9.094947017729282e-13f;  // 2^-40
 
 __device__ __forceinline__ float logit(float x) { return fmaxf(x, kMinusInf) + 0.f; }  // NaN counts as -inf, -0 as 0
 __device__ __forceinline__ float logit(__nv_bfloat16 x) { return logit(__bfloat162float(x)); }
@@ -143,20 +159,29 @@ __device__ __forceinline__ Sums block_exclusive(Shared& s, Sums mine, bool weigh
   return e;
 }
 
+// A barrier of the cluster.
+__device__ __forceinline__ void sync_all(cg::cluster_group& cluster) {
+  if (cluster.num_blocks() == 1)
+    __syncthreads();
+  else
+    cluster.sync();
+}
+
 // The sum of one value per thread over the cluster; also a barrier of the cluster. `row`: of slot, another
 // one than the last exchange's unless a barrier lies between.
 __device__ __forceinline__ u64 cluster_total(Shared& s, int row, u64 mine, u64* before = nullptr) {
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int lane = threadIdx.x % 32;
   const u64 w = warp_total(mine);
   __syncthreads();
-  if (threadIdx.x % 32 == 0) s.warp_sum[threadIdx.x / 32] = w;
+  if (lane == 0) s.warp_sum[threadIdx.x / 32] = w;
   __syncthreads();
-  u64 block = 0;
-#pragma unroll
-  for (int q = 0; q < kWarpsS; ++q) block += s.warp_sum[q];
-  if ((int)threadIdx.x < C) cluster.map_shared_rank(&s, threadIdx.x)->slot[row][rank] = block;
-  cluster.sync();
+  if (threadIdx.x < 32) {
+    const u64 block = warp_total(lane < kWarpsS ? s.warp_sum[lane] : 0ull);
+    if (lane < C) cluster.map_shared_rank(&s, lane)->slot[row][rank] = block;
+  }
+  sync_all(cluster);
   u64 total = 0;
   for (int q = 0; q < C; ++q) {
     if (before && q < rank) *before += s.slot[row][q];
@@ -179,7 +204,7 @@ __device__ __forceinline__ void clear_histogram(Shared& s, bool weigh) {
   __syncthreads();
 }
 
-// This thread's two buckets of the cluster's histogram.
+// In the first CTA (the others go on to the next barrier): this thread's two buckets of the cluster's histogram.
 __device__ __forceinline__ void merged(Shared& s, bool weigh, Sums (&b)[2]) {
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks();
@@ -196,17 +221,21 @@ __device__ __forceinline__ void merged(Shared& s, bool weigh, Sums (&b)[2]) {
   }
 }
 
-// The first bucket after which `most` values or `reach` weight is there, from running sums `at`.
-// Written to s by the one thread that has it; s.digit stays -1 if there is none.
+// In the first CTA: the first bucket after which `most` values or `reach` weight is there, from running
+// sums `at`. Told to every CTA by the one thread that has it; digit stays as it was if there is none.
 __device__ __forceinline__ void pick(Shared& s, const Sums (&b)[2], Sums at, u64 most, u64 reach) {
+  cg::cluster_group cluster = cg::this_cluster();
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     if (b[k].count > 0 && at.count < most && at.weight < reach &&
         (at.count + b[k].count >= most || at.weight + b[k].weight >= reach)) {
-      s.digit = 2 * threadIdx.x + k;
-      s.digit_count = (unsigned)min(b[k].count, 0xffffffffull);
-      s.before_count = at.count;
-      s.before_weight = at.weight;
+      for (int q = 0; q < (int)cluster.num_blocks(); ++q) {
+        Shared* o = cluster.map_shared_rank(&s, q);
+        o->digit = 2 * threadIdx.x + k;
+        o->digit_count = (unsigned)min(b[k].count, 0xffffffffull);
+        o->before_count = at.count;
+        o->before_weight = at.weight;
+      }
     }
     at.count += b[k].count;
     at.weight += b[k].weight;
@@ -270,7 +299,7 @@ __device__ u64 list_bound(Shared& s, const Row& r, Sums before, u64 most, u64 re
       at.weight += v[k].weight;
     }
   }
-  cluster.sync();
+  sync_all(cluster);
   return s.bound;
 }
 
@@ -299,7 +328,7 @@ __device__ __noinline__ u64 find_bound(Shared& s, const T* src, int base, int n,
   Sums before{0, 0};
   int level = 0;
   for (;; ++level) {
-    cluster.sync();  // what the shared memory held is read
+    sync_all(cluster);  // what the shared memory held is read
     clear_histogram(s, true);
     if (threadIdx.x == 0) s.list_n = 0, s.digit = -1;
     for (int i = threadIdx.x; i < n; i += kThreads) {
@@ -313,16 +342,21 @@ __device__ __noinline__ u64 find_bound(Shared& s, const T* src, int base, int n,
         add_weight(s, d, w);
       }
     }
-    cluster.sync();
-    Sums b[2], all;
-    merged(s, true, b);
-    Sums at = block_exclusive(s, Sums{b[0].count + b[1].count, b[0].weight + b[1].weight}, true, all);
-    if (level == 0 && all.count <= most && all.weight <= reach) {
-      kept_weight = all.weight;
+    sync_all(cluster);
+    if (cluster.block_rank() == 0) {
+      Sums b[2], all;
+      merged(s, true, b);
+      const Sums at = block_exclusive(s, Sums{b[0].count + b[1].count, b[0].weight + b[1].weight}, true, all);
+      pick(s, b, Sums{at.count + before.count, at.weight + before.weight}, most, reach);
+    }
+    sync_all(cluster);
+    if (s.digit < 0) {  // neither is reached: all are kept
+      u64 mine = 0;
+      for (int i = threadIdx.x; i < n; i += kThreads)
+        if (order_of(logit(src[i]), base + i) <= bound) mine += r.weight(logit(src[i]));
+      kept_weight = cluster_total(s, 1, mine);
       return bound;
     }
-    pick(s, b, Sums{at.count + before.count, at.weight + before.weight}, most, reach);
-    cluster.sync();
     path[level] = s.digit;
     before = Sums{s.before_count, s.before_weight};
     if (s.digit_count <= kList || level + 1 == kLevels) break;
@@ -334,7 +368,7 @@ __device__ __noinline__ u64 find_bound(Shared& s, const T* src, int base, int n,
     for (int q = 0; q <= level; ++q) on = on && digit_of(q, r, l, base + i) == path[q];
     if (on && r.weight(l)) push(first, order_of(l, base + i));
   }
-  cluster.sync();
+  sync_all(cluster);
   bound = list_bound(s, r, before, most, reach, nullptr);
   // the weight of the kept: of what lies before the bound and of itself
   u64 mine = 0;
@@ -351,50 +385,50 @@ __device__ __forceinline__ u64 share_of(u64 total, float p) {
   return want > 1.0 ? (u64)want : 1ull;
 }
 
-// top-k (and, inside it, top-p)
+// top-k (and, inside it, top-p). `own`: the largest logit this thread has read.
 template <typename T>
-__device__ __forceinline__ u64 bound_of_k(Shared& s, const float* x, const T* src, int base, int n, const Row& r, int k,
-                                          const float* p) {
+__device__ __forceinline__ u64 bound_of_k(Shared& s, const float* x, const T* src, int V, int base, int n, const Row& r,
+                                          int k, const float* p, float own) {
   cg::cluster_group cluster = cg::this_cluster();
   clear_histogram(s, false);
   if (threadIdx.x == 0) s.list_n = 0, s.digit = -1;
-  const float4* x4 = reinterpret_cast<const float4*>(x);
-  const int n4 = (n + 3) / 4;
-  for (int i = threadIdx.x; i < n4; i += kThreads) {
-    const float4 l = x4[i];
-    // the last bucket holds weights of zero only: 2^-40 is (top - l) / T = 27.7 of 32
-    const int b[4] = {r.bucket(l.x), r.bucket(l.y), r.bucket(l.z), r.bucket(l.w)};
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (b[q] < kBuckets - 1) atomicAdd(&s.count[b[q]], 1u);
+  // the last bucket holds weights of zero only: 2^-40 is (top - l) / T = 27.7 of 32
+  const int b0 = r.bucket(own);
+  if (b0 < kBuckets - 1) atomicAdd(&s.count[b0], 1u);
+  sync_all(cluster);
+  if (cluster.block_rank() == 0) {
+    Sums b[2], all;
+    merged(s, false, b);
+    const Sums at = block_exclusive(s, Sums{b[0].count + b[1].count, 0}, false, all);
+    pick(s, b, at, (u64)k, ~0ull);
   }
-  cluster.sync();
-  Sums b[2], all;
-  merged(s, false, b);
-  const Sums at = block_exclusive(s, Sums{b[0].count + b[1].count, 0}, false, all);
-  pick(s, b, at, (u64)k, ~0ull);
-  cluster.sync();
-  u64 kept = 0;
+  sync_all(cluster);
   const int last = s.digit < 0 ? kBuckets - 2 : s.digit;
-  const u64 listed = s.digit < 0 ? all.count : s.before_count + s.digit_count;
-  if (listed > kList) {
-    u64 bound = find_bound(s, src, base, n, r, ~0ull, (u64)k, ~0ull, kept);
-    if (p) {
-      const u64 reach = share_of(kept, *p);
-      if (reach < kept) bound = find_bound(s, src, base, n, r, bound, ~0ull, reach, kept);
-    }
-    return bound;
-  }
-  Shared* first = cluster.map_shared_rank(&s, 0);
-  for (int i = threadIdx.x; i < n4; i += kThreads) {
-    const float4 l = x4[i];
-    const float v[4] = {l.x, l.y, l.z, l.w};
+  bool listed = s.digit >= 0 || V <= kList;
+  if (listed) {
+    Shared* first = cluster.map_shared_rank(&s, 0);
+    const float4* x4 = reinterpret_cast<const float4*>(x);
+    const int n4 = (n + 3) / 4;
+#pragma unroll 2
+    for (int i = threadIdx.x; i < n4; i += kThreads) {
+      const float4 l = x4[i];
+      if (r.bucket(fmaxf(fmaxf(l.x, l.y), fmaxf(l.z, l.w))) > last) continue;
+      const float v[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (r.bucket(v[q]) <= last) push(first, order_of(v[q], base + 4 * i + q));
+      for (int q = 0; q < 4; ++q)
+        if (r.bucket(v[q]) <= last) push(first, order_of(v[q], base + 4 * i + q));
+    }
+    sync_all(cluster);
+    listed = first->list_n <= kList;
   }
-  cluster.sync();
-  return list_bound(s, r, Sums{0, 0}, (u64)k, ~0ull, p);
+  if (listed) return list_bound(s, r, Sums{0, 0}, (u64)k, ~0ull, p);
+  u64 kept = 0;
+  u64 bound = find_bound(s, src, base, n, r, ~0ull, (u64)k, ~0ull, kept);
+  if (p) {
+    const u64 reach = share_of(kept, *p);
+    if (reach < kept) bound = find_bound(s, src, base, n, r, bound, ~0ull, reach, kept);
+  }
+  return bound;
 }
 
 // top-p alone; replaces the logits in x by their weights w
@@ -404,65 +438,102 @@ __device__ __forceinline__ u64 bound_of_p(Shared& s, float* x, const T* src, int
   clear_histogram(s, false);
   float4* x4 = reinterpret_cast<float4*>(x);
   const int n4 = (n + 3) / 4;
-  u64 mine = 0;
+  WeightSum sum;
+#pragma unroll 2
   for (int i = threadIdx.x; i < n4; i += kThreads) {
     const float4 l = x4[i];
     const float4 w = make_float4(r.w(l.x), r.w(l.y), r.w(l.z), r.w(l.w));
     x4[i] = w;
-    const float v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const u64 f = fixed40(v[q]);
-      mine += f;
-      if (f) atomicAdd(&s.count[weight_bucket(v[q])], 1u);
-    }
+    sum.n += 4;
+    sum.add(w.x), sum.add(w.y), sum.add(w.z), sum.add(w.w);
   }
-  const u64 total = cluster_total(s, 1, mine);
+  const u64 total = cluster_total(s, 1, sum.total());
   const u64 reach = share_of(total, p);
   if (reach >= total) return ~0ull;
-  // a bucket's weight is near its count times its middle; scaled to the exact total that names the window
-  Sums b[2], all;
-  merged(s, false, b);
+  // the window from a sample: every weight above total / 4096, and each thread's first four for the rest
+  const float heavy = __fmul_rn(__ull2float_rn(total), kOne40 / 4096.f);
+  const unsigned share = 16u * (unsigned)n4 / (unsigned)max(1, min(n4, kThreads));
+  for (int i = threadIdx.x; i < n4; i += kThreads) {
+    const float4 w = x4[i];
+    if (i >= kThreads && fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)) < heavy) continue;
+    const float v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const unsigned below = ((unsigned)(2 * threadIdx.x + k) << 19) + (1u << 18);
-    b[k].weight = below < 0x3f800000u ? b[k].count * fixed40(__uint_as_float(0x3f800000u - below)) : 0ull;
+    for (int q = 0; q < 4; ++q)
+      if (v[q] >= kOne40 && (i < kThreads || v[q] >= heavy))
+        atomicAdd(&s.count[weight_bucket(v[q])], v[q] >= heavy ? 16u : share);
   }
-  Sums at = block_exclusive(s, Sums{b[0].count + b[1].count, b[0].weight + b[1].weight}, true, all);
-  if (threadIdx.x == 0) s.digit = kBuckets;  // where rounding leaves no crossing
-  __syncthreads();
-  const u64 near = (u64)(__ull2double_rn(reach) * (__ull2double_rn(all.weight) / __ull2double_rn(total)));
-  pick(s, b, at, ~0ull, near > 0 ? near : 1ull);
-  cluster.sync();
-  const int window = max(min(s.digit, weight_bucket(9.094947017729282e-13f)) - 1, 0);  // its first bucket
-  const unsigned head = 0x3f800000u - ((unsigned)window << 19);  // bits of the largest weight in it
-  __syncthreads();
+  sync_all(cluster);
+  if (cluster.block_rank() == 0) {
+    // A bucket's weight is near its count times its middle. The window: four deviations of the sampled part (a
+    // sampled weight w stands for share / 16 like it: share / 16 w^2 each), half a bucket's width for
+    // the heavy ones, and 0.2 %.
+    Sums b[2], all;
+    merged(s, false, b);
+    float spread = 0.f, big = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const unsigned below = ((unsigned)(2 * threadIdx.x + k) << 19) + (1u << 18);
+      const float mid = below < 0x3f800000u ? __uint_as_float(0x3f800000u - below) : 0.f;
+      b[k].weight = b[k].count * (fixed40(mid) >> 4);
+      const float sum = mid * (float)b[k].count * 0.0625f;
+      spread += mid < heavy ? sum * mid * (float)share * 0.0625f : 0.f;
+      big += mid < heavy ? 0.f : sum;
+    }
+    const Sums at0 = block_exclusive(s, Sums{b[0].count + b[1].count, b[0].weight + b[1].weight}, true, all);
+    const u64 both = (u64)(unsigned)__float2uint_rn(big * 1024.f) << 32;  // big <= 2^18, spread <= 2^18
+    Sums more;
+    block_exclusive(s, Sums{0, both | (u64)__float2uint_rn(fminf(spread, 262144.f) * 16.f)}, true, more);
+    spread = (float)(unsigned)more.weight * 0.0625f + 0.0625f;
+    big = (float)(unsigned)(more.weight >> 32) * (1.f / 1024.f);
+    const float sum = __ull2float_rn(all.weight) * kOne40;
+    const float near = __ull2float_rn(reach) * kOne40 * (sum / (__ull2float_rn(total) * kOne40));
+    const float margin = (share > 16u ? 4.f * sqrtf(spread) : 0.f) + big * 0.03125f + sum * 0.002f;
+    const float lo = near - margin, hi = near + margin;
+    Sums at = at0;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float w0 = __ull2float_rn(at.weight) * kOne40, w1 = __ull2float_rn(at.weight + b[k].weight) * kOne40;
+      const bool last = b[k].count > 0 && at.weight + b[k].weight == all.weight;
+      const bool opens = b[k].count > 0 && (at.weight == 0 || w0 < lo) && (w1 >= lo || last);
+      const bool ends = b[k].count > 0 && w0 < hi && (w1 >= hi || last);
+      for (int q = 0; q < (int)cluster.num_blocks(); ++q) {
+        if (opens) cluster.map_shared_rank(&s, q)->window[0] = 2 * threadIdx.x + k;
+        if (ends) cluster.map_shared_rank(&s, q)->window[1] = 2 * threadIdx.x + k;
+      }
+      at.weight += b[k].weight;
+    }
+  }
+  sync_all(cluster);
+  const int w0 = s.window[0], wide = max(1, s.window[1] - w0 + 1);
+  const unsigned head = 0x3f800000u - ((unsigned)w0 << 19);  // bits of the largest weight in the window
+  const unsigned span = (unsigned)wide << 19;
+  const int shift = 9 + (wide > 1 ? 32 - __clz(wide - 1) : 0);  // 1024 parts at most
   clear_histogram(s, true);
   if (threadIdx.x == 0) s.list_n = 0, s.digit = -1;
-  mine = 0;
+  sum = WeightSum();
+#pragma unroll 2
   for (int i = threadIdx.x; i < n4; i += kThreads) {
     const float4 w = x4[i];
     const float v[4] = {w.x, w.y, w.z, w.w};
+    sum.n += 4;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const unsigned bits = __float_as_uint(v[q]);
-      if (bits > head) {
-        mine += fixed40(v[q]);
-      } else if (head - bits < kWindowBits) {
-        const int d = (int)((head - bits) >> 11);
-        const u64 f = fixed40(v[q]);
-        if (f) {
-          atomicAdd(&s.count[d], 1u);
-          add_weight(s, d, f);
-        }
+      const unsigned under = head - __float_as_uint(v[q]);  // wraps for what is above
+      sum.add((int)under < 0 ? v[q] : 0.f);
+      if (under < span && v[q] >= kOne40) {
+        atomicAdd(&s.count[under >> shift], 1u);
+        add_weight(s, (int)(under >> shift), fixed40(v[q]));
       }
     }
   }
-  const u64 above = cluster_total(s, 2, mine);
-  merged(s, true, b);
-  at = block_exclusive(s, Sums{b[0].count + b[1].count, b[0].weight + b[1].weight}, true, all);
-  pick(s, b, Sums{at.count, at.weight + above}, ~0ull, reach);
-  cluster.sync();
+  const u64 above = cluster_total(s, 2, sum.total());
+  if (cluster.block_rank() == 0) {
+    Sums b[2], all;
+    merged(s, true, b);
+    const Sums at = block_exclusive(s, Sums{b[0].count + b[1].count, b[0].weight + b[1].weight}, true, all);
+    pick(s, b, Sums{at.count, at.weight + above}, ~0ull, reach);
+  }
+  sync_all(cluster);
   if (above >= reach || s.digit < 0 || s.digit_count > kList) {
     u64 kept;
     return find_bound(s, src, base, n, r, ~0ull, ~0ull, reach, kept);
@@ -470,17 +541,16 @@ __device__ __forceinline__ u64 bound_of_p(Shared& s, float* x, const T* src, int
   const unsigned part = (unsigned)s.digit;
   const Sums before{0, s.before_weight};
   Shared* first = cluster.map_shared_rank(&s, 0);
+#pragma unroll 2
   for (int i = threadIdx.x; i < n4; i += kThreads) {
     const float4 w = x4[i];
     const float v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const unsigned bits = __float_as_uint(v[q]);
-      if (bits <= head && (head - bits) >> 11 == part && fixed40(v[q]))
+    for (int q = 0; q < 4; ++q)
+      if ((head - __float_as_uint(v[q])) >> shift == part && v[q] >= kOne40)
         push(first, order_of(logit(src[4 * i + q]), base + 4 * i + q));
-    }
   }
-  cluster.sync();
+  sync_all(cluster);
   return list_bound(s, r, before, ~0ull, reach, nullptr);
 }
 
@@ -505,24 +575,26 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
   float top = kMinusInf;
   constexpr int VEC = 16 / sizeof(T);
   const int nv = reinterpret_cast<uintptr_t>(src) % 16 == 0 ? n / VEC : 0;
-  for (int v0 = tid; v0 < nv; v0 += 4 * kThreads) {
+  const uint4* src4 = reinterpret_cast<const uint4*>(src);
+  auto take = [&](const uint4& raw, int v) {
+    const T* t = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int e = 0; e < VEC; e += 4) {
+      const float4 l = make_float4(logit(t[e]), logit(t[e + 1]), logit(t[e + 2]), logit(t[e + 3]));
+      top = fmaxf(fmaxf(top, fmaxf(l.x, l.y)), fmaxf(l.z, l.w));
+      *reinterpret_cast<float4*>(x + v * VEC + e) = l;
+    }
+  };
+  int v = tid;
+  for (; v + 3 * kThreads < nv; v += 4 * kThreads) {
     uint4 raw[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (v0 + q * kThreads < nv) raw[q] = __ldcs(reinterpret_cast<const uint4*>(src) + v0 + q * kThreads);
+    for (int q = 0; q < 4; ++q) raw[q] = __ldcs(src4 + v + q * kThreads);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int v = v0 + q * kThreads;
-      if (v >= nv) break;
-      const T* t = reinterpret_cast<const T*>(&raw[q]);
-#pragma unroll
-      for (int e = 0; e < VEC; e += 4) {
-        const float4 l = make_float4(logit(t[e]), logit(t[e + 1]), logit(t[e + 2]), logit(t[e + 3]));
-        top = fmaxf(fmaxf(fmaxf(top, l.x), fmaxf(l.y, l.z)), l.w);
-        *reinterpret_cast<float4*>(x + v * VEC + e) = l;
-      }
-    }
+    for (int q = 0; q < 4; ++q) take(raw[q], v + q * kThreads);
   }
+#pragma unroll 3
+  for (; v < nv; v += kThreads) take(__ldcs(src4 + v), v);
 #pragma unroll 4
   for (int i = nv * VEC + tid; i < n; i += kThreads) {
     const float l = logit(src[i]);
@@ -530,6 +602,7 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
     top = fmaxf(top, l);
   }
   if (tid < 3 && n + tid < (n + 3) / 4 * 4) x[n + tid] = kMinusInf;  // the passes read whole float4
+  const float own = top;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) s.warp_sum[warp] = __float_as_uint(top);
@@ -540,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
     for (int q = 0; q < kWarpsS; ++q) top = fmaxf(top, __uint_as_float((unsigned)s.warp_sum[q]));
     cluster.map_shared_rank(&s, tid)->slot_max[rank] = top;
   }
-  cluster.sync();
+  sync_all(cluster);
   top = s.slot_max[0];
   for (int q = 1; q < C; ++q) top = fmaxf(top, s.slot_max[q]);
 
@@ -550,8 +623,14 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
   }
   if (!(temperature > 0.f)) {  // the first maximum
     int first = 0x7fffffff;
-    for (int i = tid; i < n; i += kThreads)
-      if (x[i] == top) first = min(first, base + i);
+    const float4* x4 = reinterpret_cast<const float4*>(x);
+    for (int i = tid; i < (n + 3) / 4; i += kThreads) {
+      const float4 l = x4[i];
+      if (fmaxf(fmaxf(l.x, l.y), fmaxf(l.z, l.w)) == top) {
+        first = min(first, base + 4 * i + (l.x == top ? 0 : l.y == top ? 1 : l.z == top ? 2 : 3));
+        break;
+      }
+    }
     first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0) s.warp_count[warp] = (unsigned)first;
     __syncthreads();
@@ -559,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
       for (int q = 0; q < kWarpsS; ++q) first = min(first, (int)s.warp_count[q]);
       cluster.map_shared_rank(&s, 0)->slot[2][rank] = (unsigned)first;
     }
-    cluster.sync();
+    sync_all(cluster);
     if (rank == 0 && tid == 0) {
       for (int q = 0; q < C; ++q) first = min(first, (int)s.slot[2][q]);
       a.tokens[row] = first;
@@ -575,59 +654,82 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
 
   u64 bound = ~0ull;
   if (use_k)
-    bound = bound_of_k(s, x, src, base, n, r, k, use_p ? &p : nullptr);
+    bound = bound_of_k(s, x, src, a.V, base, n, r, k, use_p ? &p : nullptr, own);
   else if (use_p)
     bound = bound_of_p(s, x, src, base, n, r, p);
   const bool weights = !use_k && use_p;  // x holds weights
-  const float border = weights && bound != ~0ull ? r.w(order_value((unsigned)(bound >> 32))) : 0.f;
 
-  // ---- sums of the kept weights: warp w owns a run of 256-value steps of the slice
-  auto weight = [&](int i) -> u64 {
-    float w = x[i];
-    if (weights) {  // equal weights may come of different logits: those are looked up
-      if (w < border || (w == border && bound != ~0ull && order_of(logit(src[i]), base + i) > bound)) return 0ull;
-    } else {
-      if (w == kMinusInf || order_of(w, base + i) > bound) return 0ull;
-      w = r.w(w);
+  // ---- sums of the kept weights: warp w owns a run of the slice
+  const float last = bound == ~0ull ? kMinusInf : order_value((unsigned)(bound >> 32));  // the border's logit
+  const float border = weights ? (bound == ~0ull ? 0.f : r.w(last)) : last;            // and as x holds it
+  auto kept = [&](int i, float v) -> float {  // the weight of x[i] = v, 0 where it is not kept
+    if (v < border) return 0.f;
+    if (v == border && bound != ~0ull) {  // equal values are kept in order; equal weights may be of other logits
+      if (order_of(weights ? logit(src[i]) : v, base + i) > bound) return 0.f;
     }
-    return w >= least ? fixed40(w) : 0ull;
+    const float w = weights ? v : r.w(v);
+    return w >= least ? w : 0.f;
   };
   const int per_warp = ((n + kWarpsS * 256 - 1) / (kWarpsS * 256)) * 256;
   const int w0 = min(warp * per_warp, n), w1 = min(w0 + per_warp, n);
-  u64 sum = 0;
-#pragma unroll 4
-  for (int i = w0 + lane; i < w1; i += 32) sum += weight(i);
+  WeightSum run;
+  const float4* x4 = reinterpret_cast<const float4*>(x);
+  if (bound == ~0ull && !weights) {  // every value counts
+#pragma unroll 2
+    for (int i = w0 + 4 * lane; i < w1; i += 128) {
+      const float4 l = x4[i / 4];
+      const float w[4] = {r.w(l.x), r.w(l.y), r.w(l.z), r.w(l.w)};
+      run.n += 4;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) run.add(w[q] >= least ? w[q] : 0.f);
+    }
+  } else {
+#pragma unroll 2
+    for (int i = w0 + 4 * lane; i < w1; i += 128) {
+      const float4 l = x4[i / 4];
+      if (fmaxf(fmaxf(l.x, l.y), fmaxf(l.z, l.w)) < border) continue;
+      const float v[4] = {l.x, l.y, l.z, l.w};
+      run.n += 4;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) run.add(kept(i + q, v[q]));
+    }
+  }
   u64 before = 0;
-  const u64 total = cluster_total(s, 0, sum, &before);
+  const u64 total = cluster_total(s, 0, run.total(), &before);
   u64 target = (u64)__dmul_rn((double)u, __ull2double_rn(total));
   target = min(target, total - 1);
-  sum = s.warp_sum[warp];
+  const u64 sum = s.warp_sum[warp];
   u64 at = before;
   for (int q = 0; q < warp; ++q) at += s.warp_sum[q];
   if (target < at || target >= at + sum) return;
-  // ---- this warp's run crosses the target: 256 values at a time, then 32
+  // ---- this warp's run crosses the target: steps of 256 values, 8 a lane
   for (int j0 = w0; j0 < w1; j0 += 256) {
-    u64 part = 0;
+    u64 part[8], mine = 0;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) part += j0 + 32 * q + lane < w1 ? weight(j0 + 32 * q + lane) : 0ull;
-    part = warp_total(part);
-    if (target >= at + part) {
-      at += part;
+    for (int q = 0; q < 8; ++q) {
+      const int i = j0 + 8 * lane + q;
+      part[q] = i < w1 ? fixed40(kept(i, x[i])) : 0ull;
+      mine += part[q];
+    }
+    const u64 end = at + warp_inclusive(mine, lane);
+    const u64 next = __shfl_sync(0xffffffffu, end, 31);
+    if (target >= next) {
+      at = next;
       continue;
     }
-    for (int i0 = j0;; i0 += 32) {
-      const int i = i0 + lane;
-      const u64 run = at + warp_inclusive(i < w1 ? weight(i) : 0ull, lane);
-      const unsigned hit = __ballot_sync(0xffffffffu, run > target);
-      if (hit) {
-        if (lane == __ffs(hit) - 1) {
+    if (target < end && target >= end - mine) {
+      u64 here = end - mine;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        if (target >= here && target < here + part[q]) {
+          const int i = j0 + 8 * lane + q;
           a.tokens[row] = base + i;
-          a.logprobs[row] = r.z(logit(src[i])) - logf(__fmul_rn(__ull2float_rn(total), 9.094947017729282e-13f));
+          a.logprobs[row] = r.z(logit(src[i])) - logf(__fmul_rn(__ull2float_rn(total), kOne40));
         }
-        return;
+        here += part[q];
       }
-      at = __shfl_sync(0xffffffffu, run, 31);
     }
+    return;
   }
 }
 
