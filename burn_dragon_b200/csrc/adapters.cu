@@ -433,54 +433,76 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
     // ------------------------------------------------ builders: one row of the tile per thread
     grid_dependency_wait();  // t is complete (and this grid does not end before the one that wrote it)
     const int r = threadIdx.x - 32 * (2 + kEpiWarps);
-    int stage = 0;
-    uint32_t granted_phase = 0;  // one bit per stage: a stage is granted again only after it was built and used
-    bool ok = true;
-    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-      const AdapterTile c = adapter_tile(p, t, BN);
+    // The t of one row and head, scaled and rounded; the next one's loads run while this one is built.
+    struct Row {
+      int slot;
+      uint4 t[8];
+    };
+    auto fetch = [&](const AdapterTile& c, int hr, Row& row) {
       const int m = c.m0 + r;
-      const int slot = p.t && m < p.M ? p.row_slot[m] : -1;
-      const float s = slot < 0 ? 0.f : p.scale ? p.scale[p.row_adapter[m]] : p.scale0;
-      for (int kb = c.kb0; kb < c.kb1; ++kb) {
-        if (kb >= p.HR * p.KB) {
-          const int e = kb - p.HR * p.KB;
-          const int h = p.HR > 1 ? e / c.ext : c.z;
-          const int j = slot - (e % c.ext) * p.per_block;  // my slot's place in this block
-          const bool here = slot >= 0 && j >= 0 && j < p.per_block;
-          const float* src = p.t + ((long long)h * p.M + m) * p.rp;
-          if (!mbar_wait_bounded(&granted_bar[stage], (granted_phase >> stage) & 1, &abort_flag, p.err,
-                                 kErrTimeoutProducer)) {
-            ok = false;
-            break;
-          }
-          granted_phase ^= 1u << stage;
-          uint8_t* dst = sA + stage * Cfg::A_BYTES;
+      row.slot = c.ext > 0 && m < p.M ? p.row_slot[m] : -1;
+      if (row.slot < 0) return;
+      const float s = p.scale ? p.scale[p.row_adapter[m]] : p.scale0;
+      const float* src = p.t + ((long long)(p.HR > 1 ? hr : c.z) * p.M + m) * p.rp;
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            const int at = 8 * q - j * p.rp;  // of my t values
-            if (here && at >= 0 && at < p.rp) {
-              float f[8];
+      for (int i = 0; i < 8; ++i) {
+        if (8 * i >= p.rp) break;
+        float f[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) f[i] = 0.f;
-              for (int part = 0; part < p.parts; ++part) {
-                const float4 lo = *reinterpret_cast<const float4*>(src + part * p.t_part + at);
-                const float4 hi = *reinterpret_cast<const float4*>(src + part * p.t_part + at + 4);
-                f[0] += lo.x, f[1] += lo.y, f[2] += lo.z, f[3] += lo.w;
-                f[4] += hi.x, f[5] += hi.y, f[6] += hi.z, f[7] += hi.w;
-              }
-#pragma unroll
-              for (int i = 0; i < 8; ++i) f[i] *= s;
-              v = to_bf16x8(f);
-            }
-            *reinterpret_cast<uint4*>(dst + sw128(r, q)) = v;
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&built_bar[stage]);
+        for (int e = 0; e < 8; ++e) f[e] = 0.f;
+#pragma unroll 4
+        for (int part = 0; part < p.parts; ++part) {
+          const float4 lo = *reinterpret_cast<const float4*>(src + part * p.t_part + 8 * i);
+          const float4 hi = *reinterpret_cast<const float4*>(src + part * p.t_part + 8 * i + 4);
+          f[0] += lo.x, f[1] += lo.y, f[2] += lo.z, f[3] += lo.w;
+          f[4] += hi.x, f[5] += hi.y, f[6] += hi.z, f[7] += hi.w;
         }
-        if (++stage == STAGES) stage = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] *= s;
+        row.t[i] = to_bf16x8(f);
       }
+    };
+    uint32_t granted_phase = 0;  // one bit per stage: a stage is granted again only after it was built and used
+    int done = 0;                // stage of the tile's first block
+    bool ok = true;
+    Row row, next;
+    int t = blockIdx.x, hr = 0;
+    AdapterTile c = adapter_tile(p, t, BN);
+    fetch(c, 0, row);
+    while (ok && t < total) {
+      const int hr2 = hr + 1 < p.HR ? hr + 1 : 0;
+      const int t2 = hr2 ? t : t + (int)gridDim.x;
+      const AdapterTile c2 = hr2 || t2 >= total ? c : adapter_tile(p, t2, BN);
+      if (t2 < total) fetch(c2, hr2, next);
+      for (int e = 0; e < c.ext; ++e) {
+        const int kb = p.HR * p.KB + hr * c.ext + e;
+        if (kb < c.kb0 || kb >= c.kb1) continue;
+        const int stage = (done + kb - c.kb0) % STAGES;
+        if (!mbar_wait_bounded(&granted_bar[stage], (granted_phase >> stage) & 1, &abort_flag, p.err,
+                               kErrTimeoutProducer)) {
+          ok = false;
+          break;
+        }
+        granted_phase ^= 1u << stage;
+        uint8_t* dst = sA + stage * Cfg::A_BYTES;
+        const int j = row.slot - e * p.per_block;  // the row's slot in this block
+        const int at = row.slot >= 0 && j >= 0 && j < p.per_block ? j * p.rp / 8 : 8;
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (q < at || q >= at + p.rp / 8) *reinterpret_cast<uint4*>(dst + sw128(r, q)) = make_uint4(0u, 0u, 0u, 0u);
+        if (at < 8) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (8 * i < p.rp) *reinterpret_cast<uint4*>(dst + sw128(r, at + i)) = row.t[i];
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&built_bar[stage]);
+      }
+      if (!hr2) done = (done + c.kb1 - c.kb0) % STAGES;
+      row = next;
+      t = t2, hr = hr2;
+      c = c2;
     }
   }
   tc_fence_before();
@@ -721,11 +743,26 @@ at::Tensor project(const Rows& x, const at::Tensor& w, bool w_mn, bool sum_heads
   }
   p.err = err.data_ptr<int>();
   p.tiles_m = (M + 127) / 128;
-  auto tiles = [&](int bn) { return (long long)p.tiles_m * ((N + bn - 1) / bn) * p.Z; };
-  const int bn = tiles(256) >= 148 ? 256 : tiles(128) >= 148 ? 128 : 64;
+  // The tile width and the number of parts of the reduction: what the busiest CTA stages (a 64-wide block is 16 KB
+  // of x and 128 B a column of w, and the operands' way into shared memory bounds the loop), and the fp32 parts
+  // that are written and read again, spread over the chip. Wide tiles stage less per column; few
+  // tiles leave SMs idle unless the reduction is split.
+  const int sms = num_sms_of(dev);
+  const long long blocks = (long long)p.HR * p.KB;
+  int bn = 64;
+  double best = 1e30;
+  p.splits = 1;
+  for (int w_ : {256, 128, 64}) {
+    const long long tiles = (long long)p.tiles_m * ((N + w_ - 1) / w_) * p.Z;
+    for (long long parts = 1; parts <= blocks / 4 || parts == 1; ++parts) {
+      if (parts > 1 && tiles * parts > sms) break;
+      const double waves = (double)((tiles * parts + sms - 1) / sms);
+      double cost = waves * ((double)((blocks + parts - 1) / parts) * (16384.0 + 128.0 * w_) + 65536.0);
+      if (parts > 1) cost += 8.0 * parts * M * N * p.Z / sms + 150000.0;
+      if (cost < best) best = cost, bn = w_, p.splits = (int)parts;
+    }
+  }
   p.tiles_n = (N + bn - 1) / bn;
-  // parts of a long reduction where there are few tiles, at least four blocks each
-  p.splits = (int)std::max<long long>(1, std::min<long long>(148 / tiles(bn), (long long)p.HR * p.KB / 4));
   at::Tensor y = at::empty({M, p.Z, N}, w.options());
   at::Tensor partial;
   if (p.splits > 1) {

@@ -155,11 +155,15 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, a: torch.Tensor, b: to
         raise ValueError(f"adapter_linear takes K and N in multiples of 8 and a rank of 1 to {MAX_RANK}, got K={K} N={N} r={r}")
     per, scale0 = None, 1.0
     if isinstance(scale, torch.Tensor):
-        per = scale.to(x.device, torch.float32).expand(G).contiguous()
+        per = scale if scale.shape == (G,) else scale.expand(G)
+        per = per.to(x.device, torch.float32).contiguous()
     else:
         scale0 = float(scale)
     if batch.rows == 0:
-        y = x.new_zeros(0, H, N)
+        return x.new_zeros((0, H, N) if heads else (0, N))
+    x, weight, a, b = _rows(x), _rows(weight), a.contiguous(), b.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad):
+        y = _AdapterLinear.apply(x, weight, a, b, batch, per, scale0)
     else:
-        y = _AdapterLinear.apply(_rows(x), _rows(weight), a.contiguous(), b.contiguous(), batch, per, scale0)
+        y = _ext.load().adapter_forward(x, weight, a, b, batch.plan, batch.dims, per, scale0, error_word(x.device))[0]
     return y if heads else y.view(batch.rows, N)
