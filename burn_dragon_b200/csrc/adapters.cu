@@ -18,7 +18,7 @@
 //    products, rows of any adapters can share a tile, and W and every b are read once per
 //    row tile. The projection's blocks need no t, so with programmatic launch they run
 //    while adapter_shrink still does; only the builders wait for it.
-//  * adapter_wgrad: da / db, one CTA per adapter, head and 128 columns.
+//  * adapter_grad: da / db, one CTA per adapter, head and slab of columns; for db it gives u in the same pass over dy.
 // t and u are kept in fp32 (partial sums over the parts of the reduction) and rounded to bf16
 // once, as an operand of the next product, like every activation of the bf16 path. All sums are
 // fp32 and in a fixed order: no atomics.
@@ -73,12 +73,17 @@ __global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const __
   const int h = blockIdx.y;
   const int k1 = min((int)(blockIdx.z + 1) * p.part_k, p.K);
   const bf16* a = p.a + ((long long)g * p.H + h) * p.r * p.K;
+  // Rows past the run or the rank repeat the last one: their sums are not kept (n), or meet rows of b that
+  // read as zero (m), and no load needs a condition.
   const bf16* xr[NT];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int i = nt * 8 + lane / 4;
-    xr[nt] = i < rows ? p.x + (long long)p.order[start + i] * p.x_row + (long long)h * p.x_head : nullptr;
-  }
+  for (int nt = 0; nt < NT; ++nt)
+    xr[nt] = p.x + (long long)p.order[start + min(nt * 8 + lane / 4, rows - 1)] * p.x_row + (long long)h * p.x_head;
+  const bf16* ar[MT][2];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ar[mt][i] = a + (long long)min(mt * 16 + i * 8 + lane / 4, p.r - 1) * p.K;
   float acc[MT][NT][4];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
@@ -86,20 +91,15 @@ __global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const __
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[mt][nt][i] = 0.f;
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll 2
-  for (int k = (int)blockIdx.z * p.part_k + warp * 32 + 8 * (lane % 4); k < k1 + 8 * (lane % 4); k += 32 * (kShrinkThreads / 32)) {
-    const bool in = k < k1;
+  auto step = [&](int k, bool in) {
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
     uint4 xv[NT], av[MT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) xv[nt] = in && xr[nt] ? *reinterpret_cast<const uint4*>(xr[nt] + k) : zero;
+    for (int nt = 0; nt < NT; ++nt) xv[nt] = in ? *reinterpret_cast<const uint4*>(xr[nt] + k) : zero;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int row = mt * 16 + i * 8 + lane / 4;
-        av[mt][i] = in && row < p.r ? *reinterpret_cast<const uint4*>(a + (long long)row * p.K + k) : zero;
-      }
+      for (int i = 0; i < 2; ++i) av[mt][i] = in ? *reinterpret_cast<const uint4*>(ar[mt][i] + k) : zero;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -107,7 +107,13 @@ __global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const __
         mma_bf16(acc[mt][nt], av[mt][0].x, av[mt][1].x, av[mt][0].y, av[mt][1].y, xv[nt].x, xv[nt].y);
         mma_bf16(acc[mt][nt], av[mt][0].z, av[mt][1].z, av[mt][0].w, av[mt][1].w, xv[nt].z, xv[nt].w);
       }
-  }
+  };
+  constexpr int SWEEP = 32 * (kShrinkThreads / 32);
+  int k0 = (int)blockIdx.z * p.part_k + warp * 32;  // of this warp's 32 values; a lane reads 8 of them
+  const int off = 8 * (lane % 4);
+#pragma unroll(NT == 1 ? 4 : 2)
+  for (; k0 + 32 <= k1; k0 += SWEEP) step(k0 + off, true);
+  if (k0 < k1) step(k0 + off, k0 + off < k1);
   // the warps' sums, folded in halves (a fixed order)
 #pragma unroll
   for (int half = 4; half > 0; half /= 2) {
@@ -513,40 +519,72 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
   }
 }
 
-// y [M, Z, N] bf16 = the sum of the parts [splits, Z, M, N], in their order.
+// y [M, Z, N] bf16 = the sum of the parts [splits, Z, M, N] in a fixed order: 32 lanes take 4 columns each, 8 warps
+// every eighth part, so that few columns of many parts do not wait for one another.
 __global__ void __launch_bounds__(256) adapter_sum_kernel(const float* __restrict__ partial, int splits, int Z, int M,
                                                           int N, bf16* __restrict__ y) {
-  const long long n = (long long)Z * M * N;
-  for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long long)gridDim.x * 1024) {
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  __shared__ float4 red[8][32];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const long long n = (long long)Z * M * N, i = ((long long)blockIdx.x * 32 + lane) * 4;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (i < n) {
 #pragma unroll 4
-    for (int q = 0; q < splits; ++q) {
+    for (int q = warp; q < splits; q += 8) {
       const float4 v = *reinterpret_cast<const float4*>(partial + q * n + i);
       s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
-    const int col = (int)(i % N);
-    const long long zm = i / N;
-    __nv_bfloat162 lo = __floats2bfloat162_rn(s.x, s.y), hi = __floats2bfloat162_rn(s.z, s.w);
-    *reinterpret_cast<uint2*>(y + ((zm % M) * Z + zm / M) * N + col) =
-        make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
   }
+  red[warp][lane] = s;
+  __syncthreads();
+  if (warp > 0 || i >= n) return;
+#pragma unroll
+  for (int q = 1; q < 8; ++q) {
+    const float4 v = red[q][lane];
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  const int col = (int)(i % N);
+  const long long zm = i / N;
+  __nv_bfloat162 lo = __floats2bfloat162_rn(s.x, s.y), hi = __floats2bfloat162_rn(s.z, s.w);
+  *reinterpret_cast<uint2*>(y + ((zm % M) * Z + zm / M) * N + col) =
+      make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
+}
+
+// t [n] = the sum of its parts [parts, n], n a multiple of 4.
+__global__ void __launch_bounds__(256) adapter_fold_kernel(const float* __restrict__ in, int parts, long long n,
+                                                           float* __restrict__ out) {
+  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int q = 0; q < parts; ++q) {
+    const float4 v = *reinterpret_cast<const float4*>(in + q * n + i);
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  *reinterpret_cast<float4*>(out + i) = s;
 }
 
 // ------------------------------------------------------------------------------- weight gradients
 
-struct WgradArgs {
-  const bf16* x;  // x or dy
+struct GradArgs {
+  const bf16* x;  // x or dy: rows of C values
   long long x_row, x_head;
-  const float* t;  // [parts, H, M, rp]
-  long long t_part;
-  int parts;
+  const float* t;  // [H, M, rp]
   const int* order;
-  const int* group;  // [G + 1]: the rows of adapter g in `order`
+  const int* group;    // [G + 1]: the rows of adapter g in `order`
+  const int* by_size;  // adapters, the ones with most rows first
   const float* scale;
   float scale0;
-  bf16* out;  // [G, H, r, C]
+  bf16* out;      // [G, H, r, C] = s t_g^T x_g
+  const bf16* w;  // [G, H, r, C]: with WITH_U also u[slab, h, m, :] = x[m] w[g]^T over the slab's columns
+  float* u;
   int M, H, r, C;
 };
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&v)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(addr));
+}
 
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&v)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -554,77 +592,156 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&v)[4], uint32_t add
                : "r"(addr));
 }
 
-constexpr int kWgradRows = 32, kWgradCols = 128;
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
 
-// out[g,h] = s t_g^T x_g: rank rows (16 MT) by 128 columns a CTA, the adapter's rows in steps of 32.
-template <int MT>
-__global__ void __launch_bounds__(256) adapter_wgrad_kernel(const __grid_constant__ WgradArgs p) {
-  constexpr int RP = 16 * MT;
-  constexpr int XP = kWgradCols + 8, TP = RP + 8;  // padded rows: ldmatrix reads without bank conflicts
-  __shared__ __align__(16) bf16 xs[2][kWgradRows][XP];
-  __shared__ __align__(16) bf16 ts[2][kWgradRows][TP];
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+constexpr int kGradRows = 32;
+
+// Padded rows: ldmatrix (x, w) and the fragments of t are read without bank conflicts.
+template <int MT, int SLAB, bool WITH_U>
+struct GradCfg {
+  static constexpr int RP = 16 * MT, XP = SLAB + 8, TP = RP + 4;
+  static constexpr int STAGES = MT == 4 && SLAB > 128 ? 2 : 3;
+  static constexpr int X_BYTES = kGradRows * XP * 2, T_BYTES = kGradRows * TP * 4;
+  static constexpr int W_BYTES = WITH_U ? RP * XP * 2 : 0, RED_BYTES = WITH_U ? 4 * kGradRows * TP * 4 : 0;
+  static constexpr int SMEM = STAGES * (X_BYTES + T_BYTES) + W_BYTES + RED_BYTES;
+};
+
+// One adapter, head and SLAB columns a CTA; the adapter's rows in steps of 32, staged by cp.async. A warp
+// holds SLAB / 8 columns of the gradient in registers. With WITH_U the same staged rows also give
+// their products with the adapter's other matrix, so that dy is read once for u and db: bound by that read.
+template <int MT, int SLAB, bool WITH_U>
+__global__ void __launch_bounds__(256) adapter_grad_kernel(const __grid_constant__ GradArgs p) {
+  using Cfg = GradCfg<MT, SLAB, WITH_U>;
+  constexpr int RP = Cfg::RP, XP = Cfg::XP, TP = Cfg::TP, ST = Cfg::STAGES, NT = SLAB / 64;
+  extern __shared__ __align__(16) uint8_t smem[];
+  bf16* xs = reinterpret_cast<bf16*>(smem);
+  float* ts = reinterpret_cast<float*>(smem + ST * Cfg::X_BYTES);
+  bf16* ws = reinterpret_cast<bf16*>(smem + ST * (Cfg::X_BYTES + Cfg::T_BYTES));
+  float* red = reinterpret_cast<float*>(smem + ST * (Cfg::X_BYTES + Cfg::T_BYTES) + Cfg::W_BYTES);
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  const int c0 = blockIdx.x * kWgradCols, h = blockIdx.y, g = blockIdx.z;
+  const int c0 = blockIdx.x * SLAB, h = blockIdx.y, g = p.by_size[blockIdx.z];
   const int r0 = p.group[g], rows = p.group[g + 1] - r0;
-  const int steps = (rows + kWgradRows - 1) / kWgradRows;
+  const int steps = (rows + kGradRows - 1) / kGradRows;
+  const long long gh = (long long)g * p.H + h;
   auto load = [&](int step, int buf) {
-    for (int i = tid; i < kWgradRows * (kWgradCols / 8); i += 256) {
-      const int row = i / (kWgradCols / 8), c = (i % (kWgradCols / 8)) * 8;
-      const int at = step * kWgradRows + row;
-      const bool in = at < rows && c0 + c < p.C;
-      const bf16* src = in ? p.x + (long long)p.order[r0 + at] * p.x_row + (long long)h * p.x_head + c0 + c : p.x;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(&xs[buf][row][c])), "l"(src),
-                   "r"(in ? 16 : 0)
-                   : "memory");
+    if (step < steps) {
+#pragma unroll 4
+      for (int i = tid; i < kGradRows * (SLAB / 8); i += 256) {
+        const int row = i / (SLAB / 8), c = (i % (SLAB / 8)) * 8;
+        const int at = step * kGradRows + row;
+        const bool in = at < rows && c0 + c < p.C;
+        cp_async16(xs + (buf * kGradRows + row) * XP + c,
+                   in ? p.x + (long long)p.order[r0 + at] * p.x_row + (long long)h * p.x_head + c0 + c : p.x, in);
+      }
+      for (int i = tid; i < kGradRows * (RP / 4); i += 256) {
+        const int row = i / (RP / 4), c = (i % (RP / 4)) * 4;
+        const int at = step * kGradRows + row;
+        const bool in = at < rows;
+        cp_async16(ts + (buf * kGradRows + row) * TP + c,
+                   in ? p.t + ((long long)h * p.M + p.order[r0 + at]) * RP + c : p.t, in);
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    for (int i = tid; i < kWgradRows * RP; i += 256) {
-      const int row = i / RP, c = i % RP;
-      const int at = step * kWgradRows + row;
-      float f = 0.f;
-      if (at < rows) {
-        const float* src = p.t + ((long long)h * p.M + p.order[r0 + at]) * RP + c;
-        for (int part = 0; part < p.parts; ++part) f += src[part * p.t_part];
-      }
-      ts[buf][row][c] = __float2bfloat16_rn(f);
-    }
   };
-  float acc[MT][2][4];
+  if constexpr (WITH_U) {
+    for (int i = tid; i < RP * (SLAB / 8); i += 256) {
+      const int row = i / (SLAB / 8), c = (i % (SLAB / 8)) * 8;
+      const bool in = row < p.r && c0 + c < p.C;
+      cp_async16(ws + row * XP + c, in ? p.w + (gh * p.r + row) * p.C + c0 + c : p.w, in);
+    }
+  }
+  float acc[MT][NT][4];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[mt][nt][i] = 0.f;
-  if (steps > 0) load(0, 0);
+#pragma unroll
+  for (int q = 0; q < ST - 1; ++q) load(q, q);
   for (int step = 0; step < steps; ++step) {
-    const int buf = step & 1;
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    const int buf = step % ST;
+    asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
     __syncthreads();
-    if (step + 1 < steps) load(step + 1, buf ^ 1);
+    load(step + ST - 1, (step + ST - 1) % ST);
+    const bf16* xb = xs + buf * kGradRows * XP;
+    const float* tb = ts + buf * kGradRows * TP;
+    // out += t^T x: rank rows, the warp's columns, a 16-row reduction each
 #pragma unroll
-    for (int kk = 0; kk < kWgradRows / 16; ++kk) {
-      uint32_t b[4];
-      ldmatrix_x4_trans(b, smem_u32(&xs[buf][kk * 16 + (lane & 15)][warp * 16 + (lane >> 4) * 8]));
+    for (int kk = 0; kk < kGradRows / 16; ++kk) {
+      uint32_t a[MT][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        uint32_t a[4];
-        ldmatrix_x4_trans(a, smem_u32(&ts[buf][kk * 16 + (lane & 7) + (lane >> 4) * 8][mt * 16 + ((lane >> 3) & 1) * 8]));
-        mma_bf16(acc[mt][0], a[0], a[1], a[2], a[3], b[0], b[1]);
-        mma_bf16(acc[mt][1], a[0], a[1], a[2], a[3], b[2], b[3]);
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float* q = tb + (kk * 16 + (i / 2) * 8 + 2 * (lane % 4)) * TP + mt * 16 + (i % 2) * 8 + lane / 4;
+          a[mt][i] = pack_bf16(q[0], q[TP]);
+        }
+#pragma unroll
+      for (int nt = 0; nt < NT; nt += 2) {
+        uint32_t b[4];
+        ldmatrix_x4_trans(b, smem_u32(xb + (kk * 16 + (lane & 15)) * XP + warp * (SLAB / 8) + nt * 8 + (lane >> 4) * 8));
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          mma_bf16(acc[mt][nt], a[mt][0], a[mt][1], a[mt][2], a[mt][3], b[0], b[1]);
+          mma_bf16(acc[mt][nt + 1], a[mt][0], a[mt][1], a[mt][2], a[mt][3], b[2], b[3]);
+        }
       }
     }
-    __syncthreads();
+    if constexpr (WITH_U) {
+      // u = x w^T: 16 rows and a quarter of the columns a warp, folded over the quarters
+      const int m0 = (warp & 1) * 16, q0 = (warp >> 1) * (SLAB / 4);
+      float uacc[2 * MT][4];
+#pragma unroll
+      for (int j = 0; j < 2 * MT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) uacc[j][i] = 0.f;
+#pragma unroll 4
+      for (int kk = 0; kk < SLAB / 64; ++kk) {
+        uint32_t a[4];
+        ldmatrix_x4(a, smem_u32(xb + (m0 + (lane & 15)) * XP + q0 + kk * 16 + (lane >> 4) * 8));
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+          uint32_t b[4];
+          ldmatrix_x4(b, smem_u32(ws + (j * 16 + (lane & 7) + (lane >> 4) * 8) * XP + q0 + kk * 16 + ((lane >> 3) & 1) * 8));
+          mma_bf16(uacc[2 * j], a[0], a[1], a[2], a[3], b[0], b[1]);
+          mma_bf16(uacc[2 * j + 1], a[0], a[1], a[2], a[3], b[2], b[3]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2 * MT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          red[((warp >> 1) * kGradRows + m0 + lane / 4 + (i / 2) * 8) * TP + j * 8 + 2 * (lane % 4) + i % 2] = uacc[j][i];
+      __syncthreads();
+      for (int i = tid; i < kGradRows * RP; i += 256) {
+        const int row = i / RP, c = i % RP, at = step * kGradRows + row;
+        if (at < rows) {
+          float f = 0.f;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) f += red[(q * kGradRows + row) * TP + c];
+          p.u[(((long long)blockIdx.x * p.H + h) * p.M + p.order[r0 + at]) * RP + c] = f;
+        }
+      }
+    }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   const float s = p.scale ? p.scale[g] : p.scale0;
-  bf16* out = p.out + ((long long)g * p.H + h) * p.r * p.C;
+  bf16* out = p.out + gh * p.r * p.C;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int row = mt * 16 + lane / 4 + 8 * i, col = c0 + warp * 16 + nt * 8 + 2 * (lane % 4);
+        const int row = mt * 16 + lane / 4 + 8 * i, col = c0 + warp * (SLAB / 8) + nt * 8 + 2 * (lane % 4);
         if (row < p.r && col < p.C)
           *reinterpret_cast<__nv_bfloat162*>(out + (long long)row * p.C + col) =
               __floats2bfloat162_rn(acc[mt][nt][2 * i] * s, acc[mt][nt][2 * i + 1] * s);
@@ -636,7 +753,7 @@ __global__ void __launch_bounds__(256) adapter_wgrad_kernel(const __grid_constan
 // The batch's plan: one int32 buffer, and where its parts lie.
 struct Plan {
   int M, G, tiles, chunks, rows_per_chunk, rows;  // rows: those with an adapter
-  const int *row_adapter, *row_slot, *tile_ptr, *slots, *order, *chunk, *group;
+  const int *row_adapter, *row_slot, *tile_ptr, *slots, *order, *chunk, *group, *by_size;
 };
 
 Plan read_plan(const at::Tensor& buf, const std::vector<int64_t>& d) {
@@ -651,8 +768,9 @@ Plan read_plan(const at::Tensor& buf, const std::vector<int64_t>& d) {
   p.slots = b, b += d[3];
   p.order = b, b += p.rows;
   p.chunk = b, b += 3 * p.chunks;
-  p.group = b;
-  TORCH_CHECK(buf.numel() == 2 * d[0] + d[2] + 1 + d[3] + d[4] + 3 * d[5] + d[1] + 1, "adapter_linear: bad batch plan");
+  p.group = b, b += p.G + 1;
+  p.by_size = b;
+  TORCH_CHECK(buf.numel() == 2 * d[0] + d[2] + 1 + d[3] + d[4] + 3 * d[5] + 2 * d[1] + 1, "adapter_linear: bad batch plan");
   return p;
 }
 
@@ -676,8 +794,8 @@ Rows rows_of(const at::Tensor& t, bool per_head) {
 at::Tensor shrink(const Rows& x, const at::Tensor& a, const Plan& p, int H, int r, cudaStream_t st) {
   const int rp = padded_rank(r);
   const long long ctas = (long long)p.chunks * H;
-  // parts of the reduction: enough CTAs for two a SM, at least 512 values each, 16 at most
-  const int parts = (int)std::max<long long>(1, std::min<long long>({16, (x.C + 511) / 512, (296 + ctas - 1) / ctas}));
+  // parts of the reduction: enough CTAs for four a SM, at least 512 values each, 32 at most
+  const int parts = (int)std::max<long long>(1, std::min<long long>({32, (x.C + 511) / 512, (592 + ctas - 1) / ctas}));
   const int part_k = ((x.C + parts - 1) / parts + 31) / 32 * 32;
   const int used = (x.C + part_k - 1) / part_k;
   at::Tensor t = at::empty({used, H, p.M, rp}, a.options().dtype(at::kFloat));
@@ -791,28 +909,71 @@ at::Tensor project(const Rows& x, const at::Tensor& w, bool w_mn, bool sum_heads
 #undef BD_ADAPTER
   if (p.splits > 1) {
     const long long n = (long long)p.Z * M * N;
-    adapter_sum_kernel<<<(unsigned)std::min<long long>((n + 1023) / 1024, 148 * 8), 256, 0, st>>>(
+    adapter_sum_kernel<<<(unsigned)((n + 127) / 128), 256, 0, st>>>(
         p.partial, p.splits, p.Z, M, N, reinterpret_cast<bf16*>(y.data_ptr()));
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
   return y;
 }
 
-at::Tensor wgrad(const Rows& x, const at::Tensor& t, const Plan& p, const at::Tensor& like, int H, int r,
-                 const c10::optional<at::Tensor>& scale, double scale0, cudaStream_t st) {
-  at::Tensor out = at::empty_like(like);
-  WgradArgs w{x.p, x.row, x.head, t.data_ptr<float>(), t.stride(0), (int)t.size(0), p.order, p.group,
-              scale ? scale->data_ptr<float>() : nullptr, (float)scale0, reinterpret_cast<bf16*>(out.data_ptr()), p.M, H,
-              r, x.C};
-  const dim3 grid((unsigned)((x.C + kWgradCols - 1) / kWgradCols), (unsigned)H, (unsigned)p.G);
-  const int rp = padded_rank(r);
-  if (rp == 16)
-    adapter_wgrad_kernel<1><<<grid, 256, 0, st>>>(w);
-  else if (rp == 32)
-    adapter_wgrad_kernel<2><<<grid, 256, 0, st>>>(w);
-  else
-    adapter_wgrad_kernel<4><<<grid, 256, 0, st>>>(w);
+// t with its parts summed.
+at::Tensor fold(const at::Tensor& t, cudaStream_t st) {
+  if (t.size(0) == 1) return t;
+  at::Tensor out = at::empty({1, t.size(1), t.size(2), t.size(3)}, t.options());
+  const long long n = out.numel();
+  adapter_fold_kernel<<<(unsigned)((n + 1023) / 1024), 256, 0, st>>>(t.data_ptr<float>(), (int)t.size(0), n,
+                                                                     out.data_ptr<float>());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return out;
+}
+
+template <int MT, int SLAB, bool WITH_U>
+void launch_grad(const GradArgs& a, int G, cudaStream_t st, int dev) {
+  constexpr int bytes = GradCfg<MT, SLAB, WITH_U>::SMEM;
+  static_assert(bytes <= 227 * 1024, "shared memory of the gradient kernel");
+  auto kern = adapter_grad_kernel<MT, SLAB, WITH_U>;
+  static bool attr_set[64] = {false};
+  if (!attr_set[dev]) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    attr_set[dev] = true;
+  }
+  kern<<<dim3((unsigned)((a.C + SLAB - 1) / SLAB), (unsigned)a.H, (unsigned)G), 256, bytes, st>>>(a);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+constexpr int kWideSlab = 512, kNarrowSlab = 128;
+
+// The gradient s t_g^T x_g of `like`; with `w` also u = x w^T in parts of 512 columns.
+at::Tensor gradient(const Rows& x, const at::Tensor& t, const Plan& p, const at::Tensor& like, int H, int r,
+                    const c10::optional<at::Tensor>& scale, double scale0, const at::Tensor* w, at::Tensor* u,
+                    cudaStream_t st, int dev) {
+  at::Tensor out = at::empty_like(like);
+  GradArgs a{x.p, x.row, x.head, t.data_ptr<float>(), p.order, p.group, p.by_size,
+             scale ? scale->data_ptr<float>() : nullptr, (float)scale0, reinterpret_cast<bf16*>(out.data_ptr()), nullptr,
+             nullptr, p.M, H, r, x.C};
+  const int rp = padded_rank(r);
+  if (w) {
+    *u = at::empty({(x.C + kWideSlab - 1) / kWideSlab, H, p.M, rp}, t.options());
+    a.w = reinterpret_cast<const bf16*>(w->data_ptr());
+    a.u = u->data_ptr<float>();
+  }
+  // narrow slabs where wide ones leave SMs without one (and nothing else comes out of them)
+  const bool narrow = !w && (long long)p.G * H * ((x.C + kWideSlab - 1) / kWideSlab) < 2 * num_sms_of(dev);
+  auto go = [&](auto mt) {
+    constexpr int MT = decltype(mt)::value;
+    if (w)
+      launch_grad<MT, kWideSlab, true>(a, p.G, st, dev);
+    else if (narrow)
+      launch_grad<MT, kNarrowSlab, false>(a, p.G, st, dev);
+    else
+      launch_grad<MT, kWideSlab, false>(a, p.G, st, dev);
+  };
+  if (rp == 16)
+    go(std::integral_constant<int, 1>());
+  else if (rp == 32)
+    go(std::integral_constant<int, 2>());
+  else
+    go(std::integral_constant<int, 4>());
   return out;
 }
 
@@ -888,10 +1049,19 @@ std::vector<at::Tensor> adapter_backward(const at::Tensor& dy, const at::Tensor&
   const bool shared = x.dim() == 2;
   const Rows rx = rows_of(x, !shared), ry = rows_of(dy, true);
   at::Tensor none = at::empty({0}, w.options()), u, dx = none, da = none, db = none;
-  if (p.rows > 0 && (want_dx || want_da)) u = shrink(ry, b, p, c.H, c.r, st);
+  const bool want_u = want_dx || want_da;
+  if (p.rows == 0) {
+    if (want_da) da = at::zeros_like(a);
+    if (want_db) db = at::zeros_like(b);
+  } else if (want_db) {
+    db = gradient(ry, fold(t, st), p, b, c.H, c.r, scale, scale0, want_u ? &b : nullptr, &u, st, c.dev);
+    if (want_u) u = fold(u, st);
+  } else if (want_u) {
+    u = shrink(ry, b, p, c.H, c.r, st);
+  }
   if (want_dx) dx = project(ry, w, false, shared, a, u, p, c.r, scale, scale0, err, st, c.dev);
-  if (want_da) da = p.rows > 0 ? wgrad(rx, u, p, a, c.H, c.r, scale, scale0, st) : at::zeros_like(a);
-  if (want_db) db = p.rows > 0 ? wgrad(ry, t, p, b, c.H, c.r, scale, scale0, st) : at::zeros_like(b);
+  if (want_da && p.rows > 0)
+    da = gradient(rx, fold(u, st), p, a, c.H, c.r, scale, scale0, nullptr, nullptr, st, c.dev);
   return {dx, da, db};
 }
 

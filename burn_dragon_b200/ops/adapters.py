@@ -66,7 +66,8 @@ class AdapterBatch:
         first = np.arange(runs.sum()) - np.repeat(np.cumsum(runs) - runs, runs)
         start = group[g] + first * self._per_chunk
         chunk = np.stack((start, np.minimum(group[g + 1] - start, self._per_chunk), g), 1)
-        flat = np.concatenate([v.reshape(-1) for v in (of_row, row_slot, tile_ptr, distinct % G, order, chunk, group)])
+        by_size = np.argsort(-count, kind="stable")  # the longest first
+        flat = np.concatenate([v.reshape(-1) for v in (of_row, row_slot, tile_ptr, distinct % G, order, chunk, group, by_size)])
         self.plan = torch.from_numpy(flat.astype(np.int32)).to(self.device)
         self.dims = [M, G, tiles, int(distinct.size), int(order.size), len(chunk), self._per_chunk]
         self._of_row = of_row

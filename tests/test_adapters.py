@@ -217,8 +217,8 @@ def test_plan_covers_every_row_once(seed):
     M, G, tiles, n_slots, n_rows, n_chunks, per = batch.dims
     of = np.repeat(ids, lengths)
     flat = batch.plan.numpy()
-    row_adapter, row_slot, tile_ptr, slots, order, chunk, group = np.split(
-        flat, np.cumsum([M, M, tiles + 1, n_slots, n_rows, 3 * n_chunks]))
+    row_adapter, row_slot, tile_ptr, slots, order, chunk, group, by_size = np.split(
+        flat, np.cumsum([M, M, tiles + 1, n_slots, n_rows, 3 * n_chunks, G + 1]))
     assert (row_adapter == of).all() and group.size == G + 1
     for m in range(M):
         if of[m] < 0:
@@ -235,6 +235,7 @@ def test_plan_covers_every_row_once(seed):
     for g in range(G):
         assert (of[order[group[g]:group[g + 1]]] == g).all()
     assert group[G] == n_rows
+    assert sorted(by_size) == list(range(G)) and (np.diff(np.diff(group)[by_size]) <= 0).all()
 
 
 def test_refusals():
