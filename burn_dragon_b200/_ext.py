@@ -33,7 +33,7 @@ if os.environ.get("BDH_PTXAS_VERBOSE"):
 
 
 # Kernels launched by one call of each binding (for the bench's launch count).
-_LAUNCHES_PER_CALL = {"grad_clip_coef": 2, "adapter_forward": 2, "adapter_backward": 4}
+_LAUNCHES_PER_CALL = {"grad_clip_coef": 2, "adapter_forward": 2, "adapter_direct": 2, "adapter_backward": 4}
 
 
 class _Counted:
@@ -53,6 +53,7 @@ class _Counted:
             self.launches += per
             return fn(*args, **kwargs)
 
+        self.__dict__[name] = call  # the next access does not come here
         return call
 
 

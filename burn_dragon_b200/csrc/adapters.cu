@@ -1017,6 +1017,43 @@ Checked check_all(const at::Tensor& x, const at::Tensor& w, const at::Tensor& a,
 
 }  // namespace
 
+std::vector<at::Tensor> adapter_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor& a, const at::Tensor& b,
+                                        const at::Tensor& plan, const std::vector<int64_t>& dims,
+                                        const c10::optional<at::Tensor>& scale, double scale0, const at::Tensor& err);
+
+namespace {
+bool direct(const at::Tensor& t, int dev, int64_t inner) {
+  if (!t.is_cuda() || t.get_device() != dev || t.scalar_type() != at::kBFloat16 || t.requires_grad()) return false;
+  if (t.stride(-1) != 1 || t.size(-1) != inner || inner % 8 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    if (t.stride(i) % 8 || t.stride(i) <= 0) return false;
+  return true;
+}
+}  // namespace
+
+// The call without gradients and without copies, with or without heads: y, or nothing where an argument needs a
+// look (a copy, a gradient, an error). One crossing from Python for a token's projection.
+c10::optional<at::Tensor> adapter_direct(const at::Tensor& x, const at::Tensor& w, const at::Tensor& a, const at::Tensor& b,
+                                         const at::Tensor& plan, const std::vector<int64_t>& dims,
+                                         const c10::optional<at::Tensor>& scale, double scale0, const at::Tensor& err) {
+  const bool heads = w.dim() == 3;
+  if (!w.is_cuda() || !(heads || w.dim() == 2) || a.dim() != w.dim() + 1 || b.dim() != w.dim() + 1) return c10::nullopt;
+  if (!(x.dim() == 2 || (heads && x.dim() == 3)) || !plan.is_cuda()) return c10::nullopt;
+  const int dev = w.get_device();
+  const int64_t H = heads ? w.size(0) : 1, K = w.size(-2), N = w.size(-1), G = a.size(0), r = a.size(-2);
+  if (!direct(x, dev, K) || !direct(w, dev, N) || !direct(a, dev, K) || !direct(b, dev, N)) return c10::nullopt;
+  if (!a.is_contiguous() || !b.is_contiguous() || r < 1 || r > 64 || G != dims[1] || dims[0] == 0 || x.size(0) != dims[0])
+    return c10::nullopt;
+  if (b.size(0) != G || b.size(-2) != r || (heads && (a.size(1) != H || b.size(1) != H || (x.dim() == 3 && x.size(1) != H))))
+    return c10::nullopt;
+  if (scale && (!scale->is_cuda() || scale->get_device() != dev || scale->scalar_type() != at::kFloat || scale->dim() != 1 ||
+                scale->size(0) != G || !scale->is_contiguous()))
+    return c10::nullopt;
+  if (heads) return adapter_forward(x, w, a, b, plan, dims, scale, scale0, err)[0];
+  return adapter_forward(x, w.unsqueeze(0), a.unsqueeze(1), b.unsqueeze(1), plan, dims, scale, scale0, err)[0].view(
+      {x.size(0), N});
+}
+
 // y [M, H, N], and t [parts, H, M, rp] fp32 (empty without adapters) for the backward pass.
 std::vector<at::Tensor> adapter_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor& a, const at::Tensor& b,
                                         const at::Tensor& plan, const std::vector<int64_t>& dims,

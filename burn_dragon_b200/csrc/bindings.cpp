@@ -117,6 +117,9 @@ void percentile_thresholds(const at::Tensor& values, double q, const at::Tensor&
 std::vector<at::Tensor> adapter_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor& a, const at::Tensor& b,
                                         const at::Tensor& plan, const std::vector<int64_t>& dims,
                                         const c10::optional<at::Tensor>& scale, double scale0, const at::Tensor& err);
+c10::optional<at::Tensor> adapter_direct(const at::Tensor& x, const at::Tensor& w, const at::Tensor& a, const at::Tensor& b,
+                                         const at::Tensor& plan, const std::vector<int64_t>& dims,
+                                         const c10::optional<at::Tensor>& scale, double scale0, const at::Tensor& err);
 std::vector<at::Tensor> adapter_backward(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& w,
                                          const at::Tensor& a, const at::Tensor& b, const at::Tensor& t,
                                          const at::Tensor& plan, const std::vector<int64_t>& dims,
@@ -189,6 +192,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("tp_gather_bytes", &bd::tp_gather_bytes);
   m.def("percentile_thresholds", &bd::percentile_thresholds);
   m.def("adapter_forward", &bd::adapter_forward);
+  m.def("adapter_direct", &bd::adapter_direct);
   m.def("adapter_backward", &bd::adapter_backward);
   m.def("sample_tokens", &bd::sample_tokens);
   m.def("adamw_many", &bd::adamw_many);

@@ -210,7 +210,9 @@ __device__ __forceinline__ void merged(Shared& s, bool weigh, Sums (&b)[2]) {
   const int C = (int)cluster.num_blocks();
   b[0] = b[1] = Sums{0, 0};
   const int at = 2 * threadIdx.x;
-  for (int q = 0; q < C; ++q) {
+#pragma unroll
+  for (int q = 0; q < kMaxCluster; ++q) {  // unrolled: the loads of all CTAs are in flight together
+    if (q >= C) break;
     const Shared* o = cluster.map_shared_rank(&s, q);
     const uint2 c = *reinterpret_cast<const uint2*>(&o->count[at]);
     b[0].count += c.x, b[1].count += c.y;
@@ -247,21 +249,44 @@ __device__ __forceinline__ void push(Shared* first, u64 order) {
   if (at < kList) first->list[at] = order;
 }
 
-// Ascending bitonic sort of the first CTA's list.
+// Ascending bitonic sort of the first CTA's list, two values a thread (t and t + 512): partners within a warp
+// exchange by shuffles, only the six widest distances go through shared memory.
 __device__ void sort_list(Shared& s, int n) {
-  int size = 2;
+  const int t = threadIdx.x;
+  int size = 32;
   while (size < n) size <<= 1;
-  for (int i = n + threadIdx.x; i < size; i += kThreads) s.list[i] = ~0ull;
-  __syncthreads();
+  u64 v[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) v[e] = t + e * kThreads < n ? s.list[t + e * kThreads] : ~0ull;
+  const int live = size > kThreads ? 2 : 1;  // values of a thread that take part
   for (int k = 2; k <= size; k <<= 1)
     for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int t = threadIdx.x; t < size / 2; t += kThreads) {
-        const int i = 2 * t - (t & (j - 1)), l = i + j;
-        const u64 a = s.list[i], b = s.list[l];
-        if ((a > b) == ((i & k) == 0)) s.list[i] = b, s.list[l] = a;
+      if (j == kThreads) {
+        if (v[0] > v[1]) {
+          const u64 o = v[0];
+          v[0] = v[1], v[1] = o;
+        }
+        continue;
       }
-      __syncthreads();
+      u64 o[2];
+      if (j >= 32) {
+        __syncthreads();
+        for (int e = 0; e < live; ++e) s.list[t + e * kThreads] = v[e];
+        __syncthreads();
+        for (int e = 0; e < live; ++e) o[e] = s.list[(t + e * kThreads) ^ j];
+      } else {
+        if (t >= size) continue;  // whole warps
+        for (int e = 0; e < live; ++e) o[e] = __shfl_xor_sync(0xffffffffu, v[e], j);
+      }
+      for (int e = 0; e < live; ++e) {
+        const int i = t + e * kThreads;
+        const bool low = ((i & j) == 0) == ((i & k) == 0);  // this place gets the smaller one
+        if ((v[e] > o[e]) == low) v[e] = o[e];
+      }
     }
+  __syncthreads();
+  for (int e = 0; e < live; ++e) s.list[t + e * kThreads] = v[e];
+  __syncthreads();
 }
 
 // After the gather's barrier: the first CTA sorts the list and finds the last value that is kept: fewer
@@ -387,8 +412,8 @@ __device__ __forceinline__ u64 share_of(u64 total, float p) {
 
 // top-k (and, inside it, top-p). `own`: the largest logit this thread has read.
 template <typename T>
-__device__ __forceinline__ u64 bound_of_k(Shared& s, const float* x, const T* src, int V, int base, int n, const Row& r,
-                                          int k, const float* p, float own) {
+__device__ __forceinline__ u64 bound_of_k(Shared& s, const float* x, const T* src, int base, int n, const Row& r, int k,
+                                          const float* p, float own) {
   cg::cluster_group cluster = cg::this_cluster();
   clear_histogram(s, false);
   if (threadIdx.x == 0) s.list_n = 0, s.digit = -1;
@@ -403,8 +428,8 @@ __device__ __forceinline__ u64 bound_of_k(Shared& s, const float* x, const T* sr
     pick(s, b, at, (u64)k, ~0ull);
   }
   sync_all(cluster);
-  const int last = s.digit < 0 ? kBuckets - 2 : s.digit;
-  bool listed = s.digit >= 0 || V <= kList;
+  const int last = s.digit;
+  bool listed = last >= 0;  // else fewer than k threads have a value
   if (listed) {
     Shared* first = cluster.map_shared_rank(&s, 0);
     const float4* x4 = reinterpret_cast<const float4*>(x);
@@ -653,11 +678,16 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
   const bool use_k = k > 0 && k < a.V, use_p = p < 1.f;
 
   u64 bound = ~0ull;
-  if (use_k)
-    bound = bound_of_k(s, x, src, a.V, base, n, r, k, use_p ? &p : nullptr, own);
+  if (a.V <= kList && (use_k || use_p)) {  // a short row (in one CTA) is the list
+    for (int i = tid; i < n; i += kThreads) s.list[i] = order_of(x[i], i);
+    if (tid == 0) s.list_n = n;
+    __syncthreads();
+    bound = list_bound(s, r, Sums{0, 0}, use_k ? (u64)k : ~0ull, ~0ull, use_p ? &p : nullptr);
+  } else if (use_k)
+    bound = bound_of_k(s, x, src, base, n, r, k, use_p ? &p : nullptr, own);
   else if (use_p)
     bound = bound_of_p(s, x, src, base, n, r, p);
-  const bool weights = !use_k && use_p;  // x holds weights
+  const bool weights = !use_k && use_p && a.V > kList;  // x holds weights
 
   // ---- sums of the kept weights: warp w owns a run of the slice
   const float last = bound == ~0ull ? kMinusInf : order_value((unsigned)(bound >> 32));  // the border's logit

@@ -126,6 +126,12 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, a: torch.Tensor, b: to
     """See the module. ``scale``: a number, or an fp32 tensor of one per adapter (a constant: no
     gradient). On CUDA all operands are bf16, K and N multiples of 8, r <= 64; sums are fp32. Tensors
     that are not laid out in aligned rows are copied first."""
+    if x.is_cuda:
+        tensor = isinstance(scale, torch.Tensor)
+        y = _ext.load().adapter_direct(x, weight, a, b, batch.plan, batch.dims, scale if tensor else None,
+                                       1.0 if tensor else float(scale), error_word(x.device))
+        if y is not None:
+            return y
     heads = weight.dim() == 3
     if not heads:
         if weight.dim() != 2 or a.dim() != 3 or b.dim() != 3 or x.dim() != 2:
