@@ -37,12 +37,15 @@ namespace {
 namespace cg = cooperative_groups;
 using u64 = unsigned long long;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarpsS = kThreads / 32;
-constexpr int kBuckets = 1024;  // two a thread
-constexpr int kList = 1024;     // values that are sorted
+constexpr int kBuckets = 1024;
+constexpr int kList = 1024;  // values that are sorted
+constexpr int kEach = kBuckets / kThreads;  // buckets, and values of the list, of a thread
+static_assert(kBuckets == kList, "one count for both");
 constexpr int kMaxCluster = 8;
 constexpr int kMaxSlice = 32768;  // logits a CTA can hold
+constexpr int kWhole = 8192;      // a slice whose weights all go through one exact histogram
 constexpr float kMinusInf = -INFINITY;
 
 struct SampleArgs {
@@ -58,7 +61,7 @@ struct SampleArgs {
 };
 
 // With a slice of 64,000 bytes (128,000 tokens over 8 CTAs) three CTAs share an SM.
-struct Shared {
+struct __align__(16) Shared {
   union {
     struct {
       unsigned count[kBuckets];
@@ -204,36 +207,44 @@ __device__ __forceinline__ void clear_histogram(Shared& s, bool weigh) {
   __syncthreads();
 }
 
-// In the first CTA (the others go on to the next barrier): this thread's two buckets of the cluster's histogram.
-__device__ __forceinline__ void merged(Shared& s, bool weigh, Sums (&b)[2]) {
+// In the first CTA (the others go on to the next barrier): this thread's buckets of the cluster's
+// histogram, and their sum.
+__device__ __forceinline__ Sums merged(Shared& s, bool weigh, Sums (&b)[kEach]) {
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks();
-  b[0] = b[1] = Sums{0, 0};
-  const int at = 2 * threadIdx.x;
+  const int at = kEach * threadIdx.x;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) b[k] = Sums{0, 0};
 #pragma unroll
   for (int q = 0; q < kMaxCluster; ++q) {  // unrolled: the loads of all CTAs are in flight together
     if (q >= C) break;
     const Shared* o = cluster.map_shared_rank(&s, q);
-    const uint2 c = *reinterpret_cast<const uint2*>(&o->count[at]);
-    b[0].count += c.x, b[1].count += c.y;
+    const uint4 c = *reinterpret_cast<const uint4*>(&o->count[at]);
+    b[0].count += c.x, b[1].count += c.y, b[2].count += c.z, b[3].count += c.w;
     if (weigh) {
-      const uint2 lo = *reinterpret_cast<const uint2*>(&o->lo[at]), hi = *reinterpret_cast<const uint2*>(&o->hi[at]);
+      const uint4 lo = *reinterpret_cast<const uint4*>(&o->lo[at]), hi = *reinterpret_cast<const uint4*>(&o->hi[at]);
       b[0].weight += (u64)hi.x << 32 | lo.x, b[1].weight += (u64)hi.y << 32 | lo.y;
+      b[2].weight += (u64)hi.z << 32 | lo.z, b[3].weight += (u64)hi.w << 32 | lo.w;
     }
   }
+  Sums all{0, 0};
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) all.count += b[k].count, all.weight += b[k].weight;
+  return all;
 }
+static_assert(kEach == 4, "merged reads four buckets a thread");
 
 // In the first CTA: the first bucket after which `most` values or `reach` weight is there, from running
 // sums `at`. Told to every CTA by the one thread that has it; digit stays as it was if there is none.
-__device__ __forceinline__ void pick(Shared& s, const Sums (&b)[2], Sums at, u64 most, u64 reach) {
+__device__ __forceinline__ void pick(Shared& s, const Sums (&b)[kEach], Sums at, u64 most, u64 reach) {
   cg::cluster_group cluster = cg::this_cluster();
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < kEach; ++k) {
     if (b[k].count > 0 && at.count < most && at.weight < reach &&
         (at.count + b[k].count >= most || at.weight + b[k].weight >= reach)) {
       for (int q = 0; q < (int)cluster.num_blocks(); ++q) {
         Shared* o = cluster.map_shared_rank(&s, q);
-        o->digit = 2 * threadIdx.x + k;
+        o->digit = kEach * threadIdx.x + k;
         o->digit_count = (unsigned)min(b[k].count, 0xffffffffull);
         o->before_count = at.count;
         o->before_weight = at.weight;
@@ -249,43 +260,63 @@ __device__ __forceinline__ void push(Shared* first, u64 order) {
   if (at < kList) first->list[at] = order;
 }
 
-// Ascending bitonic sort of the first CTA's list, two values a thread (t and t + 512): partners within a warp
-// exchange by shuffles, only the six widest distances go through shared memory.
+// Ascending order of up to 256 values of the first CTA's list, a value a thread: each counts the ones before it.
+// One broadcast read and four instructions a value, all independent, where a step of a sorting
+// network is a chain of about 300 cycles (256 values: 1.6 against 5.5 us).
+__device__ void rank_list(Shared& s, int n) {
+  const int t = threadIdx.x;
+  const u64 mine = t < n ? s.list[t] : ~0ull;
+  int before = 0;
+  if (t < (n + 31) / 32 * 32) {
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) before += s.list[j] < mine ? 1 : 0;
+  }
+  __syncthreads();
+  if (t < n) s.list[before] = mine;
+  __syncthreads();
+}
+
+// Ascending bitonic sort of the first CTA's list, value t + 256 e in register e of thread t: partners in one
+// thread and in one warp exchange without shared memory.
 __device__ void sort_list(Shared& s, int n) {
   const int t = threadIdx.x;
   int size = 32;
   while (size < n) size <<= 1;
-  u64 v[2];
+  u64 v[kEach];
 #pragma unroll
-  for (int e = 0; e < 2; ++e) v[e] = t + e * kThreads < n ? s.list[t + e * kThreads] : ~0ull;
-  const int live = size > kThreads ? 2 : 1;  // values of a thread that take part
+  for (int e = 0; e < kEach; ++e) v[e] = t + e * kThreads < n ? s.list[t + e * kThreads] : ~0ull;
+  auto keep = [&](int e, u64 o, int j, int k) {
+    const int i = t + e * kThreads;
+    const bool low = ((i & j) == 0) == ((i & k) == 0);  // this place gets the smaller one
+    if ((v[e] > o) == low) v[e] = o;
+  };
   for (int k = 2; k <= size; k <<= 1)
     for (int j = k >> 1; j > 0; j >>= 1) {
-      if (j == kThreads) {
-        if (v[0] > v[1]) {
-          const u64 o = v[0];
-          v[0] = v[1], v[1] = o;
-        }
-        continue;
-      }
-      u64 o[2];
-      if (j >= 32) {
+      u64 o[kEach];
+      if (j >= kThreads) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) o[e] = j == kThreads ? v[e ^ 1] : v[e ^ 2];
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) keep(e, o[e], j, k);
+      } else if (j >= 32) {
         __syncthreads();
-        for (int e = 0; e < live; ++e) s.list[t + e * kThreads] = v[e];
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+          if (e * kThreads < size) s.list[t + e * kThreads] = v[e];
         __syncthreads();
-        for (int e = 0; e < live; ++e) o[e] = s.list[(t + e * kThreads) ^ j];
-      } else {
-        if (t >= size) continue;  // whole warps
-        for (int e = 0; e < live; ++e) o[e] = __shfl_xor_sync(0xffffffffu, v[e], j);
-      }
-      for (int e = 0; e < live; ++e) {
-        const int i = t + e * kThreads;
-        const bool low = ((i & j) == 0) == ((i & k) == 0);  // this place gets the smaller one
-        if ((v[e] > o[e]) == low) v[e] = o[e];
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+          if (e * kThreads < size) keep(e, s.list[(t + e * kThreads) ^ j], j, k);
+      } else if (t < size) {  // whole warps
+#pragma unroll
+        for (int e = 0; e < kEach; ++e)
+          if (e * kThreads < size) keep(e, __shfl_xor_sync(0xffffffffu, v[e], j), j, k);
       }
     }
   __syncthreads();
-  for (int e = 0; e < live; ++e) s.list[t + e * kThreads] = v[e];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e)
+    if (e * kThreads < size) s.list[t + e * kThreads] = v[e];
   __syncthreads();
 }
 
@@ -296,17 +327,21 @@ __device__ u64 list_bound(Shared& s, const Row& r, Sums before, u64 most, u64 re
   cg::cluster_group cluster = cg::this_cluster();
   if (cluster.block_rank() == 0) {
     const int n = (int)min(s.list_n, (unsigned)kList);
-    sort_list(s, n);
-    Sums v[2], all;
-    u64 order[2];
+    if (n <= kThreads)
+      rank_list(s, n);
+    else
+      sort_list(s, n);
+    Sums v[kEach], all, own{0, 0};
+    u64 order[kEach];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int i = 2 * threadIdx.x + k;
+    for (int k = 0; k < kEach; ++k) {
+      const int i = kEach * threadIdx.x + k;
       order[k] = i < n ? s.list[i] : ~0ull;
       v[k] = Sums{i < n ? 1ull : 0ull, 0};
       if (i < n && (share || reach != ~0ull) && before.count + i < most) v[k].weight = r.weight(order_value((unsigned)(order[k] >> 32)));
+      own.count += v[k].count, own.weight += v[k].weight;
     }
-    Sums at = block_exclusive(s, Sums{v[0].count + v[1].count, v[0].weight + v[1].weight}, true, all);
+    Sums at = block_exclusive(s, own, true, all);
     if (share) {
       const double want = ceil(__dmul_rn(__ull2double_rn(all.weight), (double)*share));
       reach = want > 1.0 ? (u64)want : 1ull;
@@ -315,7 +350,7 @@ __device__ u64 list_bound(Shared& s, const Row& r, Sums before, u64 most, u64 re
     at.weight += before.weight;
     const u64 end = min(most, before.count + n);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < kEach; ++k) {
       if (v[k].count && at.count < most && at.weight < reach &&
           (at.count + 1 >= end || at.weight + v[k].weight >= reach)) {
         for (int q = 0; q < (int)cluster.num_blocks(); ++q) cluster.map_shared_rank(&s, q)->bound = order[k];
@@ -369,9 +404,8 @@ __device__ __noinline__ u64 find_bound(Shared& s, const T* src, int base, int n,
     }
     sync_all(cluster);
     if (cluster.block_rank() == 0) {
-      Sums b[2], all;
-      merged(s, true, b);
-      const Sums at = block_exclusive(s, Sums{b[0].count + b[1].count, b[0].weight + b[1].weight}, true, all);
+      Sums b[kEach], all;
+      const Sums at = block_exclusive(s, merged(s, true, b), true, all);
       pick(s, b, Sums{at.count + before.count, at.weight + before.weight}, most, reach);
     }
     sync_all(cluster);
@@ -422,9 +456,8 @@ __device__ __forceinline__ u64 bound_of_k(Shared& s, const float* x, const T* sr
   if (b0 < kBuckets - 1) atomicAdd(&s.count[b0], 1u);
   sync_all(cluster);
   if (cluster.block_rank() == 0) {
-    Sums b[2], all;
-    merged(s, false, b);
-    const Sums at = block_exclusive(s, Sums{b[0].count + b[1].count, 0}, false, all);
+    Sums b[kEach], all;
+    const Sums at = block_exclusive(s, merged(s, false, b), false, all);
     pick(s, b, at, (u64)k, ~0ull);
   }
   sync_all(cluster);
@@ -458,9 +491,12 @@ __device__ __forceinline__ u64 bound_of_k(Shared& s, const float* x, const T* sr
 
 // top-p alone; replaces the logits in x by their weights w
 template <typename T>
-__device__ __forceinline__ u64 bound_of_p(Shared& s, float* x, const T* src, int base, int n, const Row& r, float p) {
+__device__ __forceinline__ u64 bound_of_p(Shared& s, float* x, const T* src, int base, int n, int slice, const Row& r,
+                                          float p) {
   cg::cluster_group cluster = cg::this_cluster();
-  clear_histogram(s, false);
+  const bool whole = slice <= kWhole;
+  clear_histogram(s, whole);
+  if (threadIdx.x == 0) s.list_n = 0, s.digit = -1;
   float4* x4 = reinterpret_cast<float4*>(x);
   const int n4 = (n + 3) / 4;
   WeightSum sum;
@@ -470,66 +506,100 @@ __device__ __forceinline__ u64 bound_of_p(Shared& s, float* x, const T* src, int
     const float4 w = make_float4(r.w(l.x), r.w(l.y), r.w(l.z), r.w(l.w));
     x4[i] = w;
     sum.n += 4;
-    sum.add(w.x), sum.add(w.y), sum.add(w.z), sum.add(w.w);
+    const float v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      sum.add(v[q]);
+      if (whole && v[q] >= kOne40) {
+        atomicAdd(&s.count[weight_bucket(v[q])], 1u);
+        add_weight(s, weight_bucket(v[q]), fixed40(v[q]));
+      }
+    }
   }
   const u64 total = cluster_total(s, 1, sum.total());
   const u64 reach = share_of(total, p);
   if (reach >= total) return ~0ull;
-  // the window from a sample: every weight above total / 4096, and each thread's first four for the rest
-  const float heavy = __fmul_rn(__ull2float_rn(total), kOne40 / 4096.f);
-  const unsigned share = 16u * (unsigned)n4 / (unsigned)max(1, min(n4, kThreads));
-  for (int i = threadIdx.x; i < n4; i += kThreads) {
-    const float4 w = x4[i];
-    if (i >= kThreads && fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)) < heavy) continue;
-    const float v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (v[q] >= kOne40 && (i < kThreads || v[q] >= heavy))
-        atomicAdd(&s.count[weight_bucket(v[q])], v[q] >= heavy ? 16u : share);
-  }
-  sync_all(cluster);
-  if (cluster.block_rank() == 0) {
-    // A bucket's weight is near its count times its middle. The window: four deviations of the sampled part (a
-    // sampled weight w stands for share / 16 like it: share / 16 w^2 each), half a bucket's width for
-    // the heavy ones, and 0.2 %.
-    Sums b[2], all;
-    merged(s, false, b);
-    float spread = 0.f, big = 0.f;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const unsigned below = ((unsigned)(2 * threadIdx.x + k) << 19) + (1u << 18);
-      const float mid = below < 0x3f800000u ? __uint_as_float(0x3f800000u - below) : 0.f;
-      b[k].weight = b[k].count * (fixed40(mid) >> 4);
-      const float sum = mid * (float)b[k].count * 0.0625f;
-      spread += mid < heavy ? sum * mid * (float)share * 0.0625f : 0.f;
-      big += mid < heavy ? 0.f : sum;
+  Shared* first = cluster.map_shared_rank(&s, 0);
+  int w0 = 0, wide = 1;  // the window: its first bucket, and their number
+  if (whole) {
+    if (cluster.block_rank() == 0) {
+      Sums b[kEach], all;
+      const Sums at = block_exclusive(s, merged(s, true, b), true, all);
+      pick(s, b, at, ~0ull, reach);
     }
-    const Sums at0 = block_exclusive(s, Sums{b[0].count + b[1].count, b[0].weight + b[1].weight}, true, all);
-    const u64 both = (u64)(unsigned)__float2uint_rn(big * 1024.f) << 32;  // big <= 2^18, spread <= 2^18
-    Sums more;
-    block_exclusive(s, Sums{0, both | (u64)__float2uint_rn(fminf(spread, 262144.f) * 16.f)}, true, more);
-    spread = (float)(unsigned)more.weight * 0.0625f + 0.0625f;
-    big = (float)(unsigned)(more.weight >> 32) * (1.f / 1024.f);
-    const float sum = __ull2float_rn(all.weight) * kOne40;
-    const float near = __ull2float_rn(reach) * kOne40 * (sum / (__ull2float_rn(total) * kOne40));
-    const float margin = (share > 16u ? 4.f * sqrtf(spread) : 0.f) + big * 0.03125f + sum * 0.002f;
-    const float lo = near - margin, hi = near + margin;
-    Sums at = at0;
+    sync_all(cluster);
+    w0 = s.digit;
+    if (s.digit_count <= kList) {
+      const Sums before{0, s.before_weight};
+      for (int i = threadIdx.x; i < n4; i += kThreads) {
+        const float4 w = x4[i];
+        const float v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float w0 = __ull2float_rn(at.weight) * kOne40, w1 = __ull2float_rn(at.weight + b[k].weight) * kOne40;
-      const bool last = b[k].count > 0 && at.weight + b[k].weight == all.weight;
-      const bool opens = b[k].count > 0 && (at.weight == 0 || w0 < lo) && (w1 >= lo || last);
-      const bool ends = b[k].count > 0 && w0 < hi && (w1 >= hi || last);
-      for (int q = 0; q < (int)cluster.num_blocks(); ++q) {
-        if (opens) cluster.map_shared_rank(&s, q)->window[0] = 2 * threadIdx.x + k;
-        if (ends) cluster.map_shared_rank(&s, q)->window[1] = 2 * threadIdx.x + k;
+        for (int q = 0; q < 4; ++q)
+          if (weight_bucket(v[q]) == w0 && v[q] >= kOne40) push(first, order_of(logit(src[4 * i + q]), base + 4 * i + q));
       }
-      at.weight += b[k].weight;
+      sync_all(cluster);
+      return list_bound(s, r, before, ~0ull, reach, nullptr);
     }
+  } else {
+    // the window from a sample: every weight above total / 4096, and each thread's first eight for the rest
+    const float heavy = __fmul_rn(__ull2float_rn(total), kOne40 / 4096.f);
+    const unsigned share = 16u * (unsigned)n4 / (unsigned)max(1, min(n4, 2 * kThreads));
+    for (int i = threadIdx.x; i < n4; i += kThreads) {
+      const float4 w = x4[i];
+      if (i >= 2 * kThreads && fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)) < heavy) continue;
+      const float v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (v[q] >= kOne40 && (i < 2 * kThreads || v[q] >= heavy))
+          atomicAdd(&s.count[weight_bucket(v[q])], v[q] >= heavy ? 16u : share);
+    }
+    sync_all(cluster);
+    if (cluster.block_rank() == 0) {
+      // A bucket's weight is near its count times its middle. The window: four deviations of the sampled part (a
+      // sampled weight w stands for share / 16 like it: share / 16 w^2 each), half a bucket's width for
+      // the heavy ones, and 0.2 %.
+      Sums b[kEach], all, own{0, 0};
+      merged(s, false, b);
+      float spread = 0.f, big = 0.f;
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) {
+        const unsigned below = ((unsigned)(kEach * threadIdx.x + k) << 19) + (1u << 18);
+        const float mid = below < 0x3f800000u ? __uint_as_float(0x3f800000u - below) : 0.f;
+        b[k].weight = b[k].count * (fixed40(mid) >> 4);
+        own.weight += b[k].weight;
+        const float sum = mid * (float)b[k].count * 0.0625f;
+        spread += mid < heavy ? sum * mid * (float)share * 0.0625f : 0.f;
+        big += mid < heavy ? 0.f : sum;
+      }
+      const Sums at0 = block_exclusive(s, own, true, all);
+      const u64 both = (u64)(unsigned)__float2uint_rn(big * 1024.f) << 32;  // big <= 2^18, spread <= 2^18
+      Sums more;
+      block_exclusive(s, Sums{0, both | (u64)__float2uint_rn(fminf(spread, 262144.f) * 16.f)}, true, more);
+      spread = (float)(unsigned)more.weight * 0.0625f + 0.0625f;
+      big = (float)(unsigned)(more.weight >> 32) * (1.f / 1024.f);
+      const float sum = __ull2float_rn(all.weight) * kOne40;
+      const float near = __ull2float_rn(reach) * kOne40 * (sum / (__ull2float_rn(total) * kOne40));
+      const float margin = (share > 16u ? 4.f * sqrtf(spread) : 0.f) + big * 0.03125f + sum * 0.002f;
+      const float lo = near - margin, hi = near + margin;
+      Sums at = at0;
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) {
+        const float w0 = __ull2float_rn(at.weight) * kOne40, w1 = __ull2float_rn(at.weight + b[k].weight) * kOne40;
+        const bool last = b[k].count > 0 && at.weight + b[k].weight == all.weight;
+        const bool opens = b[k].count > 0 && (at.weight == 0 || w0 < lo) && (w1 >= lo || last);
+        const bool ends = b[k].count > 0 && w0 < hi && (w1 >= hi || last);
+        for (int q = 0; q < (int)cluster.num_blocks(); ++q) {
+          if (opens) cluster.map_shared_rank(&s, q)->window[0] = kEach * threadIdx.x + k;
+          if (ends) cluster.map_shared_rank(&s, q)->window[1] = kEach * threadIdx.x + k;
+        }
+        at.weight += b[k].weight;
+      }
+    }
+    sync_all(cluster);
+    w0 = s.window[0], wide = max(1, s.window[1] - w0 + 1);
   }
-  sync_all(cluster);
-  const int w0 = s.window[0], wide = max(1, s.window[1] - w0 + 1);
+  __syncthreads();
   const unsigned head = 0x3f800000u - ((unsigned)w0 << 19);  // bits of the largest weight in the window
   const unsigned span = (unsigned)wide << 19;
   const int shift = 9 + (wide > 1 ? 32 - __clz(wide - 1) : 0);  // 1024 parts at most
@@ -553,9 +623,8 @@ __device__ __forceinline__ u64 bound_of_p(Shared& s, float* x, const T* src, int
   }
   const u64 above = cluster_total(s, 2, sum.total());
   if (cluster.block_rank() == 0) {
-    Sums b[2], all;
-    merged(s, true, b);
-    const Sums at = block_exclusive(s, Sums{b[0].count + b[1].count, b[0].weight + b[1].weight}, true, all);
+    Sums b[kEach], all;
+    const Sums at = block_exclusive(s, merged(s, true, b), true, all);
     pick(s, b, Sums{at.count, at.weight + above}, ~0ull, reach);
   }
   sync_all(cluster);
@@ -565,7 +634,6 @@ __device__ __forceinline__ u64 bound_of_p(Shared& s, float* x, const T* src, int
   }
   const unsigned part = (unsigned)s.digit;
   const Sums before{0, s.before_weight};
-  Shared* first = cluster.map_shared_rank(&s, 0);
 #pragma unroll 2
   for (int i = threadIdx.x; i < n4; i += kThreads) {
     const float4 w = x4[i];
@@ -611,12 +679,12 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
     }
   };
   int v = tid;
-  for (; v + 3 * kThreads < nv; v += 4 * kThreads) {
-    uint4 raw[4];
+  for (; v + 7 * kThreads < nv; v += 8 * kThreads) {
+    uint4 raw[8];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) raw[q] = __ldcs(src4 + v + q * kThreads);
+    for (int q = 0; q < 8; ++q) raw[q] = __ldcs(src4 + v + q * kThreads);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) take(raw[q], v + q * kThreads);
+    for (int q = 0; q < 8; ++q) take(raw[q], v + q * kThreads);
   }
 #pragma unroll 3
   for (; v < nv; v += kThreads) take(__ldcs(src4 + v), v);
@@ -686,7 +754,7 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
   } else if (use_k)
     bound = bound_of_k(s, x, src, base, n, r, k, use_p ? &p : nullptr, own);
   else if (use_p)
-    bound = bound_of_p(s, x, src, base, n, r, p);
+    bound = bound_of_p(s, x, src, base, n, a.slice, r, p);
   const bool weights = !use_k && use_p && a.V > kList;  // x holds weights
 
   // ---- sums of the kept weights: warp w owns a run of the slice
