@@ -51,7 +51,7 @@ constexpr float kMinusInf = -INFINITY;
 struct SampleArgs {
   const void* logits;
   long long row_stride;
-  int V, slice;
+  int rows, V, slice;
   const float *u, *temperature, *top_p, *min_p;
   const int* top_k;
   float temperature0, top_p0, min_p0;
@@ -69,6 +69,7 @@ struct __align__(16) Shared {
     };
     u64 list[kList];  // order bits : index, ascending = the order of the row
   };
+  float4 warp_estimate[kWarpsS];
   u64 warp_sum[kWarpsS];
   unsigned warp_count[kWarpsS];
   u64 slot[3][kMaxCluster];  // one value per CTA of the cluster; the next exchange uses another row
@@ -348,7 +349,11 @@ __device__ u64 list_bound(Shared& s, const Row& r, Sums before, u64 most, u64 re
     }
     at.count += before.count;
     at.weight += before.weight;
-    const u64 end = min(most, before.count + n);
+    // without a reach the last value is the bound; with one it has to be reached
+    const u64 end = reach == ~0ull ? min(most, before.count + n) : most;
+    if (threadIdx.x == 0)
+      for (int q = 0; q < (int)cluster.num_blocks(); ++q) cluster.map_shared_rank(&s, q)->bound = 0;
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
       if (v[k].count && at.count < most && at.weight < reach &&
@@ -545,6 +550,7 @@ __device__ __forceinline__ u64 bound_of_p(Shared& s, float* x, const T* src, int
     // the window from a sample: every weight above total / 4096, and each thread's first eight for the rest
     const float heavy = __fmul_rn(__ull2float_rn(total), kOne40 / 4096.f);
     const unsigned share = 16u * (unsigned)n4 / (unsigned)max(1, min(n4, 2 * kThreads));
+    if (threadIdx.x == 0) s.window[0] = 0, s.window[1] = weight_bucket(kOne40);
     for (int i = threadIdx.x; i < n4; i += kThreads) {
       const float4 w = x4[i];
       if (i >= 2 * kThreads && fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)) < heavy) continue;
@@ -558,42 +564,54 @@ __device__ __forceinline__ u64 bound_of_p(Shared& s, float* x, const T* src, int
     if (cluster.block_rank() == 0) {
       // A bucket's weight is near its count times its middle. The window: four deviations of the sampled part (a
       // sampled weight w stands for share / 16 like it: share / 16 w^2 each), half a bucket's width for
-      // the heavy ones, and 0.2 %.
-      Sums b[kEach], all, own{0, 0};
+      // the heavy ones, and 0.2 %. fp32: a window that misses the border is found out.
+      Sums b[kEach];
       merged(s, false, b);
-      float spread = 0.f, big = 0.f;
+      float w[kEach], sum = 0.f, spread = 0.f, big = 0.f;
 #pragma unroll
       for (int k = 0; k < kEach; ++k) {
         const unsigned below = ((unsigned)(kEach * threadIdx.x + k) << 19) + (1u << 18);
         const float mid = below < 0x3f800000u ? __uint_as_float(0x3f800000u - below) : 0.f;
-        b[k].weight = b[k].count * (fixed40(mid) >> 4);
-        own.weight += b[k].weight;
-        const float sum = mid * (float)b[k].count * 0.0625f;
-        spread += mid < heavy ? sum * mid * (float)share * 0.0625f : 0.f;
-        big += mid < heavy ? 0.f : sum;
+        w[k] = mid * (float)(unsigned)b[k].count * 0.0625f;
+        sum += w[k];
+        spread += mid < heavy ? w[k] * mid * (float)share * 0.0625f : 0.f;
+        big += mid < heavy ? 0.f : w[k];
       }
-      const Sums at0 = block_exclusive(s, own, true, all);
-      const u64 both = (u64)(unsigned)__float2uint_rn(big * 1024.f) << 32;  // big <= 2^18, spread <= 2^18
-      Sums more;
-      block_exclusive(s, Sums{0, both | (u64)__float2uint_rn(fminf(spread, 262144.f) * 16.f)}, true, more);
-      spread = (float)(unsigned)more.weight * 0.0625f + 0.0625f;
-      big = (float)(unsigned)(more.weight >> 32) * (1.f / 1024.f);
-      const float sum = __ull2float_rn(all.weight) * kOne40;
-      const float near = __ull2float_rn(reach) * kOne40 * (sum / (__ull2float_rn(total) * kOne40));
-      const float margin = (share > 16u ? 4.f * sqrtf(spread) : 0.f) + big * 0.03125f + sum * 0.002f;
-      const float lo = near - margin, hi = near + margin;
-      Sums at = at0;
+      const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+      float run = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const float t = __shfl_up_sync(0xffffffffu, run, o);
+        run += lane >= o ? t : 0.f;
+        spread += __shfl_xor_sync(0xffffffffu, spread, o);
+        big += __shfl_xor_sync(0xffffffffu, big, o);
+      }
+      if (lane == 31) s.warp_estimate[warp] = make_float4(run, spread, big, 0.f);
+      __syncthreads();
+      float at = run - sum, all = 0.f;
+      spread = 0.0625f, big = 0.f;
+#pragma unroll
+      for (int q = 0; q < kWarpsS; ++q) {
+        const float4 e = s.warp_estimate[q];
+        at += q < warp ? e.x : 0.f;
+        all += e.x, spread += e.y, big += e.z;
+      }
+      const float near = __ull2float_rn(reach) / __ull2float_rn(total) * all;
+      const float margin = (share > 16u ? 4.f * sqrtf(spread) : 0.f) + big * 0.03125f + all * 0.002f;
+      const float lo = fmaxf(near - margin, 0.f), hi = fminf(near + margin, all * 0.99999f);
+      // the first bucket that reaches lo, and the first that reaches hi
+      int opens = -1, ends = -1;
 #pragma unroll
       for (int k = 0; k < kEach; ++k) {
-        const float w0 = __ull2float_rn(at.weight) * kOne40, w1 = __ull2float_rn(at.weight + b[k].weight) * kOne40;
-        const bool last = b[k].count > 0 && at.weight + b[k].weight == all.weight;
-        const bool opens = b[k].count > 0 && (at.weight == 0 || w0 < lo) && (w1 >= lo || last);
-        const bool ends = b[k].count > 0 && w0 < hi && (w1 >= hi || last);
-        for (int q = 0; q < (int)cluster.num_blocks(); ++q) {
-          if (opens) cluster.map_shared_rank(&s, q)->window[0] = kEach * threadIdx.x + k;
-          if (ends) cluster.map_shared_rank(&s, q)->window[1] = kEach * threadIdx.x + k;
+        if (b[k].count > 0) {
+          if (at <= lo && at + w[k] > lo) opens = kEach * threadIdx.x + k;
+          if (at < hi && at + w[k] >= hi) ends = kEach * threadIdx.x + k;
         }
-        at.weight += b[k].weight;
+        at += w[k];
+      }
+      for (int q = 0; q < (int)cluster.num_blocks(); ++q) {
+        if (opens >= 0) cluster.map_shared_rank(&s, q)->window[0] = opens;
+        if (ends >= 0) cluster.map_shared_rank(&s, q)->window[1] = ends;
       }
     }
     sync_all(cluster);
@@ -603,7 +621,7 @@ __device__ __forceinline__ u64 bound_of_p(Shared& s, float* x, const T* src, int
   const unsigned head = 0x3f800000u - ((unsigned)w0 << 19);  // bits of the largest weight in the window
   const unsigned span = (unsigned)wide << 19;
   const int shift = 9 + (wide > 1 ? 32 - __clz(wide - 1) : 0);  // 1024 parts at most
-  clear_histogram(s, true);
+  clear_histogram(s, false);
   if (threadIdx.x == 0) s.list_n = 0, s.digit = -1;
   sum = WeightSum();
 #pragma unroll 2
@@ -615,36 +633,50 @@ __device__ __forceinline__ u64 bound_of_p(Shared& s, float* x, const T* src, int
     for (int q = 0; q < 4; ++q) {
       const unsigned under = head - __float_as_uint(v[q]);  // wraps for what is above
       sum.add((int)under < 0 ? v[q] : 0.f);
-      if (under < span && v[q] >= kOne40) {
-        atomicAdd(&s.count[under >> shift], 1u);
-        add_weight(s, (int)(under >> shift), fixed40(v[q]));
-      }
+      if (under < span && v[q] >= kOne40) atomicAdd(&s.count[under >> shift], 1u);
     }
   }
   const u64 above = cluster_total(s, 2, sum.total());
-  if (cluster.block_rank() == 0) {
-    Sums b[kEach], all;
-    const Sums at = block_exclusive(s, merged(s, true, b), true, all);
-    pick(s, b, Sums{at.count, at.weight + above}, ~0ull, reach);
-  }
-  sync_all(cluster);
-  if (above >= reach || s.digit < 0 || s.digit_count > kList) {
+  if (above >= reach) {
     u64 kept;
     return find_bound(s, src, base, n, r, ~0ull, ~0ull, reach, kept);
   }
-  const unsigned part = (unsigned)s.digit;
-  const Sums before{0, s.before_weight};
+  // A part is 2^-9 of its weight wide at most: counts times middles miss the border by one part at most.
+  if (cluster.block_rank() == 0) {
+    Sums b[kEach], all, own{0, 0};
+    merged(s, false, b);
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const unsigned below = ((unsigned)(kEach * threadIdx.x + k) << shift) + (1u << shift) / 2;
+      b[k].weight = below < head ? b[k].count * fixed40(__uint_as_float(head - below)) : 0ull;
+      own.count += b[k].count, own.weight += b[k].weight;
+    }
+    Sums at = block_exclusive(s, own, true, all);
+    pick(s, b, Sums{at.count, at.weight + above}, ~0ull, min(reach, above + all.weight));
+  }
+  sync_all(cluster);
+  const int part = max(s.digit, 1) - 1;  // the first of three parts that are sorted
+  sum = WeightSum();
 #pragma unroll 2
   for (int i = threadIdx.x; i < n4; i += kThreads) {
     const float4 w = x4[i];
     const float v[4] = {w.x, w.y, w.z, w.w};
+    sum.n += 4;
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if ((head - __float_as_uint(v[q])) >> shift == part && v[q] >= kOne40)
-        push(first, order_of(logit(src[4 * i + q]), base + 4 * i + q));
+    for (int q = 0; q < 4; ++q) {
+      const int at = (int)(head - __float_as_uint(v[q])) >> shift;  // its part; negative for what is above
+      sum.add(at < part ? v[q] : 0.f);
+      if (at >= part && at < part + 3 && v[q] >= kOne40) push(first, order_of(logit(src[4 * i + q]), base + 4 * i + q));
+    }
   }
-  sync_all(cluster);
-  return list_bound(s, r, before, ~0ull, reach, nullptr);
+  const u64 before = cluster_total(s, 1, sum.total());
+  const bool listed = s.digit >= 0 && before < reach && first->list_n <= kList;
+  if (listed) {
+    const u64 bound = list_bound(s, r, Sums{0, before}, ~0ull, reach, nullptr);
+    if (bound) return bound;  // 0: the border is not in the list
+  }
+  u64 kept;
+  return find_bound(s, src, base, n, r, ~0ull, ~0ull, reach, kept);
 }
 
 template <typename T>
@@ -652,11 +684,11 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
   extern __shared__ __align__(16) float x[];
   __shared__ Shared s;
   cg::cluster_group cluster = cg::this_cluster();
-  cluster.barrier_arrive();  // waited for before the first access to another CTA's memory
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int row = blockIdx.x / C;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int base = min(rank * a.slice, a.V), n = min(a.slice, a.V - base);
+  cluster.barrier_arrive();  // waited for before the first access to another CTA's memory
+  const int row = blockIdx.x / C;
   const T* src = static_cast<const T*>(a.logits) + (long long)row * a.row_stride + base;
   const float temperature = a.temperature ? a.temperature[row] : a.temperature0;
   const int k = a.top_k ? a.top_k[row] : a.top_k0;
@@ -781,6 +813,24 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
 #pragma unroll
       for (int q = 0; q < 4; ++q) run.add(w[q] >= least ? w[q] : 0.f);
     }
+  } else if (weights) {
+#pragma unroll 2
+    for (int i = w0 + 4 * lane; i < w1; i += 128) {
+      const float4 l = x4[i / 4];
+      const float v[4] = {l.x, l.y, l.z, l.w};
+      run.n += 4;
+      bool equal = false;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        run.add(v[q] > border && v[q] >= least ? v[q] : 0.f);
+        equal |= v[q] == border;
+      }
+      if (equal && border > 0.f) {
+        run.n += 4;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) run.add(v[q] == border ? kept(i + q, v[q]) : 0.f);
+      }
+    }
   } else {
 #pragma unroll 2
     for (int i = w0 + 4 * lane; i < w1; i += 128) {
@@ -799,8 +849,8 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
   const u64 sum = s.warp_sum[warp];
   u64 at = before;
   for (int q = 0; q < warp; ++q) at += s.warp_sum[q];
+  // ---- the warp whose run crosses the target: steps of 256 values, 8 a lane
   if (target < at || target >= at + sum) return;
-  // ---- this warp's run crosses the target: steps of 256 values, 8 a lane
   for (int j0 = w0; j0 < w1; j0 += 256) {
     u64 part[8], mine = 0;
 #pragma unroll
@@ -832,7 +882,7 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
 }
 
 template <typename T>
-void launch(const SampleArgs& a, int rows, int C, cudaStream_t st, int dev) {
+void launch(const SampleArgs& a, int C, cudaStream_t st, int dev) {
   auto kern = sample_kernel<T>;
   const size_t bytes = (size_t)a.slice * sizeof(float);
   static bool attr_set[64] = {false};
@@ -841,7 +891,6 @@ void launch(const SampleArgs& a, int rows, int C, cudaStream_t st, int dev) {
     attr_set[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(rows * C));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = st;
@@ -851,6 +900,7 @@ void launch(const SampleArgs& a, int rows, int C, cudaStream_t st, int dev) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  cfg.gridDim = dim3((unsigned)(a.rows * C));
   C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a));
 }
 
@@ -884,7 +934,7 @@ void sample_tokens(const at::Tensor& logits, const at::Tensor& u, const c10::opt
   SampleArgs a;
   a.logits = logits.data_ptr();
   a.row_stride = logits.stride(0);
-  a.V = (int)V;
+  a.rows = (int)B, a.V = (int)V;
   a.u = setting<float>(u, B, at::kFloat, dev, "u (fp32)");
   a.temperature = setting<float>(temperature, B, at::kFloat, dev, "temperature (fp32)");
   a.top_k = setting<int>(top_k, B, at::kInt, dev, "top_k (int32)");
@@ -902,9 +952,9 @@ void sample_tokens(const at::Tensor& logits, const at::Tensor& u, const c10::opt
   a.slice = (int)(((V + C - 1) / C + 7) / 8 * 8);
   auto st = at::cuda::getCurrentCUDAStream(dev).stream();
   if (bf16)
-    launch<__nv_bfloat16>(a, (int)B, C, st, dev);
+    launch<__nv_bfloat16>(a, C, st, dev);
   else
-    launch<float>(a, (int)B, C, st, dev);
+    launch<float>(a, C, st, dev);
 }
 
 }  // namespace bd
