@@ -16,9 +16,12 @@
 //   top-k   a histogram of the threads' largest logits, in 1024 linear buckets of (m - l) / T (1/32
 //           wide), names a bucket that k of them reach: all values up to it, few more than k, are sorted;
 //   top-p   the weights replace the logits in shared memory; a sample of them (an eighth, and all
-//           heavy ones), in 16 buckets an octave, names a window around the border that holds
-//           5 % of the weight; the sum above it and a histogram of the window's weights are exact and
-//           name one of up to 1024 parts of it, which is sorted.
+//           heavy ones), in 16 buckets an octave, names a window around the border; the sum above it is exact, and
+//           counts in up to 1024 parts of it name three parts, which are sorted, after the exact sum above
+//           them (or, where they hold more than kList, are the next window). Slices of up to kWhole
+//           values take one exact histogram instead.
+// Few values go through the histograms: an addition to shared memory costs a warp more than all
+// arithmetic of a pass.
 // Where more than kList values are left (many equal ones), or the border is not in the window,
 // find_bound refines exact histograms over the row's bits, read again from memory.
 //
@@ -547,8 +550,8 @@ __device__ __forceinline__ u64 bound_of_p(Shared& s, float* x, const T* src, int
       return list_bound(s, r, before, ~0ull, reach, nullptr);
     }
   } else {
-    // the window from a sample: every weight above total / 4096, and each thread's first eight for the rest
-    const float heavy = __fmul_rn(__ull2float_rn(total), kOne40 / 4096.f);
+    // the window from a sample: every weight above total / 16384, and each thread's first eight for the rest
+    const float heavy = __fmul_rn(__ull2float_rn(total), kOne40 / 16384.f);
     const unsigned share = 16u * (unsigned)n4 / (unsigned)max(1, min(n4, 2 * kThreads));
     if (threadIdx.x == 0) s.window[0] = 0, s.window[1] = weight_bucket(kOne40);
     for (int i = threadIdx.x; i < n4; i += kThreads) {
@@ -562,7 +565,7 @@ __device__ __forceinline__ u64 bound_of_p(Shared& s, float* x, const T* src, int
     }
     sync_all(cluster);
     if (cluster.block_rank() == 0) {
-      // A bucket's weight is near its count times its middle. The window: four deviations of the sampled part (a
+      // A bucket's weight is near its count times its middle. The window: 3.5 deviations of the sampled part (a
       // sampled weight w stands for share / 16 like it: share / 16 w^2 each), half a bucket's width for
       // the heavy ones, and 0.2 %. fp32: a window that misses the border is found out.
       Sums b[kEach];
@@ -597,7 +600,7 @@ __device__ __forceinline__ u64 bound_of_p(Shared& s, float* x, const T* src, int
         all += e.x, spread += e.y, big += e.z;
       }
       const float near = __ull2float_rn(reach) / __ull2float_rn(total) * all;
-      const float margin = (share > 16u ? 4.f * sqrtf(spread) : 0.f) + big * 0.03125f + all * 0.002f;
+      const float margin = (share > 16u ? 3.5f * sqrtf(spread) : 0.f) + big * 0.03125f + all * 0.002f;
       const float lo = fmaxf(near - margin, 0.f), hi = fminf(near + margin, all * 0.99999f);
       // the first bucket that reaches lo, and the first that reaches hi
       int opens = -1, ends = -1;
@@ -618,62 +621,68 @@ __device__ __forceinline__ u64 bound_of_p(Shared& s, float* x, const T* src, int
     w0 = s.window[0], wide = max(1, s.window[1] - w0 + 1);
   }
   __syncthreads();
-  const unsigned head = 0x3f800000u - ((unsigned)w0 << 19);  // bits of the largest weight in the window
-  const unsigned span = (unsigned)wide << 19;
-  const int shift = 9 + (wide > 1 ? 32 - __clz(wide - 1) : 0);  // 1024 parts at most
-  clear_histogram(s, false);
-  if (threadIdx.x == 0) s.list_n = 0, s.digit = -1;
-  sum = WeightSum();
+  unsigned head = 0x3f800000u - ((unsigned)w0 << 19);  // bits of the largest weight in the window
+  unsigned span = (unsigned)wide << 19;
+  int shift = 9 + (wide > 1 ? 32 - __clz(wide - 1) : 0);  // of a part's width: 1024 parts at most
+  for (;;) {
+    clear_histogram(s, false);
+    if (threadIdx.x == 0) s.list_n = 0, s.digit = -1;
+    sum = WeightSum();
 #pragma unroll 2
-  for (int i = threadIdx.x; i < n4; i += kThreads) {
-    const float4 w = x4[i];
-    const float v[4] = {w.x, w.y, w.z, w.w};
-    sum.n += 4;
+    for (int i = threadIdx.x; i < n4; i += kThreads) {
+      const float4 w = x4[i];
+      const float v[4] = {w.x, w.y, w.z, w.w};
+      sum.n += 4;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const unsigned under = head - __float_as_uint(v[q]);  // wraps for what is above
-      sum.add((int)under < 0 ? v[q] : 0.f);
-      if (under < span && v[q] >= kOne40) atomicAdd(&s.count[under >> shift], 1u);
+      for (int q = 0; q < 4; ++q) {
+        const unsigned under = head - __float_as_uint(v[q]);  // wraps for what is above
+        sum.add((int)under < 0 ? v[q] : 0.f);
+        if (under < span && v[q] >= kOne40) atomicAdd(&s.count[under >> shift], 1u);
+      }
     }
-  }
-  const u64 above = cluster_total(s, 2, sum.total());
-  if (above >= reach) {
-    u64 kept;
-    return find_bound(s, src, base, n, r, ~0ull, ~0ull, reach, kept);
-  }
-  // A part is 2^-9 of its weight wide at most: counts times middles miss the border by one part at most.
-  if (cluster.block_rank() == 0) {
-    Sums b[kEach], all, own{0, 0};
-    merged(s, false, b);
+    const u64 above = cluster_total(s, 2, sum.total());
+    if (above >= reach) break;
+    // counts times the parts' middles miss the border by one part at most
+    if (cluster.block_rank() == 0) {
+      Sums b[kEach], all, own{0, 0};
+      merged(s, false, b);
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-      const unsigned below = ((unsigned)(kEach * threadIdx.x + k) << shift) + (1u << shift) / 2;
-      b[k].weight = below < head ? b[k].count * fixed40(__uint_as_float(head - below)) : 0ull;
-      own.count += b[k].count, own.weight += b[k].weight;
+      for (int k = 0; k < kEach; ++k) {
+        const unsigned below = ((unsigned)(kEach * threadIdx.x + k) << shift) + (1u << shift) / 2;
+        b[k].weight = below < head ? b[k].count * fixed40(__uint_as_float(head - below)) : 0ull;
+        own.count += b[k].count, own.weight += b[k].weight;
+      }
+      const Sums at = block_exclusive(s, own, true, all);
+      pick(s, b, Sums{at.count, at.weight + above}, ~0ull, min(reach, above + all.weight));
     }
-    Sums at = block_exclusive(s, own, true, all);
-    pick(s, b, Sums{at.count, at.weight + above}, ~0ull, min(reach, above + all.weight));
-  }
-  sync_all(cluster);
-  const int part = max(s.digit, 1) - 1;  // the first of three parts that are sorted
-  sum = WeightSum();
+    sync_all(cluster);
+    const int part = max(s.digit, 1) - 1;  // the first of three parts that are sorted
+    sum = WeightSum();
 #pragma unroll 2
-  for (int i = threadIdx.x; i < n4; i += kThreads) {
-    const float4 w = x4[i];
-    const float v[4] = {w.x, w.y, w.z, w.w};
-    sum.n += 4;
+    for (int i = threadIdx.x; i < n4; i += kThreads) {
+      const float4 w = x4[i];
+      const float v[4] = {w.x, w.y, w.z, w.w};
+      sum.n += 4;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int at = (int)(head - __float_as_uint(v[q])) >> shift;  // its part; negative for what is above
-      sum.add(at < part ? v[q] : 0.f);
-      if (at >= part && at < part + 3 && v[q] >= kOne40) push(first, order_of(logit(src[4 * i + q]), base + 4 * i + q));
+      for (int q = 0; q < 4; ++q) {
+        const int at = (int)(head - __float_as_uint(v[q])) >> shift;  // its part; negative for what is above
+        sum.add(at < part ? v[q] : 0.f);
+        if (at >= part && at < part + 3 && v[q] >= kOne40) push(first, order_of(logit(src[4 * i + q]), base + 4 * i + q));
+      }
     }
-  }
-  const u64 before = cluster_total(s, 1, sum.total());
-  const bool listed = s.digit >= 0 && before < reach && first->list_n <= kList;
-  if (listed) {
-    const u64 bound = list_bound(s, r, Sums{0, before}, ~0ull, reach, nullptr);
-    if (bound) return bound;  // 0: the border is not in the list
+    const u64 before = cluster_total(s, 1, sum.total());
+    if (s.digit < 0 || before >= reach) break;
+    const unsigned listed = first->list_n;
+    if (listed <= kList) {
+      const u64 bound = list_bound(s, r, Sums{0, before}, ~0ull, reach, nullptr);
+      if (bound) return bound;
+      break;  // the border is not in the list
+    }
+    if (shift == 0) break;  // equal weights
+    head -= (unsigned)part << shift;  // too many: the three parts are the next window
+    span = 3u << shift;
+    shift = max(shift - 8, 0);
+    sync_all(cluster);  // list_n is read
   }
   u64 kept;
   return find_bound(s, src, base, n, r, ~0ull, ~0ull, reach, kept);
