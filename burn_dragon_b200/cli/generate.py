@@ -6,7 +6,7 @@ context_strategy, output_format: ``decoded_text`` prints text, ``token_ids`` pri
 is decoded text); burn_dragon_language/src/config/core.rs:18-60.
 
   python -m burn_dragon_b200.cli.generate --run runs/language/cuda/NAME --prompt "hello" [--max-tokens 64]
-         [--temperature 0.8 --top-k 40] [--batch 1] [--output-format token_ids]
+         [--temperature 0.8 --top-k 40 --top-p 0.95 --min-p 0.05] [--batch 1] [--output-format token_ids]
 """
 
 from __future__ import annotations
@@ -32,6 +32,8 @@ def main(argv=None) -> None:
     ap.add_argument("--max-chars", type=int, default=None)
     ap.add_argument("--temperature", type=float, default=None)
     ap.add_argument("--top-k", type=int, default=None)
+    ap.add_argument("--top-p", type=float, default=None)
+    ap.add_argument("--min-p", type=float, default=None)
     ap.add_argument("--output-format", choices=("auto", "decoded_text", "token_ids"), default=None)
     ap.add_argument("--batch", type=int, default=1)
     ap.add_argument("--seed", type=int, default=0)
@@ -79,7 +81,8 @@ def main(argv=None) -> None:
     if window is not None and len(prompt) > window:
         prompt = prompt[-window:]  # the recurrent state carries the rest; nothing to trim later
     x = torch.tensor([prompt] * a.batch, dtype=torch.long, device=dev)
-    out = Generator(model).generate(x, max_tokens, temperature=temperature, top_k=top_k, seed=a.seed)
+    out = Generator(model).generate(x, max_tokens, temperature=temperature, top_k=top_k, seed=a.seed,
+                                    top_p=a.top_p, min_p=a.min_p)
     for row in out.tolist():
         if fmt == "token_ids":
             print(json.dumps(row))

@@ -1,0 +1,179 @@
+"""A bank of low-rank adapters on one frozen BDH model: trained together, served together.
+
+Where a random scaffold (``models.scaffold``) trains one adapter per model, an ``AdapterBank`` keeps G of
+them for the three shared projections, W = W_frozen + s A_g^T B_g with s = alpha / r or alpha / sqrt(r), and
+a batch may name another adapter for every sequence. ``AdapterBDH`` is the BDH forward with the three
+projections through ``ops.adapters.adapter_linear`` (bf16 operands on CUDA, the plain form on CPU);
+norms, RoPE and the linear attention are ``models.reference``'s. ``train_step`` updates the adapters of
+the batch with ``AdamWMany``; ``generate`` serves requests of different lengths, adapters and sampling
+settings in one batch (``ops.sampling.sample_tokens``).
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from ..ops.adapters import AdapterBatch, adapter_linear
+from ..ops.sampling import sample_tokens
+from ..train.optim import AdamWMany
+from . import reference as R
+from .state import ModelState
+
+PROJECTIONS = ("encoder", "encoder_v", "decoder")
+
+
+def bank_shapes(cfg, rank: int) -> dict[str, tuple[int, ...]]:
+    """One adapter's matrices; rows contiguous over the projection's inputs (a) and outputs (b)."""
+    D, H, Nh = cfg.n_embd, cfg.n_head, cfg.latent_per_head
+    return {"encoder.a": (H, rank, D), "encoder.b": (H, rank, Nh), "encoder_v.a": (H, rank, D),
+            "encoder_v.b": (H, rank, Nh), "decoder.a": (rank, H * Nh), "decoder.b": (rank, D)}
+
+
+class AdapterBank:
+    """fp32 masters of G adapters and, on CUDA, the bf16 copies that the projections read."""
+
+    def __init__(self, cfg, n_adapters: int, rank: int = 16, alpha: float = 16.0, scaling: str = "rank_stabilized",
+                 device="cpu", seed: int = 0):
+        if scaling not in ("standard", "rank_stabilized"):
+            raise ValueError(f"unknown adapter scaling {scaling!r}")
+        self.cfg, self.n_adapters, self.rank = cfg, n_adapters, rank
+        self.scale = alpha / rank if scaling == "standard" else alpha / math.sqrt(rank)
+        gen = torch.Generator().manual_seed(seed)
+        self.master, self.work = {}, {}
+        for name, shape in bank_shapes(cfg, rank).items():
+            t = torch.zeros(n_adapters, *shape)
+            if name.endswith(".a"):  # b starts at zero: a fresh adapter changes nothing
+                t.uniform_(-1.0 / math.sqrt(shape[-1]), 1.0 / math.sqrt(shape[-1]), generator=gen)
+            self.master[name] = t.to(device)
+            cuda = self.master[name].is_cuda
+            self.work[name] = self.master[name].bfloat16() if cuda else self.master[name]
+
+    def load_scaffold(self, g: int, tensors: dict[str, torch.Tensor]) -> None:
+        """Adapter ``g`` from a random-scaffold model's ``<projection>.a`` [.., in, r] / ``.b`` [.., r, out]."""
+        for name, t in self.master.items():
+            src = tensors[name]
+            t[g].copy_(src.transpose(-1, -2) if name.endswith(".a") else src)
+            if self.work[name] is not t:
+                self.work[name][g].copy_(t[g])
+
+    def tensors(self, which: dict[str, torch.Tensor]) -> list[torch.Tensor]:
+        """Every adapter's own matrices, adapter by adapter."""
+        return [which[name][g] for g in range(self.n_adapters) for name in self.master]
+
+
+class AdapterBDH:
+    """BDH with an adapter per sequence; the model's own weights stay as they are."""
+
+    def __init__(self, model, bank: AdapterBank):
+        cfg = model.cfg
+        if getattr(cfg, "mhc_streams", 1) > 1 or getattr(cfg, "latent_fanout_schedule", None):
+            raise ValueError("adapters run on the plain BDH layer: no mHC streams, no latent fan-out")
+        if getattr(cfg, "sequence_memory_system", "linear_attention") != "linear_attention":
+            raise ValueError("adapters run on the linear-attention memory")
+        self.cfg, self.bank = cfg, bank
+        with torch.no_grad():
+            p = {k: None if v is None else v.detach() for k, v in model.param_dict().items()}
+        dev = p["embed"].device
+        self.p, self.dtype = p, torch.bfloat16 if dev.type == "cuda" else torch.float32
+        self.weights = {n: p[n].to(self.dtype).contiguous() for n in PROJECTIONS}
+        self.norm = R.make_norm(cfg.norm_kind, p["norm_gamma"], p["norm_beta"], cfg.norm_eps, p.get("norm_alpha"),
+                                p.get("norm_shift"))
+        make = {"rope": R.rope_freqs, "pope": R.pope_freqs}.get(cfg.rotary_embedding)
+        self.freqs = None if make is None else make(cfg.latent_per_head, cfg.rope_theta, device=dev)
+        self.decay = R.decay_vector(cfg.decay_slopes(), device=dev) if cfg.uses_decay() else None
+
+    def batch(self, adapters, length: int) -> AdapterBatch:
+        """The plan of ``len(adapters)`` sequences of ``length`` tokens."""
+        return AdapterBatch(adapters, [length] * len(adapters), self.bank.n_adapters, device=self.p["embed"].device)
+
+    def _linear(self, name: str, x: torch.Tensor, batch: AdapterBatch, work) -> torch.Tensor:
+        return adapter_linear(x.to(self.dtype), self.weights[name], work[name + ".a"], work[name + ".b"], batch,
+                              self.bank.scale).float()
+
+    def forward(self, tokens: torch.Tensor, batch: AdapterBatch, state: ModelState | None = None, work=None):
+        """Logits [B, T, V] of tokens [B, T], row b T + t of the batch being token t of sequence b."""
+        cfg, work = self.cfg, work or self.bank.work
+        B, T = tokens.shape
+        D, H, Nh = cfg.n_embd, cfg.n_head, cfg.latent_per_head
+        pos = state.position if state is not None else 0
+        thr, thr_y = cfg.thresholds()
+        phases = None
+        if self.freqs is not None:
+            phases = R.rope_phases(torch.arange(pos, pos + T, device=tokens.device), self.freqs)[None, None]
+        v = self.norm(self.p["embed"][tokens])
+        rhos = []
+        for layer in range(cfg.n_layer):
+            x = torch.relu(self._linear("encoder", v.reshape(B * T, D), batch, work) - thr)  # [B T, H, Nh]
+            q = x.view(B, T, H, Nh).transpose(1, 2)
+            if phases is not None:
+                q = R.pope_apply(q, phases) if cfg.rotary_embedding == "pope" else R.rope_apply(q, phases)
+            rho0 = state.rhos[layer] if state is not None and state.rhos is not None else None
+            a, rho = R.linear_attention_chunked(q, v[:, None], rho0=rho0, decay=self.decay, need_state=state is not None)
+            a = self.norm(a).transpose(1, 2).reshape(B * T, H, D)
+            y = torch.relu(self._linear("encoder_v", a, batch, work) - thr_y)
+            m = self._linear("decoder", (x * y).reshape(B * T, H * Nh), batch, work)
+            v = self.norm(v + self.norm(m).view(B, T, D))
+            rhos.append(rho)
+        if state is not None:
+            state.rhos = rhos
+            state.position += T
+        head = self.p["embed"].t() if self.p["lm_head"] is None else self.p["lm_head"]
+        return v @ head
+
+    # ---------------------------------------------------------------- training
+    def optimizer(self, lr: float = 1e-3, state_bits: int = 32, weight_decay: float = 0.0, seed: int = 0) -> AdamWMany:
+        """AdamW over every adapter's matrices; on CUDA it writes the bf16 copies too."""
+        bank = self.bank
+        cuda = bank.master["encoder.a"].is_cuda
+        return AdamWMany(bank.tensors(bank.master), lr=lr, weight_decay=weight_decay, state_bits=state_bits, seed=seed,
+                         shadows=bank.tensors(bank.work) if cuda else None)
+
+    def train_step(self, opt: AdamWMany, tokens: torch.Tensor, targets: torch.Tensor, adapters,
+                   batch: AdapterBatch | None = None, lr: float | None = None) -> torch.Tensor:
+        """One step on sequences [B, T] with the given adapters; those of no sequence are left alone.
+        ``batch``: the plan of an earlier step with the same adapters. Returns the mean loss."""
+        bank = self.bank
+        batch = batch or self.batch(adapters, tokens.shape[1])
+        names = list(bank.master)
+        work = {n: t.detach().requires_grad_(True) for n, t in bank.work.items()}
+        loss = R.cross_entropy(self.forward(tokens, batch, work=work), targets)
+        grads = dict(zip(names, torch.autograd.grad(loss, [work[n] for n in names])))
+        used = {int(g) for g in adapters}
+        opt.step([grads[n][g] if g in used else None for g in range(bank.n_adapters) for n in names], lr=lr)
+        return loss.detach()
+
+    # ---------------------------------------------------------------- serving
+    @torch.no_grad()
+    def generate(self, prompts: list[list[int]], adapters, max_new_tokens: int, temperature=1.0, top_k=0, top_p=1.0,
+                 min_p=0.0, seed: int = 0) -> tuple[list[list[int]], list[list[float]]]:
+        """Continuations of prompts of different lengths, each with its adapter (-1: none) and settings (numbers,
+        or one value per request), and the tokens' log-probabilities. Every row advances at the same
+        position; one still inside its prompt takes its next prompt token."""
+        if len(prompts) != len(adapters) or not prompts or any(not p for p in prompts):
+            raise ValueError("one adapter per prompt, and no empty prompts")
+        dev = self.p["embed"].device
+        lens = torch.tensor([len(p) for p in prompts], device=dev)
+        width, shared = int(lens.max()), int(lens.min())
+        table = torch.tensor([p + [0] * (width - len(p)) for p in prompts], device=dev)
+        setting = lambda v, dt: torch.as_tensor(v, dtype=dt, device=dev).expand(len(prompts)).contiguous()  # noqa: E731
+        settings = [setting(temperature, torch.float32), setting(top_k, torch.int32), setting(top_p, torch.float32),
+                    setting(min_p, torch.float32)]
+        gen = torch.Generator(device=dev).manual_seed(seed)
+        state = ModelState.empty()
+        logits = self.forward(table[:, :shared], self.batch(adapters, shared), state)[:, -1]
+        step = self.batch(adapters, 1)  # one plan for all single-token steps
+        tokens, logprobs = [], []
+        for pos in range(shared, width + max_new_tokens):
+            drawn, lp = sample_tokens(logits.contiguous(), torch.rand(len(prompts), generator=gen, device=dev), *settings)
+            nxt = torch.where(lens > pos, table[:, min(pos, width - 1)], drawn)
+            tokens.append(nxt)
+            logprobs.append(lp)
+            if pos + 1 < width + max_new_tokens:
+                logits = self.forward(nxt[:, None], step, state)[:, -1]
+        host_t = torch.stack(tokens, 1).tolist()
+        host_l = torch.stack(logprobs, 1).tolist()
+        start = [len(p) - shared for p in prompts]
+        return ([t[s:s + max_new_tokens] for t, s in zip(host_t, start)],
+                [t[s:s + max_new_tokens] for t, s in zip(host_l, start)])

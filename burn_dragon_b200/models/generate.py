@@ -23,15 +23,21 @@ import torch
 from .. import _ext
 from ..ops import gemm as G
 from ..ops.gemm import Operand
+from ..ops.sampling import sample_tokens
 from .reference import rope_freqs
 from .state import ModelState
 
 
 def sample_next(logits: torch.Tensor, temperature: float = 0.0, top_k: int | None = None,
-                generator: torch.Generator | None = None) -> torch.Tensor:
-    """Greedy for temperature 0, else softmax(logits / T) restricted to the top-k."""
+                generator: torch.Generator | None = None, top_p: float | None = None,
+                min_p: float | None = None) -> torch.Tensor:
+    """Greedy for temperature 0, else softmax(logits / T) restricted to the top-k. With ``top_p`` or
+    ``min_p`` the draw is ``ops.sampling.sample_tokens`` on uniform numbers from ``generator``."""
     if temperature <= 0.0:
         return logits.argmax(dim=-1)
+    if top_p is not None or min_p is not None:
+        u = torch.rand(logits.shape[0], generator=generator, device=logits.device)
+        return sample_tokens(logits, u, temperature, top_k or 0, 1.0 if top_p is None else top_p, min_p or 0.0)[0]
     z = logits.float() / temperature
     if top_k is not None and top_k < z.shape[-1]:
         kth = torch.topk(z, top_k, dim=-1).values[..., -1:]
@@ -250,7 +256,7 @@ class Generator:
     def generate_stream(self, prompt: list[int], max_new_tokens: int, chunk_tokens: int = 16,
                         temperature: float = 0.0, top_k: int | None = None, stop_token: int | None = None,
                         sliding_window: int | None = None, on_chunk=None, seed: int | None = None,
-                        device=None) -> list[int]:
+                        device=None, top_p: float | None = None, min_p: float | None = None) -> list[int]:
         """One sequence, tokens handed to ``on_chunk`` every ``chunk_tokens`` steps
         (generation.rs:1174-1275). ``sliding_window`` keeps only the last ``window``
         prompt tokens (the recurrent state needs no trimming afterwards)."""
@@ -266,7 +272,7 @@ class Generator:
         pending = []
         done = 0
         while done < max_new_tokens:
-            nxt = sample_next(logits, temperature, top_k, gen)
+            nxt = sample_next(logits, temperature, top_k, gen, top_p, min_p)
             pending.append(nxt)
             done += 1
             if done < max_new_tokens:
@@ -288,7 +294,8 @@ class Generator:
     # ---------------------------------------------------------------- loop
     @torch.no_grad()
     def generate(self, prompt: torch.Tensor, max_new_tokens: int, temperature: float = 0.0,
-                 top_k: int | None = None, device_buffer_tokens: int = 64, seed: int | None = None):
+                 top_k: int | None = None, device_buffer_tokens: int = 64, seed: int | None = None,
+                 top_p: float | None = None, min_p: float | None = None):
         """Returns [B, max_new_tokens] generated tokens (host tensor)."""
         gen = None
         if seed is not None:
@@ -297,7 +304,7 @@ class Generator:
         logits, state = self.prefill(prompt)
         buf = torch.empty(prompt.shape[0], max_new_tokens, dtype=torch.long, device=prompt.device)
         out = []
-        nxt = sample_next(logits, temperature, top_k, gen)
+        nxt = sample_next(logits, temperature, top_k, gen, top_p, min_p)
         for i in range(max_new_tokens):
             buf[:, i] = nxt
             if (i + 1) % device_buffer_tokens == 0 or i + 1 == max_new_tokens:
@@ -305,5 +312,5 @@ class Generator:
                 out.append(buf[:, start:i + 1].cpu())
             if i + 1 < max_new_tokens:
                 logits = self.decode_step(nxt, state)
-                nxt = sample_next(logits, temperature, top_k, gen)
+                nxt = sample_next(logits, temperature, top_k, gen, top_p, min_p)
         return torch.cat(out, dim=1)
