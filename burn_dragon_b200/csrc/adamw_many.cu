@@ -215,7 +215,7 @@ __device__ __forceinline__ void update_block(const ManyTensor& t, const ManyHype
 }
 
 template <int CAP, bool EIGHT>
-__global__ void __launch_bounds__(32 * kWarps) adamw_many_kernel(const __grid_constant__ ManyTable<CAP> table,
+__global__ void __launch_bounds__(32 * kWarps, EIGHT ? 5 : 4) adamw_many_kernel(const __grid_constant__ ManyTable<CAP> table,
                                                                  const __grid_constant__ ManyHyper h,
                                                                  const int* __restrict__ owner, int first,
                                                                  long long block0, long long block1, void* M, void* V,

@@ -607,7 +607,7 @@ constexpr int kGradRows = 32;
 template <int MT, int SLAB, bool WITH_U>
 struct GradCfg {
   static constexpr int RP = 16 * MT, XP = SLAB + 8, TP = RP + 4;
-  static constexpr int STAGES = MT == 4 && SLAB > 128 ? 2 : 3;
+  static constexpr int STAGES = SLAB > 128 ? 2 : 3;  // wide: two CTAs an SM (MT = 1) hide more than a third stage
   static constexpr int X_BYTES = kGradRows * XP * 2, T_BYTES = kGradRows * TP * 4;
   static constexpr int W_BYTES = WITH_U ? RP * XP * 2 : 0, RED_BYTES = WITH_U ? 4 * kGradRows * TP * 4 : 0;
   static constexpr int SMEM = STAGES * (X_BYTES + T_BYTES) + W_BYTES + RED_BYTES;
