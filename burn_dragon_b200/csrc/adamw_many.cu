@@ -47,7 +47,7 @@ struct ManyTable {
 };
 
 struct ManyHyper {
-  float lr, decay, b1, nb1, b2, nb2, eps, inv_bc1, inv_bc2;
+  float step, decay, b1, nb1, b2, nb2, eps, inv_bc2;  // step = lr / (1 - b1^t)
   unsigned key;
   const float* gscale;
 };
@@ -110,22 +110,28 @@ __device__ __forceinline__ void store8(void* base, bool bf16, long long at, int 
   }
 }
 
-__device__ __forceinline__ float e4m3_value(unsigned char c) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+// Four e4m3 codes, two a conversion.
+__device__ __forceinline__ void e4m3_values(unsigned u, float* v) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(u >> (16 * k)), __NV_E4M3);
+    const float2 f = __half22float2(__half2(h));
+    v[2 * k] = f.x, v[2 * k + 1] = f.y;
+  }
 }
 
 template <bool WIDE>
-__device__ __forceinline__ void load_codes(const unsigned char* s, int lane, unsigned char (&c)[8]) {
-  if constexpr (WIDE) {
+__device__ __forceinline__ void load_codes(const unsigned char* s, int lane, float (&v)[8]) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const unsigned u = *reinterpret_cast<const unsigned*>(s + h * 128 + lane * 4);
+  for (int h = 0; h < 2; ++h) {
+    unsigned u = 0;
+    if constexpr (WIDE) {
+      u = *reinterpret_cast<const unsigned*>(s + h * 128 + lane * 4);
+    } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) c[4 * h + k] = (unsigned char)(u >> (8 * k));
+      for (int k = 0; k < 4; ++k) u |= (unsigned)s[elem<false>(lane, 4 * h + k)] << (8 * k);
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) c[j] = s[elem<false>(lane, j)];
+    e4m3_values(u, v + 4 * h);
   }
 }
 
@@ -134,12 +140,19 @@ __device__ __forceinline__ void store_codes(unsigned char* s, int lane, const un
   if constexpr (WIDE) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      *reinterpret_cast<unsigned*>(s + h * 128 + lane * 4) =
-          c[4 * h] | c[4 * h + 1] << 8 | c[4 * h + 2] << 16 | c[4 * h + 3] << 24;
+      *reinterpret_cast<unsigned*>(s + h * 128 + lane * 4) = __byte_perm(
+          __byte_perm(c[4 * h], c[4 * h + 1], 0x0040), __byte_perm(c[4 * h + 2], c[4 * h + 3], 0x0040), 0x5410);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) s[elem<false>(lane, j)] = (unsigned char)c[j];
   }
+}
+
+// p's own update needs no correctly rounded root and quotient (2^-22 of a step of lr); the states do not use them.
+__device__ __forceinline__ float root(float x) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 // absmax over the warp's block as bits: NaN and infinity win, as they have to
@@ -173,12 +186,11 @@ __device__ __forceinline__ void update_block(const ManyTensor& t, const ManyHype
   load8<WIDE>(t.g, t.flags & kGradBf16, at, lane, n, g);
   load8<WIDE>(t.p, t.flags & kParamBf16, at, lane, n, p);
   if constexpr (EIGHT) {
-    unsigned char cm[8], cv[8];
-    load_codes<WIDE>(static_cast<unsigned char*>(M) + st, lane, cm);
-    load_codes<WIDE>(static_cast<unsigned char*>(V) + st, lane, cv);
+    load_codes<WIDE>(static_cast<unsigned char*>(M) + st, lane, m);
+    load_codes<WIDE>(static_cast<unsigned char*>(V) + st, lane, v);
     const float sm = MS[block], sv = VS[block];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m[j] = __fmul_rn(e4m3_value(cm[j]), sm), v[j] = __fmul_rn(e4m3_value(cv[j]), sv);
+    for (int j = 0; j < 8; ++j) m[j] = __fmul_rn(m[j], sm), v[j] = __fmul_rn(v[j], sv);
   } else {
     load8<WIDE>(M, false, st, lane, kBlock, m);
     load8<WIDE>(V, false, st, lane, kBlock, v);
@@ -189,21 +201,26 @@ __device__ __forceinline__ void update_block(const ManyTensor& t, const ManyHype
     const float gi = __fmul_rn(g[j], gs);
     m[j] = __fadd_rn(__fmul_rn(m[j], h.b1), __fmul_rn(gi, h.nb1));
     v[j] = __fadd_rn(__fmul_rn(v[j], h.b2), __fmul_rn(__fmul_rn(gi, gi), h.nb2));
-    p[j] = p[j] * h.decay - h.lr * ((m[j] * h.inv_bc1) / (sqrtf(v[j] * h.inv_bc2) + h.eps));
+    p[j] = p[j] * h.decay - __fdividef(m[j] * h.step, root(v[j] * h.inv_bc2) + h.eps);
   }
   store8<WIDE>(t.p, t.flags & kParamBf16, at, lane, n, p);
   if (t.shadow) store8<WIDE>(t.shadow, true, at, lane, n, p);
   if constexpr (EIGHT) {
     const float2 fm = block_scale(block_amax(m)), fv = block_scale(block_amax(v));
     unsigned cm[8], cv[8];
+    const unsigned first = (unsigned)st * 0x9E3779B1u + h.key;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      unsigned x = (unsigned)(st + elem<WIDE>(lane, j)) * 0x9E3779B1u + h.key;
+      unsigned x = first + (unsigned)elem<WIDE>(lane, j) * 0x9E3779B1u;
       x = (x ^ (x >> 16)) * 0x85EBCA6Bu;
       x = (x ^ (x >> 13)) * 0xC2B2AE35u;
       x ^= x >> 16;
-      cm[j] = fm.y == 0.f ? 0u : e4m3_stochastic(m[j], fm.y, x & 0xffffu) | (m[j] < 0.f ? 0x80u : 0u);
-      cv[j] = fv.y == 0.f ? 0u : max(e4m3_stochastic(v[j], fv.y, x >> 16), v[j] > 0.f ? 1u : 0u);
+      cm[j] = e4m3_stochastic(m[j], fm.y, x & 0xffffu) | (m[j] < 0.f ? 0x80u : 0u);
+      cv[j] = max(e4m3_stochastic(v[j], fv.y, x >> 16), v[j] > 0.f ? 1u : 0u);
+    }
+    if (fm.y == 0.f || fv.y == 0.f) {  // a block of zeros, or one that is not finite (of the whole warp)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) cm[j] = fm.y == 0.f ? 0u : cm[j], cv[j] = fv.y == 0.f ? 0u : cv[j];
     }
     store_codes<WIDE>(static_cast<unsigned char*>(M) + st, lane, cm);
     store_codes<WIDE>(static_cast<unsigned char*>(V) + st, lane, cv);
@@ -283,9 +300,9 @@ void adamw_many(const std::vector<at::Tensor>& params, const std::vector<c10::op
   if (eight) TORCH_CHECK(v_scale && m_scale->numel() == total && v_scale->numel() == total, "adamw_many: scale sizes");
   if (gscale) TORCH_CHECK(gscale->scalar_type() == at::kFloat && gscale->get_device() == dev, "adamw_many: gradient scale");
   ManyHyper h;
-  h.lr = (float)lr, h.decay = (float)(1.0 - lr * wd);
+  h.step = (float)(lr / bc1), h.decay = (float)(1.0 - lr * wd);
   h.b1 = (float)b1, h.nb1 = (float)(1.0 - b1), h.b2 = (float)b2, h.nb2 = (float)(1.0 - b2);
-  h.eps = (float)eps, h.inv_bc1 = (float)(1.0 / bc1), h.inv_bc2 = (float)(1.0 / bc2);
+  h.eps = (float)eps, h.inv_bc2 = (float)(1.0 / bc2);
   h.key = (unsigned)key;
   h.gscale = gscale ? gscale->data_ptr<float>() : nullptr;
   std::vector<ManyTensor> all(n);

@@ -180,17 +180,22 @@ struct AdapterTile {
   int m0, n0, z, slot0, nslots, ext, kb0, kb1, split;
 };
 
-__device__ __forceinline__ AdapterTile adapter_tile(const AdapterGemm& p, int t, int BN) {
+// Coordinates of tile t; its slots are read from memory by adapter_tile, which every role calls one tile ahead.
+__device__ __forceinline__ AdapterTile adapter_place(const AdapterGemm& p, int t, int BN) {
   AdapterTile c;
   c.n0 = (t % p.tiles_n) * BN;
   t /= p.tiles_n;
-  const int mb = t % p.tiles_m;
-  c.m0 = mb * 128;
+  c.m0 = (t % p.tiles_m) * 128;
   t /= p.tiles_m;
   c.split = t % p.splits;
   c.z = t / p.splits;
-  c.slot0 = p.t ? p.tile_ptr[mb] : 0;
-  c.nslots = p.t ? p.tile_ptr[mb + 1] - c.slot0 : 0;
+  return c;
+}
+
+__device__ __forceinline__ AdapterTile adapter_tile(const AdapterGemm& p, int t, int BN) {
+  AdapterTile c = adapter_place(p, t, BN);
+  c.slot0 = p.t ? p.tile_ptr[c.m0 / 128] : 0;
+  c.nslots = (p.t ? p.tile_ptr[c.m0 / 128 + 1] : 0) - c.slot0;
   c.ext = (c.nslots + p.per_block - 1) / p.per_block;
   const long long total = (long long)p.HR * (p.KB + c.ext);
   c.kb0 = (int)(total * c.split / p.splits);
@@ -270,8 +275,17 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
       uint32_t phase = 0;
       long long issued = 0;
       bool ok = true;
+      AdapterTile next = adapter_tile(p, blockIdx.x, BN);
+      int ids[4];  // adapters of the next adapter block, read while other blocks are on their way
+      auto read_ids = [&](const AdapterTile& c, int e) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          ids[j] = e * p.per_block + j < c.nslots && j < p.per_block ? p.slots[c.slot0 + e * p.per_block + j] : 0;
+      };
       for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-        const AdapterTile c = adapter_tile(p, t, BN);
+        const AdapterTile c = next;
+        if (t + (int)gridDim.x < total) next = adapter_tile(p, t + gridDim.x, BN);
+        if (c.ext > 0) read_ids(c, max(c.kb0 - p.HR * p.KB, 0) % c.ext);
         for (int kb = c.kb0; kb < c.kb1; ++kb) {
           if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutProducer)) {
             ok = false;
@@ -298,12 +312,15 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
             const int n = min(p.per_block, c.nslots - j0);
             mbar_arrive(&granted_bar[stage]);
             mbar_arrive_expect_tx(&full_bar[stage], n * p.rp * 2 * BN);
-            for (int j = 0; j < n; ++j) {
-              const int gh = p.slots[c.slot0 + j0 + j] * p.H + h;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (j >= n) break;
+              const int gh = ids[j] * p.H + h;
 #pragma unroll
               for (int i = 0; i < BN / 64; ++i)
                 tma_load_4d(b_dst + i * 8192 + j * p.rp * 128, &p.tb, &full_bar[stage], c.n0 + 64 * i, 0, gh, 0);
             }
+            read_ids(c, (e + 1) % c.ext);
           }
           ++issued;
           if (++stage == STAGES) {
@@ -335,8 +352,10 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0, built_phase = 0;  // built_phase: one bit per stage
       bool ok = true;
+      AdapterTile next = adapter_tile(p, blockIdx.x, BN);
       for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-        const AdapterTile c = adapter_tile(p, t, BN);
+        const AdapterTile c = next;
+        if (t + (int)gridDim.x < total) next = adapter_tile(p, t + gridDim.x, BN);
         if (!mbar_wait_bounded(&tempty_bar[acc], acc_phase ^ 1, &abort_flag, p.err, kErrTimeoutMma)) {
           ok = false;
           break;
@@ -397,7 +416,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int t = blockIdx.x; t < total; t += gridDim.x) {
-      const AdapterTile c = adapter_tile(p, t, BN);
+      const AdapterTile c = adapter_place(p, t, BN);
       if (!mbar_wait_bounded(&tfull_bar[acc], acc_phase, &abort_flag, p.err, kErrTimeoutEpilogue)) break;
       tc_fence_after();
       const int row0 = c.m0 + quad * 32;
