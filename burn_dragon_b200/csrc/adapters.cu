@@ -156,7 +156,8 @@ __global__ void __launch_bounds__(kShrinkThreads) adapter_shrink_kernel(const __
 // ------------------------------------------------------------------------------- projection
 
 struct AdapterGemm {
-  CUtensorMap tx, tw, tb, ty;
+  CUtensorMap tx, tw, tb;
+  bf16* y;  // [M, Z, N]
   int M, N, KB;      // rows, output columns, 64-wide blocks of one head's reduction
   int HR, Z;         // heads summed in the reduction, heads of the output
   int x_heads;       // x has a head coordinate
@@ -206,14 +207,17 @@ __device__ __forceinline__ AdapterTile adapter_tile(const AdapterGemm& p, int t,
 constexpr int kEpiWarps = 8, kBuildWarps = 4;
 constexpr int kAdapterThreads = 32 * (2 + kEpiWarps + kBuildWarps);
 
-template <int BN>
+// EXT: buffers of the built operand (16 KB each), apart from the ring of x and w, so that the builders work ahead of
+// the products. A 256-wide tile has room for three stages and two buffers, which short reductions want
+// (an adapter block every few blocks), or four and one, which long ones want.
+template <int BN, int EXT>
 struct AdapterCfg {
   static constexpr int A_BYTES = 128 * 64 * 2;
   static constexpr int B_BYTES = BN * 64 * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;  // 192 KB of operands
-  static constexpr int EPI_BYTES = kEpiWarps * 4096;                // a 32 x 64 bf16 tile per epilogue warp
-  static constexpr int SMEM = STAGES * STAGE_BYTES + EPI_BYTES + 1024;
+  static constexpr int STAGES = BN == 256 ? (EXT == 1 ? 4 : 3) : BN == 128 ? 5 : 6;
+  static constexpr int EPI_BYTES = kEpiWarps * 2048;  // a 32 x 32 bf16 tile per epilogue warp
+  static constexpr int SMEM = STAGES * STAGE_BYTES + EXT * A_BYTES + EPI_BYTES + 1024;
   static constexpr int TMEM_COLS = 2 * BN;
 };
 
@@ -228,14 +232,13 @@ __device__ __forceinline__ uint4 to_bf16x8(const float* v) {
 }
 
 // W_MN: W's rows are the reduction (y = x W); else its columns are (dx = dy W^T).
-template <int BN, bool W_MN>
+template <int BN, bool W_MN, int EXT>
 __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const __grid_constant__ AdapterGemm p) {
-  using Cfg = AdapterCfg<BN>;
+  using Cfg = AdapterCfg<BN, EXT>;
   constexpr int STAGES = Cfg::STAGES;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES];
-  // an adapter block's stage passes from the producer (granted) over the builders (built) to the MMA warp
-  __shared__ uint64_t granted_bar[STAGES], built_bar[STAGES];
+  __shared__ uint64_t built_bar[EXT], used_bar[EXT];  // of the built operands
   __shared__ uint64_t tfull_bar[2], tempty_bar[2], drain_bar;
   __shared__ uint32_t tmem_base_s;
   __shared__ volatile int abort_flag;
@@ -243,14 +246,17 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
   uint8_t* sB = smem + STAGES * Cfg::A_BYTES;
-  uint8_t* sEpi = smem + STAGES * Cfg::STAGE_BYTES;
+  uint8_t* sExt = smem + STAGES * Cfg::STAGE_BYTES;
+  uint8_t* sEpi = sExt + EXT * Cfg::A_BYTES;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
-      mbar_init(&granted_bar[s], 1);
-      mbar_init(&built_bar[s], kBuildWarps);
+    }
+    for (int e = 0; e < EXT; ++e) {
+      mbar_init(&built_bar[e], kBuildWarps);
+      mbar_init(&used_bar[e], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull_bar[a], 1);
@@ -310,7 +316,6 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
             const int h = p.HR > 1 ? e / c.ext : c.z;
             const int j0 = (e % c.ext) * p.per_block;
             const int n = min(p.per_block, c.nslots - j0);
-            mbar_arrive(&granted_bar[stage]);
             mbar_arrive_expect_tx(&full_bar[stage], n * p.rp * 2 * BN);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -349,8 +354,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
       // ------------------------------------------------ MMA issuer
       constexpr uint32_t idesc_w = make_idesc_bf16(128, BN, false, W_MN);
       constexpr uint32_t idesc_b = make_idesc_bf16(128, BN, false, true);
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0, built_phase = 0;  // built_phase: one bit per stage
+      int stage = 0, acc = 0, buf = 0;  // buf: the next built operand
+      uint32_t phase = 0, acc_phase = 0, buf_phase = 0;
       bool ok = true;
       AdapterTile next = adapter_tile(p, blockIdx.x, BN);
       for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
@@ -365,8 +370,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
         for (int kb = c.kb0; kb < c.kb1; ++kb) {
           const bool ext = kb >= p.HR * p.KB;
           if (!mbar_wait_bounded(&full_bar[stage], phase, &abort_flag, p.err, kErrTimeoutMma) ||
-              (ext && !mbar_wait_bounded(&built_bar[stage], (built_phase >> stage) & 1, &abort_flag, p.err,
-                                         kErrTimeoutMma))) {
+              (ext && !mbar_wait_bounded(&built_bar[buf], buf_phase, &abort_flag, p.err, kErrTimeoutMma))) {
             ok = false;
             break;
           }
@@ -381,12 +385,17 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
                              : make_sdesc_sw128(b_base + kk * 32, 16, 1024),
                         idesc_w, (kb > c.kb0 || kk > 0) ? 1u : 0u);
           } else {
-            built_phase ^= 1u << stage;
+            const uint32_t e_base = smem_u32(sExt + buf * Cfg::A_BYTES);
             const int j0 = ((kb - p.HR * p.KB) % c.ext) * p.per_block;
             const int steps = min(p.per_block, c.nslots - j0) * p.rp / 16;
             for (int kk = 0; kk < steps; ++kk)
-              umma_bf16(d_tmem, make_sdesc_sw128(a_base + kk * 32, 16, 1024),
+              umma_bf16(d_tmem, make_sdesc_sw128(e_base + kk * 32, 16, 1024),
                         make_sdesc_sw128(b_base + kk * 2048, 8192, 1024), idesc_b, (kb > c.kb0 || kk > 0) ? 1u : 0u);
+            umma_commit(&used_bar[buf]);
+            if (++buf == EXT) {
+              buf = 0;
+              buf_phase ^= 1;
+            }
           }
           umma_commit(&empty_bar[stage]);
           if (++stage == STAGES) {
@@ -407,11 +416,11 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
       mbar_wait_bounded(&drain_bar, 0, (volatile int*)&dummy_abort, p.err, kErrTimeoutDrain);
     }
   } else if (warp < 2 + kEpiWarps) {
-    // ------------------------------------------------ epilogue: bf16 tiles by TMA, or fp32 parts
+    // ------------------------------------------------ epilogue: bf16 rows, or fp32 parts
     const int quad = warp & 3;         // TMEM lane quadrant of this warp
     const int half = (warp - 2) >> 2;  // half of the tile's columns
-    uint8_t* buf = sEpi + (warp - 2) * 4096;
-    constexpr int COLS = BN >= 128 ? BN / 2 : 64;
+    uint8_t* buf = sEpi + (warp - 2) * 2048;
+    constexpr int COLS = BN / 2;
     const int col0 = half * COLS;
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -421,26 +430,30 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
       tc_fence_after();
       const int row0 = c.m0 + quad * 32;
 #pragma unroll 1
-      for (int cc = 0; cc < COLS; cc += 64) {
+      for (int cc = 0; cc < COLS; cc += 32) {
         const int col = c.n0 + col0 + cc;
-        if (col0 >= BN || row0 >= p.M || col >= p.N) continue;
-        float v[64];
-        tmem_ld64(tmem_base + ((uint32_t)(quad * 32) << 16) + acc * BN + col0 + cc, v);
+        if (row0 >= p.M || col >= p.N) continue;
+        float v[32];
+        tmem_ld32(tmem_base + ((uint32_t)(quad * 32) << 16) + acc * BN + col0 + cc, v);
         if (p.splits == 1) {
-          if (lane == 0) bulk_wait_group_read0();  // the previous tile has left the buffer
+          // a lane holds a row: turned over in shared memory so that four lanes store 64 bytes of one row
           __syncwarp();
 #pragma unroll
-          for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(buf + sw128(lane, q)) = to_bf16x8(v + 8 * q);
-          fence_proxy_async_smem();
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = to_bf16x8(v + 8 * q);
           __syncwarp();
-          if (lane == 0) {
-            tma_store_4d(&p.ty, buf, col, row0, c.z, 0);
-            bulk_commit_group();
+          const int q = lane & 3;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 8 * i + lane / 4;
+            const uint4 w = *reinterpret_cast<const uint4*>(buf + r * 64 + ((q ^ ((r >> 1) & 3)) << 4));
+            if (row0 + r < p.M && col + 8 * q < p.N)
+              *reinterpret_cast<uint4*>(p.y + (long long)(row0 + r) * p.Z * p.N + (long long)c.z * p.N + col + 8 * q) = w;
           }
         } else if (row0 + lane < p.M) {
           float* o = p.partial + (((long long)c.split * p.Z + c.z) * p.M + row0 + lane) * p.N + col;
 #pragma unroll
-          for (int q = 0; q < 16; ++q)
+          for (int q = 0; q < 8; ++q)
             if (col + 4 * q < p.N)
               reinterpret_cast<float4*>(o)[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
         }
@@ -453,7 +466,6 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
         acc_phase ^= 1;
       }
     }
-    if (lane == 0) bulk_wait_group0();
   } else {
     // ------------------------------------------------ builders: one row of the tile per thread
     grid_dependency_wait();  // t is complete (and this grid does not end before the one that wrote it)
@@ -487,8 +499,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
         row.t[i] = to_bf16x8(f);
       }
     };
-    uint32_t granted_phase = 0;  // one bit per stage: a stage is granted again only after it was built and used
-    int done = 0;                // stage of the tile's first block
+    int buf = 0;
+    uint32_t buf_phase = 0;
     bool ok = true;
     Row row, next;
     int t = blockIdx.x, hr = 0;
@@ -502,14 +514,11 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
       for (int e = 0; e < c.ext; ++e) {
         const int kb = p.HR * p.KB + hr * c.ext + e;
         if (kb < c.kb0 || kb >= c.kb1) continue;
-        const int stage = (done + kb - c.kb0) % STAGES;
-        if (!mbar_wait_bounded(&granted_bar[stage], (granted_phase >> stage) & 1, &abort_flag, p.err,
-                               kErrTimeoutProducer)) {
+        if (!mbar_wait_bounded(&used_bar[buf], buf_phase ^ 1, &abort_flag, p.err, kErrTimeoutProducer)) {
           ok = false;
           break;
         }
-        granted_phase ^= 1u << stage;
-        uint8_t* dst = sA + stage * Cfg::A_BYTES;
+        uint8_t* dst = sExt + buf * Cfg::A_BYTES;
         const int j = row.slot - e * p.per_block;  // the row's slot in this block
         const int at = row.slot >= 0 && j >= 0 && j < p.per_block ? j * p.rp / 8 : 8;
 #pragma unroll
@@ -522,9 +531,12 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&built_bar[stage]);
+        if (lane == 0) mbar_arrive(&built_bar[buf]);
+        if (++buf == EXT) {
+          buf = 0;
+          buf_phase ^= 1;
+        }
       }
-      if (!hr2) done = (done + c.kb1 - c.kb0) % STAGES;
       row = next;
       t = t2, hr = hr2;
       c = c2;
@@ -837,10 +849,11 @@ at::Tensor shrink(const Rows& x, const at::Tensor& a, const Plan& p, int H, int 
   return t;
 }
 
-template <int BN, bool W_MN>
+template <int BN, bool W_MN, int EXT>
 void launch_gemm(const AdapterGemm& p, cudaStream_t st, int dev, bool after_shrink) {
-  using Cfg = AdapterCfg<BN>;
-  auto kern = adapter_gemm_kernel<BN, W_MN>;
+  using Cfg = AdapterCfg<BN, EXT>;
+  static_assert(Cfg::SMEM <= 226 * 1024, "shared memory of the projection kernel");
+  auto kern = adapter_gemm_kernel<BN, W_MN, EXT>;
   static bool attr_set[64] = {false};
   if (!attr_set[dev]) {
     C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
@@ -914,18 +927,24 @@ at::Tensor project(const Rows& x, const at::Tensor& w, bool w_mn, bool sum_heads
     p.tw = tensor_map_bf16(w.data_ptr(), {K, N, H}, {w.stride(1), w.stride(0)}, 64, (uint32_t)bn);
   if (adapters)
     p.tb = tensor_map_bf16(b.data_ptr(), {N, r, b.size(0) * H}, {N, (int64_t)r * N}, 64, (uint32_t)p.rp);
-  p.ty = tensor_map_bf16(y.data_ptr(), {N, M, p.Z}, {(int64_t)p.Z * N, N}, 64, 32);
-#define BD_ADAPTER(BN)                                 \
-  if (bn == BN) {                                      \
-    if (w_mn)                                          \
-      launch_gemm<BN, true>(p, st, dev, adapters);     \
-    else                                               \
-      launch_gemm<BN, false>(p, st, dev, adapters);    \
-  }
-  BD_ADAPTER(64)
-  BD_ADAPTER(128)
-  BD_ADAPTER(256)
-#undef BD_ADAPTER
+  p.y = reinterpret_cast<bf16*>(y.data_ptr());
+  // short: at most 16 blocks of the reduction between two adapter blocks' tiles
+  const bool brief = blocks / p.splits <= 16;
+  auto go = [&](auto width, auto ext) {
+    constexpr int W = decltype(width)::value, E = decltype(ext)::value;
+    if (w_mn)
+      launch_gemm<W, true, E>(p, st, dev, adapters);
+    else
+      launch_gemm<W, false, E>(p, st, dev, adapters);
+  };
+  if (bn == 256 && brief)
+    go(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
+  else if (bn == 256)
+    go(std::integral_constant<int, 256>(), std::integral_constant<int, 1>());
+  else if (bn == 128)
+    go(std::integral_constant<int, 128>(), std::integral_constant<int, 3>());
+  else
+    go(std::integral_constant<int, 64>(), std::integral_constant<int, 3>());
   if (p.splits > 1) {
     const long long n = (long long)p.Z * M * N;
     adapter_sum_kernel<<<(unsigned)((n + 127) / 128), 256, 0, st>>>(
