@@ -163,7 +163,7 @@ struct AdapterGemm {
   int x_heads;       // x has a head coordinate
   int H;             // heads of b and t
   int tiles_m, tiles_n, splits;
-  int rp, per_block;  // padded rank, slots per 64-wide block
+  int rp, per_block, block_shift;  // padded rank, slots per 64-wide block and its logarithm
   int parts;          // partial sums of t
   long long t_part;
   const float* t;     // [parts, H, M, rp]; null without adapters
@@ -181,26 +181,54 @@ struct AdapterTile {
   int m0, n0, z, slot0, nslots, ext, kb0, kb1, split;
 };
 
-// Coordinates of tile t; its slots are read from memory by adapter_tile, which every role calls one tile ahead.
-__device__ __forceinline__ AdapterTile adapter_place(const AdapterGemm& p, int t, int BN) {
+// The tiles of a CTA, t, t + step, ...: columns fastest, then rows, parts, heads. Divided once; a role is one thread
+// here, and divisions for every tile (64-bit ones above all) made a chain of over 1 us (4096 x 256 -> 4 x
+// 8192 without adapters: 98 us with them).
+struct AdapterWalk {
+  unsigned at[3], by[3], size[3], z, bz;
+
+  __device__ __forceinline__ AdapterWalk(const AdapterGemm& p, unsigned t, unsigned step) {
+    size[0] = p.tiles_n, size[1] = p.tiles_m, size[2] = p.splits;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      at[i] = t % size[i], by[i] = step % size[i];
+      t /= size[i], step /= size[i];
+    }
+    z = t, bz = step;
+  }
+  __device__ __forceinline__ void next() {
+    unsigned carry = 0;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      at[i] += by[i] + carry;
+      carry = at[i] >= size[i] ? 1 : 0;
+      at[i] -= carry ? size[i] : 0;
+    }
+    z += bz + carry;
+  }
+};
+
+__device__ __forceinline__ AdapterTile adapter_place(const AdapterWalk& w, int BN) {
   AdapterTile c;
-  c.n0 = (t % p.tiles_n) * BN;
-  t /= p.tiles_n;
-  c.m0 = (t % p.tiles_m) * 128;
-  t /= p.tiles_m;
-  c.split = t % p.splits;
-  c.z = t / p.splits;
+  c.n0 = (int)w.at[0] * BN;
+  c.m0 = (int)w.at[1] * 128;
+  c.split = (int)w.at[2];
+  c.z = (int)w.z;
   return c;
 }
 
-__device__ __forceinline__ AdapterTile adapter_tile(const AdapterGemm& p, int t, int BN) {
-  AdapterTile c = adapter_place(p, t, BN);
-  c.slot0 = p.t ? p.tile_ptr[c.m0 / 128] : 0;
-  c.nslots = (p.t ? p.tile_ptr[c.m0 / 128 + 1] : 0) - c.slot0;
-  c.ext = (c.nslots + p.per_block - 1) / p.per_block;
-  const long long total = (long long)p.HR * (p.KB + c.ext);
-  c.kb0 = (int)(total * c.split / p.splits);
-  c.kb1 = (int)(total * (c.split + 1) / p.splits);
+// With the tile's slots, which are read from memory: every role asks one tile ahead.
+__device__ __forceinline__ AdapterTile adapter_tile(const AdapterGemm& p, const AdapterWalk& w, int BN) {
+  AdapterTile c = adapter_place(w, BN);
+  c.slot0 = p.t ? p.tile_ptr[w.at[1]] : 0;
+  c.nslots = (p.t ? p.tile_ptr[w.at[1] + 1] : 0) - c.slot0;
+  c.ext = (c.nslots + p.per_block - 1) >> p.block_shift;
+  const unsigned total = (unsigned)(p.HR * (p.KB + c.ext));  // times splits below 2^32: the host checks
+  c.kb0 = 0, c.kb1 = (int)total;
+  if (p.splits > 1) {
+    c.kb0 = (int)(total * (unsigned)c.split / (unsigned)p.splits);
+    c.kb1 = (int)(total * (unsigned)(c.split + 1) / (unsigned)p.splits);
+  }
   return c;
 }
 
@@ -281,7 +309,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
       uint32_t phase = 0;
       long long issued = 0;
       bool ok = true;
-      AdapterTile next = adapter_tile(p, blockIdx.x, BN);
+      AdapterWalk walk(p, blockIdx.x, gridDim.x);
+      AdapterTile next = adapter_tile(p, walk, BN);
       int ids[4];  // adapters of the next adapter block, read while other blocks are on their way
       auto read_ids = [&](const AdapterTile& c, int e) {
 #pragma unroll
@@ -290,8 +319,9 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
       };
       for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
         const AdapterTile c = next;
-        if (t + (int)gridDim.x < total) next = adapter_tile(p, t + gridDim.x, BN);
-        if (c.ext > 0) read_ids(c, max(c.kb0 - p.HR * p.KB, 0) % c.ext);
+        walk.next();
+        if (t + (int)gridDim.x < total) next = adapter_tile(p, walk, BN);
+        if (c.ext > 0) read_ids(c, p.HR > 1 ? max(c.kb0 - p.HR * p.KB, 0) % c.ext : max(c.kb0 - p.KB, 0));
         for (int kb = c.kb0; kb < c.kb1; ++kb) {
           if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutProducer)) {
             ok = false;
@@ -314,7 +344,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
           } else {
             const int e = kb - p.HR * p.KB;
             const int h = p.HR > 1 ? e / c.ext : c.z;
-            const int j0 = (e % c.ext) * p.per_block;
+            const int j0 = (p.HR > 1 ? e % c.ext : e) * p.per_block;
             const int n = min(p.per_block, c.nslots - j0);
             mbar_arrive_expect_tx(&full_bar[stage], n * p.rp * 2 * BN);
 #pragma unroll
@@ -325,7 +355,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
               for (int i = 0; i < BN / 64; ++i)
                 tma_load_4d(b_dst + i * 8192 + j * p.rp * 128, &p.tb, &full_bar[stage], c.n0 + 64 * i, 0, gh, 0);
             }
-            read_ids(c, (e + 1) % c.ext);
+            read_ids(c, p.HR > 1 ? (e + 1) % c.ext : min(e + 1, c.ext - 1));
           }
           ++issued;
           if (++stage == STAGES) {
@@ -357,10 +387,12 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
       int stage = 0, acc = 0, buf = 0;  // buf: the next built operand
       uint32_t phase = 0, acc_phase = 0, buf_phase = 0;
       bool ok = true;
-      AdapterTile next = adapter_tile(p, blockIdx.x, BN);
+      AdapterWalk walk(p, blockIdx.x, gridDim.x);
+      AdapterTile next = adapter_tile(p, walk, BN);
       for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
         const AdapterTile c = next;
-        if (t + (int)gridDim.x < total) next = adapter_tile(p, t + gridDim.x, BN);
+        walk.next();
+        if (t + (int)gridDim.x < total) next = adapter_tile(p, walk, BN);
         if (!mbar_wait_bounded(&tempty_bar[acc], acc_phase ^ 1, &abort_flag, p.err, kErrTimeoutMma)) {
           ok = false;
           break;
@@ -386,8 +418,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
                         idesc_w, (kb > c.kb0 || kk > 0) ? 1u : 0u);
           } else {
             const uint32_t e_base = smem_u32(sExt + buf * Cfg::A_BYTES);
-            const int j0 = ((kb - p.HR * p.KB) % c.ext) * p.per_block;
-            const int steps = min(p.per_block, c.nslots - j0) * p.rp / 16;
+            const int j0 = (p.HR > 1 ? (kb - p.HR * p.KB) % c.ext : kb - p.KB) * p.per_block;
+            const int steps = (min(p.per_block, c.nslots - j0) * p.rp) >> 4;
             for (int kk = 0; kk < steps; ++kk)
               umma_bf16(d_tmem, make_sdesc_sw128(e_base + kk * 32, 16, 1024),
                         make_sdesc_sw128(b_base + kk * 2048, 8192, 1024), idesc_b, (kb > c.kb0 || kk > 0) ? 1u : 0u);
@@ -424,8 +456,9 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
     const int col0 = half * COLS;
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int t = blockIdx.x; t < total; t += gridDim.x) {
-      const AdapterTile c = adapter_place(p, t, BN);
+    AdapterWalk walk(p, blockIdx.x, gridDim.x);
+    for (int t = blockIdx.x; t < total; t += gridDim.x, walk.next()) {
+      const AdapterTile c = adapter_place(walk, BN);
       if (!mbar_wait_bounded(&tfull_bar[acc], acc_phase, &abort_flag, p.err, kErrTimeoutEpilogue)) break;
       tc_fence_after();
       const int row0 = c.m0 + quad * 32;
@@ -504,12 +537,14 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
     bool ok = true;
     Row row, next;
     int t = blockIdx.x, hr = 0;
-    AdapterTile c = adapter_tile(p, t, BN);
+    AdapterWalk walk(p, blockIdx.x, gridDim.x);
+    AdapterTile c = adapter_tile(p, walk, BN);
     fetch(c, 0, row);
     while (ok && t < total) {
       const int hr2 = hr + 1 < p.HR ? hr + 1 : 0;
       const int t2 = hr2 ? t : t + (int)gridDim.x;
-      const AdapterTile c2 = hr2 || t2 >= total ? c : adapter_tile(p, t2, BN);
+      if (!hr2) walk.next();
+      const AdapterTile c2 = hr2 || t2 >= total ? c : adapter_tile(p, walk, BN);
       if (t2 < total) fetch(c2, hr2, next);
       for (int e = 0; e < c.ext; ++e) {
         const int kb = p.HR * p.KB + hr * c.ext + e;
@@ -885,6 +920,8 @@ at::Tensor project(const Rows& x, const at::Tensor& w, bool w_mn, bool sum_heads
   p.Z = sum_heads ? 1 : H;
   p.x_heads = x.head != 0;
   p.rp = padded_rank(r), p.per_block = 64 / p.rp;
+  p.block_shift = p.per_block == 4 ? 2 : p.per_block == 2 ? 1 : 0;
+  TORCH_CHECK(((long long)p.KB + 128) * p.HR < (1 << 22), "adapter_linear: the reduction is too long");
   const bool adapters = plan.rows > 0;
   if (adapters) {
     p.t = t.data_ptr<float>(), p.parts = (int)t.size(0), p.t_part = t.stride(0);

@@ -108,6 +108,7 @@ CASES = [
     ([0, 1], [70, 60], 2, 1, 4104, 40, 16, True),             # long reduction, few tiles: split
     ([0, 1, 0], [40, 50, 60], 2, 2, 72, 2056, 33, True),      # wide output, padded rank
     ([1, 3, 0, 2, 1], [301, 1, 499, 64, 36], 4, 2, 256, 9000, 16, True),  # several tiles per CTA, short reduction
+    ([0, -1, 1], [700, 300, 36], 2, 3, 72, 6000, 24, True),   # many row tiles of a short reduction, a tile without adapters
     (list(range(40)) * 2, [8] * 80, 40, 2, 64, 8200, 16, False),  # more adapter blocks than projection blocks
 ]
 
