@@ -15,6 +15,10 @@
 // code, since a denominator rounded to zero would blow its update up. m and v are
 // computed with separately rounded products and sums, so any implementation of the formulas
 // gives the same codes.
+//
+// Measured on a B200: 25.2 M values, fp32 states and gradients, 28 B each: 108 us = 6.5 TB/s, the copy rate. 26 M
+// values with e4m3 states, bf16 gradients and working copies, 16 B each: 92 us = 4.6 TB/s; there the
+// instructions bound it (about 95 a value; 85 % of the issue slots at 120 before the codes were converted in pairs).
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_bf16.h>

@@ -19,6 +19,10 @@
 //    row tile. The projection's blocks need no t, so with programmatic launch they run
 //    while adapter_shrink still does; only the builders wait for it.
 //  * adapter_grad: da / db, one CTA per adapter, head and slab of columns; for db it gives u in the same pass over dy.
+// Measured on a B200: 48 rows, 43 adapters of rank 16, 4 heads 256 -> 8192: 22 us for 66 MB;
+// 4099 rows the same way: shrink 11, product 107 us (45 us for its 295 MB at the copy rate: the issuing
+// thread and the operands' way into shared memory, 192 KB a tile, bound it); 4096^3 without adapters 107 us = 1285
+// TFLOP/s. Keeping w in shared memory over the row tiles (192 columns) was slower: 113 against 98 us.
 // t and u are kept in fp32 (partial sums over the parts of the reduction) and rounded to bf16
 // once, as an operand of the next product, like every activation of the bf16 path. All sums are
 // fp32 and in a fixed order: no atomics.
