@@ -826,8 +826,9 @@ struct Plan {
   const int *row_adapter, *row_slot, *tile_ptr, *slots, *order, *chunk, *group, *by_size;
 };
 
-Plan read_plan(const at::Tensor& buf, const std::vector<int64_t>& d) {
-  TORCH_CHECK(buf.is_cuda() && buf.scalar_type() == at::kInt && buf.is_contiguous() && d.size() == 7,
+Plan read_plan(const at::Tensor& buf, const std::vector<int64_t>& d, int dev) {
+  TORCH_CHECK(buf.is_cuda() && buf.get_device() == dev, "adapter_linear: the batch's plan must be on the operands' GPU");
+  TORCH_CHECK(buf.scalar_type() == at::kInt && buf.is_contiguous() && d.size() == 7,
               "adapter_linear: bad batch plan");
   Plan p;
   p.M = (int)d[0], p.G = (int)d[1], p.tiles = (int)d[2], p.rows = (int)d[4], p.chunks = (int)d[5], p.rows_per_chunk = (int)d[6];
@@ -1117,8 +1118,8 @@ c10::optional<at::Tensor> adapter_direct(const at::Tensor& x, const at::Tensor& 
                                          const c10::optional<at::Tensor>& scale, double scale0, const at::Tensor& err) {
   const bool heads = w.dim() == 3;
   if (!w.is_cuda() || !(heads || w.dim() == 2) || a.dim() != w.dim() + 1 || b.dim() != w.dim() + 1) return c10::nullopt;
-  if (!(x.dim() == 2 || (heads && x.dim() == 3)) || !plan.is_cuda()) return c10::nullopt;
   const int dev = w.get_device();
+  if (!(x.dim() == 2 || (heads && x.dim() == 3)) || !plan.is_cuda() || plan.get_device() != dev) return c10::nullopt;
   const int64_t H = heads ? w.size(0) : 1, K = w.size(-2), N = w.size(-1), G = a.size(0), r = a.size(-2);
   if (!direct(x, dev, K) || !direct(w, dev, N) || !direct(a, dev, K) || !direct(b, dev, N)) return c10::nullopt;
   if (!a.is_contiguous() || !b.is_contiguous() || r < 1 || r > 64 || G != dims[1] || dims[0] == 0 || x.size(0) != dims[0])
@@ -1137,7 +1138,7 @@ c10::optional<at::Tensor> adapter_direct(const at::Tensor& x, const at::Tensor& 
 std::vector<at::Tensor> adapter_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor& a, const at::Tensor& b,
                                         const at::Tensor& plan, const std::vector<int64_t>& dims,
                                         const c10::optional<at::Tensor>& scale, double scale0, const at::Tensor& err) {
-  const Plan p = read_plan(plan, dims);
+  const Plan p = read_plan(plan, dims, w.get_device());
   const Checked c = check_all(x, w, a, b, p, scale);
   c10::cuda::CUDAGuard guard(c.dev);
   auto st = at::cuda::getCurrentCUDAStream(c.dev).stream();
@@ -1156,7 +1157,7 @@ std::vector<at::Tensor> adapter_backward(const at::Tensor& dy, const at::Tensor&
                                          const at::Tensor& plan, const std::vector<int64_t>& dims,
                                          const c10::optional<at::Tensor>& scale, double scale0, const at::Tensor& err,
                                          bool want_dx, bool want_da, bool want_db) {
-  const Plan p = read_plan(plan, dims);
+  const Plan p = read_plan(plan, dims, w.get_device());
   const Checked c = check_all(x, w, a, b, p, scale);
   check_operand(dy, c.dev, "dy");
   TORCH_CHECK(dy.dim() == 3 && dy.size(0) == p.M && dy.size(1) == c.H && dy.size(2) == c.N, "adapter_linear: dy [M, H, N]");

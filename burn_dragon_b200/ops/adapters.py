@@ -151,13 +151,13 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, a: torch.Tensor, b: to
         raise ValueError("the shared projection is frozen: adapter_linear has no gradient for it")
     if isinstance(scale, torch.Tensor) and scale.dim() > 0 and scale.shape != (G,):
         raise ValueError(f"scale must be a number or one value per adapter, got shape {tuple(scale.shape)}")
+    if any(t.device != x.device for t in (weight, a, b, batch.plan)):
+        raise ValueError("adapter_linear: all operands and the batch must be on one device")
     if not x.is_cuda:
         y = adapter_linear_ref(x, weight, a, b, batch, scale)
         return y if heads else y.view(batch.rows, N)
     if any(t.dtype != torch.bfloat16 for t in (x, weight, a, b)):
         raise TypeError("adapter_linear takes bf16 tensors on CUDA")
-    if any(t.device != x.device for t in (weight, a, b)) or batch.device.type != "cuda":
-        raise ValueError("adapter_linear: all operands and the batch must be on one device")
     if K % 8 or N % 8 or not 1 <= r <= MAX_RANK:
         raise ValueError(f"adapter_linear takes K and N in multiples of 8 and a rank of 1 to {MAX_RANK}, got K={K} N={N} r={r}")
     per, scale0 = None, 1.0
