@@ -68,6 +68,9 @@ def main(argv=None) -> None:
     prompts = [list(t.encode()[:max(1, len(t.encode()) // 2)]) for t in a.text]
     out, logprobs = net.generate(prompts, list(range(G)), a.max_tokens, a.temperature, a.top_k, a.top_p, a.min_p, a.seed)
     for g, (p, o, lp) in enumerate(zip(prompts, out, logprobs)):
+        if -1 in o:
+            print(f"adapter {g}: no token to draw after {o.index(-1)} tokens: the logits are NaN or -inf")
+            continue
         text = bytes(t & 0xFF for t in p + o).decode("utf-8", errors="replace")
         print(f"adapter {g}: {text!r} (mean log-probability {sum(lp) / max(len(lp), 1):.3f})")
 

@@ -84,6 +84,8 @@ def main(argv=None) -> None:
     out = Generator(model).generate(x, max_tokens, temperature=temperature, top_k=top_k, seed=a.seed,
                                     top_p=a.top_p, min_p=a.min_p)
     for row in out.tolist():
+        if -1 in row:
+            raise SystemExit(f"no token to draw after {row.index(-1)} tokens: the logits are NaN or -inf")
         if fmt == "token_ids":
             print(json.dumps(row))
         else:

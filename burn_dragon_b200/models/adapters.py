@@ -19,6 +19,7 @@ from ..ops.adapters import AdapterBatch, adapter_linear
 from ..ops.sampling import sample_tokens
 from ..train.optim import AdamWMany
 from . import reference as R
+from .generate import feed, hold
 from .state import ModelState
 
 PROJECTIONS = ("encoder", "encoder_v", "decoder")
@@ -150,7 +151,8 @@ class AdapterBDH:
                  min_p=0.0, seed: int = 0) -> tuple[list[list[int]], list[list[float]]]:
         """Continuations of prompts of different lengths, each with its adapter (-1: none) and settings (numbers,
         or one value per request), and the tokens' log-probabilities. Every row advances at the same
-        position; one still inside its prompt takes its next prompt token."""
+        position; one still inside its prompt takes its next prompt token. A request whose logits leave
+        nothing to draw from answers -1 (log-probability -inf) from there on; the others go on."""
         if len(prompts) != len(adapters) or not prompts or any(not p for p in prompts):
             raise ValueError("one adapter per prompt, and no empty prompts")
         dev = self.p["embed"].device
@@ -165,13 +167,14 @@ class AdapterBDH:
         logits = self.forward(table[:, :shared], self.batch(adapters, shared), state)[:, -1]
         step = self.batch(adapters, 1)  # one plan for all single-token steps
         tokens, logprobs = [], []
+        nxt = None
         for pos in range(shared, width + max_new_tokens):
             drawn, lp = sample_tokens(logits.contiguous(), torch.rand(len(prompts), generator=gen, device=dev), *settings)
-            nxt = torch.where(lens > pos, table[:, min(pos, width - 1)], drawn)
+            nxt = torch.where(lens > pos, table[:, min(pos, width - 1)], hold(drawn, nxt))
             tokens.append(nxt)
-            logprobs.append(lp)
+            logprobs.append(torch.where(nxt < 0, float("-inf"), lp))
             if pos + 1 < width + max_new_tokens:
-                logits = self.forward(nxt[:, None], step, state)[:, -1]
+                logits = self.forward(feed(nxt)[:, None], step, state)[:, -1]
         host_t = torch.stack(tokens, 1).tolist()
         host_l = torch.stack(logprobs, 1).tolist()
         start = [len(p) - shared for p in prompts]

@@ -32,7 +32,8 @@ def sample_next(logits: torch.Tensor, temperature: float = 0.0, top_k: int | Non
                 generator: torch.Generator | None = None, top_p: float | None = None,
                 min_p: float | None = None) -> torch.Tensor:
     """Greedy for temperature 0, else softmax(logits / T) restricted to the top-k. With ``top_p`` or
-    ``min_p`` the draw is ``ops.sampling.sample_tokens`` on uniform numbers from ``generator``."""
+    ``min_p`` the draw is ``ops.sampling.sample_tokens`` on uniform numbers from ``generator``: -1 for a row
+    whose logits leave nothing to draw from (``hold`` and ``feed`` carry it through a loop)."""
     if temperature <= 0.0:
         return logits.argmax(dim=-1)
     if top_p is not None or min_p is not None:
@@ -44,6 +45,16 @@ def sample_next(logits: torch.Tensor, temperature: float = 0.0, top_k: int | Non
         z = z.masked_fill(z < kth, float("-inf"))
     p = torch.softmax(z, dim=-1)
     return torch.multinomial(p, 1, generator=generator).squeeze(-1)
+
+
+def hold(drawn: torch.Tensor, before: torch.Tensor | None) -> torch.Tensor:
+    """``drawn``, with -1 for every row that had no token ``before`` either: such a row has ended."""
+    return drawn if before is None else torch.where(before < 0, before, drawn)
+
+
+def feed(tokens: torch.Tensor) -> torch.Tensor:
+    """``tokens`` as the model may read them: a row without one goes on with token 0, and is not answered."""
+    return tokens.clamp_min(0)
 
 
 class _DecodeWorkspace:
@@ -259,7 +270,8 @@ class Generator:
                         device=None, top_p: float | None = None, min_p: float | None = None) -> list[int]:
         """One sequence, tokens handed to ``on_chunk`` every ``chunk_tokens`` steps
         (generation.rs:1174-1275). ``sliding_window`` keeps only the last ``window``
-        prompt tokens (the recurrent state needs no trimming afterwards)."""
+        prompt tokens (the recurrent state needs no trimming afterwards). Logits that leave nothing to
+        draw from raise RuntimeError, after the tokens before them were handed out."""
         dev = torch.device(device) if device is not None else self.model.store.data.device
         if sliding_window and len(prompt) > sliding_window:
             prompt = prompt[-sliding_window:]
@@ -271,21 +283,30 @@ class Generator:
         full = list(prompt)
         pending = []
         done = 0
+        may_end = top_p is not None or min_p is not None  # draws of sample_tokens, which may be -1
+        nxt = None
         while done < max_new_tokens:
-            nxt = sample_next(logits, temperature, top_k, gen, top_p, min_p)
+            nxt = sample_next(logits, temperature, top_k, gen, top_p, min_p) if not may_end else \
+                hold(sample_next(logits, temperature, top_k, gen, top_p, min_p), nxt)
             pending.append(nxt)
             done += 1
             if done < max_new_tokens:
-                logits = self.decode_step(nxt.contiguous(), state)
+                logits = self.decode_step((feed(nxt) if may_end else nxt).contiguous(), state)
             if len(pending) >= chunk_tokens or done == max_new_tokens:
                 chunk = torch.cat(pending).cpu().tolist()
                 pending.clear()
+                failed = -1 in chunk
+                chunk = chunk[:chunk.index(-1)] if failed else chunk
                 if stop_token is not None and stop_token in chunk:
                     chunk = chunk[:chunk.index(stop_token) + 1]
                     full.extend(chunk)
                     if on_chunk:
                         on_chunk(chunk)
                     break
+                if failed:
+                    if on_chunk and chunk:
+                        on_chunk(chunk)
+                    raise RuntimeError("no token to draw: the logits are NaN or -inf")
                 full.extend(chunk)
                 if on_chunk:
                     on_chunk(chunk)
@@ -296,7 +317,8 @@ class Generator:
     def generate(self, prompt: torch.Tensor, max_new_tokens: int, temperature: float = 0.0,
                  top_k: int | None = None, device_buffer_tokens: int = 64, seed: int | None = None,
                  top_p: float | None = None, min_p: float | None = None):
-        """Returns [B, max_new_tokens] generated tokens (host tensor)."""
+        """Returns [B, max_new_tokens] generated tokens (host tensor). With ``top_p`` or ``min_p`` a row whose
+        logits leave nothing to draw from holds -1 from there on; the other rows go on."""
         gen = None
         if seed is not None:
             gen = torch.Generator(device=prompt.device)
@@ -304,6 +326,7 @@ class Generator:
         logits, state = self.prefill(prompt)
         buf = torch.empty(prompt.shape[0], max_new_tokens, dtype=torch.long, device=prompt.device)
         out = []
+        may_end = top_p is not None or min_p is not None
         nxt = sample_next(logits, temperature, top_k, gen, top_p, min_p)
         for i in range(max_new_tokens):
             buf[:, i] = nxt
@@ -311,6 +334,7 @@ class Generator:
                 start = (i // device_buffer_tokens) * device_buffer_tokens
                 out.append(buf[:, start:i + 1].cpu())
             if i + 1 < max_new_tokens:
-                logits = self.decode_step(nxt, state)
-                nxt = sample_next(logits, temperature, top_k, gen, top_p, min_p)
+                logits = self.decode_step(feed(nxt) if may_end else nxt, state)
+                drawn = sample_next(logits, temperature, top_k, gen, top_p, min_p)
+                nxt = hold(drawn, nxt) if may_end else drawn
         return torch.cat(out, dim=1)
