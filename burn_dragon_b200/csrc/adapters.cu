@@ -14,7 +14,9 @@
 //    with the adapters as an extension of its reduction: after the K-blocks of x and W
 //    come blocks of 64 / rp adapter slots. A 128-row tile lists the distinct adapters of its rows
 //    ("slots"); four builder warps write t s into the columns of each row's slot and zeros
-//    elsewhere, and TMA loads the slots' b rows beside each other. So one accumulator takes both
+//    elsewhere, and TMA loads the slots' b rows beside each other. A slot's product leaves the accumulator's
+//    rows of other slots as they are (they are masked off: zeros alone would let an infinity or NaN in one
+//    adapter's b into them, since 0 b is NaN then). So one accumulator takes both
 //    products, rows of any adapters can share a tile, and W and every b are read once per
 //    row tile. The projection's blocks need no t, so with programmatic launch they run
 //    while adapter_shrink still does; only the builders wait for it.
@@ -45,6 +47,16 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// umma_bf16 with accumulation into the rows (TMEM lanes) whose bit in `off` is clear; the others keep what they hold.
+__device__ __forceinline__ void umma_bf16_rows(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint4 off) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.eq.b32 p, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off.x), "r"(off.y), "r"(off.z), "r"(off.w)
+      : "memory");
 }
 
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -167,7 +179,7 @@ struct AdapterGemm {
   int x_heads;       // x has a head coordinate
   int H;             // heads of b and t
   int tiles_m, tiles_n, splits;
-  int rp, per_block, block_shift;  // padded rank, slots per 64-wide block and its logarithm
+  int r, rp, per_block, block_shift;  // rank, padded rank, slots per 64-wide block and its logarithm
   int parts;          // partial sums of t
   long long t_part;
   const float* t;     // [parts, H, M, rp]; null without adapters
@@ -182,7 +194,7 @@ struct AdapterGemm {
 };
 
 struct AdapterTile {
-  int m0, n0, z, slot0, nslots, ext, kb0, kb1, split;
+  int m0, n0, z, slot0, nslots, ext, kb0, kb1, e0, e1, split;
 };
 
 // The tiles of a CTA, t, t + step, ...: columns fastest, then rows, parts, heads. Divided once; a role is one thread
@@ -227,11 +239,15 @@ __device__ __forceinline__ AdapterTile adapter_tile(const AdapterGemm& p, const 
   c.slot0 = p.t ? p.tile_ptr[w.at[1]] : 0;
   c.nslots = (p.t ? p.tile_ptr[w.at[1] + 1] : 0) - c.slot0;
   c.ext = (c.nslots + p.per_block - 1) >> p.block_shift;
-  const unsigned total = (unsigned)(p.HR * (p.KB + c.ext));  // times splits below 2^32: the host checks
-  c.kb0 = 0, c.kb1 = (int)total;
+  // Blocks of the projection, then adapter blocks. A part takes its share of both (of the projection's at least four):
+  // the first product of a tile writes every row of the accumulator, which an adapter's does not.
+  // Times splits below 2^32: the host checks.
+  const unsigned blocks = (unsigned)(p.HR * p.KB), adapters = (unsigned)(p.HR * c.ext);
+  c.kb0 = 0, c.kb1 = (int)blocks, c.e0 = 0, c.e1 = (int)adapters;
   if (p.splits > 1) {
-    c.kb0 = (int)(total * (unsigned)c.split / (unsigned)p.splits);
-    c.kb1 = (int)(total * (unsigned)(c.split + 1) / (unsigned)p.splits);
+    const unsigned i = (unsigned)c.split, parts = (unsigned)p.splits;
+    c.kb0 = (int)(blocks * i / parts), c.kb1 = (int)(blocks * (i + 1) / parts);
+    c.e0 = (int)(adapters * i / parts), c.e1 = (int)(adapters * (i + 1) / parts);
   }
   return c;
 }
@@ -271,6 +287,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES];
   __shared__ uint64_t built_bar[EXT], used_bar[EXT];  // of the built operands
+  __shared__ uint4 rows_off[EXT][4];  // of each slot of a built operand: the tile's rows that are not its own
   __shared__ uint64_t tfull_bar[2], tempty_bar[2], drain_bar;
   __shared__ uint32_t tmem_base_s;
   __shared__ volatile int abort_flag;
@@ -325,28 +342,30 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
         const AdapterTile c = next;
         walk.next();
         if (t + (int)gridDim.x < total) next = adapter_tile(p, walk, BN);
-        if (c.ext > 0) read_ids(c, p.HR > 1 ? max(c.kb0 - p.HR * p.KB, 0) % c.ext : max(c.kb0 - p.KB, 0));
-        for (int kb = c.kb0; kb < c.kb1; ++kb) {
+        if (c.ext > 0) read_ids(c, c.e0 % c.ext);
+        const int projection = c.kb1 - c.kb0, blocks = projection + c.e1 - c.e0;
+        for (int i = 0; i < blocks; ++i) {
           if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutProducer)) {
             ok = false;
             break;
           }
           uint8_t* a_dst = sA + stage * Cfg::A_BYTES;
           uint8_t* b_dst = sB + stage * Cfg::B_BYTES;
-          if (kb < p.HR * p.KB) {
+          if (i < projection) {
+            const int kb = c.kb0 + i;
             const int h = p.HR > 1 ? kb / p.KB : c.z;
             const int k0 = (p.HR > 1 ? kb % p.KB : kb) * 64;
             mbar_arrive_expect_tx(&full_bar[stage], Cfg::STAGE_BYTES);
             tma_load_4d(a_dst, &p.tx, &full_bar[stage], k0, c.m0, p.x_heads ? h : 0, 0);
             if constexpr (W_MN) {
 #pragma unroll
-              for (int i = 0; i < BN / 64; ++i)
-                tma_load_4d(b_dst + i * 8192, &p.tw, &full_bar[stage], c.n0 + 64 * i, k0, h, 0);
+              for (int q = 0; q < BN / 64; ++q)
+                tma_load_4d(b_dst + q * 8192, &p.tw, &full_bar[stage], c.n0 + 64 * q, k0, h, 0);
             } else {
               tma_load_4d(b_dst, &p.tw, &full_bar[stage], k0, c.n0, h, 0);
             }
           } else {
-            const int e = kb - p.HR * p.KB;
+            const int e = c.e0 + i - projection;
             const int h = p.HR > 1 ? e / c.ext : c.z;
             const int j0 = (p.HR > 1 ? e % c.ext : e) * p.per_block;
             const int n = min(p.per_block, c.nslots - j0);
@@ -356,8 +375,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
               if (j >= n) break;
               const int gh = ids[j] * p.H + h;
 #pragma unroll
-              for (int i = 0; i < BN / 64; ++i)
-                tma_load_4d(b_dst + i * 8192 + j * p.rp * 128, &p.tb, &full_bar[stage], c.n0 + 64 * i, 0, gh, 0);
+              for (int q = 0; q < BN / 64; ++q)
+                tma_load_4d(b_dst + q * 8192 + j * p.rp * 128, &p.tb, &full_bar[stage], c.n0 + 64 * q, 0, gh, 0);
             }
             read_ids(c, p.HR > 1 ? (e + 1) % c.ext : min(e + 1, c.ext - 1));
           }
@@ -403,8 +422,9 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
         }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
-        for (int kb = c.kb0; kb < c.kb1; ++kb) {
-          const bool ext = kb >= p.HR * p.KB;
+        const int projection = c.kb1 - c.kb0, blocks = projection + c.e1 - c.e0;
+        for (int i = 0; i < blocks; ++i) {
+          const bool ext = i >= projection;
           if (!mbar_wait_bounded(&full_bar[stage], phase, &abort_flag, p.err, kErrTimeoutMma) ||
               (ext && !mbar_wait_bounded(&built_bar[buf], buf_phase, &abort_flag, p.err, kErrTimeoutMma))) {
             ok = false;
@@ -419,14 +439,16 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
               umma_bf16(d_tmem, make_sdesc_sw128(a_base + kk * 32, 16, 1024),
                         W_MN ? make_sdesc_sw128(b_base + kk * 2048, 8192, 1024)
                              : make_sdesc_sw128(b_base + kk * 32, 16, 1024),
-                        idesc_w, (kb > c.kb0 || kk > 0) ? 1u : 0u);
+                        idesc_w, (i > 0 || kk > 0) ? 1u : 0u);
           } else {
             const uint32_t e_base = smem_u32(sExt + buf * Cfg::A_BYTES);
-            const int j0 = (p.HR > 1 ? (kb - p.HR * p.KB) % c.ext : kb - p.KB) * p.per_block;
-            const int steps = (min(p.per_block, c.nslots - j0) * p.rp) >> 4;
+            const int e = c.e0 + i - projection;
+            const int j0 = (p.HR > 1 ? e % c.ext : e) * p.per_block;
+            const int steps = (min(p.per_block, c.nslots - j0) * p.rp) >> 4;  // 1, 2 or 4 a slot
             for (int kk = 0; kk < steps; ++kk)
-              umma_bf16(d_tmem, make_sdesc_sw128(e_base + kk * 32, 16, 1024),
-                        make_sdesc_sw128(b_base + kk * 2048, 8192, 1024), idesc_b, (kb > c.kb0 || kk > 0) ? 1u : 0u);
+              umma_bf16_rows(d_tmem, make_sdesc_sw128(e_base + kk * 32, 16, 1024),
+                             make_sdesc_sw128(b_base + kk * 2048, 8192, 1024), idesc_b,
+                             rows_off[buf][kk >> (2 - p.block_shift)]);
             umma_commit(&used_bar[buf]);
             if (++buf == EXT) {
               buf = 0;
@@ -532,7 +554,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
           f[4] += hi.x, f[5] += hi.y, f[6] += hi.z, f[7] += hi.w;
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= s;
+        for (int e = 0; e < 8; ++e) f[e] = 8 * i + e < p.r ? f[e] * s : 0.f;  // b reads as zero past the rank
         row.t[i] = to_bf16x8(f);
       }
     };
@@ -551,9 +573,11 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
       const AdapterTile c2 = hr2 || t2 >= total ? c : adapter_tile(p, walk, BN);
       if (t2 < total) fetch(c2, hr2, next);
       for (int e = 0; e < c.ext; ++e) {
-        const int kb = p.HR * p.KB + hr * c.ext + e;
-        if (kb < c.kb0 || kb >= c.kb1) continue;
-        if (!mbar_wait_bounded(&used_bar[buf], buf_phase ^ 1, &abort_flag, p.err, kErrTimeoutProducer)) {
+        const int block = hr * c.ext + e;
+        if (block < c.e0 || block >= c.e1) continue;
+        // the same answer for the whole warp: its lanes go on together
+        if (!__all_sync(0xffffffffu,
+                        mbar_wait_bounded(&used_bar[buf], buf_phase ^ 1, &abort_flag, p.err, kErrTimeoutProducer))) {
           ok = false;
           break;
         }
@@ -567,6 +591,11 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             if (8 * i < p.rp) *reinterpret_cast<uint4*>(dst + sw128(r, at + i)) = row.t[i];
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const uint32_t own = __ballot_sync(0xffffffffu, at < 8 && j == s);
+          if (lane == 0) reinterpret_cast<uint32_t*>(&rows_off[buf][s])[r / 32] = ~own;
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -803,7 +832,7 @@ __global__ void __launch_bounds__(256) adapter_grad_kernel(const __grid_constant
     }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
-  const float s = p.scale ? p.scale[g] : p.scale0;
+  const float s = rows == 0 ? 0.f : p.scale ? p.scale[g] : p.scale0;  // 0 even where the scale is not finite
   bf16* out = p.out + gh * p.r * p.C;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
@@ -924,7 +953,7 @@ at::Tensor project(const Rows& x, const at::Tensor& w, bool w_mn, bool sum_heads
   p.HR = sum_heads ? H : 1;
   p.Z = sum_heads ? 1 : H;
   p.x_heads = x.head != 0;
-  p.rp = padded_rank(r), p.per_block = 64 / p.rp;
+  p.r = r, p.rp = padded_rank(r), p.per_block = 64 / p.rp;
   p.block_shift = p.per_block == 4 ? 2 : p.per_block == 2 ? 1 : 0;
   TORCH_CHECK(((long long)p.KB + 128) * p.HR < (1 << 22), "adapter_linear: the reduction is too long");
   const bool adapters = plan.rows > 0;

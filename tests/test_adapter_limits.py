@@ -33,3 +33,75 @@ def test_the_binding_refuses_a_plan_of_another_device():
     assert mod.adapter_direct(x, w, a, b, batch.plan, batch.dims, None, 1.0, err) is None
     with pytest.raises(RuntimeError, match="operands' GPU"):
         mod.adapter_forward(x, w, a, b, batch.plan, batch.dims, None, 1.0, err)
+
+
+LAYOUTS = [
+    # ids, rows, adapters, H, K, N, r, x shared: several requests to a tile
+    ([0, 1, -1, 2, 0], [3, 2, 4, 5, 1], 3, 2, 64, 72, 16, True),            # one block of adapters
+    (list(range(9)) + [-1, 1], [1] * 11, 9, 1, 128, 264, 8, True),          # several blocks, single tokens
+    ([2, 1, 0, -1], [100, 20, 60, 9], 3, 2, 72, 136, 33, False),            # one slot a block, two tiles
+    (list(range(20)) + [-1] * 3, [2] * 23, 20, 1, 8200, 40, 16, True),      # a reduction in parts
+    ([0, 1, 2, -1, 1], [30, 40, 50, 7, 9], 3, 4, 128, 520, 24, True),       # two slots a block, dx sums the heads
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("where", ["a", "b", "one of b"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("layout", LAYOUTS, ids=range(len(LAYOUTS)))
+def test_a_not_finite_adapter_stays_with_its_rows(layout, value, where):
+    """Rows of other adapters, rows without one and the other adapters' gradients are what they are beside a finite
+    adapter, bit for bit; the adapter's own rows are not finite where the formula's are not."""
+    ids, lengths, G, H, K, N, r, shared = layout
+    M = sum(lengths)
+    gen = torch.Generator().manual_seed(4)
+    rn = lambda *s: torch.randn(*s, generator=gen).to("cuda", torch.bfloat16)  # noqa: E731
+    x, w = (rn(M, K) if shared else rn(M, H, K)), rn(H, K, N) * 0.1
+    a, b, dy = rn(G, H, r, K) * K ** -0.5, rn(G, H, r, N) * 0.2, rn(M, H, N)
+    batch = AdapterBatch(ids, lengths, G)
+    of = batch.adapter_of_row()
+
+    def run(a, b):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, a, b)]
+        y = adapter_linear(leaves[0], w, leaves[1], leaves[2], batch, 0.7)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    want = run(a, b)
+    bad = (a if where == "a" else b).clone()
+    if where == "one of b":
+        bad[1, H - 1, r - 1, N - 3] = value
+    else:
+        bad[1, H - 1] = value
+    got = run(bad, b) if where == "a" else run(a, bad)
+    other, rest = of != 1, torch.arange(G, device="cuda") != 1
+    assert torch.equal(got[0][other], want[0][other]) and torch.equal(got[1][other], want[1][other])
+    assert torch.equal(got[2][rest], want[2][rest]) and torch.equal(got[3][rest], want[3][rest])
+    assert not got[0][of == 1].isfinite().all()
+    if where == "one of b":  # only its column of y
+        columns = torch.ones(H, N, dtype=torch.bool, device="cuda")
+        columns[H - 1, N - 3] = False
+        assert torch.equal(got[0][:, columns], want[0][:, columns])
+        assert not got[0][of == 1][:, H - 1, N - 3].isfinite().any()
+    else:
+        assert not got[0][of == 1][:, H - 1].isfinite().any()
+
+
+@pytest.mark.gpu
+def test_an_infinite_t_gives_the_formulas_infinity():
+    """Ranks are padded to 16, 32 or 64: what pads them adds nothing to an infinite row, not 0 * inf."""
+    x, w, a, b = make(6, G=1, H=1, K=64, N=64, r=5, dev="cuda", dtype=torch.bfloat16)
+    x, a, b = x.abs(), a.abs(), b.abs()
+    a[0, 0, 4, 0] = float("inf")
+    y = adapter_linear(x, w, a, b, AdapterBatch([0], [6], 1))
+    keep = (x[:, :1] > 0) & (b[0, 0, 4] > 0)
+    assert (y[:, 0][keep] == float("inf")).all()
+
+
+@pytest.mark.gpu
+def test_the_gradient_of_an_unused_adapter_is_zero_whatever_its_scale():
+    x, w, a, b = make(6, G=3, H=1, K=64, N=64, dev="cuda", dtype=torch.bfloat16)
+    scale = torch.tensor([1.0, float("nan"), 2.0], device="cuda")
+    a.requires_grad_(True), b.requires_grad_(True)
+    y = adapter_linear(x, w, a, b, AdapterBatch([0, 2], [2, 4], 3), scale)
+    for g in torch.autograd.grad(y, (a, b), torch.ones_like(y)):
+        assert (g[1] == 0).all() and g.isfinite().all()
