@@ -3,6 +3,7 @@
 //   g' = g c;  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2
 //   p  = p (1 - lr wd) - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps);  shadow = bf16(p)
 //
+// t counts the tensor's own steps: one without a gradient keeps its moments, and its count.
 // The states of all tensors lie in one buffer, each tensor padded to blocks of 256 values;
 // one warp owns one block and `owner[block]` names its tensor. The tensors' addresses are
 // kernel arguments (up to 32 KB of them), so a step is one launch and copies no table.
@@ -25,6 +26,7 @@
 #include <cuda_fp8.h>
 #include <torch/extension.h>
 
+#include <cmath>
 #include <vector>
 
 namespace bd {
@@ -43,6 +45,7 @@ struct ManyTensor {
   long long n;
   int block0;  // first state block
   int flags;
+  float step, inv_bc2;  // lr / (1 - b1^t), 1 / (1 - b2^t)
 };
 
 template <int CAP>
@@ -51,7 +54,7 @@ struct ManyTable {
 };
 
 struct ManyHyper {
-  float step, decay, b1, nb1, b2, nb2, eps, inv_bc2;  // step = lr / (1 - b1^t)
+  float decay, b1, nb1, b2, nb2, eps;
   unsigned key;
   const float* gscale;
 };
@@ -205,7 +208,7 @@ __device__ __forceinline__ void update_block(const ManyTensor& t, const ManyHype
     const float gi = __fmul_rn(g[j], gs);
     m[j] = __fadd_rn(__fmul_rn(m[j], h.b1), __fmul_rn(gi, h.nb1));
     v[j] = __fadd_rn(__fmul_rn(v[j], h.b2), __fmul_rn(__fmul_rn(gi, gi), h.nb2));
-    p[j] = p[j] * h.decay - __fdividef(m[j] * h.step, root(v[j] * h.inv_bc2) + h.eps);
+    p[j] = p[j] * h.decay - __fdividef(m[j] * t.step, root(v[j] * t.inv_bc2) + h.eps);
   }
   store8<WIDE>(t.p, t.flags & kParamBf16, at, lane, n, p);
   if (t.shadow) store8<WIDE>(t.shadow, true, at, lane, n, p);
@@ -277,21 +280,23 @@ void launch(const std::vector<ManyTensor>& all, size_t first, size_t count, cons
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-constexpr int kFew = 64, kMany = 640;  // tensors a launch names: 2.5 KB or 25 KB of arguments
+constexpr int kFew = 64, kMany = 640;  // tensors a launch names: 3 KB or 30 KB of arguments
+static_assert(sizeof(ManyTable<kMany>) + sizeof(ManyHyper) + 128 <= 32764, "arguments of a launch");
 
 }  // namespace
 
 // params / grads / shadows: one entry per tensor (a gradient may be None, shadows may be
 // empty); block0[i]: the first 256-value state block of tensor i, with the total last;
 // owner [total] int32: the tensor of each block. m, v: [total * 256] fp32, or e4m3 with
-// m_scale, v_scale [total] fp32.
+// m_scale, v_scale [total] fp32. steps[i]: tensor i's own steps, this one included.
 void adamw_many(const std::vector<at::Tensor>& params, const std::vector<c10::optional<at::Tensor>>& grads,
                 const std::vector<at::Tensor>& shadows, const std::vector<int64_t>& block0, const at::Tensor& owner,
                 const at::Tensor& m, const at::Tensor& v, const c10::optional<at::Tensor>& m_scale,
                 const c10::optional<at::Tensor>& v_scale, double lr, double b1, double b2, double eps, double wd,
-                double bc1, double bc2, int64_t key, const c10::optional<at::Tensor>& gscale) {
+                const std::vector<int64_t>& steps, int64_t key, const c10::optional<at::Tensor>& gscale) {
   const size_t n = params.size();
-  TORCH_CHECK(n > 0 && grads.size() == n && block0.size() == n + 1, "adamw_many: one gradient and state range per tensor");
+  TORCH_CHECK(n > 0 && grads.size() == n && block0.size() == n + 1 && steps.size() == n,
+              "adamw_many: one gradient, state range and step count per tensor");
   TORCH_CHECK(shadows.empty() || shadows.size() == n, "adamw_many: no shadows or one per tensor");
   const int dev = m.get_device();
   c10::cuda::CUDAGuard guard(dev);
@@ -304,12 +309,14 @@ void adamw_many(const std::vector<at::Tensor>& params, const std::vector<c10::op
   if (eight) TORCH_CHECK(v_scale && m_scale->numel() == total && v_scale->numel() == total, "adamw_many: scale sizes");
   if (gscale) TORCH_CHECK(gscale->scalar_type() == at::kFloat && gscale->get_device() == dev, "adamw_many: gradient scale");
   ManyHyper h;
-  h.step = (float)(lr / bc1), h.decay = (float)(1.0 - lr * wd);
+  h.decay = (float)(1.0 - lr * wd);
   h.b1 = (float)b1, h.nb1 = (float)(1.0 - b1), h.b2 = (float)b2, h.nb2 = (float)(1.0 - b2);
-  h.eps = (float)eps, h.inv_bc2 = (float)(1.0 / bc2);
+  h.eps = (float)eps;
   h.key = (unsigned)key;
   h.gscale = gscale ? gscale->data_ptr<float>() : nullptr;
   std::vector<ManyTensor> all(n);
+  int64_t last = 0;  // of most tensors the same
+  float step = 0.f, inv_bc2 = 0.f;
   for (size_t i = 0; i < n; ++i) {
     ManyTensor& t = all[i];
     const at::Tensor& p = params[i];
@@ -321,7 +328,15 @@ void adamw_many(const std::vector<at::Tensor>& params, const std::vector<c10::op
     t.flags = dtype_of(p, kParamBf16);
     bool w = wide(t.p, t.flags & kParamBf16);
     t.g = nullptr;
+    t.step = t.inv_bc2 = 0.f;
     if (grads[i]) {
+      TORCH_CHECK(steps[i] >= 1, "adamw_many: steps are counted from 1");
+      if (steps[i] != last) {
+        last = steps[i];
+        step = (float)(lr / (1.0 - std::pow(b1, (double)last)));
+        inv_bc2 = (float)(1.0 / (1.0 - std::pow(b2, (double)last)));
+      }
+      t.step = step, t.inv_bc2 = inv_bc2;
       const at::Tensor& g = *grads[i];
       TORCH_CHECK(g.get_device() == dev && g.is_contiguous() && g.numel() == t.n, "adamw_many: a gradient like its tensor");
       t.flags |= dtype_of(g, kGradBf16);

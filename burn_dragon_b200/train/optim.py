@@ -149,9 +149,11 @@ class AdamWMany:
     step of v by a thousandth of itself is kept on average and a run repeats bit for bit.
 
     ``state``: ``m`` and ``v`` (and ``m_scale`` / ``v_scale``), every tensor padded to blocks of 256
-    values in the order of ``params``. A tensor whose gradient is None is left alone. The step
-    count and the learning rate are arguments of the launch, so a captured CUDA graph would
-    repeat one step; ``FusedAdamW`` keeps them on the device for that."""
+    values in the order of ``params``. A tensor whose gradient is None is left alone, and its moments are
+    corrected for the steps that it has had itself (``steps``), not for those of the others (``t``): an adapter
+    that joins late or is trained rarely moves as it would alone. The step counts and the learning rate are
+    arguments of the launch, so a captured CUDA graph would repeat one step; ``FusedAdamW`` keeps
+    them on the device for that."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.1,
                  state_bits: int = 32, shadows=None, seed: int = 0):
@@ -172,6 +174,7 @@ class AdamWMany:
                 raise ValueError("a shadow is a contiguous bf16 tensor of its tensor's size")
         self.lr, (self.b1, self.b2), self.eps, self.wd = lr, betas, eps, weight_decay
         self.state_bits, self.seed, self.t = state_bits, int(seed), 0
+        self.steps = [0] * len(self.params)
         sizes = [-(-p.numel() // BLOCK) for p in self.params]
         self.block0 = [0]
         for n in sizes:
@@ -185,14 +188,19 @@ class AdamWMany:
             self.state |= {k: torch.zeros(total, device=dev) for k in ("m_scale", "v_scale")}
 
     def state_dict(self) -> dict:
-        return {**self.state, "t": self.t, "lr": self.lr, "seed": self.seed}
+        return {**self.state, "t": self.t, "steps": list(self.steps), "lr": self.lr, "seed": self.seed}
 
     def load_state_dict(self, sd: dict) -> None:
+        """A state without ``steps``: every tensor has had all ``t`` steps."""
         for k, t in self.state.items():
             if sd[k].dtype != t.dtype or sd[k].shape != t.shape:
                 raise ValueError(f"state {k!r} is {tuple(sd[k].shape)} {sd[k].dtype}, not {tuple(t.shape)} {t.dtype}")
+        steps = [int(n) for n in sd.get("steps", [sd["t"]] * len(self.params))]
+        if len(steps) != len(self.params):
+            raise ValueError(f"{len(steps)} step counts for {len(self.params)} tensors")
+        for k, t in self.state.items():
             t.copy_(sd[k])
-        self.t = int(sd["t"])
+        self.t, self.steps = int(sd["t"]), steps
         self.seed = int(sd.get("seed", self.seed))
 
     def moments(self, i: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -215,21 +223,21 @@ class AdamWMany:
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} tensors")
         t = self.t + 1
         lr = self.lr if lr is None else lr
-        bc1, bc2 = 1.0 - self.b1 ** t, 1.0 - self.b2 ** t
+        steps = [n if g is None else n + 1 for n, g in zip(self.steps, grads)]
         key = (self.seed * 0x9E3779B1 + t * 0x85EBCA77) & 0xFFFFFFFF
         if self.state["m"].is_cuda:
             grads = [g if g is None or g.is_contiguous() else g.contiguous() for g in grads]
             _ext.load().adamw_many(self.params, grads, self.shadows, self.block0, self.owner, self.state["m"],
                                    self.state["v"], self.state.get("m_scale"), self.state.get("v_scale"), lr, self.b1,
-                                   self.b2, self.eps, self.wd, bc1, bc2, key, grad_scale)
+                                   self.b2, self.eps, self.wd, steps, key, grad_scale)
         else:
             for p, g in zip(self.params, grads):
                 if g is not None and g.numel() != p.numel():
                     raise ValueError("a gradient has its tensor's size")
             for i, (p, g) in enumerate(zip(self.params, grads)):
                 if g is not None:
-                    self._step_cpu(i, p, g, lr, bc1, bc2, key, grad_scale)
-        self.t = t
+                    self._step_cpu(i, p, g, lr, 1.0 - self.b1 ** steps[i], 1.0 - self.b2 ** steps[i], key, grad_scale)
+        self.t, self.steps = t, steps
 
     def _step_cpu(self, i, p, g, lr, bc1, bc2, key, grad_scale) -> None:
         blocks = slice(self.block0[i], self.block0[i + 1])
