@@ -2,7 +2,9 @@
 
 Where a random scaffold (``models.scaffold``) trains one adapter per model, an ``AdapterBank`` keeps G of
 them for the three shared projections, W = W_frozen + s A_g^T B_g with s = alpha / r or alpha / sqrt(r), and
-a batch may name another adapter for every sequence. ``AdapterBDH`` is the BDH forward with the three
+a batch may name another adapter for every sequence. ``load_scaffold`` takes adapters over from scaffold models
+of one seed, W = gain_g W_seed + s_g A_g^T B_g with the scaling and the gains that they were trained with; the
+embedding, the head and the norms are those of the model that ``AdapterBDH`` is given. ``AdapterBDH`` is the BDH forward with the three
 projections through ``ops.adapters.adapter_linear`` (bf16 operands on CUDA, the plain form on CPU);
 norms, RoPE and the linear attention are ``models.reference``'s. ``train_step`` updates the adapters of
 the batch with ``AdamWMany``; ``generate`` serves requests of different lengths, adapters and sampling
@@ -19,7 +21,9 @@ from ..ops.adapters import AdapterBatch, adapter_linear
 from ..ops.sampling import sample_tokens
 from ..train.optim import AdamWMany
 from . import reference as R
+from .bdh import SCAFFOLD_RECORD
 from .generate import feed, hold
+from .scaffold import PATHS, scaffold_tensor_cpu
 from .state import ModelState
 
 PROJECTIONS = ("encoder", "encoder_v", "decoder")
@@ -42,6 +46,10 @@ class AdapterBank:
         self.cfg, self.n_adapters, self.rank = cfg, n_adapters, rank
         self.scale = alpha / rank if scaling == "standard" else alpha / math.sqrt(rank)
         gen = torch.Generator().manual_seed(seed)
+        # of adapters from a scaffold, per projection [G]: s / gain (None while all are the bank's own) and the gain of
+        # W_seed (None while all are 1)
+        self.scales, self.gain = None, None
+        self.scaffold = None  # what W_seed was made from, where it is known
         self.master, self.work = {}, {}
         for name, shape in bank_shapes(cfg, rank).items():
             t = torch.zeros(n_adapters, *shape)
@@ -51,13 +59,64 @@ class AdapterBank:
             cuda = self.master[name].is_cuda
             self.work[name] = self.master[name].bfloat16() if cuda else self.master[name]
 
-    def load_scaffold(self, g: int, tensors: dict[str, torch.Tensor]) -> None:
-        """Adapter ``g`` from a random-scaffold model's ``<projection>.a`` [.., in, r] / ``.b`` [.., r, out]."""
+    def load_scaffold(self, g: int, source, scale: float | None = None) -> None:
+        """Adapter ``g`` from a random-scaffold model, or from the tensors of one by their names in its
+        ``state_dict`` (``encoder_a``), in its record (``random_scaffold_adapters.fast.encoder.a``) or
+        ``encoder.a``: a [.., in, r], b [.., r, out] and the trained gain. A model brings its scaling along; for
+        tensors it is ``scale``, or that of the bank's configuration if that is a scaffold's, else the bank's own.
+        ``AdapterBDH`` then takes W_seed, without the model's own adapter, for the frozen projections."""
+        cfg = self.cfg
+        if isinstance(source, torch.nn.Module):
+            if not getattr(source, "scaffold", False):
+                raise ValueError("load_scaffold takes a random-scaffold model or its tensors")
+            cfg = source.cfg
+            with torch.no_grad():
+                source = {f"{n}.{k}": t.detach() for n in PROJECTIONS for k, t in zip(("a", "b", "gain"), source._scaffold_parts(n))}
+            scale = cfg.random_scaffold.adapter_scale()
+        rs = cfg.random_scaffold
+        if scale is None:
+            scale = rs.adapter_scale() if rs.enabled else self.scale
+        made = (rs.seed, rs.distribution, cfg.init_std) if rs.enabled else None
+        if made and self.scaffold and made != self.scaffold:
+            raise ValueError(f"adapters of one bank share W_seed: {made} is not {self.scaffold} (seed, distribution, std)")
+
+        def tensor(name: str):
+            proj, part = name.split(".")
+            for key in (name, f"{proj}_{part}", f"{SCAFFOLD_RECORD}.{name}"):
+                if key in source:
+                    return source[key].detach()
+            return None
+
+        values, gains = {}, {}
         for name, t in self.master.items():
-            src = tensors[name]
-            t[g].copy_(src.transpose(-1, -2) if name.endswith(".a") else src)
+            v = tensor(name)
+            if v is None:
+                raise KeyError(f"no {name!r} among the scaffold's tensors")
+            v = v.transpose(-1, -2) if name.endswith(".a") else v
+            if v.shape != t.shape[1:]:
+                raise ValueError(f"{name} is {tuple(v.shape)}, the bank's adapters are {tuple(t.shape[1:])}")
+            values[name] = v
+        for proj in PROJECTIONS:
+            v = tensor(proj + ".gain")
+            gains[proj] = 1.0 if v is None else float(v)
+            if gains[proj] == 0.0 or not math.isfinite(gains[proj]):
+                raise ValueError(f"{proj}: a gain of {gains[proj]} cannot be served beside others")
+        like = self.master["encoder.a"]
+        if self.scales is None:
+            self.scales = {n: like.new_full((self.n_adapters,), self.scale) for n in PROJECTIONS}
+        if self.gain is None and any(gain != 1.0 for gain in gains.values()):
+            self.gain = {n: like.new_ones(self.n_adapters) for n in PROJECTIONS}
+        for name, v in values.items():
+            t = self.master[name]
+            t[g].copy_(v)
             if self.work[name] is not t:
                 self.work[name][g].copy_(t[g])
+        for proj, gain in gains.items():
+            # y = gain x W_seed + s t b, as the operator computes it: x' W + (s / gain) t' b with x' = gain x
+            self.scales[proj][g] = scale / gain
+            if self.gain is not None:
+                self.gain[proj][g] = gain
+        self.scaffold = self.scaffold or made
 
     def tensors(self, which: dict[str, torch.Tensor]) -> list[torch.Tensor]:
         """Every adapter's own matrices, adapter by adapter."""
@@ -78,25 +137,52 @@ class AdapterBDH:
             p = {k: None if v is None else v.detach() for k, v in model.param_dict().items()}
         dev = p["embed"].device
         self.p, self.dtype = p, torch.bfloat16 if dev.type == "cuda" else torch.float32
-        self.weights = {n: p[n].to(self.dtype).contiguous() for n in PROJECTIONS}
+        self.model = model
+        self._freeze()
         self.norm = R.make_norm(cfg.norm_kind, p["norm_gamma"], p["norm_beta"], cfg.norm_eps, p.get("norm_alpha"),
                                 p.get("norm_shift"))
         make = {"rope": R.rope_freqs, "pope": R.pope_freqs}.get(cfg.rotary_embedding)
         self.freqs = None if make is None else make(cfg.latent_per_head, cfg.rope_theta, device=dev)
         self.decay = R.decay_vector(cfg.decay_slopes(), device=dev) if cfg.uses_decay() else None
 
+    @torch.no_grad()
+    def _freeze(self) -> None:
+        """The frozen projections: the model's, or for a scaffold's adapters what they were trained beside."""
+        model, bank = self.model, self.bank
+        self.on_scaffold = bank.scales is not None
+        frozen = {n: self.p[n] for n in PROJECTIONS}
+        if self.on_scaffold and getattr(model, "scaffold", False):
+            frozen = {n: model.scaffold_base(n) for n in PROJECTIONS}
+        if bank.scaffold is not None:
+            seed, distribution, std = bank.scaffold
+            for n in PROJECTIONS:
+                some = min(4096, frozen[n].numel())
+                want = scaffold_tensor_cpu(seed, PATHS[n], (some,), std, distribution)
+                if not torch.allclose(frozen[n].reshape(-1)[:some].float().cpu(), want, rtol=1e-4, atol=1e-4 * std):
+                    raise ValueError(f"{n} is not the W_seed of the scaffold that the adapters were trained on")
+        self.weights = {n: frozen[n].to(self.dtype).contiguous() for n in PROJECTIONS}
+
     def batch(self, adapters, length: int) -> AdapterBatch:
         """The plan of ``len(adapters)`` sequences of ``length`` tokens."""
         return AdapterBatch(adapters, [length] * len(adapters), self.bank.n_adapters, device=self.p["embed"].device)
 
-    def _linear(self, name: str, x: torch.Tensor, batch: AdapterBatch, work) -> torch.Tensor:
+    def _linear(self, name: str, x: torch.Tensor, batch: AdapterBatch, work, gains) -> torch.Tensor:
+        scale = self.bank.scales[name] if self.on_scaffold else self.bank.scale
+        if gains is not None:
+            x = x * gains[name].view(-1, *[1] * (x.dim() - 1))
         return adapter_linear(x.to(self.dtype), self.weights[name], work[name + ".a"], work[name + ".b"], batch,
-                              self.bank.scale).float()
+                              scale).float()
 
     def forward(self, tokens: torch.Tensor, batch: AdapterBatch, state: ModelState | None = None, work=None):
         """Logits [B, T, V] of tokens [B, T], row b T + t of the batch being token t of sequence b."""
-        cfg, work = self.cfg, work or self.bank.work
+        cfg, work, bank = self.cfg, work or self.bank.work, self.bank
         B, T = tokens.shape
+        if self.on_scaffold != (bank.scales is not None):  # the bank's first adapter from a scaffold came later
+            self._freeze()
+        gains = None
+        if bank.gain is not None:
+            of = batch.adapter_of_row()
+            gains = {n: torch.where(of < 0, 1.0, bank.gain[n][of.clamp_min(0)]) for n in PROJECTIONS}
         D, H, Nh = cfg.n_embd, cfg.n_head, cfg.latent_per_head
         pos = state.position if state is not None else 0
         thr, thr_y = cfg.thresholds()
@@ -106,15 +192,15 @@ class AdapterBDH:
         v = self.norm(self.p["embed"][tokens])
         rhos = []
         for layer in range(cfg.n_layer):
-            x = torch.relu(self._linear("encoder", v.reshape(B * T, D), batch, work) - thr)  # [B T, H, Nh]
+            x = torch.relu(self._linear("encoder", v.reshape(B * T, D), batch, work, gains) - thr)  # [B T, H, Nh]
             q = x.view(B, T, H, Nh).transpose(1, 2)
             if phases is not None:
                 q = R.pope_apply(q, phases) if cfg.rotary_embedding == "pope" else R.rope_apply(q, phases)
             rho0 = state.rhos[layer] if state is not None and state.rhos is not None else None
             a, rho = R.linear_attention_chunked(q, v[:, None], rho0=rho0, decay=self.decay, need_state=state is not None)
             a = self.norm(a).transpose(1, 2).reshape(B * T, H, D)
-            y = torch.relu(self._linear("encoder_v", a, batch, work) - thr_y)
-            m = self._linear("decoder", (x * y).reshape(B * T, H * Nh), batch, work)
+            y = torch.relu(self._linear("encoder_v", a, batch, work, gains) - thr_y)
+            m = self._linear("decoder", (x * y).reshape(B * T, H * Nh), batch, work, gains)
             v = self.norm(v + self.norm(m).view(B, T, D))
             rhos.append(rho)
         if state is not None:
