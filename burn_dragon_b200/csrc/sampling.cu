@@ -40,6 +40,8 @@
 #include <cuda_bf16.h>
 #include <torch/extension.h>
 
+#include <cfloat>
+
 namespace bd {
 namespace {
 
@@ -788,7 +790,7 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
   }
   Row r;
   r.top = top;
-  r.inv_t = __fdiv_rn(1.f, temperature);
+  r.inv_t = __fdiv_rn(1.f, fminf(temperature, FLT_MAX));  // never 0, which would make a weight of -inf * 0
   r.per_bucket = r.inv_t * 32.f;
   const bool use_k = k > 0 && k < a.V, use_p = p < 1.f;
 

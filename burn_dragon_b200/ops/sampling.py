@@ -4,7 +4,8 @@
 repeated, and returns its log-probability under the distribution it was drawn from (what the
 policy-gradient objectives need). In the order "value descending, index ascending":
 
-1. ``temperature`` T: weights exp((l - max) / T); T <= 0 answers the first maximum, log-probability 0;
+1. ``temperature`` T: weights exp((l - max) / T); T <= 0 answers the first maximum, log-probability 0, and +inf
+   counts as the largest fp32 number (every token that is not masked by -inf is as likely as another);
 2. ``top_k`` k > 0: the first k;
 3. ``top_p`` p < 1: of those, the shortest prefix whose share reaches p (the first token at least);
 4. ``min_p``: those whose weight is at least min_p times the largest;
@@ -75,7 +76,7 @@ def sample_tokens_ref(logits, u, temperature, top_k, top_p, min_p):
     B, V = l.shape
     l = torch.where(l.isnan(), float("-inf"), l)
     top = l.amax(1, keepdim=True)
-    z = torch.where(l == top, 0.0, (l - top) * (1.0 / temperature[:, None]))
+    z = torch.where(l == top, 0.0, (l - top) * (1.0 / temperature[:, None].clamp_max(torch.finfo(torch.float32).max)))
     w = torch.where(l == float("-inf"), 0.0, z.exp())
     W = (w * _ONE).to(torch.int64)
     order = l.sort(dim=1, descending=True, stable=True).indices
