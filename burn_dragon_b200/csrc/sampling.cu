@@ -110,7 +110,8 @@ __device__ __forceinline__ u64 fixed40(float w) {  // floor(w 2^40) for 0 <= w <
 // floored at 2^-40 by adding 1.5 * 2^-17 rounded down; both sums leave their bits in the low mantissa. Six
 // single-rate instructions a value against about twenty for 64-bit shifts and adds.
 struct WeightSum {
-  unsigned high = 0, low = 0, n = 0;  // at most 2^14 values
+  // At most 511 values: each puts a signed rest of up to 2^22 units into the 32 bits of `low`.
+  unsigned high = 0, low = 0, n = 0;
   __device__ __forceinline__ void add(float w) {
     const float t = __fadd_rn(w, 96.f);
     const float rest = __fsub_rn(w, __fsub_rn(t, 96.f));
@@ -121,6 +122,9 @@ struct WeightSum {
     return ((u64)(high - n * 0x42c00000u) << 23) + (u64)(long long)(int)(low - n * 0x37400000u);
   }
 };
+
+// A thread sums its share of a slice (a warp's run is a whole number of 256 values), twice where values equal the border.
+static_assert(2 * (kMaxSlice / kThreads) < 512, "WeightSum holds a thread's values");
 
 struct Row {
   float top, inv_t, per_bucket;

@@ -54,3 +54,30 @@ def test_hard_rows_at_an_infinite_temperature(V, k, p, low):
     u = torch.rand(len(names), generator=torch.Generator().manual_seed(V))
     full = [torch.full((len(names),), v, device="cuda") for v in (INF, k, p, low)]
     same(sample_tokens(logits.cuda(), u.cuda(), INF, k, p, low), sample_tokens_ref(logits.cuda(), u.cuda(), *full), names)
+
+
+def long_rows(V):
+    """hard_rows, and rows whose border lies among equal or nearly equal weights."""
+    names, logits = hard_rows(V)
+    more = {
+        "two values": torch.arange(V).remainder(2).float() * 1e-6,
+        "one heavy value": torch.zeros(V).index_fill(0, torch.tensor([V // 2]), 12.0),
+        "a geometric fall": -torch.arange(V).float() * 1e-2,
+        "equal but for the last bits": torch.full((V,), 2.0).add(torch.arange(V).remainder(3).float() * 2.0 ** -22),
+        "a plateau below a few": torch.zeros(V).index_fill(0, torch.arange(0, V, 997), 3.0),
+    }
+    return names + list(more), torch.cat((logits, torch.stack(list(more.values()))))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [70001, 131073, 262144])  # slices of more than 8192 values: windows from a sample
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t,k,p,low", [(1.0, 0, 0.3, 0.0), (0.7, 0, 0.95, 0.0), (1.0, 0, 0.0, 0.0), (1e-3, 0, 0.5, 0.0),
+                                       (1e30, 0, 0.5, 0.0), (1.0, 300, 0.6, 0.0), (1.0, 2000, 1.0, 0.0), (1.0, 0, 0.9, 0.4),
+                                       (INF, 0, 0.7, 0.0)])
+def test_hard_rows_of_long_vocabularies(V, dtype, t, k, p, low):
+    names, logits = long_rows(V)
+    logits = logits.to(dtype).cuda()
+    u = torch.rand(len(names), generator=torch.Generator().manual_seed(V)).cuda()
+    full = [torch.full((len(names),), v, device="cuda") for v in (t, k, p, low)]
+    same(sample_tokens(logits, u, t, k, p, low), sample_tokens_ref(logits, u, *full), names)
