@@ -155,11 +155,15 @@ __device__ __forceinline__ void store_codes(unsigned char* s, int lane, const un
   }
 }
 
-// p's own update needs no correctly rounded root and quotient (2^-22 of a step of lr); the states do not use them.
-__device__ __forceinline__ float root(float x) {
+// m / (sqrt(v) + eps). Beside 8-bit states, whose own rounding is 2^-4 and which the instructions bound (102 us
+// with the correctly rounded forms, 90 without), root and quotient are good to 2^-22 of the step; the states do not use
+// them. With 32-bit states the bytes bound the step, and both are rounded correctly.
+template <bool EIGHT>
+__device__ __forceinline__ float ratio(float m, float v, float eps) {
+  if constexpr (!EIGHT) return __fdiv_rn(m, __fadd_rn(__fsqrt_rn(v), eps));
   float r;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return __fdividef(m, r + eps);
 }
 
 // absmax over the warp's block as bits: NaN and infinity win, as they have to
@@ -208,7 +212,7 @@ __device__ __forceinline__ void update_block(const ManyTensor& t, const ManyHype
     const float gi = __fmul_rn(g[j], gs);
     m[j] = __fadd_rn(__fmul_rn(m[j], h.b1), __fmul_rn(gi, h.nb1));
     v[j] = __fadd_rn(__fmul_rn(v[j], h.b2), __fmul_rn(__fmul_rn(gi, gi), h.nb2));
-    p[j] = p[j] * h.decay - __fdividef(m[j] * t.step, root(v[j] * t.inv_bc2) + h.eps);
+    p[j] = p[j] * h.decay - ratio<EIGHT>(m[j] * t.step, v[j] * t.inv_bc2, h.eps);
   }
   store8<WIDE>(t.p, t.flags & kParamBf16, at, lane, n, p);
   if (t.shadow) store8<WIDE>(t.shadow, true, at, lane, n, p);

@@ -1,4 +1,5 @@
-"""AdamWMany where tensors have had different numbers of steps: each is corrected for its own, as torch.optim.AdamW does."""
+"""AdamWMany where tensors have had different numbers of steps: each is corrected for its own, as torch.optim.AdamW does.
+And the rounding of its update."""
 
 import pytest
 import torch
@@ -145,3 +146,15 @@ def test_an_adapter_trains_as_it_would_alone():
         moved.append({n: t[1].clone() for n, t in net.bank.master.items()})
     for n in moved[0]:
         assert torch.equal(moved[0][n], moved[1][n])
+
+
+@pytest.mark.gpu
+def test_a_step_in_32_bits_rounds_root_and_quotient_correctly():
+    """From p = 0 the step is -(m lr / bc1) / (sqrt(v / bc2) + eps), operation by operation in fp32."""
+    p, g = torch.zeros(70001, device="cuda"), gradient(70001, 3, "cuda")
+    opt = AdamWMany([p], lr=LR, weight_decay=0.1)
+    opt.step([g])
+    m, v = opt.moments(0)
+    f32 = lambda x: torch.tensor(x, dtype=torch.float32, device="cuda")  # noqa: E731
+    want = (m * f32(LR / (1 - 0.9))) / ((v * f32(1 / (1 - 0.999))).sqrt() + f32(1e-8))
+    assert torch.equal(p, -want)
