@@ -292,15 +292,18 @@ static_assert(sizeof(ManyTable<kMany>) + sizeof(ManyHyper) + 128 <= 32764, "argu
 // params / grads / shadows: one entry per tensor (a gradient may be None, shadows may be
 // empty); block0[i]: the first 256-value state block of tensor i, with the total last;
 // owner [total] int32: the tensor of each block. m, v: [total * 256] fp32, or e4m3 with
-// m_scale, v_scale [total] fp32. steps[i]: tensor i's own steps, this one included.
+// m_scale, v_scale [total] fp32. steps [n] int64 on the host: each tensor's own steps so far; those of the
+// tensors with a gradient are advanced.
 void adamw_many(const std::vector<at::Tensor>& params, const std::vector<c10::optional<at::Tensor>>& grads,
                 const std::vector<at::Tensor>& shadows, const std::vector<int64_t>& block0, const at::Tensor& owner,
                 const at::Tensor& m, const at::Tensor& v, const c10::optional<at::Tensor>& m_scale,
                 const c10::optional<at::Tensor>& v_scale, double lr, double b1, double b2, double eps, double wd,
-                const std::vector<int64_t>& steps, int64_t key, const c10::optional<at::Tensor>& gscale) {
+                const at::Tensor& steps, int64_t key, const c10::optional<at::Tensor>& gscale) {
   const size_t n = params.size();
-  TORCH_CHECK(n > 0 && grads.size() == n && block0.size() == n + 1 && steps.size() == n,
-              "adamw_many: one gradient, state range and step count per tensor");
+  TORCH_CHECK(n > 0 && grads.size() == n && block0.size() == n + 1, "adamw_many: one gradient and state range per tensor");
+  TORCH_CHECK(steps.device().is_cpu() && steps.scalar_type() == at::kLong && steps.is_contiguous() && steps.numel() == (int64_t)n,
+              "adamw_many: one step count per tensor, on the host");
+  int64_t* had = steps.data_ptr<int64_t>();
   TORCH_CHECK(shadows.empty() || shadows.size() == n, "adamw_many: no shadows or one per tensor");
   const int dev = m.get_device();
   c10::cuda::CUDAGuard guard(dev);
@@ -334,9 +337,9 @@ void adamw_many(const std::vector<at::Tensor>& params, const std::vector<c10::op
     t.g = nullptr;
     t.step = t.inv_bc2 = 0.f;
     if (grads[i]) {
-      TORCH_CHECK(steps[i] >= 1, "adamw_many: steps are counted from 1");
-      if (steps[i] != last) {
-        last = steps[i];
+      TORCH_CHECK(had[i] >= 0, "adamw_many: step counts below 0");
+      if (had[i] + 1 != last) {
+        last = had[i] + 1;
         step = (float)(lr / (1.0 - std::pow(b1, (double)last)));
         inv_bc2 = (float)(1.0 / (1.0 - std::pow(b2, (double)last)));
       }
@@ -370,6 +373,7 @@ void adamw_many(const std::vector<at::Tensor>& params, const std::vector<c10::op
     }
     i += count;
   }
+  for (size_t i = 0; i < n; ++i) had[i] += grads[i].has_value();
 }
 
 }  // namespace bd

@@ -133,7 +133,7 @@ void adamw_many(const std::vector<at::Tensor>& params, const std::vector<c10::op
                 const std::vector<at::Tensor>& shadows, const std::vector<int64_t>& block0, const at::Tensor& owner,
                 const at::Tensor& m, const at::Tensor& v, const c10::optional<at::Tensor>& m_scale,
                 const c10::optional<at::Tensor>& v_scale, double lr, double b1, double b2, double eps, double wd,
-                const std::vector<int64_t>& steps, int64_t key, const c10::optional<at::Tensor>& gscale);
+                const at::Tensor& steps, int64_t key, const c10::optional<at::Tensor>& gscale);
 }  // namespace bd
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {

@@ -174,7 +174,7 @@ class AdamWMany:
                 raise ValueError("a shadow is a contiguous bf16 tensor of its tensor's size")
         self.lr, (self.b1, self.b2), self.eps, self.wd = lr, betas, eps, weight_decay
         self.state_bits, self.seed, self.t = state_bits, int(seed), 0
-        self.steps = [0] * len(self.params)
+        self._steps = torch.zeros(len(self.params), dtype=torch.int64)  # on the host; the launch reads and advances it
         sizes = [-(-p.numel() // BLOCK) for p in self.params]
         self.block0 = [0]
         for n in sizes:
@@ -187,8 +187,13 @@ class AdamWMany:
         if state_bits == 8:
             self.state |= {k: torch.zeros(total, device=dev) for k in ("m_scale", "v_scale")}
 
+    @property
+    def steps(self) -> list[int]:
+        """The steps that each tensor has had."""
+        return self._steps.tolist()
+
     def state_dict(self) -> dict:
-        return {**self.state, "t": self.t, "steps": list(self.steps), "lr": self.lr, "seed": self.seed}
+        return {**self.state, "t": self.t, "steps": self.steps, "lr": self.lr, "seed": self.seed}
 
     def load_state_dict(self, sd: dict) -> None:
         """A state without ``steps``: every tensor has had all ``t`` steps."""
@@ -200,7 +205,8 @@ class AdamWMany:
             raise ValueError(f"{len(steps)} step counts for {len(self.params)} tensors")
         for k, t in self.state.items():
             t.copy_(sd[k])
-        self.t, self.steps = int(sd["t"]), steps
+        self.t = int(sd["t"])
+        self._steps.copy_(torch.tensor(steps))
         self.seed = int(sd.get("seed", self.seed))
 
     def moments(self, i: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -223,21 +229,22 @@ class AdamWMany:
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} tensors")
         t = self.t + 1
         lr = self.lr if lr is None else lr
-        steps = [n if g is None else n + 1 for n, g in zip(self.steps, grads)]
         key = (self.seed * 0x9E3779B1 + t * 0x85EBCA77) & 0xFFFFFFFF
         if self.state["m"].is_cuda:
             grads = [g if g is None or g.is_contiguous() else g.contiguous() for g in grads]
             _ext.load().adamw_many(self.params, grads, self.shadows, self.block0, self.owner, self.state["m"],
                                    self.state["v"], self.state.get("m_scale"), self.state.get("v_scale"), lr, self.b1,
-                                   self.b2, self.eps, self.wd, steps, key, grad_scale)
+                                   self.b2, self.eps, self.wd, self._steps, key, grad_scale)
         else:
             for p, g in zip(self.params, grads):
                 if g is not None and g.numel() != p.numel():
                     raise ValueError("a gradient has its tensor's size")
             for i, (p, g) in enumerate(zip(self.params, grads)):
                 if g is not None:
-                    self._step_cpu(i, p, g, lr, 1.0 - self.b1 ** steps[i], 1.0 - self.b2 ** steps[i], key, grad_scale)
-        self.t, self.steps = t, steps
+                    n = int(self._steps[i]) + 1
+                    self._step_cpu(i, p, g, lr, 1.0 - self.b1 ** n, 1.0 - self.b2 ** n, key, grad_scale)
+                    self._steps[i] = n
+        self.t = t
 
     def _step_cpu(self, i, p, g, lr, bc1, bc2, key, grad_scale) -> None:
         blocks = slice(self.block0[i], self.block0[i + 1])
