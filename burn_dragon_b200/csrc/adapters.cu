@@ -1133,6 +1133,7 @@ std::vector<at::Tensor> adapter_forward(const at::Tensor& x, const at::Tensor& w
 namespace {
 bool direct(const at::Tensor& t, int dev, int64_t inner) {
   if (!t.is_cuda() || t.get_device() != dev || t.scalar_type() != at::kBFloat16 || t.requires_grad()) return false;
+  if (t._fw_grad(0).defined()) return false;  // a forward-mode tangent: refused, not dropped
   if (t.stride(-1) != 1 || t.size(-1) != inner || inner % 8 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
   for (int64_t i = 0; i + 1 < t.dim(); ++i)
     if (t.stride(i) % 8 || t.stride(i) <= 0) return false;
@@ -1156,7 +1157,7 @@ c10::optional<at::Tensor> adapter_direct(const at::Tensor& x, const at::Tensor& 
   if (b.size(0) != G || b.size(-2) != r || (heads && (a.size(1) != H || b.size(1) != H || (x.dim() == 3 && x.size(1) != H))))
     return c10::nullopt;
   if (scale && (!scale->is_cuda() || scale->get_device() != dev || scale->scalar_type() != at::kFloat || scale->dim() != 1 ||
-                scale->size(0) != G || !scale->is_contiguous()))
+                scale->size(0) != G || !scale->is_contiguous() || scale->requires_grad() || scale->_fw_grad(0).defined()))
     return c10::nullopt;
   if (heads) return adapter_forward(x, w, a, b, plan, dims, scale, scale0, err)[0];
   return adapter_forward(x, w.unsqueeze(0), a.unsqueeze(1), b.unsqueeze(1), plan, dims, scale, scale0, err)[0].view(

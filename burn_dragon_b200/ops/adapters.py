@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import numpy as np
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from .. import _ext
 from .gemm import error_word
@@ -123,8 +124,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 def adapter_linear(x: torch.Tensor, weight: torch.Tensor, a: torch.Tensor, b: torch.Tensor, batch: AdapterBatch,
                    scale=1.0) -> torch.Tensor:
-    """See the module. ``scale``: a number, or an fp32 tensor of one per adapter (a constant: no
-    gradient). On CUDA all operands are bf16, K and N multiples of 8, r <= 64; sums are fp32. Tensors
+    """See the module. ``scale``: a number, or an fp32 tensor of one per adapter (on CUDA a constant: one that
+    wants a gradient is refused, and so are forward-mode tangents). On CUDA all operands are bf16, K and N multiples of 8, r <= 64; sums are fp32. Tensors
     that are not laid out in aligned rows are copied first."""
     if x.is_cuda:
         tensor = isinstance(scale, torch.Tensor)
@@ -160,8 +161,13 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, a: torch.Tensor, b: to
         raise TypeError("adapter_linear takes bf16 tensors on CUDA")
     if K % 8 or N % 8 or not 1 <= r <= MAX_RANK:
         raise ValueError(f"adapter_linear takes K and N in multiples of 8 and a rank of 1 to {MAX_RANK}, got K={K} N={N} r={r}")
+    tensors = (x, weight, a, b, scale) if isinstance(scale, torch.Tensor) else (x, weight, a, b)
+    if any(unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("adapter_linear has no forward-mode derivative on CUDA")
     per, scale0 = None, 1.0
     if isinstance(scale, torch.Tensor):
+        if scale.requires_grad and torch.is_grad_enabled():
+            raise ValueError("scale is a constant: adapter_linear has no gradient for it on CUDA")
         per = scale if scale.shape == (G,) else scale.expand(G)
         per = per.to(x.device, torch.float32).contiguous()
     else:

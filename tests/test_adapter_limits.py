@@ -105,3 +105,27 @@ def test_the_gradient_of_an_unused_adapter_is_zero_whatever_its_scale():
     y = adapter_linear(x, w, a, b, AdapterBatch([0, 2], [2, 4], 3), scale)
     for g in torch.autograd.grad(y, (a, b), torch.ones_like(y)):
         assert (g[1] == 0).all() and g.isfinite().all()
+
+
+@pytest.mark.gpu
+def test_derivatives_that_the_kernels_do_not_have_are_refused():
+    """A tangent or a gradient of the scale must not disappear."""
+    import torch.autograd.forward_ad as fwd
+
+    x, w, a, b = make(5, dev="cuda", dtype=torch.bfloat16)
+    batch = AdapterBatch([0, 1], [2, 3], 2)
+    scale = torch.ones(2, device="cuda")
+    with fwd.dual_level():
+        for i in range(4):
+            args = [x, w, a, b]
+            args[i] = fwd.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                adapter_linear(*args, batch, scale)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            adapter_linear(x, w, a, b, batch, fwd.make_dual(scale, scale))
+        adapter_linear(x, w, a, b, batch, scale)
+    scale.requires_grad_(True)
+    with pytest.raises(ValueError, match="scale is a constant"):
+        adapter_linear(x, w, a, b, batch, scale)
+    with torch.no_grad():
+        adapter_linear(x, w, a, b, batch, scale)
