@@ -1,8 +1,9 @@
 """Next-token sampling with each request's own settings (``csrc/sampling.cu``).
 
 ``sample_tokens`` draws one token per row of logits from given uniform numbers, so a run can be
-repeated, and returns its log-probability under the distribution it was drawn from (what the
-policy-gradient objectives need). In the order "value descending, index ascending":
+repeated, and returns its log-probability under the distribution it was drawn from (the behaviour
+policy's, which policy-gradient objectives divide by): a constant, without a graph. The policy's own
+log-probability, with its gradient, is computed from the logits. In the order "value descending, index ascending":
 
 1. ``temperature`` T: weights exp((l - max) / T); T <= 0 answers the first maximum, log-probability 0, and +inf
    counts as the largest fp32 number (every token that is not masked by -inf is as likely as another);
@@ -56,8 +57,9 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     k0 = 0 if k0 is None else int(k0)
     if not logits.is_cuda:
         full = lambda x, x0, dt: torch.full((B,), x0, dtype=dt) if x is None else x  # noqa: E731
-        return sample_tokens_ref(logits, u, full(t, t0, f32), full(k, k0, torch.int32), full(p, p0, f32),
-                                 full(m, m0, f32))
+        with torch.no_grad():  # whole-number sums have no derivative: a graph would lack the normaliser's part
+            return sample_tokens_ref(logits, u, full(t, t0, f32), full(k, k0, torch.int32), full(p, p0, f32),
+                                     full(m, m0, f32))
     if logits.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"sample_tokens takes fp32 or bf16 logits, not {logits.dtype}")
     if V > MAX_VOCAB:

@@ -46,6 +46,14 @@ def test_an_infinite_logit_at_an_infinite_temperature(k, p, dev):
     assert torch.allclose(logprobs.cpu(), torch.full((2,), 0.5).log(), atol=1e-6)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_log_probabilities_are_constants_on_every_device(dev):
+    logits = torch.randn(3, 50, device=dev, requires_grad=True)
+    temperature = torch.ones(3, device=dev, requires_grad=True)
+    tokens, logprobs = sample_tokens(logits, torch.rand(3, device=dev), temperature, 5, 0.9)
+    assert not logprobs.requires_grad and not tokens.requires_grad
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("V", [64, 5000, 33000])
 @pytest.mark.parametrize("k,p,low", [(0, 1.0, 0.0), (0, 0.3, 0.0), (40, 0.6, 0.0), (0, 0.9, 0.5)])
