@@ -93,7 +93,14 @@ def adapter_linear_ref(x, weight, a, b, batch: AdapterBatch, scale=1.0):
             out.append((rows, s[g] * torch.einsum("mhr,hrn->mhn", t, b[g])))
     for rows, d in out:
         y = y.index_add(0, rows, d.to(y.dtype))
-    return y
+    return y if out else _reach(y, a, b)
+
+
+def _reach(y, *inputs):
+    """``y`` with a gradient of zeros for each of ``inputs``: no row reads them."""
+    if not (torch.is_grad_enabled() and any(t.requires_grad for t in inputs)):
+        return y
+    return y + sum(t[:0].sum() for t in inputs).to(y.dtype)
 
 
 class _AdapterLinear(torch.autograd.Function):
@@ -173,7 +180,7 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, a: torch.Tensor, b: to
     else:
         scale0 = float(scale)
     if batch.rows == 0:
-        return x.new_zeros((0, H, N) if heads else (0, N))
+        return _reach(x.new_zeros((0, H, N) if heads else (0, N)), x, a, b)
     x, weight, a, b = _rows(x), _rows(weight), a.contiguous(), b.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad):
         y = _AdapterLinear.apply(x, weight, a, b, batch, per, scale0)

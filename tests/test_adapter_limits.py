@@ -129,3 +129,22 @@ def test_derivatives_that_the_kernels_do_not_have_are_refused():
         adapter_linear(x, w, a, b, batch, scale)
     with torch.no_grad():
         adapter_linear(x, w, a, b, batch, scale)
+
+
+@pytest.mark.parametrize("dev,dtype", [("cpu", torch.float32), pytest.param("cuda", torch.bfloat16, marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("ids,lengths", [([], []), ([0], [0]), ([-1, -1], [2, 1])], ids=("no request", "no rows", "no adapters"))
+@pytest.mark.parametrize("heads", [True, False])
+def test_gradients_where_no_row_has_an_adapter(ids, lengths, heads, dev, dtype):
+    """Zeros for a and b, and an empty gradient of no rows: a training step may hold such a batch."""
+    x, w, a, b = make(sum(lengths), H=1, dev=dev, dtype=dtype)
+    w, a, b = (w, a, b) if heads else (w[0], a[:, 0], b[:, 0])
+    leaves = [t.detach().clone().requires_grad_(True) for t in (x, a, b)]
+    y = adapter_linear(leaves[0], w, leaves[1], leaves[2], AdapterBatch(ids, lengths, 2, device=dev))
+    dx, da, db = torch.autograd.grad(y.sum(), leaves)
+    assert y.shape == ((x.shape[0], 1, 24) if heads else (x.shape[0], 24)) and dx.shape == x.shape
+    assert (da == 0).all() and (db == 0).all() and da.shape == a.shape and db.shape == b.shape
+    if x.shape[0]:
+        want = w.double().sum(-1).expand(x.shape)  # one rounding of the result, fp32 sums
+        assert ((dx.double() - want).abs() <= torch.finfo(dtype).eps * w.double().abs().sum(-1)).all()
+    with torch.no_grad():
+        assert not adapter_linear(*[leaves[0], w, *leaves[1:]], AdapterBatch(ids, lengths, 2, device=dev)).requires_grad
