@@ -181,7 +181,7 @@ def adapter_linear(x: torch.Tensor, weight: torch.Tensor, a: torch.Tensor, b: to
         scale0 = float(scale)
     if batch.rows == 0:
         return _reach(x.new_zeros((0, H, N) if heads else (0, N)), x, a, b)
-    x, weight, a, b = _rows(x), _rows(weight), a.contiguous(), b.contiguous()
+    x, weight, a, b = _rows(x), _rows(weight), _rows(a.contiguous()), _rows(b.contiguous())
     if torch.is_grad_enabled() and (x.requires_grad or a.requires_grad or b.requires_grad):
         y = _AdapterLinear.apply(x, weight, a, b, batch, per, scale0)
     else:

@@ -148,3 +148,21 @@ def test_gradients_where_no_row_has_an_adapter(ids, lengths, heads, dev, dtype):
         assert ((dx.double() - want).abs() <= torch.finfo(dtype).eps * w.double().abs().sum(-1)).all()
     with torch.no_grad():
         assert not adapter_linear(*[leaves[0], w, *leaves[1:]], AdapterBatch(ids, lengths, 2, device=dev)).requires_grad
+
+
+@pytest.mark.gpu
+def test_adapters_at_odd_addresses_and_strides():
+    """a and b that do not start on 16 bytes (parts of one buffer) or are not contiguous are copied, as x is."""
+    x, w, a, b = make(9, G=3, H=2, K=64, N=72, r=5, dev="cuda", dtype=torch.bfloat16)
+    batch = AdapterBatch([2, 0, 1], [4, 3, 2], 3)
+    want = adapter_linear(x, w, a, b, batch, 1.5)
+    whole = torch.cat((x.new_zeros(3), a.flatten(), b.flatten()))
+    oa, ob = whole[3:3 + a.numel()].view(a.shape), whole[3 + a.numel():].view(b.shape)
+    assert oa.data_ptr() % 16 and ob.data_ptr() % 16
+    turned = a.transpose(2, 3).contiguous().transpose(2, 3)
+    for p, q in ((oa, b), (a, ob), (oa, ob), (turned, b)):
+        assert torch.equal(adapter_linear(x, w, p, q, batch, 1.5), want)
+    p, q = oa.detach().requires_grad_(True), ob.detach().requires_grad_(True)
+    y = adapter_linear(x, w, p, q, batch, 1.5)
+    assert torch.equal(y.detach(), want)
+    assert [g.shape for g in torch.autograd.grad(y, (p, q), torch.ones_like(y))] == [a.shape, b.shape]
