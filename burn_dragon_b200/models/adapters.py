@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import math
 
+import numpy as np
 import torch
 
 from ..ops.adapters import AdapterBatch, adapter_linear
@@ -223,6 +224,8 @@ class AdapterBDH:
         ``batch``: the plan of an earlier step with the same adapters. Returns the mean loss."""
         bank = self.bank
         batch = batch or self.batch(adapters, tokens.shape[1])
+        if not np.array_equal(batch._of_row, np.repeat(np.asarray(adapters, dtype=np.int64), tokens.shape[1])):
+            raise ValueError("the batch was planned for other adapters or another length")
         names = list(bank.master)
         work = {n: t.detach().requires_grad_(True) for n, t in bank.work.items()}
         loss = R.cross_entropy(self.forward(tokens, batch, work=work), targets)
