@@ -174,8 +174,10 @@ class AdapterBDH:
         return adapter_linear(x.to(self.dtype), self.weights[name], work[name + ".a"], work[name + ".b"], batch,
                               scale).float()
 
-    def forward(self, tokens: torch.Tensor, batch: AdapterBatch, state: ModelState | None = None, work=None):
-        """Logits [B, T, V] of tokens [B, T], row b T + t of the batch being token t of sequence b."""
+    def forward(self, tokens: torch.Tensor, batch: AdapterBatch, state: ModelState | None = None, work=None,
+                training: bool = False):
+        """Logits [B, T, V] of tokens [B, T], row b T + t of the batch being token t of sequence b.
+        ``training``: with the model's dropout."""
         cfg, work, bank = self.cfg, work or self.bank.work, self.bank
         B, T = tokens.shape
         if self.on_scaffold != (bank.scales is not None):  # the bank's first adapter from a scaffold came later
@@ -201,7 +203,10 @@ class AdapterBDH:
             a, rho = R.linear_attention_chunked(q, v[:, None], rho0=rho0, decay=self.decay, need_state=state is not None)
             a = self.norm(a).transpose(1, 2).reshape(B * T, H, D)
             y = torch.relu(self._linear("encoder_v", a, batch, work, gains) - thr_y)
-            m = self._linear("decoder", (x * y).reshape(B * T, H * Nh), batch, work, gains)
+            yn = x * y
+            if training and cfg.dropout > 0.0:
+                yn = torch.nn.functional.dropout(yn, cfg.dropout)
+            m = self._linear("decoder", yn.reshape(B * T, H * Nh), batch, work, gains)
             v = self.norm(v + self.norm(m).view(B, T, D))
             rhos.append(rho)
         if state is not None:
@@ -220,7 +225,8 @@ class AdapterBDH:
 
     def train_step(self, opt: AdamWMany, tokens: torch.Tensor, targets: torch.Tensor, adapters,
                    batch: AdapterBatch | None = None, lr: float | None = None) -> torch.Tensor:
-        """One step on sequences [B, T] with the given adapters; those of no sequence are left alone.
+        """One step on sequences [B, T] with the given adapters; those of no sequence are left alone. Dropout
+        as in the model's own training: its configuration's rate, unless the model is in evaluation mode.
         ``batch``: the plan of an earlier step with the same adapters. Returns the mean loss."""
         bank = self.bank
         batch = batch or self.batch(adapters, tokens.shape[1])
@@ -228,7 +234,7 @@ class AdapterBDH:
             raise ValueError("the batch was planned for other adapters or another length")
         names = list(bank.master)
         work = {n: t.detach().requires_grad_(True) for n, t in bank.work.items()}
-        loss = R.cross_entropy(self.forward(tokens, batch, work=work), targets)
+        loss = R.cross_entropy(self.forward(tokens, batch, work=work, training=self.model.training), targets)
         grads = dict(zip(names, torch.autograd.grad(loss, [work[n] for n in names])))
         used = {int(g) for g in adapters}
         opt.step([grads[n][g] if g in used else None for g in range(bank.n_adapters) for n in names], lr=lr)

@@ -24,7 +24,26 @@ def test_a_plan_of_other_adapters_is_refused():
     x, y = TOKENS[:, :-1], TOKENS[:, 1:]
     net.train_step(opt, x, y, range(2), batch=net.batch([0, 1], 8))
     before = {n: t.clone() for n, t in net.bank.master.items()}
-    for plan in (net.batch([0, 2], 8), net.batch([1, 0], 8), net.batch([0, 1], 9), net.batch([0, 0, 1, 1], 4)):
+    for plan in (net.batch([0, 2], 8), net.batch([1, 0], 8), net.batch([0, 1], 9)):
         with pytest.raises(ValueError, match="planned for other"):
             net.train_step(opt, x, y, [0, 1], batch=plan)
     assert all(torch.equal(t, before[n]) for n, t in net.bank.master.items()) and opt.t == 1
+    net.train_step(opt, x, y, [0, 1], batch=net.batch([0, 0, 1, 1], 4))  # the same adapter for every row
+
+
+def test_a_step_trains_with_the_models_dropout():
+    """At a rate of 1 the layers add nothing, which needs no equal random numbers: the loss is the model's own."""
+    for mode, rate in ((True, 1.0), (False, 0.0)):
+        model, net = make(dropout=1.0)
+        model.train(mode)
+        x, y = TOKENS[:, :-1], TOKENS[:, 1:]
+        want = float(model.loss(x, y).detach())
+        assert abs(float(net.train_step(net.optimizer(), x, y, [0, 1])) - want) < 1e-5
+        p = {k: v.detach() for k, v in model.param_dict().items() if v is not None}
+        model.cfg.dropout = rate
+        assert abs(float(R.cross_entropy(R.bdh_forward(x, p, model.cfg, training=True)[0], y)) - want) < 1e-5
+    model, net = make(dropout=0.5)
+    losses = {float(net.train_step(net.optimizer(lr=0.0), TOKENS[:, :-1], TOKENS[:, 1:], [0, 1])) for _ in range(4)}
+    assert len(losses) == 4  # drawn anew each step
+    logits = [net.forward(TOKENS, net.batch([0, 1], 9)) for _ in range(2)]
+    assert torch.equal(*logits)  # and not in answers
