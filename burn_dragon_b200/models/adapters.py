@@ -250,6 +250,8 @@ class AdapterBDH:
         nothing to draw from answers -1 (log-probability -inf) from there on; the others go on."""
         if len(prompts) != len(adapters) or not prompts or any(not p for p in prompts):
             raise ValueError("one adapter per prompt, and no empty prompts")
+        if max_new_tokens <= 0:
+            return [[] for _ in prompts], [[] for _ in prompts]
         dev = self.p["embed"].device
         lens = torch.tensor([len(p) for p in prompts], device=dev)
         width, shared = int(lens.max()), int(lens.min())

@@ -47,3 +47,11 @@ def test_a_step_trains_with_the_models_dropout():
     assert len(losses) == 4  # drawn anew each step
     logits = [net.forward(TOKENS, net.batch([0, 1], 9)) for _ in range(2)]
     assert torch.equal(*logits)  # and not in answers
+
+
+@pytest.mark.parametrize("prompts", [[[1, 2], [3, 4]], [[1, 2, 3], [4]]])
+def test_no_new_tokens_are_an_empty_answer(prompts):
+    _, net = make()
+    assert net.generate(prompts, [0, -1], 0) == ([[], []], [[], []])
+    out, lp = net.generate(prompts, [0, -1], 1)
+    assert [len(o) for o in out] == [1, 1] == [len(v) for v in lp]
