@@ -6,18 +6,21 @@ Each given text gets an adapter of its own; one batch per step trains them toget
   python -m burn_dragon_b200.cli.adapters --text "the quick brown fox" --text "0123456789" [--run runs/language/cuda/NAME]
          [--steps 200] [--rank 16] [--state-bits 8] [--max-tokens 32] [--temperature 0.8 --top-k 40 --top-p 0.95 --min-p 0.05]
 
-Without ``--run`` the frozen model is the tiny byte configuration with random weights.
+Without ``--run`` the frozen model is the tiny byte configuration with random weights. A run's texts go through
+its own ``tokenizer.json`` (bytes where it has none).
 """
 
 from __future__ import annotations
 
 import argparse
+import os
 
 import torch
 
 from ..config import DragonConfig, training_config_from_dict
 from ..models.adapters import AdapterBank, AdapterBDH
 from ..models.bdh import BDH
+from ..utils.tokenizer import ByteTokenizer, load_tokenizer
 
 
 def main(argv=None) -> None:
@@ -37,23 +40,26 @@ def main(argv=None) -> None:
     ap.add_argument("--seed", type=int, default=0)
     a = ap.parse_args(argv)
     dev = torch.device("cuda", 0) if torch.cuda.is_available() else torch.device("cpu")
+    tok = ByteTokenizer()
     if a.run:
         from ..train.checkpoint import RunDir
 
         run = RunDir(a.run)
         model = BDH(training_config_from_dict(run.read_json("training_config.json")).model, device=dev)
         run.load(None, model)
+        path = os.path.join(a.run, "tokenizer.json")
+        tok = load_tokenizer(path) if os.path.exists(path) else tok
     else:
         cfg = DragonConfig.tiny()
         cfg.init_std = 0.1  # a random head that can tell bytes apart
         model = BDH(cfg, device=dev, seed=a.seed)
-    if model.cfg.vocab_size < 256:
-        raise SystemExit("the adapter example trains on bytes: a vocabulary of at least 256")
+    if model.cfg.vocab_size < tok.vocab_size:
+        raise SystemExit(f"the model has {model.cfg.vocab_size} tokens, the tokenizer {tok.vocab_size}")
     G = len(a.text)
     net = AdapterBDH(model, AdapterBank(model.cfg, G, rank=a.rank, device=dev, seed=a.seed))
     opt = net.optimizer(lr=a.lr, state_bits=a.state_bits, seed=a.seed)
-    data = [torch.tensor(list((t.encode() + b"\n") * (2 + (a.length + 1) // len(t.encode() + b"\n"))), dtype=torch.long)
-            for t in a.text]
+    lines = [tok.encode(t + "\n") for t in a.text]
+    data = [torch.tensor(ids * (2 + (a.length + 1) // len(ids)), dtype=torch.long) for ids in lines]
     gen = torch.Generator().manual_seed(a.seed)
     plan = net.batch(range(G), a.length)
     for step in range(a.steps):
@@ -65,13 +71,13 @@ def main(argv=None) -> None:
         loss = net.train_step(opt, xy[:, :-1], xy[:, 1:], range(G), batch=plan)
         if step % 50 == 0 or step + 1 == a.steps:
             print(f"step {step}: loss {float(loss):.4f}")
-    prompts = [list(t.encode()[:max(1, len(t.encode()) // 2)]) for t in a.text]
+    prompts = [ids[:max(1, len(ids) // 2)] for ids in map(tok.encode, a.text)]
     out, logprobs = net.generate(prompts, list(range(G)), a.max_tokens, a.temperature, a.top_k, a.top_p, a.min_p, a.seed)
     for g, (p, o, lp) in enumerate(zip(prompts, out, logprobs)):
         if -1 in o:
             print(f"adapter {g}: no token to draw after {o.index(-1)} tokens: the logits are NaN or -inf")
             continue
-        text = bytes(t & 0xFF for t in p + o).decode("utf-8", errors="replace")
+        text = tok.decode([t for t in p + o if t < tok.vocab_size])  # a model may have more tokens than its tokenizer
         print(f"adapter {g}: {text!r} (mean log-probability {sum(lp) / max(len(lp), 1):.3f})")
 
 
