@@ -33,7 +33,10 @@ if os.environ.get("BDH_PTXAS_VERBOSE"):
 
 
 # Kernels launched by one call of each binding (for the bench's launch count).
-_LAUNCHES_PER_CALL = {"grad_clip_coef": 2, "adapter_forward": 2, "adapter_direct": 2, "adapter_backward": 4}
+_LAUNCHES_PER_CALL = {"grad_clip_coef": 2}
+# These count their launches themselves: how many there are depends on the arguments.
+_LAUNCHES_PER_CALL.update(dict.fromkeys(("adapter_forward", "adapter_direct", "adapter_backward", "sample_tokens",
+                                         "adamw_many"), 0))
 
 
 class _Counted:
@@ -65,7 +68,7 @@ def add_launches(n: int) -> None:
 
 def launch_count() -> int:
     """Kernels of this package launched so far in this process."""
-    return _MOD.launches if _MOD is not None else 0
+    return _MOD.launches + _MOD._mod.counted_launches() if _MOD is not None else 0
 
 
 def load(verbose: bool = False):

@@ -29,6 +29,8 @@
 #include <cmath>
 #include <vector>
 
+#include "launches.h"
+
 namespace bd {
 namespace {
 
@@ -282,6 +284,7 @@ void launch(const std::vector<ManyTensor>& all, size_t first, size_t count, cons
     adamw_many_kernel<CAP, false><<<grid, 32 * kWarps, 0, st>>>(table, h, owner.data_ptr<int>(), (int)first, block0,
                                                                 block1, m.data_ptr(), v.data_ptr(), ms, vs);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  ++counted_launches;
 }
 
 constexpr int kFew = 64, kMany = 640;  // tensors a launch names: 3 KB or 30 KB of arguments

@@ -33,6 +33,7 @@
 #include <torch/extension.h>
 
 #include "gemm_table.h"
+#include "launches.h"
 #include "sm100_ptx.cuh"
 #include "tensor_map.h"
 
@@ -915,6 +916,7 @@ at::Tensor shrink(const Rows& x, const at::Tensor& a, const Plan& p, int H, int 
   else
     go(std::integral_constant<int, 4>());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  ++counted_launches;
   return t;
 }
 
@@ -940,6 +942,7 @@ void launch_gemm(const AdapterGemm& p, cudaStream_t st, int dev, bool after_shri
   cfg.attrs = attr;
   cfg.numAttrs = after_shrink ? 1 : 0;
   C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, p));
+  ++counted_launches;
 }
 
 // out [M, Z, N] = sum over the reduction's heads of x w (+ s t b).
@@ -1021,6 +1024,7 @@ at::Tensor project(const Rows& x, const at::Tensor& w, bool w_mn, bool sum_heads
     adapter_sum_kernel<<<(unsigned)((n + 127) / 128), 256, 0, st>>>(
         p.partial, p.splits, p.Z, M, N, reinterpret_cast<bf16*>(y.data_ptr()));
     C10_CUDA_KERNEL_LAUNCH_CHECK();
+    ++counted_launches;
   }
   return y;
 }
@@ -1033,6 +1037,7 @@ at::Tensor fold(const at::Tensor& t, cudaStream_t st) {
   adapter_fold_kernel<<<(unsigned)((n + 1023) / 1024), 256, 0, st>>>(t.data_ptr<float>(), (int)t.size(0), n,
                                                                      out.data_ptr<float>());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  ++counted_launches;
   return out;
 }
 
@@ -1048,6 +1053,7 @@ void launch_grad(const GradArgs& a, int G, cudaStream_t st, int dev) {
   }
   kern<<<dim3((unsigned)((a.C + SLAB - 1) / SLAB), (unsigned)a.H, (unsigned)G), 256, bytes, st>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  ++counted_launches;
 }
 
 constexpr int kWideSlab = 512, kNarrowSlab = 128;

@@ -3,6 +3,8 @@
 
 #include <vector>
 
+#include "launches.h"
+
 namespace bd {
 void gemm(int64_t epi, int64_t bn, const at::Tensor& a, bool a_mn, std::vector<int64_t> a_geom,
           const at::Tensor& b, bool b_mn, std::vector<int64_t> b_geom, int64_t M, int64_t N, int64_t K,
@@ -136,6 +138,10 @@ void adamw_many(const std::vector<at::Tensor>& params, const std::vector<c10::op
                 const at::Tensor& steps, int64_t key, const c10::optional<at::Tensor>& gscale);
 }  // namespace bd
 
+namespace bd {
+std::atomic<int64_t> counted_launches{0};
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "burn_dragon_b200 sm_100a kernels (tcgen05 GEMM engine + row kernels)";
   m.def("gemm", &bd::gemm);
@@ -196,4 +202,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("adapter_backward", &bd::adapter_backward);
   m.def("sample_tokens", &bd::sample_tokens);
   m.def("adamw_many", &bd::adamw_many);
+  m.def("counted_launches", [] { return bd::counted_launches.load(); });
 }

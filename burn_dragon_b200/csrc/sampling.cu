@@ -42,6 +42,8 @@
 
 #include <cfloat>
 
+#include "launches.h"
+
 namespace bd {
 namespace {
 
@@ -923,6 +925,7 @@ void launch(const SampleArgs& a, int C, cudaStream_t st, int dev) {
   cfg.numAttrs = 1;
   cfg.gridDim = dim3((unsigned)(a.rows * C));
   C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, a));
+  ++counted_launches;
 }
 
 template <typename S>
