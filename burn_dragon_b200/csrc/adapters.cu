@@ -486,7 +486,9 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
     AdapterWalk walk(p, blockIdx.x, gridDim.x);
     for (int t = blockIdx.x; t < total; t += gridDim.x, walk.next()) {
       const AdapterTile c = adapter_place(walk, BN);
-      if (!mbar_wait_bounded(&tfull_bar[acc], acc_phase, &abort_flag, p.err, kErrTimeoutEpilogue)) break;
+      // the same answer for the whole warp: the loads from TMEM need all of its lanes, also where a wait has run out
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&tfull_bar[acc], acc_phase, &abort_flag, p.err, kErrTimeoutEpilogue)))
+        break;
       tc_fence_after();
       const int row0 = c.m0 + quad * 32;
 #pragma unroll 1
