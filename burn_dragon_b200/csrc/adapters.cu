@@ -13,12 +13,11 @@
 //  * adapter_gemm: the projection on tcgen05 (TMA, TMEM, warp roles as in the GEMM engine),
 //    with the adapters as an extension of its reduction: after the K-blocks of x and W
 //    come blocks of 64 / rp adapter slots. A 128-row tile lists the distinct adapters of its rows
-//    ("slots"); four builder warps write t s into the columns of each row's slot and zeros
-//    elsewhere, and TMA loads the slots' b rows beside each other. A slot's product leaves the accumulator's
-//    rows of other slots as they are (they are masked off: zeros alone would let an infinity or NaN in one
-//    adapter's b into them, since 0 b is NaN then). So one accumulator takes both
-//    products, rows of any adapters can share a tile, and W and every b are read once per
-//    row tile. The projection's blocks need no t, so with programmatic launch they run
+//    ("slots"); four builder warps write t s into the columns of each row's slot, and TMA loads the
+//    slots' b rows beside each other. A slot's product leaves the accumulator's rows of other slots as they
+//    are: they are masked off (zeros in their columns would not do: 0 b is NaN where another adapter's b is not
+//    finite). So one accumulator takes both products, rows of any adapters can share a tile, and W and every b are
+//    read once per row tile. The projection's blocks need no t, so with programmatic launch they run
 //    while adapter_shrink still does; only the builders wait for it.
 //  * adapter_grad: da / db, one CTA per adapter, head and slab of columns; for db it gives u in the same pass over dy.
 // Measured on a B200: 48 rows, 43 adapters of rank 16, 4 heads 256 -> 8192: 22 us for 66 MB;
@@ -426,8 +425,13 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
         const int projection = c.kb1 - c.kb0, blocks = projection + c.e1 - c.e0;
         for (int i = 0; i < blocks; ++i) {
           const bool ext = i >= projection;
-          if (!mbar_wait_bounded(&full_bar[stage], phase, &abort_flag, p.err, kErrTimeoutMma) ||
-              (ext && !mbar_wait_bounded(&built_bar[buf], buf_phase, &abort_flag, p.err, kErrTimeoutMma))) {
+          uint4 off[4];  // of each step: read while the block's b is still on its way
+          if (ext) {
+            ok = mbar_wait_bounded(&built_bar[buf], buf_phase, &abort_flag, p.err, kErrTimeoutMma);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) off[kk] = rows_off[buf][kk >> (2 - p.block_shift)];
+          }
+          if (!ok || !mbar_wait_bounded(&full_bar[stage], phase, &abort_flag, p.err, kErrTimeoutMma)) {
             ok = false;
             break;
           }
@@ -446,10 +450,11 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
             const int e = c.e0 + i - projection;
             const int j0 = (p.HR > 1 ? e % c.ext : e) * p.per_block;
             const int steps = (min(p.per_block, c.nslots - j0) * p.rp) >> 4;  // 1, 2 or 4 a slot
-            for (int kk = 0; kk < steps; ++kk)
-              umma_bf16_rows(d_tmem, make_sdesc_sw128(e_base + kk * 32, 16, 1024),
-                             make_sdesc_sw128(b_base + kk * 2048, 8192, 1024), idesc_b,
-                             rows_off[buf][kk >> (2 - p.block_shift)]);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              if (kk < steps)
+                umma_bf16_rows(d_tmem, make_sdesc_sw128(e_base + kk * 32, 16, 1024),
+                               make_sdesc_sw128(b_base + kk * 2048, 8192, 1024), idesc_b, off[kk]);
             umma_commit(&used_bar[buf]);
             if (++buf == EXT) {
               buf = 0;
@@ -585,19 +590,17 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_gemm_kernel(const 
           break;
         }
         uint8_t* dst = sExt + buf * Cfg::A_BYTES;
-        const int j = row.slot - e * p.per_block;  // the row's slot in this block
-        const int at = row.slot >= 0 && j >= 0 && j < p.per_block ? j * p.rp / 8 : 8;
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-          if (q < at || q >= at + p.rp / 8) *reinterpret_cast<uint4*>(dst + sw128(r, q)) = make_uint4(0u, 0u, 0u, 0u);
-        if (at < 8) {
+        // The row's slot in this block. Its other columns hold what they held: those products are masked off.
+        const int j = row.slot - e * p.per_block;
+        const bool here = row.slot >= 0 && j >= 0 && j < p.per_block;
+        if (here) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (8 * i < p.rp) *reinterpret_cast<uint4*>(dst + sw128(r, at + i)) = row.t[i];
+            if (8 * i < p.rp) *reinterpret_cast<uint4*>(dst + sw128(r, j * p.rp / 8 + i)) = row.t[i];
         }
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          const uint32_t own = __ballot_sync(0xffffffffu, at < 8 && j == s);
+          const uint32_t own = __ballot_sync(0xffffffffu, here && j == s);
           if (lane == 0) reinterpret_cast<uint32_t*>(&rows_off[buf][s])[r / 32] = ~own;
         }
         fence_proxy_async_smem();
