@@ -63,8 +63,8 @@ class AdapterBank:
     def load_scaffold(self, g: int, source, scale: float | None = None) -> None:
         """Adapter ``g`` from a random-scaffold model, or from the tensors of one by their names in its
         ``state_dict`` (``encoder_a``), in its record (``random_scaffold_adapters.fast.encoder.a``) or
-        ``encoder.a``: a [.., in, r], b [.., r, out] and the trained gain. A model brings its scaling along; for
-        tensors it is ``scale``, or that of the bank's configuration if that is a scaffold's, else the bank's own.
+        ``encoder.a``: a [.., in, r], b [.., r, out] and the trained gain. ``scale``: the scaffold's s; by default
+        that of the model, of the bank's configuration if that is a scaffold's, or the bank's own.
         ``AdapterBDH`` then takes W_seed, without the model's own adapter, for the frozen projections."""
         cfg = self.cfg
         if isinstance(source, torch.nn.Module):
@@ -73,7 +73,6 @@ class AdapterBank:
             cfg = source.cfg
             with torch.no_grad():
                 source = {f"{n}.{k}": t.detach() for n in PROJECTIONS for k, t in zip(("a", "b", "gain"), source._scaffold_parts(n))}
-            scale = cfg.random_scaffold.adapter_scale()
         rs = cfg.random_scaffold
         if scale is None:
             scale = rs.adapter_scale() if rs.enabled else self.scale
@@ -119,6 +118,25 @@ class AdapterBank:
                 self.gain[proj][g] = gain
         self.scaffold = self.scaffold or made
 
+    def state_dict(self) -> dict:
+        """The masters, and how they are applied: ``scale``, and of adapters from a scaffold ``scales``, ``gain`` and
+        ``scaffold``."""
+        return {**self.master, "scale": self.scale, "scales": self.scales, "gain": self.gain, "scaffold": self.scaffold}
+
+    def load_state_dict(self, sd: dict) -> None:
+        """A state of a bank of the same shapes. An ``AdapterBDH`` of this bank takes it over on its next call."""
+        for name, t in self.master.items():
+            if sd[name].shape != t.shape:
+                raise ValueError(f"{name} is {tuple(sd[name].shape)}, the bank's is {tuple(t.shape)}")
+        like = self.master["encoder.a"]
+        for name, t in self.master.items():
+            t.copy_(sd[name])
+            if self.work[name] is not t:
+                self.work[name].copy_(t)
+        own = lambda d: None if d is None else {n: v.to(like.device, torch.float32).clone() for n, v in d.items()}  # noqa: E731
+        self.scale, self.scales, self.gain = float(sd["scale"]), own(sd["scales"]), own(sd["gain"])
+        self.scaffold = None if sd["scaffold"] is None else tuple(sd["scaffold"])
+
     def tensors(self, which: dict[str, torch.Tensor]) -> list[torch.Tensor]:
         """Every adapter's own matrices, adapter by adapter."""
         return [which[name][g] for g in range(self.n_adapters) for name in self.master]
@@ -162,6 +180,7 @@ class AdapterBDH:
                 if not torch.allclose(frozen[n].reshape(-1)[:some].float().cpu(), want, rtol=1e-4, atol=1e-4 * std):
                     raise ValueError(f"{n} is not the W_seed of the scaffold that the adapters were trained on")
         self.weights = {n: frozen[n].to(self.dtype).contiguous() for n in PROJECTIONS}
+        self.frozen_for = (self.on_scaffold, bank.scaffold)
 
     def batch(self, adapters, length: int) -> AdapterBatch:
         """The plan of ``len(adapters)`` sequences of ``length`` tokens."""
@@ -180,7 +199,7 @@ class AdapterBDH:
         ``training``: with the model's dropout."""
         cfg, work, bank = self.cfg, work or self.bank.work, self.bank
         B, T = tokens.shape
-        if self.on_scaffold != (bank.scales is not None):  # the bank's first adapter from a scaffold came later
+        if self.frozen_for != (bank.scales is not None, bank.scaffold):  # adapters of a scaffold came, or went, later
             self._freeze()
         gains = None
         if bank.gain is not None:

@@ -115,6 +115,29 @@ def test_what_does_not_belong_together_is_refused():
         bank.load_scaffold(1, model)
 
 
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("from_scaffold", [True, False])
+def test_a_bank_is_saved_and_loaded(from_scaffold, dev, tmp_path):
+    model = scaffold_model(1, dev=dev)
+    bank = AdapterBank(model.cfg, 2, rank=4, alpha=3.0, device=dev, seed=8)
+    if from_scaffold:
+        bank.load_scaffold(0, model)
+    net = AdapterBDH(model, bank)
+    opt = net.optimizer(lr=1e-2)
+    tokens = TOKENS.to(dev)
+    for _ in range(3):
+        net.train_step(opt, tokens[:, :-1], tokens[:, 1:], [0, 1, -1])
+    want = net.forward(tokens, net.batch([0, 1, -1], 11))
+    torch.save(bank.state_dict(), tmp_path / "bank.pt")
+    other = AdapterBank(model.cfg, 2, rank=4, device=dev)
+    before = AdapterBDH(model, other)
+    other.load_state_dict(torch.load(tmp_path / "bank.pt"))
+    for got in (before, AdapterBDH(model, other)):
+        assert torch.equal(got.forward(tokens, got.batch([0, 1, -1], 11)), want)
+    with pytest.raises(ValueError, match="the bank's is"):
+        AdapterBank(model.cfg, 3, rank=4, device=dev).load_state_dict(bank.state_dict())
+
+
 @pytest.mark.gpu
 def test_on_the_device():
     """bf16 projections against the fp32 model: each of the 6 rounds inputs, weights and outputs to 2^-8."""
