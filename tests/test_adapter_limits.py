@@ -166,3 +166,28 @@ def test_adapters_at_odd_addresses_and_strides():
     y = adapter_linear(x, w, p, q, batch, 1.5)
     assert torch.equal(y.detach(), want)
     assert [g.shape for g in torch.autograd.grad(y, (p, q), torch.ones_like(y))] == [a.shape, b.shape]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", LAYOUTS, ids=range(len(LAYOUTS)))
+def test_a_request_alone_answers_as_among_others(layout):
+    """Up to the order of fp32 sums: how a reduction is split depends on the batch's size. Each way is within one
+    rounding of y and one of each t of the formula."""
+    from test_adapters import BF, formula
+
+    ids, lengths, G, H, K, N, r, shared = layout
+    gen = torch.Generator().manual_seed(6)
+    rn = lambda *s: torch.randn(*s, generator=gen).to("cuda", torch.bfloat16)  # noqa: E731
+    M = sum(lengths)
+    x, w = (rn(M, K) if shared else rn(M, H, K)), rn(H, K, N) * 0.1
+    a, b, scale = rn(G, H, r, K) * K ** -0.5, rn(G, H, r, N) * 0.2, torch.ones(G, device="cuda")
+    batch = AdapterBatch(ids, lengths, G)
+    y = adapter_linear(x, w, a, b, batch, scale)
+    want, low, size, _ = formula(x, w, a, b, batch.adapter_of_row(), scale)
+    bound = 2 * (BF * 1.01 * (want.abs() + low) + (K + 64) * 2.0 ** -23 * size)
+    at = 0
+    for g, n in zip(ids, lengths):
+        rows = slice(at, at + n)
+        alone = adapter_linear(x[rows], w, a, b, AdapterBatch([g], [n], G), scale)
+        assert ((alone.double() - y[rows].double()).abs() <= bound[rows]).all()
+        at += n
