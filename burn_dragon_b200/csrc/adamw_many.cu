@@ -17,9 +17,9 @@
 // computed with separately rounded products and sums, so any implementation of the formulas
 // gives the same codes.
 //
-// Measured on a B200: 25.2 M values, fp32 states and gradients, 28 B each: 108 us = 6.5 TB/s, the copy rate. 26 M
-// values with e4m3 states, bf16 gradients and working copies, 16 B each: 92 us = 4.6 TB/s; there the
-// instructions bound it (about 95 a value; 85 % of the issue slots at 120 before the codes were converted in pairs).
+// Measured on a B200: 25.2 M values, fp32 states and gradients, 28 B each: 109 us = 6.5 TB/s, the copy rate. 26 M
+// values with e4m3 states, bf16 gradients and working copies, 16 B each: 93 us = 4.5 TB/s; there the
+// instructions bound it (about 84 a value: 71 % of the issue slots, with DRAM busy for half of the time).
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_bf16.h>
@@ -158,7 +158,7 @@ __device__ __forceinline__ void store_codes(unsigned char* s, int lane, const un
 }
 
 // m / (sqrt(v) + eps). Beside 8-bit states, whose own rounding is 2^-4 and which the instructions bound (102 us
-// with the correctly rounded forms, 90 without), root and quotient are good to 2^-22 of the step; the states do not use
+// with the correctly rounded forms when 90 without), root and quotient are good to 2^-22 of the step; the states do not use
 // them. With 32-bit states the bytes bound the step, and both are rounded correctly.
 template <bool EIGHT>
 __device__ __forceinline__ float ratio(float m, float v, float eps) {

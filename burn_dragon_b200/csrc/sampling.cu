@@ -25,10 +25,10 @@
 // Where more than kList values are left (many equal ones), or the border is not in the window,
 // find_bound refines exact histograms over the row's bits, read again from memory.
 //
-// Measured on a B200: 200 x 128000 fp32 greedy 40 us, unfiltered 66, top-k 50 91, top-p 0.9 195 (the logits' bytes
-// at the copy rate: 15.6); 3 x 50000 bf16 4.5 / 11 / 16 / 33; 16 x 256 3.1 / 5.6 / 10.5 / 10.5. Bound by
-// the chain of cluster barriers and of the first CTA's steps (a top-p row lives 35 to 50 us, of which its passes
-// over the slice take a third), not by bytes or arithmetic. A grid that walks over the rows was slower
+// Measured on a B200: 200 x 128000 fp32 greedy 40 us, unfiltered 66, top-k 50 91, top-p 0.9 196 to 204 (the logits'
+// bytes at the copy rate: 15.6); 3 x 50000 bf16 4.4 / 11 / 16 / 26 to 40; 16 x 256 3.0 / 5.6 / 10.3 / 10.3. Bound by
+// the chain of cluster barriers and of the first CTA's steps (barriers are the first stall, 43 % of the issue slots are
+// used, DRAM is busy for 6 to 18 %), not by bytes or arithmetic. A grid that walks over the rows was slower
 // (unfiltered 99): a cluster then waits for its last token before the next row.
 //
 // A row is split over a cluster of C CTAs that keep their slice of it in shared memory (the
