@@ -4,11 +4,12 @@ Where a random scaffold (``models.scaffold``) trains one adapter per model, an `
 them for the three shared projections, W = W_frozen + s A_g^T B_g with s = alpha / r or alpha / sqrt(r), and
 a batch may name another adapter for every sequence. ``load_scaffold`` takes adapters over from scaffold models
 of one seed, W = gain_g W_seed + s_g A_g^T B_g with the scaling and the gains that they were trained with; the
-embedding, the head and the norms are those of the model that ``AdapterBDH`` is given. ``AdapterBDH`` is the BDH forward with the three
-projections through ``ops.adapters.adapter_linear`` (bf16 operands on CUDA, the plain form on CPU);
-norms, RoPE and the linear attention are ``models.reference``'s. ``train_step`` updates the adapters of
-the batch with ``AdamWMany``; ``generate`` serves requests of different lengths, adapters and sampling
-settings in one batch (``ops.sampling.sample_tokens``).
+embedding, the head and the norms are those of the model that ``AdapterBDH`` is given.
+
+``AdapterBDH`` is the BDH forward with the three projections through ``ops.adapters.adapter_linear`` (bf16
+operands on CUDA, the plain form on CPU); norms, RoPE and the linear attention are ``models.reference``'s.
+``train_step`` updates the adapters of the batch with ``AdamWMany``; ``generate`` serves requests of different
+lengths, adapters and sampling settings in one batch (``ops.sampling.sample_tokens``).
 """
 
 from __future__ import annotations
@@ -71,14 +72,14 @@ class AdapterBank:
             if not getattr(source, "scaffold", False):
                 raise ValueError("load_scaffold takes a random-scaffold model or its tensors")
             cfg = source.cfg
-            with torch.no_grad():
-                source = {f"{n}.{k}": t.detach() for n in PROJECTIONS for k, t in zip(("a", "b", "gain"), source._scaffold_parts(n))}
+            parts = {n: source._scaffold_parts(n) for n in PROJECTIONS}
+            source = {f"{n}.{k}": t for n in PROJECTIONS for k, t in zip(("a", "b", "gain"), parts[n])}
         rs = cfg.random_scaffold
         if scale is None:
             scale = rs.adapter_scale() if rs.enabled else self.scale
         made = (rs.seed, rs.distribution, cfg.init_std) if rs.enabled else None
         if made and self.scaffold and made != self.scaffold:
-            raise ValueError(f"adapters of one bank share W_seed: {made} is not {self.scaffold} (seed, distribution, std)")
+            raise ValueError(f"adapters of one bank share W_seed: (seed, distribution, std) {made} is not {self.scaffold}")
 
         def tensor(name: str):
             proj, part = name.split(".")
