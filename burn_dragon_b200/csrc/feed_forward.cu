@@ -67,7 +67,8 @@ __global__ void __launch_bounds__(256) ff_join_kernel(const __grid_constant__ Ff
   } else {
     if (in) {
 #pragma unroll
-      for (int s = 0; s < NB; ++s) ff_bias8(e, s, head, col, v[s]);
+      for (int s = 0; s < NB; ++s)
+        if (ff_has_bias(e, s)) ff_bias8(e, s, head, col, v[s]);
     }
     const long long rh = (long long)m * e.heads + head;
     if (!ff_backward(EPI) && e.keep != FF_KEEP_NOTHING) {
@@ -97,9 +98,13 @@ __global__ void __launch_bounds__(256) ff_join_kernel(const __grid_constant__ Ff
       ff_unpack8(*reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(e.aux) + (long long)m * e.aux_ld +
                                                  (long long)head * e.aux_head + col),
                  e.half, a);
-    ff_values<EPI, 8>(e, v[0], v[NB - 1], a);
-    if constexpr (EPI == FF_ACT) {
-      if (e.aux) {
+    if constexpr (ff_backward(EPI)) {
+      ff_with_act(e.act, [&](auto k) {
+        ff_backward_values<EPI, 8, decltype(k)::value>(e.up_relu, v[0], v[NB - 1], [&](int i) { return pair_of(a, i); });
+      });
+    } else {
+      ff_forward_values<EPI, 8>(e, v[0], v[NB - 1]);
+      if (EPI == FF_ACT && e.aux) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[0][i] += a[i];
       }
@@ -150,7 +155,9 @@ __global__ void __launch_bounds__(256) ff_held_kernel(const __grid_constant__ Ff
       }
     }
     if constexpr (KEEP != FF_KEEP_NOTHING) {
-      ff_values<EPI, 8>(e, v[0], v[1], a);
+      ff_with_act(e.act, [&](auto k) {
+        ff_backward_values<EPI, 8, decltype(k)::value>(e.up_relu, v[0], v[1], [&](int i) { return pair_of(a, i); });
+      });
       const long long to = (long long)m * e.ld + (long long)head * e.head + col;
 #pragma unroll
       for (int s = 0; s < NB; ++s)
@@ -245,7 +252,7 @@ Choice choose(int64_t rows, int64_t cols, int64_t batch, int64_t blocks, int nb,
   };
   const Option one[] = {{true, 256}, {true, 128}, {false, 128}, {false, 64}}, two[] = {{true, 128}, {false, 64}};
   const Option* options = nb == 1 ? one : two;
-  Choice best{{false, 64}, 1};
+  Choice best{{false, 64, false}, 1};
   double least = 1e300;
   for (int i = 0; i < (nb == 1 ? 4 : 2); ++i) {
     const Option o = options[i];
@@ -259,7 +266,7 @@ Choice choose(int64_t rows, int64_t cols, int64_t batch, int64_t blocks, int nb,
       const double waves = (double)((tiles * parts + workers - 1) / workers);
       double cost = waves * ((double)((blocks + parts - 1) / parts) * block + 1200.0);
       if (parts > 1) cost += 6000.0 + 8.0 * parts * rows * cols * batch * nb / 3000.0;
-      if (cost < least) least = cost, best = Choice{{o.pair, o.bn}, (int)parts};
+      if (cost < least) least = cost, best = Choice{{o.pair, o.bn, false}, (int)parts};
     }
   }
   return best;
@@ -290,12 +297,23 @@ void product(const Launch& l, int epi, FfOut e, const Mat* a, const Mat* b, int 
   p.a_mn = a_mn, p.two_a = two_a;
   p.err = l.err;
   const int64_t blocks = (int64_t)p.KB * segments, batch = (int64_t)e.heads * out_sets;
-  const Choice c = choose(e.M, e.N, batch, blocks, nb, nb == 2 && two_a ? 2 : 1, num_sms_of(l.dev), may_split);
+  Choice c = choose(e.M, e.N, batch, blocks, nb, nb == 2 && two_a ? 2 : 1, num_sms_of(l.dev), may_split);
   p.splits = c.splits;
+  // Short reductions: A stays in shared memory over the columns of its rows.
+  c.tile.resident = epi != FF_STORE && c.tile.pair && c.tile.bn == (nb == 1 ? 256 : 128) && p.splits == 1 && p.KB <= kFfResident;
   TORCH_CHECK(blocks * (c.splits + 1) < (1ll << 32), "feed_forward: the reduction is too long");
   const int rows = c.tile.pair ? 256 : 128, b_rows = c.tile.pair ? c.tile.bn / 2 : c.tile.bn;
   p.tiles_m = (e.M + rows - 1) / rows, p.tiles_n = (e.N + c.tile.bn - 1) / c.tile.bn;
   TORCH_CHECK((long long)p.tiles_m * p.tiles_n * p.splits * batch < (1ll << 31), "feed_forward: too many tiles");
+  const unsigned sizes[4] = {(unsigned)p.tiles_n, (unsigned)p.tiles_m, (unsigned)p.splits, (unsigned)e.heads};
+  const int64_t total = (int64_t)p.tiles_m * p.tiles_n * p.splits * batch;
+  unsigned step = c.tile.resident ? 1 : (unsigned)ff_workers(total, c.tile, num_sms_of(l.dev));
+  for (int i = 0; i < 4; ++i) {
+    p.size[i] = sizes[i];
+    p.step[i] = step % sizes[i];
+    step /= sizes[i];
+  }
+  p.step[4] = step;
   for (int s = 0; s < 2; ++s) {
     const int q = s < sets ? s : 0;
     p.ta[s] = a[q].map(a_mn ? 64 : 128);

@@ -16,6 +16,8 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "act8.cuh"
 #include "sm100_ptx.cuh"
 
@@ -55,6 +57,8 @@ struct alignas(64) FfGemm {
   int a_mn, b_mn;         // the reduction is not the contiguous dimension; b_mn of the gated form: a bit a projection
   int two_a;              // the second product has an A of its own
   int tiles_m, tiles_n, splits;
+  unsigned size[4];       // tiles_n, tiles_m, splits, heads of the output
+  unsigned step[5];       // how far a worker goes from tile to tile, in digits of these sizes
   uint32_t idesc;
   float* partial;         // [splits, NB, sets, heads, M, N] where the reduction is split
   int* err;
@@ -63,30 +67,99 @@ struct alignas(64) FfGemm {
 
 // ------------------------------------------------------------------------------- arithmetic
 
+// Pairs of fp32 values in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float relu_nan(float x) {  // NaN stays
+  float r;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// The normal distribution's cdf at p, and exp(-p^2 / 2) where it is wanted. The lower tail at x = |p| is
+// exp(-x^2 / 2) 2^R(x), R a least-squares fit of degree 8 on [0, 5] and constant from there: the tail is off by 8e-6 of
+// itself to x = 5, by 1.4e-7 anywhere, p cdf(p) by 2e-7. One exponential a value and no quotient: with two of the
+// latter's kind (a Chebyshev form of erfc) the special-function unit bound the epilogue (67 M outputs: 115 us).
+__device__ __forceinline__ float2 normal_cdf2(float2 p, float2* bell) {
+  const float2 x = make_float2(fminf(fabsf(p.x), 5.f), fminf(fabsf(p.y), 5.f));
+  float2 q = both(-6.862234727122996e-07f);
+  q = fma2(q, x, both(1.1530738447618205e-05f));
+  q = fma2(q, x, both(-4.327946589910425e-05f));
+  q = fma2(q, x, both(-0.0005067124147899449f));
+  q = fma2(q, x, both(0.007572786882519722f));
+  q = fma2(q, x, both(-0.05285993218421936f));
+  q = fma2(q, x, both(0.2622605562210083f));
+  q = fma2(q, x, both(-1.1511198282241821f));
+  q = fma2(q, x, both(-0.9999997019767761f));
+  const float2 e = mul2(mul2(p, p), both(-0.72134752f));
+  q = add2(q, e);
+  const float2 c = make_float2(exp2_approx(q.x), exp2_approx(q.y)), u = fma2(c, both(-1.f), both(1.f));
+  if (bell) *bell = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+  return make_float2(p.x < 0.f ? c.x : u.x, p.y < 0.f ? c.y : u.y);
+}
+
+__device__ __forceinline__ float2 sigmoid2(float2 p) {
+  const float2 e = mul2(p, both(-1.44269504f));
+  const float2 w = add2(make_float2(exp2_approx(e.x), exp2_approx(e.y)), both(1.f));
+  return make_float2(rcp_approx(w.x), rcp_approx(w.y));
+}
+
 template <int ACT>
-__device__ __forceinline__ float ff_act(float p) {
-  if constexpr (ACT == FF_RELU) return p <= 0.f ? 0.f : p;
-  if constexpr (ACT == FF_SILU) return __fdividef(p, 1.f + __expf(-p));
-  if constexpr (ACT == FF_GELU) return 0.5f * p * (1.f + erff(p * 0.70710678118654752f));
+__device__ __forceinline__ float2 ff_act(float2 p) {
+  if constexpr (ACT == FF_RELU) return make_float2(relu_nan(p.x), relu_nan(p.y));
+  if constexpr (ACT == FF_SILU) return mul2(p, sigmoid2(p));
+  if constexpr (ACT == FF_GELU) return mul2(p, normal_cdf2(p, nullptr));
   return p;
 }
 
 // act(p) and its derivative.
 template <int ACT>
-__device__ __forceinline__ void ff_act_both(float p, float& f, float& d) {
+__device__ __forceinline__ void ff_act_both(float2 p, float2& f, float2& d) {
   if constexpr (ACT == FF_RELU) {
-    f = p <= 0.f ? 0.f : p;
-    d = p > 0.f ? 1.f : 0.f;
+    f = make_float2(relu_nan(p.x), relu_nan(p.y));
+    d = make_float2(p.x > 0.f ? 1.f : 0.f, p.y > 0.f ? 1.f : 0.f);
   } else if constexpr (ACT == FF_SILU) {
-    const float s = __fdividef(1.f, 1.f + __expf(-p));
-    f = p * s;
-    d = s * (1.f + p * (1.f - s));
+    const float2 s = sigmoid2(p);
+    f = mul2(p, s);
+    d = fma2(f, fma2(s, both(-1.f), both(1.f)), s);  // s + p s (1 - s)
   } else if constexpr (ACT == FF_GELU) {
-    const float cdf = 0.5f * (1.f + erff(p * 0.70710678118654752f));
-    f = p * cdf;
-    d = cdf + p * 0.3989422804014327f * __expf(-0.5f * p * p);
+    float2 bell;
+    const float2 cdf = normal_cdf2(p, &bell);
+    f = mul2(p, cdf);
+    d = fma2(mul2(p, both(0.3989422804014327f)), bell, cdf);
   } else {
-    f = p, d = 1.f;
+    f = p, d = both(1.f);
   }
 }
 
@@ -102,31 +175,48 @@ __device__ __forceinline__ void ff_with_act(int act, F&& f) {
     f(std::integral_constant<int, FF_NONE>());
 }
 
-// n values: y = act(p) (+ r is the caller's), or dp in place.
+__device__ __forceinline__ float2 pair_of(const float* v, int i) { return make_float2(v[2 * i], v[2 * i + 1]); }
+__device__ __forceinline__ void put_pair(float* v, int i, float2 x) { v[2 * i] = x.x, v[2 * i + 1] = x.y; }
+
+// n values (even) of the forward pass, in place: p becomes act(p) or act(p) up(u).
 template <int EPI, int n>
-__device__ __forceinline__ void ff_values(const FfOut& e, float* p, float* u, const float* dy) {
-  ff_with_act(e.act, [&](auto a) {
-    constexpr int A = decltype(a)::value;
+__device__ __forceinline__ void ff_forward_values(const FfOut& e, float* p, float* u) {
+  if constexpr (EPI == FF_GATED) {
+    if (e.up_relu) {
 #pragma unroll
-    for (int i = 0; i < n; ++i) {
-      if constexpr (EPI == FF_ACT) {
-        p[i] = ff_act<A>(p[i]);
-      } else if constexpr (EPI == FF_ACT_BWD) {
-        float f, d;
-        ff_act_both<A>(p[i], f, d);
-        p[i] = dy[i] * d;
-      } else if constexpr (EPI == FF_GATED) {
-        p[i] = ff_act<A>(p[i]) * (e.up_relu && u[i] <= 0.f ? 0.f : u[i]);
-      } else if constexpr (EPI == FF_GATED_BWD) {
-        float f, d;
-        ff_act_both<A>(p[i], f, d);
-        const bool off = e.up_relu && !(u[i] > 0.f);
-        const float h = e.up_relu && u[i] <= 0.f ? 0.f : u[i];
-        p[i] = dy[i] * h * d;
-        u[i] = off ? 0.f : dy[i] * f;
-      }
+      for (int i = 0; i < n; ++i) u[i] = relu_nan(u[i]);
+    }
+  }
+  ff_with_act(e.act, [&](auto a) {
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) {
+      float2 f = ff_act<decltype(a)::value>(pair_of(p, i));
+      if constexpr (EPI == FF_GATED) f = mul2(f, pair_of(u, i));
+      put_pair(p, i, f);
     }
   });
+}
+
+// n values of the backward pass, in place: p becomes dp, or p and u become dg and du. dy(i) gives the pair i of dy.
+template <int EPI, int n, int ACT, typename DY>
+__device__ __forceinline__ void ff_backward_values(bool up_relu, float* p, float* u, DY&& dy) {
+#pragma unroll
+  for (int i = 0; i < n / 2; ++i) {
+    const float2 y = dy(i);
+    float2 f, d;
+    ff_act_both<ACT>(pair_of(p, i), f, d);
+    if constexpr (EPI == FF_ACT_BWD) {
+      put_pair(p, i, mul2(y, d));
+    } else {
+      float2 h = pair_of(u, i), du = mul2(y, f);
+      if (up_relu) {
+        du = make_float2(h.x > 0.f ? du.x : 0.f, h.y > 0.f ? du.y : 0.f);
+        h = make_float2(relu_nan(h.x), relu_nan(h.y));
+      }
+      put_pair(p, i, mul2(mul2(y, h), d));
+      put_pair(u, i, du);
+    }
+  }
 }
 
 __device__ __forceinline__ uint32_t ff_pack2(float a, float b, int half) {
@@ -142,85 +232,96 @@ __device__ __forceinline__ float2 ff_unpack2(uint32_t v, int half) {
   return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
 }
 __device__ __forceinline__ uint4 ff_pack8(const float* v, int half) {
-  return make_uint4(ff_pack2(v[0], v[1], half), ff_pack2(v[2], v[3], half), ff_pack2(v[4], v[5], half),
-                    ff_pack2(v[6], v[7], half));
+  if (half)
+    return make_uint4(ff_pack2(v[0], v[1], 1), ff_pack2(v[2], v[3], 1), ff_pack2(v[4], v[5], 1), ff_pack2(v[6], v[7], 1));
+  return make_uint4(ff_pack2(v[0], v[1], 0), ff_pack2(v[2], v[3], 0), ff_pack2(v[4], v[5], 0), ff_pack2(v[6], v[7], 0));
 }
 __device__ __forceinline__ void ff_unpack8(uint4 q, int half, float* v) {
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  if (half) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = ff_unpack2(w[i], half);
-    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    for (int i = 0; i < 4; ++i) put_pair(v, i, ff_unpack2(w[i], 1));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) put_pair(v, i, ff_unpack2(w[i], 0));
   }
 }
 
 // Adds the bias to 8 columns.
 __device__ __forceinline__ void ff_bias8(const FfOut& e, int s, int head, int col, float* v) {
   float b[8];
+  const long long at = (long long)head * e.N + col;
+  if (!e.bias[s]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) b[i] = e.bias0[s];
-  if (e.bias[s]) {
-    const long long at = (long long)head * e.N + col;
-    if (e.bias_f32) {
-      const float4* q = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(e.bias[s]) + at);
-      const float4 lo = __ldg(q), hi = __ldg(q + 1);
-      b[0] += lo.x, b[1] += lo.y, b[2] += lo.z, b[3] += lo.w, b[4] += hi.x, b[5] += hi.y, b[6] += hi.z, b[7] += hi.w;
-    } else {
-      float f[8];
-      ff_unpack8(__ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(e.bias[s]) + at)), e.half, f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) b[i] += f[i];
-    }
+    for (int i = 0; i < 8; ++i) b[i] = e.bias0[s];
+  } else if (e.bias_f32) {
+    const float4* q = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(e.bias[s]) + at);
+    const float4 lo = __ldg(q), hi = __ldg(q + 1);
+    b[0] = lo.x, b[1] = lo.y, b[2] = lo.z, b[3] = lo.w, b[4] = hi.x, b[5] = hi.y, b[6] = hi.z, b[7] = hi.w;
+  } else {
+    ff_unpack8(__ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(e.bias[s]) + at)), e.half, b);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] += b[i];
+  for (int i = 0; i < 4; ++i) put_pair(v, i, add2(pair_of(v, i), pair_of(b, i)));
 }
+
+__device__ __forceinline__ bool ff_has_bias(const FfOut& e, int s) { return e.bias[s] || e.bias0[s] != 0.f; }
 
 // ------------------------------------------------------------------------------- epilogue of 32 x 32 values a warp
 
-// A warp's 32 x 32 tile of 16-bit values in shared memory: rows of 64 bytes, their 16-byte pieces turned by the row, so
-// that a lane's row and four lanes' row are both free of bank conflicts. Global rows then move 64 bytes at a time.
+// A warp's 32 x 32 tile of 16-bit values in shared memory (2 KB): rows of 64 bytes, their 16-byte pieces turned by the
+// row, so that a lane's row and four lanes' row are both free of bank conflicts. Global rows then move 64 bytes at a time.
 __device__ __forceinline__ uint32_t ff_piece(int row, int q) { return (uint32_t)(row * 64 + ((q ^ ((row >> 1) & 3)) << 4)); }
 
 struct FfAux {
   uint4 v[4];
 };
 
-__device__ __forceinline__ FfAux ff_load_aux(const FfOut& e, int head, int row0, int col, int lane) {
-  FfAux a;
-  const int c = col + 8 * (lane & 3);
+__device__ __forceinline__ void ff_load_aux(FfAux& a, const FfOut& e, int head, int row0, int col, int lane) {
+  const int c = col + 8 * (lane & 3), r = row0 + lane / 4;
+  const uint16_t* src = reinterpret_cast<const uint16_t*>(e.aux) + (long long)r * e.aux_ld + (long long)head * e.aux_head + c;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = row0 + 8 * i + lane / 4;
     a.v[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (r < e.M && c < e.N)
-      a.v[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(e.aux) + (long long)r * e.aux_ld +
-                                               (long long)head * e.aux_head + c);
+    if (r + 8 * i < e.M && c < e.N) a.v[i] = *reinterpret_cast<const uint4*>(src + 8 * i * e.aux_ld);
   }
-  return a;
 }
 
 __device__ __forceinline__ void ff_put_aux(const FfAux& a, uint8_t* buf, int lane) {
+  __syncwarp();
 #pragma unroll
   for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(buf + ff_piece(8 * i + lane / 4, lane & 3)) = a.v[i];
+  __syncwarp();
 }
 
-// Rows [row0, row0 + 32) x 32 columns from the lanes' rows.
-__device__ __forceinline__ void ff_store_tile(const FfOut& e, void* out, long long ld, long long head_stride, int head,
-                                              const float* v, int row0, int col, uint8_t* buf, int lane) {
+// Rows [row0, row0 + 32) x 32 columns from the lanes' rows of packed values.
+__device__ __forceinline__ void ff_store_packed(const FfOut& e, void* out, long long ld, long long head_stride, int head,
+                                                uint4 (&w)[4], int row0, int col, uint8_t* buf, int lane) {
   __syncwarp();
 #pragma unroll
-  for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(buf + ff_piece(lane, q)) = ff_pack8(v + 8 * q, e.half);
+  for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(buf + ff_piece(lane, q)) = w[q];
   __syncwarp();
-  const int c = col + 8 * (lane & 3);
+  const int c = col + 8 * (lane & 3), r = lane / 4;
+  uint16_t* o = reinterpret_cast<uint16_t*>(out) + (long long)(row0 + r) * ld + (long long)head * head_stride + c;
+  const int rows = c < e.N ? e.M - row0 - r : 0;  // 8 i below it
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = 8 * i + lane / 4;
-    const uint4 w = *reinterpret_cast<const uint4*>(buf + ff_piece(r, lane & 3));
-    if (row0 + r < e.M && c < e.N)
-      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + (long long)(row0 + r) * ld + (long long)head * head_stride +
-                                c) = w;
+    w[i] = *reinterpret_cast<const uint4*>(buf + ff_piece(8 * i + r, lane & 3));
+    if (8 * i < rows) *reinterpret_cast<uint4*>(o + 8 * i * ld) = w[i];
   }
+}
+
+__device__ __forceinline__ void ff_store_tile(const FfOut& e, void* out, long long ld, long long head_stride, int head,
+                                              const float* v, int row0, int col, uint8_t* buf, int lane) {
+  uint4 w[4];
+  if (e.half) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) w[q] = ff_pack8(v + 8 * q, 1);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) w[q] = ff_pack8(v + 8 * q, 0);
+  }
+  ff_store_packed(e, out, ld, head_stride, head, w, row0, col, buf, lane);
 }
 
 // The lane's row of 32 pre-activations in 8 bits. Columns past N count as zeros.
@@ -242,10 +343,16 @@ __device__ __forceinline__ void ff_hold8(const FfOut& e, int s, int head, const 
   e.exponents[s][rh * nb + col / 32] = (uint8_t)(ex + 127);
 }
 
-// Sum over the warp's 32 rows (a row a lane) of 32 columns: lane l gets column l's. v is used up. The order is fixed.
+// Sums over the warp's 32 rows (a row a lane) of n = 16 or 32 columns: lane l gets column l % n's. v is used up. The
+// order is fixed.
+template <int n>
 __device__ __forceinline__ float ff_column_sum(float* v, int lane) {
+  if constexpr (n == 16) {
 #pragma unroll
-  for (int o = 16; o > 0; o /= 2) {
+    for (int i = 0; i < 16; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 16);
+  }
+#pragma unroll
+  for (int o = n / 2; o > 0; o /= 2) {
     const bool hi = (lane & o) != 0;
 #pragma unroll
     for (int i = 0; i < o; ++i) {
@@ -256,108 +363,178 @@ __device__ __forceinline__ float ff_column_sum(float* v, int lane) {
   return v[0];
 }
 
+template <int n>
 __device__ __forceinline__ void ff_put_sums(const FfOut& e, int s, int head, float* v, int row0, int col, int lane) {
   const bool in = row0 + lane < e.M;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = in ? v[i] : 0.f;
-  const float sum = ff_column_sum(v, lane);
-  if (col + lane < e.N) e.colsum[s][((long long)(row0 / 32) * e.heads + head) * e.N + col + lane] = sum;
+  for (int i = 0; i < n; ++i) v[i] = in ? v[i] : 0.f;
+  const float sum = ff_column_sum<n>(v, lane);
+  if (lane < n && col + lane < e.N) e.colsum[s][((long long)(row0 / 32) * e.heads + head) * e.N + col + lane] = sum;
 }
 
-// g, u: the lane's row of the products (u unused where there is one).
 template <int EPI>
-__device__ __forceinline__ void ff_epilogue(const FfOut& e, int set, int head, int row0, int col, float* g, float* u,
-                                            uint8_t* buf, int lane) {
+__device__ __forceinline__ bool ff_has_aux(const FfOut& e) {
+  return ff_backward(EPI) || (EPI == FF_ACT && e.aux != nullptr);
+}
+
+// 16 columns of one or both accumulators, one wait.
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                 "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(at));
+}
+template <int NB>
+__device__ __forceinline__ void ff_read16(uint32_t g_at, float (&g)[16], uint32_t u_at, float (&u)[16]) {
+  uint32_t a[16], b[16];
+  tmem_ld16(g_at, a);
+  if constexpr (NB == 2) tmem_ld16(u_at, b);
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    g[i] = __uint_as_float(a[i]);
+    if constexpr (NB == 2) u[i] = __uint_as_float(b[i]);
+  }
+}
+
+template <int n>
+__device__ __forceinline__ void ff_add_bias(const FfOut& e, int s, int head, int col, float* v) {
+  if (!ff_has_bias(e, s)) return;
+#pragma unroll
+  for (int q = 0; q < n / 8; ++q)
+    if (col + 8 * q < e.N) ff_bias8(e, s, head, col + 8 * q, v + 8 * q);
+}
+
+// A warp's 32 x 32 chunk. g_at, u_at: its accumulators (one or two); aux: r or dy, as ff_load_aux left it; release:
+// called once the accumulators have been read. The arithmetic goes over 16 columns at a time: sixteen warps leave a thread 96
+// registers, and with both products of 32 columns in them spills wrote as many bytes as the results.
+template <int EPI, typename R>
+__device__ __forceinline__ void ff_epilogue(const FfOut& e, int set, int head, int row0, int col, uint32_t g_at,
+                                            uint32_t u_at, const FfAux& aux, uint8_t* buf, int lane, R&& release) {
   constexpr int NB = ff_products(EPI);
   if constexpr (EPI == FF_STORE) {
+    float g[32];
+    tmem_ld32(g_at, g);
+    release();
     ff_store_tile(e, e.out[set], e.ld, e.head, head, g, row0, col, buf, lane);
     return;
   } else {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      if (col + 8 * q < e.N) {
-        ff_bias8(e, 0, head, col + 8 * q, g + 8 * q);
-        if constexpr (NB == 2) ff_bias8(e, 1, head, col + 8 * q, u + 8 * q);
-      }
-    }
-    const bool has_aux = ff_backward(EPI) || (EPI == FF_ACT && e.aux);
-    FfAux aux;
-    if (has_aux) aux = ff_load_aux(e, head, row0, col, lane);
     if constexpr (!ff_backward(EPI)) {
-      const long long hl = (long long)e.heads * e.N;
-      if (e.keep == FF_KEEP_16) {
-        ff_store_tile(e, e.held[0], hl, e.N, head, g, row0, col, buf, lane);
-        if constexpr (NB == 2) ff_store_tile(e, e.held[1], hl, e.N, head, u, row0, col, buf, lane);
-      } else if (e.keep == FF_KEEP_8) {
-        ff_hold8(e, 0, head, g, row0 + lane, col);
-        if constexpr (NB == 2) ff_hold8(e, 1, head, u, row0 + lane, col);
+      if (e.keep != FF_KEEP_NOTHING) {
+#pragma unroll
+        for (int s = 0; s < NB; ++s) {
+          float v[32];
+          tmem_ld32(s ? u_at : g_at, v);
+          ff_add_bias<32>(e, s, head, col, v);
+          if (e.keep == FF_KEEP_16)
+            ff_store_tile(e, e.held[s], (long long)e.heads * e.N, e.N, head, v, row0, col, buf, lane);
+          else
+            ff_hold8(e, s, head, v, row0 + lane, col);
+        }
       }
     }
-    float a[32];
-    if (has_aux) {
-      ff_put_aux(aux, buf + 2048, lane);
-      __syncwarp();
+    const bool has_aux = ff_has_aux<EPI>(e);
+    if (has_aux) ff_put_aux(aux, buf, lane);
+    uint4 pg[4], pu[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        ff_unpack8(*reinterpret_cast<const uint4*>(buf + 2048 + ff_piece(lane, q)), e.half, a + 8 * q);
-    }
-    ff_values<EPI, 32>(e, g, u, a);
-    if constexpr (EPI == FF_ACT) {
-      if (has_aux) {
+    for (int h = 0; h < 2; ++h) {
+      float g[16], u[16];
+      ff_read16<NB>(g_at + 16 * h, g, u_at + 16 * h, u);
+      if (h == 1) release();
+      const int c = col + 16 * h;
+      ff_add_bias<16>(e, 0, head, c, g);
+      if constexpr (NB == 2) ff_add_bias<16>(e, 1, head, c, u);
+      if constexpr (ff_backward(EPI)) {
+        ff_with_act(e.act, [&](auto a) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) g[i] += a[i];
+          for (int q = 0; q < 2; ++q) {
+            float y[8];
+            ff_unpack8(*reinterpret_cast<const uint4*>(buf + ff_piece(lane, 2 * h + q)), e.half, y);
+            ff_backward_values<EPI, 8, decltype(a)::value>(e.up_relu, g + 8 * q, u + 8 * q, [&](int i) { return pair_of(y, i); });
+          }
+        });
+      } else {
+        ff_forward_values<EPI, 16>(e, g, u);
+        if (EPI == FF_ACT && has_aux) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            float a[8];
+            ff_unpack8(*reinterpret_cast<const uint4*>(buf + ff_piece(lane, 2 * h + q)), e.half, a);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) put_pair(g + 8 * q, i, add2(pair_of(g + 8 * q, i), pair_of(a, i)));
+          }
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        pg[2 * h + q] = ff_pack8(g + 8 * q, e.half);
+        if constexpr (EPI == FF_GATED_BWD) pu[2 * h + q] = ff_pack8(u + 8 * q, e.half);
+      }
+      if constexpr (ff_backward(EPI)) {
+        if (e.colsum[0]) ff_put_sums<16>(e, 0, head, g, row0, c, lane);
+        if constexpr (NB == 2)
+          if (e.colsum[1]) ff_put_sums<16>(e, 1, head, u, row0, c, lane);
       }
     }
-    ff_store_tile(e, e.out[0], e.ld, e.head, head, g, row0, col, buf, lane);
-    if constexpr (EPI == FF_GATED_BWD) ff_store_tile(e, e.out[1], e.ld, e.head, head, u, row0, col, buf, lane);
-    if constexpr (ff_backward(EPI)) {
-      if (e.colsum[0]) ff_put_sums(e, 0, head, g, row0, col, lane);
-      if constexpr (NB == 2)
-        if (e.colsum[1]) ff_put_sums(e, 1, head, u, row0, col, lane);
-    }
+    ff_store_packed(e, e.out[0], e.ld, e.head, head, pg, row0, col, buf, lane);
+    if constexpr (EPI == FF_GATED_BWD) ff_store_packed(e, e.out[1], e.ld, e.head, head, pu, row0, col, buf, lane);
   }
 }
 
 // ------------------------------------------------------------------------------- products
 
-constexpr int kFfEpiWarps = 8;
-constexpr int kFfThreads = 64 + 32 * kFfEpiWarps;
 
-template <int NB, int BN, bool PAIR>
+constexpr int kFfResident = 4;  // blocks of a reduction whose A stays in shared memory
+
+// RES: the whole reduction of a tile's A rows stays in shared memory over a run of tiles in the same rows.
+template <int NB, int BN, bool PAIR, bool RES>
 struct FfCfg {
   static constexpr int CTAS = PAIR ? 2 : 1;
   static constexpr int B_ROWS = BN / CTAS;  // of one product, staged by this CTA
   static constexpr int A_BYTES = 128 * 64 * 2, B_BYTES = B_ROWS * 64 * 2;
-  static constexpr int STAGE_BYTES = NB * (A_BYTES + B_BYTES);
-  static constexpr int EPI_BYTES = kFfEpiWarps * 4096;
-  static constexpr int STAGES = (192 * 1024) / STAGE_BYTES;
-  static constexpr int SMEM = STAGES * STAGE_BYTES + EPI_BYTES + 1024;
+  static constexpr int A_ROOM = RES ? NB * kFfResident * A_BYTES : 0;
+  static constexpr int STAGE_BYTES = NB * ((RES ? 0 : A_BYTES) + B_BYTES);
+  // Sixteen epilogue warps, four a scheduler: with eight the epilogue of 2 x 128 columns was bound by its own latencies
+  // (gated, 4099 rows, 4 x 256 -> 8192: 240 us).
+  static constexpr int EPI_WARPS = BN >= 128 ? 16 : 8;
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int EPI_BYTES = EPI_WARPS * 2048;
+  static constexpr int STAGES = (192 * 1024 - A_ROOM) / STAGE_BYTES;
+  static constexpr int SMEM = A_ROOM + STAGES * STAGE_BYTES + EPI_BYTES + 1024;
   static constexpr int TMEM_COLS = 2 * NB * BN;
   static_assert(B_ROWS % 64 == 0 && TMEM_COLS <= 512 && SMEM <= 227 * 1024, "tile");
 };
 
-// The tiles of a CTA (or pair), t, t + step, ...: columns fastest, then rows, parts, heads, sets. Divided once.
+// The tiles of a CTA (or pair): columns fastest, then rows, parts, heads, sets. Worker w of W takes w, w + W, ..., or,
+// with RES, a run of tiles on end, so that its rows change once or twice. Divided once; the digits of the step are the host's.
 struct FfWalk {
-  unsigned at[4], by[4], size[4], set, bset;
+  unsigned at[4], set, count;
 
-  __device__ __forceinline__ FfWalk(const FfGemm& p, unsigned t, unsigned step) {
-    size[0] = p.tiles_n, size[1] = p.tiles_m, size[2] = p.splits, size[3] = p.e.heads;
+  __device__ __forceinline__ FfWalk(const FfGemm& p, unsigned worker, unsigned workers, bool runs) {
+    const unsigned total = (unsigned)(p.tiles_m * p.tiles_n * p.splits * p.e.heads * p.out_sets);
+    unsigned t = worker;
+    if (runs) {
+      t = (unsigned)((unsigned long long)total * worker / workers);
+      count = (unsigned)((unsigned long long)total * (worker + 1) / workers) - t;
+    } else {
+      count = worker < total ? (total - worker + workers - 1) / workers : 0;
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      at[i] = t % size[i], by[i] = step % size[i];
-      t /= size[i], step /= size[i];
+      at[i] = t % p.size[i];
+      t /= p.size[i];
     }
-    set = t, bset = step;
+    set = t;
   }
-  __device__ __forceinline__ void next() {
+  __device__ __forceinline__ void next(const FfGemm& p) {
     unsigned carry = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      at[i] += by[i] + carry;
-      carry = at[i] >= size[i] ? 1 : 0;
-      at[i] -= carry ? size[i] : 0;
+      at[i] += p.step[i] + carry;
+      carry = at[i] >= p.size[i] ? 1 : 0;
+      at[i] -= carry ? p.size[i] : 0;
     }
-    set += bset + carry;
+    set += p.step[4] + carry;
   }
   __device__ __forceinline__ int n() const { return (int)at[0]; }
   __device__ __forceinline__ int m() const { return (int)at[1]; }
@@ -370,6 +547,12 @@ __device__ __forceinline__ void ff_part(const FfGemm& p, int split, int& b0, int
   const unsigned blocks = (unsigned)(p.segments * p.KB);  // times the parts below 2^32: the host checks
   b0 = (int)(blocks * (unsigned)split / (unsigned)p.splits);
   b1 = (int)(blocks * (unsigned)(split + 1) / (unsigned)p.splits);
+}
+
+// Without release semantics, which would wait for this thread's global stores: what the other side waits for are loads
+// from TMEM, and those are done.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 template <bool PAIR>
@@ -392,30 +575,34 @@ __device__ __forceinline__ void ff_load(void* dst, const CUtensorMap* m, bool mn
   }
 }
 
-template <int EPI, int BN, bool PAIR>
-__global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_constant__ FfGemm p) {
+template <int EPI, int BN, bool PAIR, bool RES>
+__global__ void __launch_bounds__(FfCfg<ff_products(EPI), BN, PAIR, RES>::THREADS, 1)
+    ff_gemm_kernel(const __grid_constant__ FfGemm p) {
   constexpr int NB = ff_products(EPI);
-  using Cfg = FfCfg<NB, BN, PAIR>;
+  using Cfg = FfCfg<NB, BN, PAIR, RES>;
   constexpr int STAGES = Cfg::STAGES, ROWS = 128 * Cfg::CTAS;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES];
-  __shared__ uint64_t tfull_bar[2], tempty_bar[2], drain_bar;
+  __shared__ uint64_t tfull_bar[2], tempty_bar[2], drain_bar, afull_bar, aempty_bar;
   __shared__ uint32_t tmem_base_s;
   __shared__ volatile int abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int crank = PAIR ? (int)cluster_ctarank() : 0;
   const bool leader = crank == 0;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sEpi = smem + STAGES * Cfg::STAGE_BYTES;
+  uint8_t* sRing = smem + Cfg::A_ROOM;
+  uint8_t* sEpi = sRing + STAGES * Cfg::STAGE_BYTES;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
+    mbar_init(&afull_bar, 1);
+    mbar_init(&aempty_bar, 1);
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull_bar[a], 1);
-      mbar_init(&tempty_bar[a], Cfg::CTAS * kFfEpiWarps);
+      mbar_init(&tempty_bar[a], Cfg::CTAS * Cfg::EPI_WARPS);
     }
     mbar_init(&drain_bar, 1);
     fence_barrier_init();
@@ -436,7 +623,6 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_s;
   const unsigned worker = blockIdx.x / Cfg::CTAS, workers = gridDim.x / Cfg::CTAS;
-  const unsigned total = (unsigned)(p.tiles_m * p.tiles_n * p.splits * p.e.heads * p.out_sets);
 
   if (warp == 0) {
     if (lane == 0) {
@@ -445,11 +631,30 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
       uint32_t phase = 0;
       long long issued = 0;
       bool ok = true;
-      const uint32_t bytes = (uint32_t)(Cfg::CTAS * ((NB == 2 && !p.two_a ? 1 : NB) * Cfg::A_BYTES + NB * Cfg::B_BYTES));
-      FfWalk w(p, worker, workers);
-      for (unsigned t = worker; t < total && ok; t += workers, w.next()) {
+      const int a_count = NB == 2 && !p.two_a ? 1 : NB;
+      const uint32_t bytes = (uint32_t)(Cfg::CTAS * ((RES ? 0 : a_count * Cfg::A_BYTES) + NB * Cfg::B_BYTES));
+      unsigned rows_of = ~0u;  // RES: the rows and head whose A is there
+      uint32_t a_phase = 0;
+      FfWalk w(p, worker, workers, RES);
+      for (unsigned t = 0; t < w.count && ok; ++t, w.next(p)) {
         int b0, b1;
         ff_part(p, w.split(), b0, b1);
+        if constexpr (RES) {
+          const unsigned rows = w.at[1] + w.at[3] * p.size[1];
+          if (rows != rows_of) {
+            if (!mbar_wait_bounded(&aempty_bar, a_phase ^ 1, &abort_flag, p.err, kErrTimeoutProducer)) {
+              ok = false;
+              break;
+            }
+            if (leader) mbar_arrive_expect_tx(&afull_bar, (uint32_t)(Cfg::CTAS * a_count * p.KB * Cfg::A_BYTES));
+            for (int s = 0; s < a_count; ++s)
+              for (int kb = 0; kb < p.KB; ++kb)
+                ff_load<PAIR, 128>(smem + (s * p.KB + kb) * Cfg::A_BYTES, &p.ta[s], false, &afull_bar,
+                                   w.m() * ROWS + 128 * crank, kb * 64, (p.a_heads >> s) & 1 ? w.head() : 0);
+            a_phase ^= 1;
+            rows_of = rows;
+          }
+        }
         const int am = w.m() * ROWS + 128 * crank, bn = w.n() * BN + Cfg::B_ROWS * crank;
         int seg = b0 / p.KB, kb = b0 - seg * p.KB;
         for (int i = b0; i < b1; ++i) {
@@ -463,9 +668,12 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
           }
           uint64_t* bar = &full_bar[stage];
           if (leader) mbar_arrive_expect_tx(bar, bytes);
-          uint8_t* dst = smem + stage * Cfg::STAGE_BYTES;
+          uint8_t* dst = sRing + stage * Cfg::STAGE_BYTES;
           const int k = kb * 64;
-          if constexpr (NB == 1) {
+          if constexpr (RES) {
+            ff_load<PAIR, Cfg::B_ROWS>(dst, &p.tb[0], (p.b_mn & 1) != 0, bar, bn, k, head);
+            if constexpr (NB == 2) ff_load<PAIR, Cfg::B_ROWS>(dst + Cfg::B_BYTES, &p.tb[1], (p.b_mn & 2) != 0, bar, bn, k, head);
+          } else if constexpr (NB == 1) {
             ff_load<PAIR, 128>(dst, &p.ta[set], p.a_mn, bar, am, k, (p.a_heads >> set) & 1 ? head : 0);
             ff_load<PAIR, Cfg::B_ROWS>(dst + Cfg::A_BYTES, &p.tb[set], p.b_mn, bar, bn, k, (p.b_heads >> set) & 1 ? head : 0);
           } else {
@@ -495,6 +703,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
           }
           mbar_wait_bounded(&full_bar[s], ph, (volatile int*)&dummy_abort, p.err, kErrTimeoutDrain);
         }
+        if (RES && rows_of != ~0u) mbar_wait_bounded(&afull_bar, a_phase ^ 1, (volatile int*)&dummy_abort, p.err, kErrTimeoutDrain);
       }
     }
   } else if (warp == 1) {
@@ -503,10 +712,29 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      FfWalk w(p, worker, workers);
-      for (unsigned t = worker; t < total && ok; t += workers, w.next()) {
+      unsigned rows_of = ~0u;
+      uint32_t a_phase = 0;
+      FfWalk w(p, worker, workers, RES);
+      for (unsigned t = 0; t < w.count && ok; ++t, w.next(p)) {
         int b0, b1;
         ff_part(p, w.split(), b0, b1);
+        if constexpr (RES) {
+          const unsigned rows = w.at[1] + w.at[3] * p.size[1];
+          if (rows != rows_of) {
+            if (rows_of != ~0u) {  // once the products issued so far are done, other rows may take A's place
+              if constexpr (PAIR)
+                umma_commit_pair(&aempty_bar);
+              else
+                umma_commit(&aempty_bar);
+            }
+            if (!mbar_wait_bounded(&afull_bar, a_phase, &abort_flag, p.err, kErrTimeoutMma)) {
+              ok = false;
+              break;
+            }
+            a_phase ^= 1;
+            rows_of = rows;
+          }
+        }
         if (!mbar_wait_bounded(&tempty_bar[acc], acc_phase ^ 1, &abort_flag, p.err, kErrTimeoutMma)) {
           ok = false;
           break;
@@ -518,12 +746,14 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
             break;
           }
           tc_fence_after();
-          const uint32_t base = smem_u32(smem + stage * Cfg::STAGE_BYTES);
+          const uint32_t base = smem_u32(sRing + stage * Cfg::STAGE_BYTES);
+          const uint32_t a_at = RES ? smem_u32(smem + (i - b0) * Cfg::A_BYTES) : base;
+          const uint32_t a_next = RES ? (uint32_t)(p.KB * Cfg::A_BYTES) : (uint32_t)Cfg::A_BYTES;
 #pragma unroll
           for (int s = 0; s < NB; ++s) {
             const bool b_mn = NB == 1 ? p.b_mn != 0 : (p.b_mn & (1 << s)) != 0;
-            const uint32_t a_base = base + (s == 1 && p.two_a ? Cfg::A_BYTES : 0);
-            const uint32_t b_base = base + NB * Cfg::A_BYTES + s * Cfg::B_BYTES;
+            const uint32_t a_base = a_at + (s == 1 && p.two_a ? a_next : 0);
+            const uint32_t b_base = base + (RES ? 0 : NB * Cfg::A_BYTES) + s * Cfg::B_BYTES;
             const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
             const uint32_t a_lbo = p.a_mn ? 8192 : 16, b_lbo = b_mn ? 8192 : 16;
             const uint32_t idesc = p.idesc | (b_mn ? 1u << 16 : 0u);
@@ -568,32 +798,57 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
   } else {
     // ------------------------------------------------ epilogue (each CTA its own 128 rows)
     const int quad = warp & 3;         // TMEM lane quadrant of this warp
-    const int half = (warp - 2) >> 2;  // half of the tile's columns
-    uint8_t* buf = sEpi + (warp - 2) * 4096;
-    constexpr int COLS = BN / 2;
-    const int col0 = half * COLS;
+    const int part = (warp - 2) >> 2;  // its share of the tile's columns
+    uint8_t* buf = sEpi + (warp - 2) * 2048;
+    constexpr int COLS = BN * 4 / Cfg::EPI_WARPS;
+    static_assert(COLS % 32 == 0, "a chunk is 32 columns");
+    const int col0 = part * COLS;
     uint32_t leader_tempty0 = 0, leader_tempty1 = 0;
     if constexpr (PAIR) leader_tempty0 = map_to_cta(&tempty_bar[0], 0), leader_tempty1 = map_to_cta(&tempty_bar[1], 0);
     int acc = 0;
     uint32_t acc_phase = 0;
-    FfWalk w(p, worker, workers);
-    for (unsigned t = worker; t < total; t += workers, w.next()) {
+    FfWalk w(p, worker, workers, RES);
+    for (unsigned t = 0; t < w.count; ++t, w.next(p)) {
+      const int row0 = w.m() * ROWS + 128 * crank + quad * 32, first = w.n() * BN + col0;
+      const bool one = p.splits == 1;
+      FfAux aux;  // of the first chunk: on its way while the products are
+      if (one && ff_has_aux<EPI>(p.e)) ff_load_aux(aux, p.e, w.head(), row0, first, lane);
       // the same answer for the whole warp: the loads from TMEM need all of its lanes, also where a wait has run out
       if (!__all_sync(0xffffffffu, mbar_wait_bounded(&tfull_bar[acc], acc_phase, &abort_flag, p.err, kErrTimeoutEpilogue)))
         break;
       tc_fence_after();
-      const int row0 = w.m() * ROWS + 128 * crank + quad * 32;
+      // The accumulators go back as soon as this warp has its values in registers.
+      bool held = true;
+      auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (leader)
+            mbar_arrive(&tempty_bar[acc]);
+          else
+            mbar_arrive_cluster_relaxed(acc ? leader_tempty1 : leader_tempty0);
+        }
+        held = false;
+      };
+      const int cols = row0 < p.e.M ? min(COLS, p.e.N - first) : 0;
 #pragma unroll 1
-      for (int cc = 0; cc < COLS; cc += 32) {
-        const int col = w.n() * BN + col0 + cc;
-        if (row0 >= p.e.M || col >= p.e.N) continue;
+      for (int cc = 0; cc < cols; cc += 32) {
+        const int col = first + cc;
+        const bool last = cc + 32 >= cols;
         const uint32_t at = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * NB * BN + col0 + cc;
+        if (cc > 0 && one && ff_has_aux<EPI>(p.e)) ff_load_aux(aux, p.e, w.head(), row0, col, lane);
+        auto give_back = [&] {
+          if (last) release();
+        };
+        if (one) {
+          ff_epilogue<EPI>(p.e, (int)w.set, w.head(), row0, col, at, at + BN, aux, buf, lane, give_back);
+          continue;
+        }
         float g[32], u[32];
         tmem_ld32(at, g);
         if constexpr (NB == 2) tmem_ld32(at + BN, u);
-        if (p.splits == 1) {
-          ff_epilogue<EPI>(p.e, (int)w.set, w.head(), row0, col, g, u, buf, lane);
-        } else if (row0 + lane < p.e.M) {
+        give_back();
+        if (row0 + lane < p.e.M) {
 #pragma unroll
           for (int s = 0; s < NB; ++s) {
             const float* v = s ? u : g;
@@ -606,14 +861,7 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
           }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (leader)
-          mbar_arrive(&tempty_bar[acc]);
-        else
-          mbar_arrive_cluster(acc ? leader_tempty1 : leader_tempty0);
-      }
+      if (held) release();
       if (++acc == 2) {
         acc = 0;
         acc_phase ^= 1;
@@ -635,11 +883,13 @@ __global__ void __launch_bounds__(kFfThreads, 1) ff_gemm_kernel(const __grid_con
 }  // namespace bd
 
 namespace bd {
-// The tile of a launch: PAIR and BN. feed_forward_{a,b}.cu hold the instantiations.
+// The tile of a launch: PAIR, BN and RES. feed_forward_{a,b}.cu hold the instantiations.
 struct FfTile {
   bool pair;
   int bn;
+  bool resident;
 };
+inline int64_t ff_workers(int64_t tiles, FfTile t, int sms) { return std::min<int64_t>(tiles, sms / (t.pair ? 2 : 1)); }
 void ff_launch_one(int epi, FfTile tile, const FfGemm& p, cudaStream_t st, int dev);    // one product
 void ff_launch_gated(int epi, FfTile tile, const FfGemm& p, cudaStream_t st, int dev);  // two
 }  // namespace bd

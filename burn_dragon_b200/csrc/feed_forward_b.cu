@@ -8,11 +8,23 @@
 
 namespace bd {
 
+namespace {
+template <int EPI>
+void go(FfTile t, const FfGemm& p, cudaStream_t st, int dev) {
+  if (t.resident)
+    ff_launch<EPI, 128, true, true>(p, st, dev);
+  else if (t.pair)
+    ff_launch<EPI, 128, true>(p, st, dev);
+  else
+    ff_launch<EPI, 64, false>(p, st, dev);
+}
+}  // namespace
+
 void ff_launch_gated(int epi, FfTile t, const FfGemm& p, cudaStream_t st, int dev) {
   if (epi == FF_GATED)
-    t.pair ? ff_launch<FF_GATED, 128, true>(p, st, dev) : ff_launch<FF_GATED, 64, false>(p, st, dev);
+    go<FF_GATED>(t, p, st, dev);
   else
-    t.pair ? ff_launch<FF_GATED_BWD, 128, true>(p, st, dev) : ff_launch<FF_GATED_BWD, 64, false>(p, st, dev);
+    go<FF_GATED_BWD>(t, p, st, dev);
 }
 
 }  // namespace bd
