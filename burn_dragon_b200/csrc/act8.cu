@@ -30,6 +30,111 @@ constexpr float limit_of() {
   return sizeof(T) == 4 ? kAct8LimitF32 : std::is_same<T, __half>::value ? kAct8LimitF16 : kAct8LimitBF16;
 }
 
+// 8 values of a row a thread and step, four threads a block; kUnits steps are read before the first is coded.
+// FLAT: rows are whole blocks, so that the tensor is one row. Else N is a multiple of 8.
+constexpr int kUnits = 4;
+
+template <typename T>
+struct Eight {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void get(float* f) const {
+    const T* t = reinterpret_cast<const T*>(v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = as_float(t[i]);
+  }
+  __device__ __forceinline__ void put(const float* f) {
+    T* t = reinterpret_cast<T*>(v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = from_float<T>(f[i]);
+  }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, v[i]);
+  }
+};
+
+// Where unit u (4 a block) lies: its first value, its block, and whether it has values.
+template <bool FLAT>
+__device__ __forceinline__ bool unit_at(long long u, long long units, int N, int nb, long long& at, long long& block) {
+  block = u / 4;
+  if constexpr (FLAT) {
+    at = u * 8;
+    return u < units;
+  } else {
+    const long long r = block / nb;
+    const int c = (int)(u - r * 4 * nb) * 8;
+    at = r * N + c;
+    return u < units && c < N;
+  }
+}
+
+template <typename T, bool FLAT>
+__global__ void __launch_bounds__(256) act8_pack8_kernel(const T* __restrict__ x, long long units, int N, int nb,
+                                                         uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  const long long first = (long long)blockIdx.x * (256 * kUnits) + threadIdx.x;
+  Eight<T> raw[kUnits];
+  long long at[kUnits], block[kUnits];
+  bool in[kUnits];
+#pragma unroll
+  for (int k = 0; k < kUnits; ++k) {
+    in[k] = unit_at<FLAT>(first + 256 * k, units, N, nb, at[k], block[k]);
+    if (in[k]) raw[k].load(x + at[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < kUnits; ++k) {
+    float f[8], largest = 0.f;
+    if (in[k]) {
+      raw[k].get(f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) largest = fmaxf(largest, act8_size(f[i]));
+    }
+    largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+    largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+    if (!in[k]) continue;
+    const int e = act8_exponent(largest);
+    const float inverse = act8_power(-e);
+    __stcs(reinterpret_cast<uint2*>(codes + at[k]), make_uint2(act8_code4(f, inverse), act8_code4(f + 4, inverse)));
+    if (threadIdx.x % 4 == 0) scales[block[k]] = (uint8_t)(e + 127);
+  }
+}
+
+template <typename T, bool FLAT>
+__global__ void __launch_bounds__(256) act8_unpack8_kernel(const uint8_t* __restrict__ codes,
+                                                           const uint8_t* __restrict__ scales, long long units, int N,
+                                                           int nb, T* __restrict__ y) {
+  const long long first = (long long)blockIdx.x * (256 * kUnits) + threadIdx.x;
+  uint2 raw[kUnits];
+  uint8_t scale[kUnits];
+  long long at[kUnits], block[kUnits];
+  bool in[kUnits];
+#pragma unroll
+  for (int k = 0; k < kUnits; ++k) {
+    in[k] = unit_at<FLAT>(first + 256 * k, units, N, nb, at[k], block[k]);
+    if (in[k]) {
+      raw[k] = __ldcs(reinterpret_cast<const uint2*>(codes + at[k]));
+      scale[k] = scales[block[k]];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kUnits; ++k) {
+    if (!in[k]) continue;
+    const float power = act8_power((int)scale[k] - 127);
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = act8_value2(((i < 2 ? raw[k].x : raw[k].y) >> (16 * (i & 1))) & 0xFFFFu, power, limit_of<T>());
+      f[2 * i] = v.x, f[2 * i + 1] = v.y;
+    }
+    Eight<T> out;
+    out.put(f);
+    out.store(y + at[k]);
+  }
+}
+
 // A block of 32 a warp, a value a lane: any N.
 template <typename T>
 __global__ void __launch_bounds__(256) act8_pack_kernel(const T* __restrict__ x, long long R, int N, int nb,
@@ -76,29 +181,46 @@ void for_type(at::ScalarType t, F&& f) {
 
 unsigned grid_of(long long blocks) { return (unsigned)std::max<long long>(1, std::min<long long>((blocks + 7) / 8, 148 * 32)); }
 
+bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+unsigned unit_grid(long long units) {
+  const long long grid = (units + 256 * kUnits - 1) / (256 * kUnits);
+  TORCH_CHECK(grid < (1ll << 31), "act8: too many values");
+  return (unsigned)grid;
+}
+
 }  // namespace
 
-// x [R, N] contiguous -> codes [R, N] and exponents [R, ceil(N / 32)], uint8.
-std::vector<at::Tensor> act8_pack(const at::Tensor& x) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.is_contiguous(), "act8_pack: contiguous rows [R, N] on a GPU");
-  const int64_t R = x.size(0), N = x.size(1), nb = (N + 31) / 32;
+// x, of any shape: codes [R, N] and exponents [R, ceil(N / 32)], uint8, N its last dimension (of at least one value).
+std::vector<at::Tensor> act8_pack(const at::Tensor& given) {
+  TORCH_CHECK(given.is_cuda(), "act8_pack: values on a GPU");
+  c10::cuda::CUDAGuard guard(given.get_device());
+  const at::Tensor x = given.contiguous();
+  const int64_t N = x.numel() == 0 || x.dim() == 0 ? 1 : x.size(-1), R = x.numel() / N, nb = (N + 31) / 32;
   TORCH_CHECK(N < (1ll << 31) - 32, "act8_pack: rows of less than 2^31 - 32 values");
-  c10::cuda::CUDAGuard guard(x.get_device());
   auto st = at::cuda::getCurrentCUDAStream(x.get_device()).stream();
-  at::Tensor codes = at::empty({R, N}, x.options().dtype(at::kByte)), scales = at::empty({R, nb}, codes.options());
+  const auto bytes = x.options().dtype(at::kByte).requires_grad(false);
+  at::Tensor codes = at::empty({R, N}, bytes), scales = at::empty({R, nb}, bytes);
   if (x.numel() == 0) return {codes, scales};
   for_type(x.scalar_type(), [&](auto* p) {
     using T = std::remove_pointer_t<decltype(p)>;
-    act8_pack_kernel<T><<<grid_of(R * nb), 256, 0, st>>>(reinterpret_cast<const T*>(x.data_ptr()), R, (int)N, (int)nb,
-                                                         codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>());
+    const T* v = reinterpret_cast<const T*>(x.data_ptr());
+    uint8_t *c = codes.data_ptr<uint8_t>(), *s = scales.data_ptr<uint8_t>();
+    const long long units = R * nb * 4;
+    if (N % 32 == 0 && aligned(v))
+      act8_pack8_kernel<T, true><<<unit_grid(units), 256, 0, st>>>(v, units, (int)N, (int)nb, c, s);
+    else if (N % 8 == 0 && aligned(v))
+      act8_pack8_kernel<T, false><<<unit_grid(units), 256, 0, st>>>(v, units, (int)N, (int)nb, c, s);
+    else
+      act8_pack_kernel<T><<<grid_of(R * nb), 256, 0, st>>>(v, R, (int)N, (int)nb, c, s);
   });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   ++counted_launches;
   return {codes, scales};
 }
 
-// The values [R, N] that codes and exponents stand for, as `like`'s type.
-at::Tensor act8_unpack(const at::Tensor& codes, const at::Tensor& scales, int64_t type) {
+// The values that codes and exponents stand for, in `shape` (R N values) and type 0 fp32, 1 bf16 or 2 fp16.
+at::Tensor act8_unpack(const at::Tensor& codes, const at::Tensor& scales, const std::vector<int64_t>& shape, int64_t type) {
   TORCH_CHECK(codes.is_cuda() && codes.dim() == 2 && codes.is_contiguous() && codes.scalar_type() == at::kByte,
               "act8_unpack: contiguous codes [R, N]");
   const int64_t R = codes.size(0), N = codes.size(1), nb = (N + 31) / 32;
@@ -108,12 +230,20 @@ at::Tensor act8_unpack(const at::Tensor& codes, const at::Tensor& scales, int64_
   c10::cuda::CUDAGuard guard(codes.get_device());
   auto st = at::cuda::getCurrentCUDAStream(codes.get_device()).stream();
   const at::ScalarType t = type == 0 ? at::kFloat : type == 1 ? at::kBFloat16 : at::kHalf;
-  at::Tensor y = at::empty({R, N}, codes.options().dtype(t));
+  at::Tensor y = at::empty(shape, codes.options().dtype(t));
+  TORCH_CHECK(y.numel() == codes.numel(), "act8_unpack: the shape has another number of values");
   if (y.numel() == 0) return y;
   for_type(t, [&](auto* p) {
     using T = std::remove_pointer_t<decltype(p)>;
-    act8_unpack_kernel<T><<<grid_of(R * nb), 256, 0, st>>>(codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), R, (int)N,
-                                                           (int)nb, reinterpret_cast<T*>(y.data_ptr()));
+    T* v = reinterpret_cast<T*>(y.data_ptr());
+    const uint8_t *c = codes.data_ptr<uint8_t>(), *s = scales.data_ptr<uint8_t>();
+    const long long units = R * nb * 4;
+    if (N % 32 == 0 && aligned(c))
+      act8_unpack8_kernel<T, true><<<unit_grid(units), 256, 0, st>>>(c, s, units, (int)N, (int)nb, v);
+    else if (N % 8 == 0 && aligned(c))
+      act8_unpack8_kernel<T, false><<<unit_grid(units), 256, 0, st>>>(c, s, units, (int)N, (int)nb, v);
+    else
+      act8_unpack_kernel<T><<<grid_of(R * nb), 256, 0, st>>>(c, s, R, (int)N, (int)nb, v);
   });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   ++counted_launches;

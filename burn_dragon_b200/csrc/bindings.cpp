@@ -137,17 +137,12 @@ void adamw_many(const std::vector<at::Tensor>& params, const std::vector<c10::op
                 const c10::optional<at::Tensor>& v_scale, double lr, double b1, double b2, double eps, double wd,
                 const at::Tensor& steps, int64_t key, const c10::optional<at::Tensor>& gscale);
 std::vector<at::Tensor> act8_pack(const at::Tensor& x);
-at::Tensor act8_unpack(const at::Tensor& codes, const at::Tensor& scales, int64_t type);
-std::vector<at::Tensor> ff_forward(const at::Tensor& x, const c10::optional<at::Tensor>& z, const at::Tensor& wg,
-                                   const c10::optional<at::Tensor>& wu, const c10::optional<at::Tensor>& bg,
-                                   const c10::optional<at::Tensor>& bu, double bg0, double bu0,
-                                   const c10::optional<at::Tensor>& residual, int64_t act, bool up_relu, int64_t keep,
-                                   const at::Tensor& err);
-std::vector<at::Tensor> ff_backward(const at::Tensor& dy, const at::Tensor& x, const c10::optional<at::Tensor>& z,
-                                    const at::Tensor& wg, const c10::optional<at::Tensor>& wu,
-                                    const c10::optional<at::Tensor>& bg, const c10::optional<at::Tensor>& bu, double bg0,
-                                    double bu0, const std::vector<at::Tensor>& held, int64_t act, bool up_relu, int64_t keep,
-                                    int64_t want, const at::Tensor& err);
+at::Tensor act8_unpack(const at::Tensor& codes, const at::Tensor& scales, const std::vector<int64_t>& shape, int64_t type);
+c10::optional<at::Tensor> ff_call(const at::Tensor& x, const c10::optional<at::Tensor>& z, const at::Tensor& wg,
+                                  const c10::optional<at::Tensor>& wu, const c10::optional<at::Tensor>& bg,
+                                  const c10::optional<at::Tensor>& bu, double bg0, double bu0,
+                                  const c10::optional<at::Tensor>& residual, int64_t act, bool up_relu, int64_t keep,
+                                  const at::Tensor& err);
 }  // namespace bd
 
 namespace bd {
@@ -216,7 +211,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("adamw_many", &bd::adamw_many);
   m.def("act8_pack", &bd::act8_pack);
   m.def("act8_unpack", &bd::act8_unpack);
-  m.def("ff_forward", &bd::ff_forward);
-  m.def("ff_backward", &bd::ff_backward);
+  m.def("ff_call", &bd::ff_call);
   m.def("counted_launches", [] { return bd::counted_launches.load(); });
 }

@@ -7,6 +7,7 @@
 #include <algorithm>
 
 #include "feed_forward.cuh"
+#include "feed_forward_host.h"
 #include "gemm_table.h"
 #include "launches.h"
 #include "tensor_map.h"
@@ -316,6 +317,11 @@ void product(const Launch& l, int epi, FfOut e, const Mat* a, const Mat* b, int 
   p.step[4] = step;
   for (int s = 0; s < 2; ++s) {
     const int q = s < sets ? s : 0;
+    if (s > 0 && q == 0) {
+      p.ta[1] = p.ta[0], p.tb[1] = p.tb[0];
+      p.a_heads |= (p.a_heads & 1) << 1, p.b_heads |= (p.b_heads & 1) << 1;
+      break;
+    }
     p.ta[s] = a[q].map(a_mn ? 64 : 128);
     p.tb[s] = b[q].map(b_mn[q] ? 64 : (uint32_t)b_rows);
     if (a[q].per_head) p.a_heads |= 1 << s;
@@ -378,8 +384,6 @@ struct Layer {
   FfOut e;  // with biases, activation, sizes
   Launch l;
 };
-
-using OptTensor = c10::optional<at::Tensor>;
 
 Layer layer_of(const at::Tensor& x, const OptTensor& z, const at::Tensor& wg, const OptTensor& wu, const OptTensor& bg,
                const OptTensor& bu, double bg0, double bu0, int64_t act, bool up_relu, const at::Tensor& err) {
@@ -444,7 +448,6 @@ void forward_products(const Layer& c, int epi, const FfOut& e, bool may_split) {
 
 }  // namespace
 
-// y [M, H, N] and what the backward pass goes by: [held, exponents] a projection (none, 16-bit values, or codes).
 std::vector<at::Tensor> ff_forward(const at::Tensor& x, const OptTensor& z, const at::Tensor& wg, const OptTensor& wu,
                                    const OptTensor& bg, const OptTensor& bu, double bg0, double bu0, const OptTensor& residual,
                                    int64_t act, bool up_relu, int64_t keep, const at::Tensor& err) {
@@ -475,8 +478,6 @@ std::vector<at::Tensor> ff_forward(const at::Tensor& x, const OptTensor& z, cons
   return out;
 }
 
-// dx, dz, dwg, dwu, dbg, dbu from dy [M, H, N]; what is not wanted (a bit each in `want`) is an empty tensor. `held`: as
-// ff_forward gave it; empty: the pre-activations are computed again.
 std::vector<at::Tensor> ff_backward(const at::Tensor& dy, const at::Tensor& x, const OptTensor& z, const at::Tensor& wg,
                                     const OptTensor& wu, const OptTensor& bg, const OptTensor& bu, double bg0, double bu0,
                                     const std::vector<at::Tensor>& held, int64_t act, bool up_relu, int64_t keep,

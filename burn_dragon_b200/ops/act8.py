@@ -65,20 +65,19 @@ class PackedActivation:
     def unpack(self) -> torch.Tensor:
         """The values, in the packed tensor's shape and type."""
         if self.codes.is_cuda:
-            y = _ext.load().act8_unpack(self.codes, self.exponents, _TYPES[self.dtype])
-        else:
-            y = decode_ref(self.codes, self.exponents, self.dtype)
-        return y.view(self.shape)
+            return _ext.load().act8_unpack(self.codes, self.exponents, self.shape, _TYPES[self.dtype])
+        return decode_ref(self.codes, self.exponents, self.dtype).view(self.shape)
 
 
 def pack_activation(x: torch.Tensor) -> PackedActivation:
     """Packs an fp32, bf16 or fp16 tensor (a copy of one that is not contiguous). No graph is kept."""
     if x.dtype not in _TYPES:
         raise TypeError(f"pack_activation takes fp32, bf16 or fp16 values, not {x.dtype}")
-    rows = x.detach()
-    rows = rows.reshape(-1, x.shape[-1] if x.dim() and x.shape[-1] else 1) if x.numel() else rows.reshape(0, 1)
-    rows = rows.contiguous()
-    codes, exponents = _ext.load().act8_pack(rows) if x.is_cuda else encode_ref(rows)
+    if x.is_cuda:
+        codes, exponents = _ext.load().act8_pack(x)
+    else:
+        rows = x.detach()
+        codes, exponents = encode_ref(rows.reshape(-1, rows.shape[-1] if x.dim() else 1) if x.numel() else rows.reshape(0, 1))
     return PackedActivation(codes, exponents, x.shape, x.dtype)
 
 

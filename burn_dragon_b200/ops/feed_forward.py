@@ -35,6 +35,7 @@ from .adapters import _reach, _rows
 from .gemm import error_word
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+_UPS = {"none": False, "relu": True}
 _KEEPS = {"recompute": 0, "16bit": 1, "8bit": 2}
 
 # Reductions of at least this length hold the pre-activations in 16 bits by default, shorter ones compute them again.
@@ -102,28 +103,6 @@ def _ref(x, z, wg, wu, bg, bu, residual, act, up, keep):
 # ------------------------------------------------------------------------------ CUDA
 
 
-class _Layer(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, z, wg, wu, bg, bu, residual, bg0, bu0, act, up_relu, keep):
-        out = _ext.load().ff_forward(x, z, wg, wu, bg, bu, bg0, bu0, residual, act, up_relu, keep, error_word(x.device))
-        ctx.save_for_backward(x, z, wg, wu, bg, bu, *out[1:])
-        ctx.call = (bg0, bu0, act, up_relu, keep)
-        return out[0]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, z, wg, wu, bg, bu, *held = ctx.saved_tensors
-        bg0, bu0, act, up_relu, keep = ctx.call
-        need = ctx.needs_input_grad
-        want = sum(1 << i for i in range(6) if need[i])
-        got = [None] * 6
-        if want:
-            got = _ext.load().ff_backward(_rows(dy), x, z, wg, wu, bg, bu, bg0, bu0, held, act, up_relu, keep,
-                                          want, error_word(x.device))
-        return (*(got[i] if need[i] else None for i in range(6)), dy if need[6] else None, None, None, None, None, None)
-
-
 def _weight(w: torch.Tensor, like: torch.Tensor | None = None) -> torch.Tensor:
     """``w`` [H, K, N] as the kernels read it: K or N contiguous, the other strides multiples of 8 values."""
     def fits(t, inner):
@@ -163,7 +142,7 @@ def _layer(name, x, z, wg, wu, bg, bu, residual, act, up, keep):
     M = x.shape[0]
     if act not in ACTIVATIONS:
         raise ValueError(f"{name}: activation {act!r} (one of {', '.join(ACTIVATIONS)})")
-    if up not in ("none", "relu"):
+    if up not in _UPS:
         raise ValueError(f"{name}: up_activation {up!r} (none or relu)")
     if keep is not None and keep not in _KEEPS:
         raise ValueError(f"{name}: keep {keep!r} (one of {', '.join(_KEEPS)}, or None)")
@@ -204,22 +183,41 @@ def _layer(name, x, z, wg, wu, bg, bu, residual, act, up, keep):
     z = None if z is None else _rows(z)
     wu = None if wu is None else _weight(wu, wg)
     residual = None if residual is None else _rows(residual)
-    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, z, wg, wu, bg, bu, residual))
-    nothing = wu is None and act == "none"  # dp is dy
-    code = _KEEPS[keep] if train and not nothing else 0
-    call = (x, z, wg, wu, bg, bu, residual, bg0, bu0, ACTIVATIONS[act], up == "relu", code)
-    if train:
-        y = _Layer.apply(*call)
+    if residual is not None:  # heads are for the gated form: one head's rows
+        y = _call(x, None, wg[0], None, None if bg is None else bg[0], None, bg0, 0.0, residual[:, 0], act, up, keep)[:, None]
     else:
-        y = _ext.load().ff_forward(x, z, wg, wu, bg, bu, bg0, bu0, residual, ACTIVATIONS[act], up == "relu", 0,
-                                   error_word(x.device))[0]
+        y = _call(x, z, wg, wu, bg, bu, bg0, bu0, None, act, up, keep)
     return y if N8 == N else y[..., :N]
+
+
+def _call(x, z, wg, wu, bg, bu, bg0, bu0, residual, act, up, keep):
+    y = _ext.load().ff_call(x, z, wg, wu, bg, bu, bg0, bu0, residual, ACTIVATIONS[act], up == "relu", _KEEPS[keep],
+                            error_word(x.device))
+    if y is None:
+        raise RuntimeError("feed_forward: operands that the kernels cannot read")
+    return y
+
+
+def _direct(x, z, wg, wu, bg, bu, residual, act, up, keep):
+    """The call that needs no copy, no padding and no error: its result, or None."""
+    if not x.is_cuda or act not in ACTIVATIONS or up not in _UPS or not (keep is None or keep in _KEEPS) or wg.dim() < 2:
+        return None
+    keep = (1 if wg.shape[-2] >= KEEP_FROM else 0) if keep is None else _KEEPS[keep]
+    bg0 = bu0 = 0.0
+    if not (bg is None or isinstance(bg, torch.Tensor)):
+        bg, bg0 = None, float(bg)
+    if not (bu is None or isinstance(bu, torch.Tensor)):
+        bu, bu0 = None, float(bu)
+    return _ext.load().ff_call(x, z, wg, wu, bg, bu, bg0, bu0, residual, ACTIVATIONS[act], _UPS[up], keep, error_word(x.device))
 
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias=None, activation: str = "none", *,
                residual: torch.Tensor | None = None, keep: str | None = None) -> torch.Tensor:
     """act(x weight + bias) + residual: x [..., K], weight [K, N] (a ``torch.nn.Linear``'s is ``weight.t()``, which is
     read as it lies), bias a number or [N], residual and result [..., N]. ``activation``: none, relu, silu or gelu."""
+    y = _direct(x, None, weight, None, bias, None, residual, activation, "none", keep) if weight.dim() == 2 else None
+    if y is not None:
+        return y
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[0]:
         raise ValueError(f"linear_act takes x [..., K] and weight [K, N], got {tuple(x.shape)} and {tuple(weight.shape)}")
     K, N = weight.shape
@@ -241,6 +239,9 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
                  keep: str | None = None) -> torch.Tensor:
     """activation(x w_gate + b_gate) * up_activation(z w_up + b_up). Without heads: weights [K, N], x and z [..., K],
     biases [N]; with heads: weights [H, K, N], x and z [M, K] or [M, H, K], biases [H, N], y [M, H, N]."""
+    y = _direct(x, z, w_gate, w_up, b_gate, b_up, None, activation, up_activation, keep)
+    if y is not None:
+        return y
     if w_gate.dim() == 3:
         return _layer("gated_linear", x, z, w_gate, w_up, b_gate, b_up, None, activation, up_activation, keep)
     if w_gate.dim() != 2 or w_up.dim() != 2 or x.dim() < 1 or x.shape[-1] != w_gate.shape[0]:
