@@ -20,7 +20,7 @@ BUILD_DIR = os.path.join(CSRC, "build")
 
 SOURCES = ["bindings.cpp", "gemm_host.cu", "gemm_inst_a.cu", "gemm_inst_b.cu", "gemm_inst_c.cu", "gemm_inst_d.cu", "gemm_inst_e.cu", "rowwise.cu", "noalloc_decoder.cu", "decode.cu", "scaffold.cu", "comm.cu", "gdpo.cu", "ssd_chunk.cu",
            "adapters.cu", "sampling.cu", "adamw_many.cu", "act8.cu", "feed_forward.cu", "feed_forward_a.cu",
-           "feed_forward_b.cu", "feed_forward_autograd.cpp"]
+           "feed_forward_b.cu", "feed_forward_c.cu", "feed_forward_autograd.cpp"]
 
 NVCC_FLAGS = [
     "-gencode=arch=compute_100a,code=sm_100a",

@@ -17,103 +17,124 @@ namespace {
 
 // ------------------------------------------------------------------------------- sums of a split reduction
 
-// The parts [splits, NB, sets, heads, M, N] summed in a fixed order, then the epilogue of the unsplit form. A lane takes 8
-// columns, four lanes a block of 32; eight warps take every eighth part, so that few columns of many parts do
-// not wait for one another.
+// The parts [splits, NB, sets, heads, M, N] summed in a fixed order, then the epilogue of the unsplit form. A lane takes 4
+// columns, eight lanes a block of 32; eight warps take every eighth part, so that few columns of many parts do
+// not wait for one another. Launched while the products run (programmatic launch): it waits for them itself.
 template <int EPI>
 __global__ void __launch_bounds__(256) ff_join_kernel(const __grid_constant__ FfOut e, const float* __restrict__ partial,
                                                       int splits, int sets) {
   constexpr int NB = ff_products(EPI);
-  __shared__ float red[8][8 * NB][32];
+  __shared__ float4 red[8][NB][32];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int groups = (e.N + 31) / 32 * 4;
+  const int groups = (e.N + 31) / 32 * 8;
   const long long at = (long long)blockIdx.x * 32 + lane;
-  const int col = (int)(at % groups) * 8;
+  const int col = (int)(at % groups) * 4;
   const long long row_of_all = at / groups, rows = (long long)sets * e.heads * e.M;
   const bool in = row_of_all < rows && col < e.N;
   const long long part = rows * e.N;  // of one product
-  float v[NB][8];
-#pragma unroll
-  for (int s = 0; s < NB; ++s)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[s][i] = 0.f;
+  float v[2][4] = {};
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (in) {
-#pragma unroll 2
+#pragma unroll 4
     for (int q = warp; q < splits; q += 8)
 #pragma unroll
       for (int s = 0; s < NB; ++s) {
-        const float4* src = reinterpret_cast<const float4*>(partial + ((long long)q * NB + s) * part + row_of_all * e.N + col);
-        const float4 lo = src[0], hi = src[1];
-        v[s][0] += lo.x, v[s][1] += lo.y, v[s][2] += lo.z, v[s][3] += lo.w;
-        v[s][4] += hi.x, v[s][5] += hi.y, v[s][6] += hi.z, v[s][7] += hi.w;
+        const float4 f = *reinterpret_cast<const float4*>(partial + ((long long)q * NB + s) * part + row_of_all * e.N + col);
+        v[s][0] += f.x, v[s][1] += f.y, v[s][2] += f.z, v[s][3] += f.w;
       }
   }
 #pragma unroll
-  for (int s = 0; s < NB; ++s)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) red[warp][8 * s + i][lane] = v[s][i];
+  for (int s = 0; s < NB; ++s) red[warp][s][lane] = make_float4(v[s][0], v[s][1], v[s][2], v[s][3]);
   __syncthreads();
   if (warp > 0) return;
 #pragma unroll
   for (int q = 1; q < 8; ++q)
 #pragma unroll
-    for (int s = 0; s < NB; ++s)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[s][i] += red[q][8 * s + i][lane];
+    for (int s = 0; s < NB; ++s) {
+      const float4 f = red[q][s][lane];
+      v[s][0] += f.x, v[s][1] += f.y, v[s][2] += f.z, v[s][3] += f.w;
+    }
   const int m = (int)(row_of_all % e.M);
   const int head = (int)(row_of_all / e.M % e.heads), set = (int)(row_of_all / e.M / e.heads);
   const long long to = (long long)m * e.ld + (long long)head * e.head + col;
+  auto put = [&](void* out, long long where, const float* f) {
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + where) =
+        make_uint2(ff_pack2(f[0], f[1], e.half), ff_pack2(f[2], f[3], e.half));
+  };
   if constexpr (EPI == FF_STORE) {
-    if (in) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(e.out[set]) + to) = ff_pack8(v[0], e.half);
+    if (in) put(e.out[set], to, v[0]);
   } else {
     if (in) {
 #pragma unroll
-      for (int s = 0; s < NB; ++s)
-        if (ff_has_bias(e, s)) ff_bias8(e, s, head, col, v[s]);
+      for (int s = 0; s < NB; ++s) {
+        if (!ff_has_bias(e, s)) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const long long hn = (long long)head * e.N + col + i;
+          v[s][i] += !e.bias[s]   ? e.bias0[s]
+                     : e.bias_f32 ? reinterpret_cast<const float*>(e.bias[s])[hn]
+                                  : ff_as_float(reinterpret_cast<const uint16_t*>(e.bias[s])[hn], e.half);
+        }
+      }
     }
     const long long rh = (long long)m * e.heads + head;
     if (!ff_backward(EPI) && e.keep != FF_KEEP_NOTHING) {
 #pragma unroll
       for (int s = 0; s < NB; ++s) {
         if (e.keep == FF_KEEP_16) {
-          if (in) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(e.held[s]) + rh * e.N + col) = ff_pack8(v[s], e.half);
+          if (in) put(e.held[s], rh * e.N + col, v[s]);
         } else {
           float largest = 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) largest = fmaxf(largest, in ? act8_size(v[s][i]) : 0.f);
-          largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-          largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+          for (int i = 0; i < 4; ++i) largest = fmaxf(largest, in ? act8_size(v[s][i]) : 0.f);
+#pragma unroll
+          for (int o = 1; o < 8; o *= 2) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
           const int ex = act8_exponent(largest);
           if (in) {
-            const float inverse = act8_power(-ex);
-            *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(e.held[s]) + rh * e.N + col) =
-                make_uint2(act8_code4(v[s], inverse), act8_code4(v[s] + 4, inverse));
-            if (lane % 4 == 0) e.exponents[s][rh * (groups / 4) + col / 32] = (uint8_t)(ex + 127);
+            *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(e.held[s]) + rh * e.N + col) = act8_code4(v[s], act8_power(-ex));
+            if (lane % 8 == 0) e.exponents[s][rh * (groups / 8) + col / 32] = (uint8_t)(ex + 127);
           }
         }
       }
     }
     if (!in) return;
-    float a[8];
-    if (e.aux)
-      ff_unpack8(*reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(e.aux) + (long long)m * e.aux_ld +
-                                                 (long long)head * e.aux_head + col),
-                 e.half, a);
+    float a[4];
+    if (e.aux) {
+      const uint2 r = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(e.aux) + (long long)m * e.aux_ld +
+                                                      (long long)head * e.aux_head + col);
+      put_pair(a, 0, ff_unpack2(r.x, e.half)), put_pair(a, 1, ff_unpack2(r.y, e.half));
+    }
     if constexpr (ff_backward(EPI)) {
       ff_with_act(e.act, [&](auto k) {
-        ff_backward_values<EPI, 8, decltype(k)::value>(e.up_relu, v[0], v[NB - 1], [&](int i) { return pair_of(a, i); });
+        ff_backward_values<EPI, 4, decltype(k)::value>(e.up_relu, v[0], v[1], [&](int i) { return pair_of(a, i); });
       });
     } else {
-      ff_forward_values<EPI, 8>(e, v[0], v[NB - 1]);
+      ff_forward_values<EPI, 4>(e, v[0], v[1]);
       if (EPI == FF_ACT && e.aux) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[0][i] += a[i];
+        for (int i = 0; i < 4; ++i) v[0][i] += a[i];
       }
     }
-    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(e.out[0]) + to) = ff_pack8(v[0], e.half);
-    if constexpr (EPI == FF_GATED_BWD)
-      *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(e.out[1]) + to) = ff_pack8(v[1], e.half);
+    put(e.out[0], to, v[0]);
+    if constexpr (EPI == FF_GATED_BWD) put(e.out[1], to, v[1]);
   }
+}
+
+template <int EPI>
+void launch_join(const FfOut& e, const float* partial, int splits, int sets, cudaStream_t st) {
+  const long long n = (long long)(e.N + 31) / 32 * 8 * sets * e.heads * e.M;
+  TORCH_CHECK((n + 31) / 32 < (1ll << 31), "feed_forward: too many outputs of a split reduction");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((n + 31) / 32));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, ff_join_kernel<EPI>, e, partial, splits, sets));
+  ++counted_launches;
 }
 
 // ------------------------------------------------------------------------------- backward from held pre-activations
@@ -273,6 +294,22 @@ Choice choose(int64_t rows, int64_t cols, int64_t batch, int64_t blocks, int nb,
   return best;
 }
 
+// The same for few rows: a block is the weights' bytes at an SM's share of the memory's (23 a clock).
+constexpr int kFewRows = 128;
+
+Choice choose_few(int64_t rows, int64_t cols, int64_t batch, int64_t blocks, int nb, int sms, bool may_split) {
+  const int64_t tiles = (cols + 127) / 128 * batch;
+  Choice best{{false, rows <= 16 ? 16 : rows <= 64 ? 64 : 128, false}, 1};
+  double least = 1e300;
+  for (int64_t parts = 1; parts == 1 || (may_split && parts <= blocks / 2 && tiles * parts <= sms); ++parts) {
+    const double waves = (double)((tiles * parts + sms - 1) / sms);
+    double cost = waves * ((double)((blocks + parts - 1) / parts) * nb * 712.0 + 1200.0);
+    if (parts > 1) cost += 4000.0 + 8.0 * parts * rows * cols * batch * nb / 3000.0;
+    if (cost < least) least = cost, best.splits = (int)parts;
+  }
+  return best;
+}
+
 struct Launch {
   cudaStream_t st;
   int dev;
@@ -286,6 +323,42 @@ uint32_t idesc_of(bool pair, int bn, bool half, bool a_mn) {
   return d;
 }
 
+// The walk's constants, room for the parts of a split reduction, the launch, and their sum.
+void split_and_launch(const Launch& l, int epi, const FfOut& e, FfGemm& p, const Choice& c, int64_t batch, int out_sets, int nb,
+                      int ctas, bool few) {
+  const int64_t total = (int64_t)p.tiles_m * p.tiles_n * p.splits * batch;
+  TORCH_CHECK(total < (1ll << 31), "feed_forward: too many tiles");
+  const unsigned sizes[4] = {(unsigned)p.tiles_n, (unsigned)p.tiles_m, (unsigned)p.splits, (unsigned)e.heads};
+  unsigned step = c.tile.resident ? 1 : (unsigned)std::min<int64_t>(total, num_sms_of(l.dev) / ctas);
+  for (int i = 0; i < 4; ++i) {
+    p.size[i] = sizes[i];
+    p.step[i] = step % sizes[i];
+    step /= sizes[i];
+  }
+  p.step[4] = step;
+  at::Tensor partial;
+  if (p.splits > 1) {
+    partial = at::empty({(int64_t)p.splits * nb * batch * e.M * e.N}, l.options.dtype(at::kFloat));
+    p.partial = partial.data_ptr<float>();
+  }
+  p.e = e;
+  if (few)
+    ff_launch_few(epi, c.tile.bn, p, l.st, l.dev);
+  else if (nb == 1)
+    ff_launch_one(epi, c.tile, p, l.st, l.dev);
+  else
+    ff_launch_gated(epi, c.tile, p, l.st, l.dev);
+  if (p.splits > 1) {
+    switch (epi) {
+      case FF_STORE: launch_join<FF_STORE>(e, p.partial, p.splits, out_sets, l.st); break;
+      case FF_ACT: launch_join<FF_ACT>(e, p.partial, p.splits, out_sets, l.st); break;
+      case FF_ACT_BWD: launch_join<FF_ACT_BWD>(e, p.partial, p.splits, out_sets, l.st); break;
+      case FF_GATED: launch_join<FF_GATED>(e, p.partial, p.splits, out_sets, l.st); break;
+      default: launch_join<FF_GATED_BWD>(e, p.partial, p.splits, out_sets, l.st);
+    }
+  }
+}
+
 // One launch (two where the reduction is split): rows x cols outputs of e, the reduction `depth` long in each of
 // `segments` pairs of operands. a, b: one or two sets.
 void product(const Launch& l, int epi, FfOut e, const Mat* a, const Mat* b, int sets, int64_t depth, int segments,
@@ -295,26 +368,32 @@ void product(const Launch& l, int epi, FfOut e, const Mat* a, const Mat* b, int 
   memset(&p, 0, sizeof(p));
   p.KB = (int)((depth + 63) / 64);
   p.segments = segments, p.sum_heads = sum_heads, p.out_sets = out_sets;
-  p.a_mn = a_mn, p.two_a = two_a;
+  p.two_a = two_a;
   p.err = l.err;
   const int64_t blocks = (int64_t)p.KB * segments, batch = (int64_t)e.heads * out_sets;
-  Choice c = choose(e.M, e.N, batch, blocks, nb, nb == 2 && two_a ? 2 : 1, num_sms_of(l.dev), may_split);
+  const bool few = e.M <= kFewRows && !a_mn && out_sets == 1;
+  Choice c = few ? choose_few(e.M, e.N, batch, blocks, nb, num_sms_of(l.dev), may_split) : choose(e.M, e.N, batch, blocks, nb, nb == 2 && two_a ? 2 : 1, num_sms_of(l.dev), may_split);
   p.splits = c.splits;
   // Short reductions: A stays in shared memory over the columns of its rows.
   c.tile.resident = epi != FF_STORE && c.tile.pair && c.tile.bn == (nb == 1 ? 256 : 128) && p.splits == 1 && p.KB <= kFfResident;
   TORCH_CHECK(blocks * (c.splits + 1) < (1ll << 32), "feed_forward: the reduction is too long");
+  if (few) {
+    p.tiles_m = (e.N + 127) / 128, p.tiles_n = 1;
+    p.idesc = idesc_of(false, c.tile.bn, e.half, false);
+    for (int s = 0; s < 2; ++s) {
+      const int q = s < sets ? s : 0;
+      p.ta[s] = b[q].map(b_mn[q] ? 64 : 128);
+      p.tb[s] = a[q].map((uint32_t)c.tile.bn);
+      if (b[q].per_head) p.a_heads |= 1 << s;
+      if (a[q].per_head) p.b_heads |= 1 << s;
+      p.a_mn |= b_mn[q] ? (nb == 2 ? 1 << s : 1) : 0;
+    }
+    split_and_launch(l, epi, e, p, c, batch, out_sets, nb, 1, true);
+    return;
+  }
   const int rows = c.tile.pair ? 256 : 128, b_rows = c.tile.pair ? c.tile.bn / 2 : c.tile.bn;
   p.tiles_m = (e.M + rows - 1) / rows, p.tiles_n = (e.N + c.tile.bn - 1) / c.tile.bn;
-  TORCH_CHECK((long long)p.tiles_m * p.tiles_n * p.splits * batch < (1ll << 31), "feed_forward: too many tiles");
-  const unsigned sizes[4] = {(unsigned)p.tiles_n, (unsigned)p.tiles_m, (unsigned)p.splits, (unsigned)e.heads};
-  const int64_t total = (int64_t)p.tiles_m * p.tiles_n * p.splits * batch;
-  unsigned step = c.tile.resident ? 1 : (unsigned)ff_workers(total, c.tile, num_sms_of(l.dev));
-  for (int i = 0; i < 4; ++i) {
-    p.size[i] = sizes[i];
-    p.step[i] = step % sizes[i];
-    step /= sizes[i];
-  }
-  p.step[4] = step;
+  p.a_mn = a_mn;
   for (int s = 0; s < 2; ++s) {
     const int q = s < sets ? s : 0;
     if (s > 0 && q == 0) {
@@ -329,29 +408,7 @@ void product(const Launch& l, int epi, FfOut e, const Mat* a, const Mat* b, int 
     if (b_mn[q]) p.b_mn |= nb == 2 ? 1 << s : 1;
   }
   p.idesc = idesc_of(c.tile.pair, c.tile.bn, e.half, a_mn);
-  at::Tensor partial;
-  if (p.splits > 1) {
-    partial = at::empty({(int64_t)p.splits * nb * batch * e.M * e.N}, l.options.dtype(at::kFloat));
-    p.partial = partial.data_ptr<float>();
-  }
-  p.e = e;
-  if (nb == 1)
-    ff_launch_one(epi, c.tile, p, l.st, l.dev);
-  else
-    ff_launch_gated(epi, c.tile, p, l.st, l.dev);
-  if (p.splits > 1) {
-    const long long groups = (e.N + 31) / 32 * 4, n = groups * batch * e.M;
-    const unsigned grid = (unsigned)((n + 31) / 32);
-    switch (epi) {
-      case FF_STORE: ff_join_kernel<FF_STORE><<<grid, 256, 0, l.st>>>(e, p.partial, p.splits, out_sets); break;
-      case FF_ACT: ff_join_kernel<FF_ACT><<<grid, 256, 0, l.st>>>(e, p.partial, p.splits, out_sets); break;
-      case FF_ACT_BWD: ff_join_kernel<FF_ACT_BWD><<<grid, 256, 0, l.st>>>(e, p.partial, p.splits, out_sets); break;
-      case FF_GATED: ff_join_kernel<FF_GATED><<<grid, 256, 0, l.st>>>(e, p.partial, p.splits, out_sets); break;
-      default: ff_join_kernel<FF_GATED_BWD><<<grid, 256, 0, l.st>>>(e, p.partial, p.splits, out_sets);
-    }
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
-    ++counted_launches;
-  }
+  split_and_launch(l, epi, e, p, c, batch, out_sets, nb, c.tile.pair ? 2 : 1, false);
 }
 
 void check_rows(const at::Tensor& t, int dev, at::ScalarType type, const char* what) {

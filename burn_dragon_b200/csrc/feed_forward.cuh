@@ -883,6 +883,321 @@ __global__ void __launch_bounds__(FfCfg<ff_products(EPI), BN, PAIR, RES>::THREAD
 }  // namespace bd
 
 namespace bd {
+
+// ------------------------------------------------------------------------------- few rows
+
+// Up to MP rows: the weights take the place of A (128 columns of the output are the tensor core's rows) and the batch's
+// rows that of B, so that what is staged is the weights and little else: bound by their bytes. (With the rows as A a stage
+// held 16 KB of mostly padding for each operand: 64 rows, 4 x 256 -> 8192, 18 us; 5.2 at the copy rate.) A lane then holds a column
+// of the output and its rows lie in its registers.
+template <int NB, int MP>
+struct FfFewCfg {
+  static constexpr int W_BYTES = 128 * 64 * 2, X_BYTES = MP * 64 * 2;
+  static constexpr int STAGE_BYTES = NB * (W_BYTES + X_BYTES);
+  static constexpr int STAGES = (200 * 1024) / STAGE_BYTES;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024;
+  static constexpr int ROWS = MP < 32 ? MP : 32;  // of a chunk
+  static constexpr int EPI_WARPS = MP > 32 ? 8 : 4;
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int TMEM_COLS = 2 * NB * MP < 32 ? 32 : 2 * NB * MP;
+  static_assert(MP % 16 == 0 && X_BYTES % 1024 == 0 && TMEM_COLS <= 512 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "tile");
+};
+
+__device__ __forceinline__ float ff_as_float(uint16_t v, int half) {
+  return half ? __half2float(*reinterpret_cast<const __half*>(&v)) : __uint_as_float((uint32_t)v << 16);
+}
+__device__ __forceinline__ uint16_t ff_as_16(float v, int half) {
+  if (half) {
+    const __half h = __float2half_rn(v);
+    return *reinterpret_cast<const uint16_t*>(&h);
+  }
+  const __nv_bfloat16 h = __float2bfloat16_rn(v);
+  return *reinterpret_cast<const uint16_t*>(&h);
+}
+
+template <int n>
+__device__ __forceinline__ void ff_read_rows(uint32_t at, float* v) {
+  if constexpr (n == 32) {
+    float r[32];
+    tmem_ld32(at, r);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = r[i];
+  } else {
+    uint32_t r[16];
+    tmem_ld16(at, r);
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+  }
+}
+
+// The lane's column `col` of n rows from row0 on. All lanes of the warp call it; in: the column is one of the output's.
+template <int EPI, int n>
+__device__ __forceinline__ void ff_few_epilogue(const FfOut& e, int head, int row0, int col, bool in, float* g, float* u, int lane) {
+  constexpr int NB = ff_products(EPI);
+  const int rows = min(n, e.M - row0);
+  const long long hn = (long long)head * e.N + col;
+  uint16_t* out[2] = {reinterpret_cast<uint16_t*>(e.out[0]) + row0 * e.ld + (long long)head * e.head + col,
+                      reinterpret_cast<uint16_t*>(e.out[1]) + row0 * e.ld + (long long)head * e.head + col};
+  if constexpr (EPI != FF_STORE) {
+#pragma unroll
+    for (int s = 0; s < NB; ++s) {
+      if (!ff_has_bias(e, s) || !in) continue;
+      const float b = !e.bias[s]     ? e.bias0[s]
+                      : e.bias_f32   ? reinterpret_cast<const float*>(e.bias[s])[hn]
+                                     : ff_as_float(reinterpret_cast<const uint16_t*>(e.bias[s])[hn], e.half);
+#pragma unroll
+      for (int i = 0; i < n; ++i) (s ? u : g)[i] += b;
+    }
+    if (!ff_backward(EPI) && e.keep != FF_KEEP_NOTHING) {
+      const int nb = (e.N + 31) / 32;
+#pragma unroll
+      for (int s = 0; s < NB; ++s) {
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+          if (i >= rows) break;
+          const float v = (s ? u : g)[i];
+          const long long rh = (long long)(row0 + i) * e.heads + head;
+          if (e.keep == FF_KEEP_16) {
+            if (in) reinterpret_cast<uint16_t*>(e.held[s])[rh * e.N + col] = ff_as_16(v, e.half);
+          } else {  // the warp's 32 columns are a block
+            const uint32_t size = in ? __float_as_uint(act8_size(v)) : 0u;
+            const int ex = act8_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, size)));
+            if (in) reinterpret_cast<uint8_t*>(e.held[s])[rh * e.N + col] = (uint8_t)act8_code2(v, 0.f, act8_power(-ex));
+            if (lane == 0) e.exponents[s][rh * nb + col / 32] = (uint8_t)(ex + 127);
+          }
+        }
+      }
+    }
+    float a[n];
+    const bool has_aux = ff_has_aux<EPI>(e);
+    if (has_aux) {
+      const uint16_t* src = reinterpret_cast<const uint16_t*>(e.aux) + row0 * e.aux_ld + (long long)head * e.aux_head + col;
+#pragma unroll
+      for (int i = 0; i < n; ++i) a[i] = in && i < rows ? ff_as_float(src[i * e.aux_ld], e.half) : 0.f;
+    }
+    if constexpr (ff_backward(EPI)) {
+      ff_with_act(e.act, [&](auto k) {
+        ff_backward_values<EPI, n, decltype(k)::value>(e.up_relu, g, u, [&](int i) { return pair_of(a, i); });
+      });
+#pragma unroll
+      for (int s = 0; s < NB; ++s) {
+        if (!e.colsum[s] || !in) continue;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < n; ++i)
+          if (i < rows) sum += (s ? u : g)[i];
+        e.colsum[s][(long long)(row0 / 32) * e.heads * e.N + hn] = sum;
+      }
+    } else {
+      ff_forward_values<EPI, n>(e, g, u);
+      if (EPI == FF_ACT && has_aux) {
+#pragma unroll
+        for (int i = 0; i < n; ++i) g[i] += a[i];
+      }
+    }
+  }
+  if (!in) return;
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    if (i >= rows) break;
+    out[0][i * e.ld] = ff_as_16(g[i], e.half);
+    if constexpr (EPI == FF_GATED_BWD) out[1][i * e.ld] = ff_as_16(u[i], e.half);
+  }
+}
+
+// ta, a_mn, a_heads: of the weights; tb, b_heads: of the rows; two_a: the second product has rows of its own. tiles_m
+// counts 128 columns of the output.
+template <int EPI, int MP>
+__global__ void __launch_bounds__(FfFewCfg<ff_products(EPI), MP>::THREADS, 1) ff_few_kernel(const __grid_constant__ FfGemm p) {
+  constexpr int NB = ff_products(EPI);
+  using Cfg = FfFewCfg<NB, MP>;
+  constexpr int STAGES = Cfg::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES];
+  __shared__ uint64_t tfull_bar[2], tempty_bar[2], drain_bar;
+  __shared__ uint32_t tmem_base_s;
+  __shared__ volatile int abort_flag;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull_bar[a], 1);
+      mbar_init(&tempty_bar[a], Cfg::EPI_WARPS);
+    }
+    mbar_init(&drain_bar, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(&tmem_base_s, Cfg::TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the sum of the parts may get ready
+  const uint32_t tmem_base = tmem_base_s;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ------------------------------------------------ TMA producer
+      int stage = 0;
+      uint32_t phase = 0;
+      long long issued = 0;
+      bool ok = true;
+      const int x_count = NB == 2 && !p.two_a ? 1 : NB;
+      const uint32_t bytes = (uint32_t)(NB * Cfg::W_BYTES + x_count * Cfg::X_BYTES);
+      FfWalk w(p, blockIdx.x, gridDim.x, false);
+      for (unsigned t = 0; t < w.count && ok; ++t, w.next(p)) {
+        int b0, b1;
+        ff_part(p, w.split(), b0, b1);
+        int seg = b0 / p.KB, kb = b0 - seg * p.KB;
+        for (int i = b0; i < b1; ++i) {
+          const int set = seg / p.sum_heads;
+          const int head = p.sum_heads > 1 ? seg - set * p.sum_heads : w.head();
+          if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutProducer)) {
+            ok = false;
+            break;
+          }
+          uint64_t* bar = &full_bar[stage];
+          mbar_arrive_expect_tx(bar, bytes);
+          uint8_t* dst = smem + stage * Cfg::STAGE_BYTES;
+          const int k = kb * 64;
+#pragma unroll
+          for (int s = 0; s < NB; ++s) {
+            const int q = NB == 1 ? set : s;
+            ff_load<false, 128>(dst + s * Cfg::W_BYTES, &p.ta[q], NB == 1 ? p.a_mn != 0 : (p.a_mn >> s & 1) != 0, bar,
+                                w.m() * 128, k, (p.a_heads >> q) & 1 ? head : 0);
+            if (s < x_count)
+              ff_tma<false>(dst + NB * Cfg::W_BYTES + s * Cfg::X_BYTES, &p.tb[q], bar, k, 0, (p.b_heads >> q) & 1 ? head : 0);
+          }
+          if (++kb == p.KB) kb = 0, ++seg;
+          ++issued;
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!ok) {
+        // wait (bounded, ignoring the abort flag) for the loads still in flight
+        int dummy_abort = 0;
+        const long long inflight = issued < STAGES ? issued : STAGES;
+        int s = stage;
+        uint32_t ph = phase;
+        for (long long i = 0; i < inflight; ++i) {
+          if (--s < 0) {
+            s = STAGES - 1;
+            ph ^= 1;
+          }
+          mbar_wait_bounded(&full_bar[s], ph, (volatile int*)&dummy_abort, p.err, kErrTimeoutDrain);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // ------------------------------------------------ MMA issuer
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      FfWalk w(p, blockIdx.x, gridDim.x, false);
+      for (unsigned t = 0; t < w.count && ok; ++t, w.next(p)) {
+        int b0, b1;
+        ff_part(p, w.split(), b0, b1);
+        if (!mbar_wait_bounded(&tempty_bar[acc], acc_phase ^ 1, &abort_flag, p.err, kErrTimeoutMma)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        for (int i = b0; i < b1; ++i) {
+          if (!mbar_wait_bounded(&full_bar[stage], phase, &abort_flag, p.err, kErrTimeoutMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t base = smem_u32(smem + stage * Cfg::STAGE_BYTES);
+#pragma unroll
+          for (int s = 0; s < NB; ++s) {
+            const bool mn = NB == 1 ? p.a_mn != 0 : (p.a_mn >> s & 1) != 0;
+            const uint32_t a_base = base + s * Cfg::W_BYTES;
+            const uint32_t b_base = base + NB * Cfg::W_BYTES + (s == 1 && p.two_a ? Cfg::X_BYTES : 0);
+            const uint32_t idesc = p.idesc | (mn ? 1u << 15 : 0u);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_bf16(tmem_base + (acc * NB + s) * MP, make_sdesc_sw128(a_base + kk * (mn ? 2048 : 32), mn ? 8192 : 16, 1024),
+                        make_sdesc_sw128(b_base + kk * 32, 16, 1024), idesc, (i > b0 || kk > 0) ? 1u : 0u);
+          }
+          umma_commit(&empty_bar[stage]);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        umma_commit(&tfull_bar[acc]);
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
+      }
+      // every MMA of this thread is done before TMEM is released
+      umma_commit(&drain_bar);
+      int dummy_abort = 0;
+      mbar_wait_bounded(&drain_bar, 0, (volatile int*)&dummy_abort, p.err, kErrTimeoutDrain);
+    }
+  } else {
+    // ------------------------------------------------ epilogue
+    const int quad = warp & 3, part = (warp - 2) >> 2;
+    constexpr int SHARE = MP * 4 / Cfg::EPI_WARPS, n = Cfg::ROWS;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    FfWalk w(p, blockIdx.x, gridDim.x, false);
+    for (unsigned t = 0; t < w.count; ++t, w.next(p)) {
+      // the same answer for the whole warp: the loads from TMEM need all of its lanes, also where a wait has run out
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&tfull_bar[acc], acc_phase, &abort_flag, p.err, kErrTimeoutEpilogue)))
+        break;
+      tc_fence_after();
+      const int col = w.m() * 128 + quad * 32 + lane;
+      const bool in = col < p.e.N;
+#pragma unroll 1
+      for (int r = part * SHARE; r < (part + 1) * SHARE && r < p.e.M && w.m() * 128 + quad * 32 < p.e.N; r += n) {
+        float v[NB][n];
+#pragma unroll
+        for (int s = 0; s < NB; ++s) ff_read_rows<n>(tmem_base + ((uint32_t)(quad * 32) << 16) + (acc * NB + s) * MP + r, v[s]);
+        if (p.splits == 1) {
+          ff_few_epilogue<EPI, n>(p.e, w.head(), r, col, in, v[0], v[NB - 1], lane);
+        } else if (in) {
+#pragma unroll
+          for (int s = 0; s < NB; ++s) {
+            float* o = p.partial + ((((long long)w.split() * NB + s) * p.e.heads + w.head()) * p.e.M + r) * p.e.N + col;
+#pragma unroll
+            for (int i = 0; i < n; ++i)
+              if (r + i < p.e.M) o[(long long)i * p.e.N] = v[s][i];
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty_bar[acc]);
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
+}  // namespace bd
+
+namespace bd {
 // The tile of a launch: PAIR, BN and RES. feed_forward_{a,b}.cu hold the instantiations.
 struct FfTile {
   bool pair;
@@ -890,6 +1205,7 @@ struct FfTile {
   bool resident;
 };
 inline int64_t ff_workers(int64_t tiles, FfTile t, int sms) { return std::min<int64_t>(tiles, sms / (t.pair ? 2 : 1)); }
+void ff_launch_few(int epi, int rows, const FfGemm& p, cudaStream_t st, int dev);       // either, up to 128 rows
 void ff_launch_one(int epi, FfTile tile, const FfGemm& p, cudaStream_t st, int dev);    // one product
 void ff_launch_gated(int epi, FfTile tile, const FfGemm& p, cudaStream_t st, int dev);  // two
 }  // namespace bd
