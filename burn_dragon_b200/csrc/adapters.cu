@@ -1129,9 +1129,10 @@ Checked check_all(const at::Tensor& x, const at::Tensor& w, const at::Tensor& a,
   TORCH_CHECK(H <= 65535 && G <= 65535, "adapter_linear: at most 65535 heads and adapters");
   TORCH_CHECK(a.size(1) == H && a.size(3) == K && b.size(0) == G && b.size(1) == H && b.size(2) == r && b.size(3) == N,
               "adapter_linear: a and b do not fit the weight");
-  TORCH_CHECK(G == p.G, "adapter_linear: the batch was planned for ", p.G, " adapters, not ", G);
+  TORCH_CHECK(G == p.G, "adapter_linear: the batch was planned for ", std::to_string(p.G), " adapters, not ",
+              std::to_string(G));
   TORCH_CHECK((x.dim() == 2 || (x.dim() == 3 && x.size(1) == H)) && x.size(0) == p.M && x.size(-1) == K,
-              "adapter_linear: x must be [M, K] or [M, H, K] with the batch's ", p.M, " rows");
+              "adapter_linear: x must be [M, K] or [M, H, K] with the batch's ", std::to_string(p.M), " rows");
   if (scale)
     TORCH_CHECK(scale->is_cuda() && scale->get_device() == dev && scale->scalar_type() == at::kFloat && scale->dim() == 1 &&
                     scale->size(0) == G && scale->is_contiguous(),

@@ -20,6 +20,15 @@ namespace bd {
 namespace {
 
 PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
+  // The encoder is a driver call: it wants a current context, which a thread that has only had a device from torch (autograd's,
+  // before its first launch) does not have yet.
+  static thread_local bool ready = false;
+  if (!ready) {
+    int dev = 0;
+    C10_CUDA_CHECK(cudaGetDevice(&dev));
+    C10_CUDA_CHECK(cudaSetDevice(dev));
+    ready = true;
+  }
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -69,7 +78,7 @@ CUtensorMap encode_map(const at::Tensor& t, const Geom& g, uint32_t box_inner, u
   CUresult r = get_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, t.data_ptr(), dims, strides, box,
                                estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", (int)r);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", std::to_string((int)r));
   return m;
 }
 
@@ -89,7 +98,7 @@ CUtensorMap encode_out_map(const void* ptr, int64_t N, int64_t M, int64_t ld, in
                                estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (epilogue map) failed with code ", (int)r);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (epilogue map) failed with code ", std::to_string((int)r));
   return m;
 }
 
@@ -108,7 +117,7 @@ CUtensorMap encode_table_map(const void* ptr, int64_t pairs, int64_t T, uint32_t
                                CU_TENSOR_MAP_INTERLEAVE_NONE,
                                cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (RoPE table map) failed with code ", (int)r);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (RoPE table map) failed with code ", std::to_string((int)r));
   return m;
 }
 
@@ -138,7 +147,7 @@ CUtensorMap tensor_map_bf16(const void* base, std::array<int64_t, 3> dims, std::
   CUresult r = get_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, s, box, estr,
                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", (int)r);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", std::to_string((int)r));
   return m;
 }
 
@@ -199,7 +208,7 @@ void gemm(int64_t epi, int64_t bn, const at::Tensor& a, bool a_mn, std::vector<i
   const int KB = (int)((K + 63) / 64);
   p.kb_per_split = (KB + (int)splits - 1) / (int)splits;
   p.splits = (KB + p.kb_per_split - 1) / p.kb_per_split;
-  TORCH_CHECK(p.splits == splits, "split-K count ", splits, " does not fit ", KB, " K-blocks");
+  TORCH_CHECK(p.splits == splits, "split-K count ", std::to_string(splits), " does not fit ", std::to_string(KB), " K-blocks");
   p.a_z1 = ga.use_z1;
   p.a_z2 = ga.use_z2;
   p.b_z1 = gb.use_z1;

@@ -535,7 +535,7 @@ cudaStream_t cur_stream(const at::Tensor& t) { return at::cuda::getCurrentCUDASt
 
 template <typename F>
 void dispatch_vpl(int D, F&& f) {
-  TORCH_CHECK(D % 32 == 0, "row width ", D, " must be a multiple of 32");
+  TORCH_CHECK(D % 32 == 0, "row width ", std::to_string(D), " must be a multiple of 32");
   switch (D / 32) {
     case 1: f(std::integral_constant<int, 1>{}); break;
     case 2: f(std::integral_constant<int, 2>{}); break;
@@ -543,7 +543,7 @@ void dispatch_vpl(int D, F&& f) {
     case 8: f(std::integral_constant<int, 8>{}); break;
     case 16: f(std::integral_constant<int, 16>{}); break;
     case 32: f(std::integral_constant<int, 32>{}); break;
-    default: TORCH_CHECK(false, "row width ", D, " must be 32 * {1,2,4,8,16,32}");
+    default: TORCH_CHECK(false, "row width ", std::to_string(D), " must be 32 * {1,2,4,8,16,32}");
   }
 }
 
