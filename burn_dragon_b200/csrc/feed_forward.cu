@@ -18,16 +18,16 @@ namespace {
 // ------------------------------------------------------------------------------- sums of a split reduction
 
 // The parts [splits, NB, sets, heads, M, N] summed in a fixed order, then the epilogue of the unsplit form. A lane takes 4
-// columns, eight lanes a block of 32; eight warps take every eighth part, so that few columns of many parts do
-// not wait for one another. Launched while the products run (programmatic launch): it waits for them itself.
+// columns, eight lanes a block of 32; `ways` of the eight warps (2, 4 or 8) share the parts, so that few columns of many
+// parts do not wait for one another. Launched while the products run (programmatic launch): it waits for them itself.
 template <int EPI>
 __global__ void __launch_bounds__(256) ff_join_kernel(const __grid_constant__ FfOut e, const float* __restrict__ partial,
-                                                      int splits, int sets) {
+                                                      int splits, int sets, int ways) {
   constexpr int NB = ff_products(EPI);
   __shared__ float4 red[8][NB][32];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, way = warp % ways;
   const int groups = (e.N + 31) / 32 * 8;
-  const long long at = (long long)blockIdx.x * 32 + lane;
+  const long long at = ((long long)blockIdx.x * (8 / ways) + warp / ways) * 32 + lane;
   const int col = (int)(at % groups) * 4;
   const long long row_of_all = at / groups, rows = (long long)sets * e.heads * e.M;
   const bool in = row_of_all < rows && col < e.N;
@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(256) ff_join_kernel(const __grid_constant__ Ff
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (in) {
 #pragma unroll 4
-    for (int q = warp; q < splits; q += 8)
+    for (int q = way; q < splits; q += ways)
 #pragma unroll
       for (int s = 0; s < NB; ++s) {
         const float4 f = *reinterpret_cast<const float4*>(partial + ((long long)q * NB + s) * part + row_of_all * e.N + col);
@@ -46,12 +46,11 @@ __global__ void __launch_bounds__(256) ff_join_kernel(const __grid_constant__ Ff
 #pragma unroll
   for (int s = 0; s < NB; ++s) red[warp][s][lane] = make_float4(v[s][0], v[s][1], v[s][2], v[s][3]);
   __syncthreads();
-  if (warp > 0) return;
-#pragma unroll
-  for (int q = 1; q < 8; ++q)
+  if (way > 0) return;
+  for (int q = 1; q < ways; ++q)
 #pragma unroll
     for (int s = 0; s < NB; ++s) {
-      const float4 f = red[q][s][lane];
+      const float4 f = red[warp + q][s][lane];
       v[s][0] += f.x, v[s][1] += f.y, v[s][2] += f.z, v[s][3] += f.w;
     }
   const int m = (int)(row_of_all % e.M);
@@ -123,9 +122,11 @@ __global__ void __launch_bounds__(256) ff_join_kernel(const __grid_constant__ Ff
 template <int EPI>
 void launch_join(const FfOut& e, const float* partial, int splits, int sets, cudaStream_t st) {
   const long long n = (long long)(e.N + 31) / 32 * 8 * sets * e.heads * e.M;
-  TORCH_CHECK((n + 31) / 32 < (1ll << 31), "feed_forward: too many outputs of a split reduction");
+  const int ways = splits >= 8 ? 8 : splits >= 4 ? 4 : 2;
+  const long long a_cta = 32 * (8 / ways), grid = (n + a_cta - 1) / a_cta;
+  TORCH_CHECK(grid < (1ll << 31), "feed_forward: too many outputs of a split reduction");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((n + 31) / 32));
+  cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -133,7 +134,7 @@ void launch_join(const FfOut& e, const float* partial, int splits, int sets, cud
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, ff_join_kernel<EPI>, e, partial, splits, sets));
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, ff_join_kernel<EPI>, e, partial, splits, sets, ways));
   ++counted_launches;
 }
 
@@ -153,7 +154,7 @@ __global__ void __launch_bounds__(256) ff_held_kernel(const __grid_constant__ Ff
   for (int s = 0; s < NB; ++s)
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum[s][i] = 0.f;
-#pragma unroll 2
+#pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int m = (int)blockIdx.z * 32 + j * 8 + warp;
     if (!in || m >= e.M) continue;
@@ -259,9 +260,9 @@ Mat weight_of(const at::Tensor& w, bool& turned) {
   return Mat{w.data_ptr(), w.size(turned ? 1 : 2), w.size(turned ? 2 : 1), w.size(0), w.stride(turned ? 2 : 1), w.stride(0), true};
 }
 
-// Clocks of one launch, by a model of the busiest CTA: a 64-wide block takes what its products take on the tensor core
-// (2 NB BN at 8192 operations a clock) or what its operands take into shared memory (64 bytes a clock), a tile 1200
-// clocks of its own, and a split reduction writes and reads its parts and starts another kernel.
+// Clocks of one launch, by a model of the busiest CTA, from measured loops: a 64-wide block takes at least 800 (its way
+// through the ring where few CTAs run), 60 % of the tensor core's rate, or what its operands take into shared memory (40 bytes a
+// clock); a tile 1500 of its own; a split reduction writes and reads its parts and starts another kernel.
 struct Choice {
   FfTile tile;
   int splits;
@@ -274,7 +275,7 @@ Choice choose(int64_t rows, int64_t cols, int64_t batch, int64_t blocks, int nb,
   };
   const Option one[] = {{true, 256}, {true, 128}, {false, 128}, {false, 64}}, two[] = {{true, 128}, {false, 64}};
   const Option* options = nb == 1 ? one : two;
-  Choice best{{false, 64, false}, 1};
+  Choice best{{false, 64}, 1};
   double least = 1e300;
   for (int i = 0; i < (nb == 1 ? 4 : 2); ++i) {
     const Option o = options[i];
@@ -282,13 +283,13 @@ Choice choose(int64_t rows, int64_t cols, int64_t batch, int64_t blocks, int nb,
     const int ctas = o.pair ? 2 : 1;
     const int64_t tiles = (rows + 128 * ctas - 1) / (128 * ctas) * ((cols + o.bn - 1) / o.bn) * batch;
     const int64_t workers = sms / ctas;
-    const double block = std::max(2.0 * nb * o.bn, (a_count * 16384.0 + nb * (o.bn / ctas) * 128.0) / 64.0);
+    const double block = std::max({800.0, 3.3 * nb * o.bn, (a_count * 16384.0 + nb * (o.bn / ctas) * 128.0) / 40.0});
     for (int64_t parts = 1; parts == 1 || (may_split && parts <= blocks / 2); ++parts) {
       if (parts > 1 && tiles * parts > workers) break;
       const double waves = (double)((tiles * parts + workers - 1) / workers);
-      double cost = waves * ((double)((blocks + parts - 1) / parts) * block + 1200.0);
-      if (parts > 1) cost += 6000.0 + 8.0 * parts * rows * cols * batch * nb / 3000.0;
-      if (cost < least) least = cost, best = Choice{{o.pair, o.bn, false}, (int)parts};
+      double cost = waves * ((double)((blocks + parts - 1) / parts) * block + 1500.0);
+      if (parts > 1) cost += 5000.0 + 8.0 * parts * rows * cols * batch * nb / 3000.0;
+      if (cost < least) least = cost, best = Choice{{o.pair, o.bn}, (int)parts};
     }
   }
   return best;
@@ -299,7 +300,7 @@ constexpr int kFewRows = 128;
 
 Choice choose_few(int64_t rows, int64_t cols, int64_t batch, int64_t blocks, int nb, int sms, bool may_split) {
   const int64_t tiles = (cols + 127) / 128 * batch;
-  Choice best{{false, rows <= 16 ? 16 : rows <= 64 ? 64 : 128, false}, 1};
+  Choice best{{false, rows <= 16 ? 16 : rows <= 64 ? 64 : 128}, 1};
   double least = 1e300;
   for (int64_t parts = 1; parts == 1 || (may_split && parts <= blocks / 2 && tiles * parts <= sms); ++parts) {
     const double waves = (double)((tiles * parts + sms - 1) / sms);
@@ -329,7 +330,7 @@ void split_and_launch(const Launch& l, int epi, const FfOut& e, FfGemm& p, const
   const int64_t total = (int64_t)p.tiles_m * p.tiles_n * p.splits * batch;
   TORCH_CHECK(total < (1ll << 31), "feed_forward: too many tiles");
   const unsigned sizes[4] = {(unsigned)p.tiles_n, (unsigned)p.tiles_m, (unsigned)p.splits, (unsigned)e.heads};
-  unsigned step = c.tile.resident ? 1 : (unsigned)std::min<int64_t>(total, num_sms_of(l.dev) / ctas);
+  unsigned step = (unsigned)std::min<int64_t>(total, num_sms_of(l.dev) / ctas);
   for (int i = 0; i < 4; ++i) {
     p.size[i] = sizes[i];
     p.step[i] = step % sizes[i];
@@ -372,10 +373,8 @@ void product(const Launch& l, int epi, FfOut e, const Mat* a, const Mat* b, int 
   p.err = l.err;
   const int64_t blocks = (int64_t)p.KB * segments, batch = (int64_t)e.heads * out_sets;
   const bool few = e.M <= kFewRows && !a_mn && out_sets == 1;
-  Choice c = few ? choose_few(e.M, e.N, batch, blocks, nb, num_sms_of(l.dev), may_split) : choose(e.M, e.N, batch, blocks, nb, nb == 2 && two_a ? 2 : 1, num_sms_of(l.dev), may_split);
+  const Choice c = few ? choose_few(e.M, e.N, batch, blocks, nb, num_sms_of(l.dev), may_split) : choose(e.M, e.N, batch, blocks, nb, nb == 2 && two_a ? 2 : 1, num_sms_of(l.dev), may_split);
   p.splits = c.splits;
-  // Short reductions: A stays in shared memory over the columns of its rows.
-  c.tile.resident = epi != FF_STORE && c.tile.pair && c.tile.bn == (nb == 1 ? 256 : 128) && p.splits == 1 && p.KB <= kFfResident;
   TORCH_CHECK(blocks * (c.splits + 1) < (1ll << 32), "feed_forward: the reduction is too long");
   if (few) {
     p.tiles_m = (e.N + 127) / 128, p.tiles_n = 1;

@@ -294,34 +294,33 @@ __device__ __forceinline__ void ff_put_aux(const FfAux& a, uint8_t* buf, int lan
   __syncwarp();
 }
 
-// Rows [row0, row0 + 32) x 32 columns from the lanes' rows of packed values.
-__device__ __forceinline__ void ff_store_packed(const FfOut& e, void* out, long long ld, long long head_stride, int head,
-                                                uint4 (&w)[4], int row0, int col, uint8_t* buf, int lane) {
-  __syncwarp();
-#pragma unroll
-  for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(buf + ff_piece(lane, q)) = w[q];
+// The warp's tile in shared memory to rows [row0, row0 + 32) x 32 columns.
+__device__ __forceinline__ void ff_flush(const FfOut& e, void* out, long long ld, long long head_stride, int head, int row0,
+                                         int col, const uint8_t* buf, int lane) {
   __syncwarp();
   const int c = col + 8 * (lane & 3), r = lane / 4;
   uint16_t* o = reinterpret_cast<uint16_t*>(out) + (long long)(row0 + r) * ld + (long long)head * head_stride + c;
   const int rows = c < e.N ? e.M - row0 - r : 0;  // 8 i below it
+  uint4 w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w[i] = *reinterpret_cast<const uint4*>(buf + ff_piece(8 * i + r, lane & 3));
+  for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4*>(buf + ff_piece(8 * i + r, lane & 3));
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
     if (8 * i < rows) *reinterpret_cast<uint4*>(o + 8 * i * ld) = w[i];
-  }
 }
 
+// Rows [row0, row0 + 32) x 32 columns from the lanes' rows.
 __device__ __forceinline__ void ff_store_tile(const FfOut& e, void* out, long long ld, long long head_stride, int head,
                                               const float* v, int row0, int col, uint8_t* buf, int lane) {
-  uint4 w[4];
+  __syncwarp();
   if (e.half) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) w[q] = ff_pack8(v + 8 * q, 1);
+    for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(buf + ff_piece(lane, q)) = ff_pack8(v + 8 * q, 1);
   } else {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) w[q] = ff_pack8(v + 8 * q, 0);
+    for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(buf + ff_piece(lane, q)) = ff_pack8(v + 8 * q, 0);
   }
-  ff_store_packed(e, out, ld, head_stride, head, w, row0, col, buf, lane);
+  ff_flush(e, out, ld, head_stride, head, row0, col, buf, lane);
 }
 
 // The lane's row of 32 pre-activations in 8 bits. Columns past N count as zeros.
@@ -406,8 +405,9 @@ __device__ __forceinline__ void ff_add_bias(const FfOut& e, int s, int head, int
 }
 
 // A warp's 32 x 32 chunk. g_at, u_at: its accumulators (one or two); aux: r or dy, as ff_load_aux left it; release:
-// called once the accumulators have been read. The arithmetic goes over 16 columns at a time: sixteen warps leave a thread 96
-// registers, and with both products of 32 columns in them spills wrote as many bytes as the results.
+// called once the accumulators have been read. The arithmetic goes over 16 columns at a time, and each result takes the
+// place in shared memory that r or dy had: sixteen warps leave a thread 96 registers, and with both products of 32
+// columns in them spills wrote as many bytes as the results.
 template <int EPI, typename R>
 __device__ __forceinline__ void ff_epilogue(const FfOut& e, int set, int head, int row0, int col, uint32_t g_at,
                                             uint32_t u_at, const FfAux& aux, uint8_t* buf, int lane, R&& release) {
@@ -434,8 +434,10 @@ __device__ __forceinline__ void ff_epilogue(const FfOut& e, int set, int head, i
       }
     }
     const bool has_aux = ff_has_aux<EPI>(e);
-    if (has_aux) ff_put_aux(aux, buf, lane);
-    uint4 pg[4], pu[4];
+    if (has_aux)
+      ff_put_aux(aux, buf, lane);
+    else
+      __syncwarp();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float g[16], u[16];
@@ -467,8 +469,9 @@ __device__ __forceinline__ void ff_epilogue(const FfOut& e, int set, int head, i
       }
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        pg[2 * h + q] = ff_pack8(g + 8 * q, e.half);
-        if constexpr (EPI == FF_GATED_BWD) pu[2 * h + q] = ff_pack8(u + 8 * q, e.half);
+        *reinterpret_cast<uint4*>(buf + ff_piece(lane, 2 * h + q)) = ff_pack8(g + 8 * q, e.half);
+        if constexpr (EPI == FF_GATED_BWD)
+          *reinterpret_cast<uint4*>(buf + 2048 + ff_piece(lane, 2 * h + q)) = ff_pack8(u + 8 * q, e.half);
       }
       if constexpr (ff_backward(EPI)) {
         if (e.colsum[0]) ff_put_sums<16>(e, 0, head, g, row0, c, lane);
@@ -476,49 +479,42 @@ __device__ __forceinline__ void ff_epilogue(const FfOut& e, int set, int head, i
           if (e.colsum[1]) ff_put_sums<16>(e, 1, head, u, row0, c, lane);
       }
     }
-    ff_store_packed(e, e.out[0], e.ld, e.head, head, pg, row0, col, buf, lane);
-    if constexpr (EPI == FF_GATED_BWD) ff_store_packed(e, e.out[1], e.ld, e.head, head, pu, row0, col, buf, lane);
+    ff_flush(e, e.out[0], e.ld, e.head, head, row0, col, buf, lane);
+    if constexpr (EPI == FF_GATED_BWD) ff_flush(e, e.out[1], e.ld, e.head, head, row0, col, buf + 2048, lane);
   }
 }
 
 // ------------------------------------------------------------------------------- products
 
 
-constexpr int kFfResident = 4;  // blocks of a reduction whose A stays in shared memory
-
-// RES: the whole reduction of a tile's A rows stays in shared memory over a run of tiles in the same rows.
-template <int NB, int BN, bool PAIR, bool RES>
+template <int EPI, int BN, bool PAIR>
 struct FfCfg {
+  static constexpr int NB = ff_products(EPI);
   static constexpr int CTAS = PAIR ? 2 : 1;
   static constexpr int B_ROWS = BN / CTAS;  // of one product, staged by this CTA
   static constexpr int A_BYTES = 128 * 64 * 2, B_BYTES = B_ROWS * 64 * 2;
-  static constexpr int A_ROOM = RES ? NB * kFfResident * A_BYTES : 0;
-  static constexpr int STAGE_BYTES = NB * ((RES ? 0 : A_BYTES) + B_BYTES);
+  static constexpr int STAGE_BYTES = NB * (A_BYTES + B_BYTES);
   // Sixteen epilogue warps, four a scheduler: with eight the epilogue of 2 x 128 columns was bound by its own latencies
   // (gated, 4099 rows, 4 x 256 -> 8192: 240 us).
   static constexpr int EPI_WARPS = BN >= 128 ? 16 : 8;
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-  static constexpr int EPI_BYTES = EPI_WARPS * 2048;
-  static constexpr int STAGES = (192 * 1024 - A_ROOM) / STAGE_BYTES;
-  static constexpr int SMEM = A_ROOM + STAGES * STAGE_BYTES + EPI_BYTES + 1024;
+  static constexpr int EPI_TILE = EPI == FF_GATED_BWD ? 4096 : 2048;  // of a warp: one result, or two
+  static constexpr int EPI_BYTES = EPI_WARPS * EPI_TILE;
+  static constexpr int STAGES = (224 * 1024 - EPI_BYTES) / STAGE_BYTES;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + EPI_BYTES + 1024;
   static constexpr int TMEM_COLS = 2 * NB * BN;
   static_assert(B_ROWS % 64 == 0 && TMEM_COLS <= 512 && SMEM <= 227 * 1024, "tile");
 };
 
-// The tiles of a CTA (or pair): columns fastest, then rows, parts, heads, sets. Worker w of W takes w, w + W, ..., or,
-// with RES, a run of tiles on end, so that its rows change once or twice. Divided once; the digits of the step are the host's.
+// The tiles of a CTA (or pair): columns fastest, then rows, parts, heads, sets. Worker w of W takes w, w + W, ....
+// Divided once; the digits of the step are the host's.
 struct FfWalk {
   unsigned at[4], set, count;
 
-  __device__ __forceinline__ FfWalk(const FfGemm& p, unsigned worker, unsigned workers, bool runs) {
+  __device__ __forceinline__ FfWalk(const FfGemm& p, unsigned worker, unsigned workers) {
     const unsigned total = (unsigned)(p.tiles_m * p.tiles_n * p.splits * p.e.heads * p.out_sets);
     unsigned t = worker;
-    if (runs) {
-      t = (unsigned)((unsigned long long)total * worker / workers);
-      count = (unsigned)((unsigned long long)total * (worker + 1) / workers) - t;
-    } else {
-      count = worker < total ? (total - worker + workers - 1) / workers : 0;
-    }
+    count = worker < total ? (total - worker + workers - 1) / workers : 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       at[i] = t % p.size[i];
@@ -575,31 +571,28 @@ __device__ __forceinline__ void ff_load(void* dst, const CUtensorMap* m, bool mn
   }
 }
 
-template <int EPI, int BN, bool PAIR, bool RES>
-__global__ void __launch_bounds__(FfCfg<ff_products(EPI), BN, PAIR, RES>::THREADS, 1)
+template <int EPI, int BN, bool PAIR>
+__global__ void __launch_bounds__(FfCfg<EPI, BN, PAIR>::THREADS, 1)
     ff_gemm_kernel(const __grid_constant__ FfGemm p) {
   constexpr int NB = ff_products(EPI);
-  using Cfg = FfCfg<NB, BN, PAIR, RES>;
+  using Cfg = FfCfg<EPI, BN, PAIR>;
   constexpr int STAGES = Cfg::STAGES, ROWS = 128 * Cfg::CTAS;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES];
-  __shared__ uint64_t tfull_bar[2], tempty_bar[2], drain_bar, afull_bar, aempty_bar;
+  __shared__ uint64_t tfull_bar[2], tempty_bar[2], drain_bar;
   __shared__ uint32_t tmem_base_s;
   __shared__ volatile int abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int crank = PAIR ? (int)cluster_ctarank() : 0;
   const bool leader = crank == 0;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sRing = smem + Cfg::A_ROOM;
-  uint8_t* sEpi = sRing + STAGES * Cfg::STAGE_BYTES;
+  uint8_t* sEpi = smem + STAGES * Cfg::STAGE_BYTES;
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
-    mbar_init(&afull_bar, 1);
-    mbar_init(&aempty_bar, 1);
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull_bar[a], 1);
       mbar_init(&tempty_bar[a], Cfg::CTAS * Cfg::EPI_WARPS);
@@ -632,29 +625,11 @@ __global__ void __launch_bounds__(FfCfg<ff_products(EPI), BN, PAIR, RES>::THREAD
       long long issued = 0;
       bool ok = true;
       const int a_count = NB == 2 && !p.two_a ? 1 : NB;
-      const uint32_t bytes = (uint32_t)(Cfg::CTAS * ((RES ? 0 : a_count * Cfg::A_BYTES) + NB * Cfg::B_BYTES));
-      unsigned rows_of = ~0u;  // RES: the rows and head whose A is there
-      uint32_t a_phase = 0;
-      FfWalk w(p, worker, workers, RES);
+      const uint32_t bytes = (uint32_t)(Cfg::CTAS * (a_count * Cfg::A_BYTES + NB * Cfg::B_BYTES));
+      FfWalk w(p, worker, workers);
       for (unsigned t = 0; t < w.count && ok; ++t, w.next(p)) {
         int b0, b1;
         ff_part(p, w.split(), b0, b1);
-        if constexpr (RES) {
-          const unsigned rows = w.at[1] + w.at[3] * p.size[1];
-          if (rows != rows_of) {
-            if (!mbar_wait_bounded(&aempty_bar, a_phase ^ 1, &abort_flag, p.err, kErrTimeoutProducer)) {
-              ok = false;
-              break;
-            }
-            if (leader) mbar_arrive_expect_tx(&afull_bar, (uint32_t)(Cfg::CTAS * a_count * p.KB * Cfg::A_BYTES));
-            for (int s = 0; s < a_count; ++s)
-              for (int kb = 0; kb < p.KB; ++kb)
-                ff_load<PAIR, 128>(smem + (s * p.KB + kb) * Cfg::A_BYTES, &p.ta[s], false, &afull_bar,
-                                   w.m() * ROWS + 128 * crank, kb * 64, (p.a_heads >> s) & 1 ? w.head() : 0);
-            a_phase ^= 1;
-            rows_of = rows;
-          }
-        }
         const int am = w.m() * ROWS + 128 * crank, bn = w.n() * BN + Cfg::B_ROWS * crank;
         int seg = b0 / p.KB, kb = b0 - seg * p.KB;
         for (int i = b0; i < b1; ++i) {
@@ -668,12 +643,9 @@ __global__ void __launch_bounds__(FfCfg<ff_products(EPI), BN, PAIR, RES>::THREAD
           }
           uint64_t* bar = &full_bar[stage];
           if (leader) mbar_arrive_expect_tx(bar, bytes);
-          uint8_t* dst = sRing + stage * Cfg::STAGE_BYTES;
+          uint8_t* dst = smem + stage * Cfg::STAGE_BYTES;
           const int k = kb * 64;
-          if constexpr (RES) {
-            ff_load<PAIR, Cfg::B_ROWS>(dst, &p.tb[0], (p.b_mn & 1) != 0, bar, bn, k, head);
-            if constexpr (NB == 2) ff_load<PAIR, Cfg::B_ROWS>(dst + Cfg::B_BYTES, &p.tb[1], (p.b_mn & 2) != 0, bar, bn, k, head);
-          } else if constexpr (NB == 1) {
+          if constexpr (NB == 1) {
             ff_load<PAIR, 128>(dst, &p.ta[set], p.a_mn, bar, am, k, (p.a_heads >> set) & 1 ? head : 0);
             ff_load<PAIR, Cfg::B_ROWS>(dst + Cfg::A_BYTES, &p.tb[set], p.b_mn, bar, bn, k, (p.b_heads >> set) & 1 ? head : 0);
           } else {
@@ -703,7 +675,6 @@ __global__ void __launch_bounds__(FfCfg<ff_products(EPI), BN, PAIR, RES>::THREAD
           }
           mbar_wait_bounded(&full_bar[s], ph, (volatile int*)&dummy_abort, p.err, kErrTimeoutDrain);
         }
-        if (RES && rows_of != ~0u) mbar_wait_bounded(&afull_bar, a_phase ^ 1, (volatile int*)&dummy_abort, p.err, kErrTimeoutDrain);
       }
     }
   } else if (warp == 1) {
@@ -712,29 +683,10 @@ __global__ void __launch_bounds__(FfCfg<ff_products(EPI), BN, PAIR, RES>::THREAD
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      unsigned rows_of = ~0u;
-      uint32_t a_phase = 0;
-      FfWalk w(p, worker, workers, RES);
+      FfWalk w(p, worker, workers);
       for (unsigned t = 0; t < w.count && ok; ++t, w.next(p)) {
         int b0, b1;
         ff_part(p, w.split(), b0, b1);
-        if constexpr (RES) {
-          const unsigned rows = w.at[1] + w.at[3] * p.size[1];
-          if (rows != rows_of) {
-            if (rows_of != ~0u) {  // once the products issued so far are done, other rows may take A's place
-              if constexpr (PAIR)
-                umma_commit_pair(&aempty_bar);
-              else
-                umma_commit(&aempty_bar);
-            }
-            if (!mbar_wait_bounded(&afull_bar, a_phase, &abort_flag, p.err, kErrTimeoutMma)) {
-              ok = false;
-              break;
-            }
-            a_phase ^= 1;
-            rows_of = rows;
-          }
-        }
         if (!mbar_wait_bounded(&tempty_bar[acc], acc_phase ^ 1, &abort_flag, p.err, kErrTimeoutMma)) {
           ok = false;
           break;
@@ -746,14 +698,12 @@ __global__ void __launch_bounds__(FfCfg<ff_products(EPI), BN, PAIR, RES>::THREAD
             break;
           }
           tc_fence_after();
-          const uint32_t base = smem_u32(sRing + stage * Cfg::STAGE_BYTES);
-          const uint32_t a_at = RES ? smem_u32(smem + (i - b0) * Cfg::A_BYTES) : base;
-          const uint32_t a_next = RES ? (uint32_t)(p.KB * Cfg::A_BYTES) : (uint32_t)Cfg::A_BYTES;
+          const uint32_t base = smem_u32(smem + stage * Cfg::STAGE_BYTES);
 #pragma unroll
           for (int s = 0; s < NB; ++s) {
             const bool b_mn = NB == 1 ? p.b_mn != 0 : (p.b_mn & (1 << s)) != 0;
-            const uint32_t a_base = a_at + (s == 1 && p.two_a ? a_next : 0);
-            const uint32_t b_base = base + (RES ? 0 : NB * Cfg::A_BYTES) + s * Cfg::B_BYTES;
+            const uint32_t a_base = base + (s == 1 && p.two_a ? Cfg::A_BYTES : 0);
+            const uint32_t b_base = base + NB * Cfg::A_BYTES + s * Cfg::B_BYTES;
             const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
             const uint32_t a_lbo = p.a_mn ? 8192 : 16, b_lbo = b_mn ? 8192 : 16;
             const uint32_t idesc = p.idesc | (b_mn ? 1u << 16 : 0u);
@@ -799,7 +749,7 @@ __global__ void __launch_bounds__(FfCfg<ff_products(EPI), BN, PAIR, RES>::THREAD
     // ------------------------------------------------ epilogue (each CTA its own 128 rows)
     const int quad = warp & 3;         // TMEM lane quadrant of this warp
     const int part = (warp - 2) >> 2;  // its share of the tile's columns
-    uint8_t* buf = sEpi + (warp - 2) * 2048;
+    uint8_t* buf = sEpi + (warp - 2) * Cfg::EPI_TILE;
     constexpr int COLS = BN * 4 / Cfg::EPI_WARPS;
     static_assert(COLS % 32 == 0, "a chunk is 32 columns");
     const int col0 = part * COLS;
@@ -807,7 +757,7 @@ __global__ void __launch_bounds__(FfCfg<ff_products(EPI), BN, PAIR, RES>::THREAD
     if constexpr (PAIR) leader_tempty0 = map_to_cta(&tempty_bar[0], 0), leader_tempty1 = map_to_cta(&tempty_bar[1], 0);
     int acc = 0;
     uint32_t acc_phase = 0;
-    FfWalk w(p, worker, workers, RES);
+    FfWalk w(p, worker, workers);
     for (unsigned t = 0; t < w.count; ++t, w.next(p)) {
       const int row0 = w.m() * ROWS + 128 * crank + quad * 32, first = w.n() * BN + col0;
       const bool one = p.splits == 1;
@@ -1049,7 +999,7 @@ __global__ void __launch_bounds__(FfFewCfg<ff_products(EPI), MP>::THREADS, 1) ff
       bool ok = true;
       const int x_count = NB == 2 && !p.two_a ? 1 : NB;
       const uint32_t bytes = (uint32_t)(NB * Cfg::W_BYTES + x_count * Cfg::X_BYTES);
-      FfWalk w(p, blockIdx.x, gridDim.x, false);
+      FfWalk w(p, blockIdx.x, gridDim.x);
       for (unsigned t = 0; t < w.count && ok; ++t, w.next(p)) {
         int b0, b1;
         ff_part(p, w.split(), b0, b1);
@@ -1102,7 +1052,7 @@ __global__ void __launch_bounds__(FfFewCfg<ff_products(EPI), MP>::THREADS, 1) ff
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      FfWalk w(p, blockIdx.x, gridDim.x, false);
+      FfWalk w(p, blockIdx.x, gridDim.x);
       for (unsigned t = 0; t < w.count && ok; ++t, w.next(p)) {
         int b0, b1;
         ff_part(p, w.split(), b0, b1);
@@ -1153,7 +1103,7 @@ __global__ void __launch_bounds__(FfFewCfg<ff_products(EPI), MP>::THREADS, 1) ff
     constexpr int SHARE = MP * 4 / Cfg::EPI_WARPS, n = Cfg::ROWS;
     int acc = 0;
     uint32_t acc_phase = 0;
-    FfWalk w(p, blockIdx.x, gridDim.x, false);
+    FfWalk w(p, blockIdx.x, gridDim.x);
     for (unsigned t = 0; t < w.count; ++t, w.next(p)) {
       // the same answer for the whole warp: the loads from TMEM need all of its lanes, also where a wait has run out
       if (!__all_sync(0xffffffffu, mbar_wait_bounded(&tfull_bar[acc], acc_phase, &abort_flag, p.err, kErrTimeoutEpilogue)))
@@ -1198,11 +1148,10 @@ __global__ void __launch_bounds__(FfFewCfg<ff_products(EPI), MP>::THREADS, 1) ff
 }  // namespace bd
 
 namespace bd {
-// The tile of a launch: PAIR, BN and RES. feed_forward_{a,b}.cu hold the instantiations.
+// The tile of a launch: PAIR and BN. feed_forward_{a,b}.cu hold the instantiations.
 struct FfTile {
   bool pair;
   int bn;
-  bool resident;
 };
 inline int64_t ff_workers(int64_t tiles, FfTile t, int sms) { return std::min<int64_t>(tiles, sms / (t.pair ? 2 : 1)); }
 void ff_launch_few(int epi, int rows, const FfGemm& p, cudaStream_t st, int dev);       // either, up to 128 rows

@@ -11,9 +11,6 @@ namespace bd {
 namespace {
 template <int EPI>
 void go(FfTile t, const FfGemm& p, cudaStream_t st, int dev) {
-  if constexpr (EPI != FF_STORE) {
-    if (t.resident) return ff_launch<EPI, 256, true, true>(p, st, dev);
-  }
   if (t.pair && t.bn == 256)
     ff_launch<EPI, 256, true>(p, st, dev);
   else if (t.pair)

@@ -11,9 +11,7 @@ namespace bd {
 namespace {
 template <int EPI>
 void go(FfTile t, const FfGemm& p, cudaStream_t st, int dev) {
-  if (t.resident)
-    ff_launch<EPI, 128, true, true>(p, st, dev);
-  else if (t.pair)
+  if (t.pair)
     ff_launch<EPI, 128, true>(p, st, dev);
   else
     ff_launch<EPI, 64, false>(p, st, dev);

@@ -8,17 +8,17 @@
 
 namespace bd {
 
-template <int EPI, int BN, bool PAIR, bool RES = false>
+template <int EPI, int BN, bool PAIR>
 void ff_launch(const FfGemm& p, cudaStream_t st, int dev) {
-  using Cfg = FfCfg<ff_products(EPI), BN, PAIR, RES>;
-  auto kern = ff_gemm_kernel<EPI, BN, PAIR, RES>;
+  using Cfg = FfCfg<EPI, BN, PAIR>;
+  auto kern = ff_gemm_kernel<EPI, BN, PAIR>;
   static bool attr_set[64] = {false};
   if (!attr_set[dev]) {
     C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
     attr_set[dev] = true;
   }
   const long long total = (long long)p.tiles_m * p.tiles_n * p.splits * p.e.heads * p.out_sets;
-  const long long workers = ff_workers(total, FfTile{PAIR, BN, RES}, num_sms_of(dev));
+  const long long workers = ff_workers(total, FfTile{PAIR, BN}, num_sms_of(dev));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(workers * Cfg::CTAS));
   cfg.blockDim = dim3(Cfg::THREADS);
