@@ -311,6 +311,10 @@ class DragonConfig:
     # dense_score_short_context | gated_delta_chunk_wy
     sequence_memory_system: str = "linear_attention"
     sequence_executor: str = "reference"
+    # products of the layer-loop variants (ops/feed_forward.py): "torch", or "kernels" (bf16
+    # operands, fp32 sums on CUDA) for the gated step of layers whose memory reads the dense
+    # stream (Mamba-3), the latent refiner and the next-latent transition
+    feed_forward: str = "torch"
     mamba: MambaSequenceConfig = field(default_factory=MambaSequenceConfig)
     gated_deltanet2: GatedDeltaNet2Config = field(default_factory=GatedDeltaNet2Config)
     # residual connector: vanilla | mhc | attention_residual | block_attention_residual
@@ -451,6 +455,8 @@ class DragonConfig:
         ok = {("linear_attention", "reference"), ("linear_attention", "dense_score_short_context"),
               ("mamba3_state_space_duality", "reference"), ("gated_deltanet2", "reference"),
               ("gated_deltanet2", "gated_delta_chunk_wy")}
+        if self.feed_forward not in ("torch", "kernels"):
+            raise ValueError(f"model.feed_forward {self.feed_forward!r} (torch | kernels)")
         if (self.sequence_memory_system, self.sequence_executor) not in ok:
             raise ValueError(f"sequence kernel family {self.sequence_memory_system!r} with executor "
                              f"{self.sequence_executor!r} is not supported")
@@ -869,6 +875,9 @@ class TrainingSection:
     # SequenceBatchingMode)
     sequence_batching: str = "auto"  # auto | random | streaming
     gradient_accumulation_steps: int = 1
+    # what the layer-loop variants' autograd holds between the passes (ops/act8.py): "full",
+    # or "8bit" (e4m3 with a scale for 32 values)
+    activation_checkpoints: str = "full"
     seed: int = 1337
     log_frequency: int = 10
     checkpoint_interval_iters: int | None = None
@@ -1013,6 +1022,8 @@ class TrainingConfig:
         if t.gdpo and t.gdpo.get("enabled"):
             raise ValueError("training.gdpo.enabled is a legacy objective flag; use training.objective.type = "
                              "\"sdpo\" for self-distilled policy optimization")
+        if t.activation_checkpoints not in ("full", "8bit"):
+            raise ValueError(f"training.activation_checkpoints {t.activation_checkpoints!r} (full | 8bit)")
         if t.launch_mode not in (None, "fresh", "resume_exact_run", "resume_latest_checkpoint_if_present",
                                  "init_from_checkpoint"):
             raise ValueError(f"training.launch_mode {t.launch_mode!r}")

@@ -39,6 +39,8 @@ import torch.nn.functional as F
 from torch import nn
 
 from ..config import DragonConfig
+from ..ops.act8 import activations_in_8bit
+from ..ops.feed_forward import gated_linear, linear_act
 from . import reference as R
 from .bdh import BDH
 
@@ -224,6 +226,8 @@ class DragonRuntime(nn.Module):
         D, L = cfg.n_embd, cfg.n_layer
         self.connector = cfg.resolved_residual_connector()
         self.rollout_mode = rollout_mode
+        self.activations_8bit = False  # hold what the layers save for the backward pass in 8 bits
+        self._low: dict | None = None  # the operands of this forward pass in the kernels' type, by parameter
         if self.connector == "attention_residual":
             c = cfg.attention_residual
             self.attn_res = AttentionResidual(D, c.num_heads, c.history_window, c.recency_bias, c.dropout)
@@ -294,6 +298,38 @@ class DragonRuntime(nn.Module):
         self._decay = R.decay_vector(cfg.decay_slopes(), device=dev) if cfg.uses_decay() else None
 
     # ------------------------------------------------------------------ pieces
+    def _operand(self, w: torch.Tensor) -> torch.Tensor:
+        """A weight as the products read it: bf16 on CUDA, cast once a forward pass."""
+        if not w.is_cuda or w.dtype in (torch.bfloat16, torch.float16):
+            return w
+        if self._low is None:
+            return w.to(torch.bfloat16)
+        if id(w) not in self._low:
+            self._low[id(w)] = (w, w.to(torch.bfloat16))  # w too: its id stays its own
+        return self._low[id(w)][1]
+
+    def _product(self, x, lin: "Linear", activation: str = "none", residual=None):
+        """act(x W + b) + residual of a head's Linear."""
+        if self.cfg.feed_forward != "kernels":
+            y = lin(x)
+            y = F.gelu(y) if activation == "gelu" else y
+            return y if residual is None else residual + y
+        w = self._operand(lin.weight)
+        r = None if residual is None else residual.to(w.dtype)
+        return linear_act(x.to(w.dtype), w, lin.bias, activation, residual=r).to(x.dtype)
+
+    def _gated_step(self, v, a, enc, enc_v, dec, thr, thr_y):
+        """relu(v E - thr) * relu(a E_v - thr_y) and its decoder projection: [B, H, T, Nh], [B, T, D]."""
+        B, T, D = v.shape
+        H, _, Nh = enc.shape
+        E, Ev, W = (self._operand(w) for w in (enc, enc_v, dec))
+        rows = lambda t: t.reshape(B * T, D).to(E.dtype)  # noqa: E731
+        yn = gated_linear(rows(v), E, Ev, -float(thr), -float(thr_y), z=rows(a), activation="relu", up_activation="relu")
+        if self.cfg.dropout > 0 and self.training:
+            yn = F.dropout(yn, self.cfg.dropout, True)
+        m = linear_act(yn.reshape(B * T, H * Nh), W)
+        return yn.view(B, T, H, Nh).permute(0, 2, 1, 3), m.view(B, T, D).to(v.dtype)
+
     def _weights(self, slow: bool = False):
         p = self.core.param_dict()
         if slow and hasattr(self, "slow_encoder"):
@@ -352,6 +388,13 @@ class DragonRuntime(nn.Module):
         nf = self._norm(p)
         thr, thr_y = self.cfg.thresholds()
         lm = self._latent_mask
+        if self.cfg.feed_forward == "kernels" and lm is None and x_inject is None and \
+                self.cfg.sequence_memory_system == "mamba3_state_space_duality":
+            # this memory reads the dense stream, so nothing but the gate wants x
+            a = nf(self._attend(v[:, None], v, ls, pos, fixed, slot))
+            yn, m = self._gated_step(v, a[:, 0], enc, enc_v, dec, thr, thr_y)
+            out = nf(v + nf(m))
+            return (out, yn) if want_y else out
         x = torch.relu(torch.einsum("btd,hdn->bhtn", v, enc) - thr)
         if lm is not None:
             x = x * lm
@@ -571,13 +614,34 @@ class DragonRuntime(nn.Module):
         return R.cross_entropy(self.forward(tokens, state, event_mask), targets, mask)
 
     def _forward(self, tokens, state, event_mask, logits: bool):
+        self._low = {}
+        try:
+            return self._run(tokens, state, event_mask, logits)
+        finally:
+            self._low = None
+
+    def _layers(self, *args):
+        """``hidden_single_pass``, with what it saves held in 8 bits where that is wanted."""
+        if not (self.activations_8bit and torch.is_grad_enabled()):
+            return self.hidden_single_pass(*args)
+        if self.core.scaffold:
+            raise ValueError("activations in 8 bits are not for a random scaffold: its effective weights are computed in the "
+                             "layers and would be held in 8 bits too")
+        if self.cfg.feed_forward == "kernels":  # cast before: a weight is no activation
+            slow = (self.slow_encoder, self.slow_encoder_v, self.slow_decoder) if hasattr(self, "slow_encoder") else ()
+            for w in (*self._weights()[:3], *slow):
+                self._operand(w)
+        with activations_in_8bit(exclude=[low for _, low in (self._low or {}).values()]):
+            return self.hidden_single_pass(*args)
+
+    def _run(self, tokens, state, event_mask, logits: bool):
         if state is None:
             state = RuntimeState.new(self.cfg.n_layer)
         p = self.core.param_dict()
         emb = p["embed"][tokens]
         Fs = self.cfg.rollout_fast_steps_per_slow_step
         if Fs <= 1:
-            h = self.hidden_single_pass(emb, state, state.position, False, event_mask)
+            h = self._layers(emb, state, state.position, False, event_mask)
             state.position += tokens.shape[1]
             h = self.reason_hidden_final(h)
             return h, (self.logits_from_hidden(h) if logits else None)
@@ -587,9 +651,9 @@ class DragonRuntime(nn.Module):
             em = None if event_mask is None else event_mask[:, t:t + 1]
             if self.rollout_mode == "host_loop":
                 for _ in range(Fs):
-                    h = self.hidden_single_pass(tok, state, state.position, False, em)
+                    h = self._layers(tok, state, state.position, False, em)
             else:  # the token repeated F times in one pass at a fixed position
-                h = self.hidden_single_pass(tok.expand(-1, Fs, -1), state, state.position, True, em)[:, -1:]
+                h = self._layers(tok.expand(-1, Fs, -1), state, state.position, True, em)[:, -1:]
             hs.append(self.reason_hidden_final(h))
             state.position += 1
         h = torch.cat(hs, 1)
@@ -602,10 +666,11 @@ class DragonRuntime(nn.Module):
             (not lr.adaptive_halting or hasattr(self, "stop_head"))
 
     def _refine(self, cur):
-        upd = self.refiner_out(F.gelu(self.refiner_in(cur)))
+        h = self._product(cur, self.refiner_in, "gelu")
         if hasattr(self, "refiner_gate"):
-            upd = upd * torch.sigmoid(self.refiner_gate)
-        nxt = cur + upd
+            nxt = cur + self._product(h, self.refiner_out) * torch.sigmoid(self.refiner_gate)
+        else:
+            nxt = self._product(h, self.refiner_out, residual=cur)
         return self._norm(self.core.param_dict())(nxt) if self.cfg.latent_reasoning.normalize_steps else nxt
 
     def reason_hidden(self, hidden) -> LatentReasoningOutput:
@@ -660,7 +725,8 @@ class DragonRuntime(nn.Module):
             mu = x.mean(-1, keepdim=True)
             c = x - mu
             x = c / (c.pow(2).mean(-1, keepdim=True) + 1e-5).sqrt()
-        return hidden + self.transition_out(F.gelu(self.transition_mid(F.gelu(self.transition_in(x)))))
+        h = self._product(self._product(x, self.transition_in, "gelu"), self.transition_mid, "gelu")
+        return self._product(h, self.transition_out, residual=hidden)
 
     def sequence_scores(self, hidden):
         return self.score_out(self.score_candidate(hidden)) if hasattr(self, "score_out") else None

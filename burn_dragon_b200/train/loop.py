@@ -194,8 +194,12 @@ def train(cfg: TrainingConfig, run_name: str | None = None, resume: bool = True,
         trainer = RuntimeTrainer(cfg.model, dev, lr=o.learning_rate, weight_decay=o.weight_decay,
                                  betas=(o.beta1, o.beta2), eps=o.eps, grad_clip_norm=o.grad_clip_norm,
                                  grad_clip_value=o.grad_clip_value, seed=t.seed,
-                                 lr_schedule=o.lr_schedule, max_iters=t.max_iters)
+                                 lr_schedule=o.lr_schedule, max_iters=t.max_iters,
+                                 activation_checkpoints=t.activation_checkpoints)
     else:
+        if t.activation_checkpoints != "full":
+            raise ValueError("training.activation_checkpoints = \"8bit\" is for the layer-loop variants (the fused step "
+                             "keeps its own activations)")
         trainer = Trainer(cfg.model, dev, lr=o.learning_rate, weight_decay=o.weight_decay,
                           betas=(o.beta1, o.beta2), eps=o.eps, grad_clip_norm=o.grad_clip_norm,
                           grad_clip_value=o.grad_clip_value, seed=t.seed,

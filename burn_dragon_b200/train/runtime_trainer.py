@@ -23,10 +23,15 @@ from .optim import FusedAdamW, lr_at
 class RuntimeTrainer:
     def __init__(self, cfg: DragonConfig, device, lr=1e-3, weight_decay=0.1, betas=(0.9, 0.999), eps=1e-8,
                  grad_clip_norm=None, seed=1337, lr_schedule=None, max_iters=1000, rollout_mode: str = "fused",
-                 grad_clip_value=None):
+                 grad_clip_value=None, activation_checkpoints: str = "full"):
+        """``activation_checkpoints`` "8bit": what the layers save for the backward pass is held in 8 bits
+        (``ops.act8``); the head and the loss keep theirs."""
+        if activation_checkpoints not in ("full", "8bit"):
+            raise ValueError(f"activation_checkpoints {activation_checkpoints!r} (full | 8bit)")
         self.cfg = cfg
         self.device = torch.device(device)
         self.model = DragonRuntime(cfg, device=self.device, seed=seed, rollout_mode=rollout_mode)
+        self.model.activations_8bit = activation_checkpoints == "8bit"
         self.core = self.model.core
         self.opt = FusedAdamW(self.core.store, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
                               grad_clip_norm=grad_clip_norm, grad_clip_value=grad_clip_value)
