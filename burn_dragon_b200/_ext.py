@@ -37,7 +37,7 @@ if os.environ.get("BDH_PTXAS_VERBOSE"):
 _LAUNCHES_PER_CALL = {"grad_clip_coef": 2}
 # These count their launches themselves: how many there are depends on the arguments.
 _LAUNCHES_PER_CALL.update(dict.fromkeys(("adapter_forward", "adapter_direct", "adapter_backward", "sample_tokens",
-                                         "adamw_many", "act8_pack", "act8_unpack", "ff_call"), 0))
+                                         "adamw_many", "act8_pack", "act8_unpack", "ff_call", "ff_pad"), 0))
 
 
 class _Counted:

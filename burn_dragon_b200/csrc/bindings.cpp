@@ -138,6 +138,7 @@ void adamw_many(const std::vector<at::Tensor>& params, const std::vector<c10::op
                 const at::Tensor& steps, int64_t key, const c10::optional<at::Tensor>& gscale);
 std::vector<at::Tensor> act8_pack(const at::Tensor& x);
 at::Tensor act8_unpack(const at::Tensor& codes, const at::Tensor& scales, const std::vector<int64_t>& shape, int64_t type);
+at::Tensor ff_pad(const at::Tensor& t, int64_t R8, int64_t C8);
 c10::optional<at::Tensor> ff_call(const at::Tensor& x, const c10::optional<at::Tensor>& z, const at::Tensor& wg,
                                   const c10::optional<at::Tensor>& wu, const c10::optional<at::Tensor>& bg,
                                   const c10::optional<at::Tensor>& bu, double bg0, double bu0,
@@ -212,5 +213,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("act8_pack", &bd::act8_pack);
   m.def("act8_unpack", &bd::act8_unpack);
   m.def("ff_call", &bd::ff_call);
+  m.def("ff_pad", &bd::ff_pad);
   m.def("counted_launches", [] { return bd::counted_launches.load(); });
 }

@@ -211,6 +211,25 @@ __global__ void __launch_bounds__(256) ff_held_kernel(const __grid_constant__ Ff
   }
 }
 
+// [B, R, C] of any strides (the last 1) to [B, R8, C8], zeros behind: 8 values a thread. Rows of odd lengths cannot be read
+// by TMA; torch's constant padding took 150 us for a weight of 32 MB.
+__global__ void __launch_bounds__(256) ff_pad_kernel(const uint16_t* __restrict__ in, long long in_batch, long long in_row,
+                                                     int R, int C, uint4* __restrict__ out, int R8, int C8, long long units) {
+  const int per_row = C8 / 8;
+  for (long long u = (long long)blockIdx.x * 256 + threadIdx.x; u < units; u += (long long)gridDim.x * 256) {
+    const long long row = u / per_row;
+    const int c = (int)(u - row * per_row) * 8, b = (int)(row / R8), r = (int)(row - (long long)b * R8);
+    uint32_t v[4] = {0, 0, 0, 0};
+    if (r < R) {
+      const uint16_t* src = in + b * in_batch + r * in_row + c;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i < C) v[i / 2] |= (uint32_t)src[i] << (16 * (i & 1));
+    }
+    out[u] = make_uint4(v[0], v[1], v[2], v[3]);
+  }
+}
+
 // out [C] = the sum over R rows of part [R, C], in a fixed order: a column a lane, every eighth row a warp.
 template <typename T>
 __global__ void __launch_bounds__(256) ff_colsum_kernel(const float* __restrict__ part, int R, long long C, T* __restrict__ out) {
@@ -678,6 +697,24 @@ std::vector<at::Tensor> ff_backward(const at::Tensor& dy, const at::Tensor& x, c
     if (want_w[0]) weight_grad(0, 1);
     if (want_w[1] && c.nb == 2) weight_grad(1, 1);
   }
+  return out;
+}
+
+// t [B, R, C] of 16-bit values, the last dimension contiguous, grown to [B, R8, C8] by zeros (C8 a multiple of 8).
+at::Tensor ff_pad(const at::Tensor& t, int64_t R8, int64_t C8) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 3 && t.element_size() == 2 && (t.stride(2) == 1 || t.size(2) <= 1) && C8 % 8 == 0 &&
+                  R8 >= t.size(1) && C8 >= t.size(2) && R8 < (1ll << 31) && C8 < (1ll << 31),
+              "ff_pad: [B, R, C] of 16-bit values, contiguous in C");
+  c10::cuda::CUDAGuard guard(t.get_device());
+  at::Tensor out = at::empty({t.size(0), R8, C8}, t.options().requires_grad(false));
+  const long long units = out.numel() / 8;
+  if (units == 0) return out;
+  ff_pad_kernel<<<(unsigned)std::min<long long>((units + 255) / 256, 148 * 16), 256, 0,
+                  at::cuda::getCurrentCUDAStream(t.get_device()).stream()>>>(
+      reinterpret_cast<const uint16_t*>(t.data_ptr()), t.stride(0), t.stride(1), (int)t.size(1), (int)t.size(2),
+      reinterpret_cast<uint4*>(out.data_ptr()), (int)R8, (int)C8, units);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  ++counted_launches;
   return out;
 }
 
