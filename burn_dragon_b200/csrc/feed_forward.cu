@@ -700,7 +700,6 @@ std::vector<at::Tensor> ff_backward(const at::Tensor& dy, const at::Tensor& x, c
   return out;
 }
 
-// t [B, R, C] of 16-bit values, the last dimension contiguous, grown to [B, R8, C8] by zeros (C8 a multiple of 8).
 at::Tensor ff_pad(const at::Tensor& t, int64_t R8, int64_t C8) {
   TORCH_CHECK(t.is_cuda() && t.dim() == 3 && t.element_size() == 2 && (t.stride(2) == 1 || t.size(2) <= 1) && C8 % 8 == 0 &&
                   R8 >= t.size(1) && C8 >= t.size(2) && R8 < (1ll << 31) && C8 < (1ll << 31),

@@ -114,6 +114,56 @@ bool bias(const at::Tensor& b, const at::Tensor& w, bool heads) {
          (heads ? b.dim() == 2 && b.size(0) == w.size(0) && b.size(1) == w.size(2) : b.dim() == 1 && b.size(0) == w.size(1));
 }
 
+// Rows, or a weight (turned as it lies), with zeros behind.
+at::Tensor grow_rows(const at::Tensor& t, int64_t cols) {
+  if (t.size(-1) == cols) return t;
+  auto shape = t.sizes().vec();
+  shape.back() = cols;
+  const at::Tensor flat = t.reshape({1, -1, t.size(-1)});
+  return ff_pad(flat.stride(2) == 1 || flat.size(2) == 1 ? flat : flat.contiguous(), flat.size(1), cols).view(shape);
+}
+at::Tensor grow_weight(const at::Tensor& w, int64_t K8, int64_t N8) {
+  if (w.size(0) == K8 && w.size(1) == N8) return w;
+  if (w.stride(1) != 1 && w.stride(0) == 1) return ff_pad(w.t().unsqueeze(0), N8, K8).squeeze(0).t();
+  return ff_pad((w.stride(1) == 1 ? w : w.contiguous()).unsqueeze(0), K8, N8).squeeze(0);
+}
+
+}  // namespace
+
+OptTensor ff_call(const at::Tensor& x, const OptTensor& z, const at::Tensor& wg, const OptTensor& wu, const OptTensor& bg,
+                  const OptTensor& bu, double bg0, double bu0, const OptTensor& residual, int64_t act, bool up_relu,
+                  int64_t keep, const at::Tensor& err);
+
+namespace {
+
+// The call without gradients and heads at sizes that are not multiples of 8: operands padded by a kernel each.
+OptTensor padded(const at::Tensor& x, const OptTensor& z, const at::Tensor& wg, const OptTensor& wu, const OptTensor& bg,
+                 const OptTensor& bu, double bg0, double bu0, const OptTensor& residual, int64_t act, bool up_relu,
+                 const at::Tensor& err) {
+  const int64_t K = wg.size(0), N = wg.size(1), K8 = (K + 7) / 8 * 8, N8 = (N + 7) / 8 * 8;
+  auto rows_like = [&](const at::Tensor& t, int64_t cols) {
+    if (!operand(t, wg) || t.dim() != x.dim() || t.dim() < 1 || t.size(-1) != cols || t.numel() == 0) return false;
+    for (int64_t i = 0; i + 1 < x.dim(); ++i)
+      if (t.size(i) != x.size(i)) return false;
+    return true;
+  };
+  if (K == 0 || N == 0 || !operand(wg, wg) || !rows_like(x, K) || (z && (!wu || !rows_like(*z, K))) ||
+      (residual && (wu || !rows_like(*residual, N))) ||
+      (wu && (!operand(*wu, wg) || wu->dim() != 2 || wu->sizes() != wg.sizes())))
+    return c10::nullopt;
+  for (const OptTensor* b : {&bg, &bu})
+    if (*b && (!(*b)->is_cuda() || (*b)->get_device() != wg.get_device() || (*b)->dim() != 1 || (*b)->size(0) != N ||
+               ((*b)->scalar_type() != wg.scalar_type() && (*b)->scalar_type() != at::kFloat) || (*b)->_fw_grad(0).defined()))
+      return c10::nullopt;
+  auto bias8 = [&](const OptTensor& b) { return b ? OptTensor(at::constant_pad_nd(*b, {0, N8 - N}).contiguous()) : b; };
+  at::Tensor w2 = wu ? grow_weight(*wu, K8, N8) : at::Tensor();
+  const at::Tensor w1 = grow_weight(wg, K8, N8);
+  if (wu && (w2.stride(-1) == 1) != (w1.stride(-1) == 1)) return c10::nullopt;
+  const OptTensor y = ff_call(grow_rows(x, K8), z ? OptTensor(grow_rows(*z, K8)) : z, w1, wu ? OptTensor(w2) : wu, bias8(bg),
+                              bias8(bu), bg0, bu0, residual ? OptTensor(grow_rows(*residual, N8)) : residual, act, up_relu, 0, err);
+  return y ? OptTensor(y->narrow(-1, 0, N)) : y;
+}
+
 }  // namespace
 
 // y of linear_act (no wu) or gated_linear, with its node of the graph where a gradient is wanted; nothing where an argument
@@ -125,6 +175,13 @@ OptTensor ff_call(const at::Tensor& x, const OptTensor& z, const at::Tensor& wg,
   const bool heads = wg.dim() == 3;
   if (!heads && wg.dim() != 2) return c10::nullopt;
   const int64_t H = heads ? wg.size(0) : 1, K = wg.size(-2), N = wg.size(-1);
+  if (!heads && (K % 8 || N % 8)) {
+    bool wants = x.requires_grad() || wg.requires_grad();
+    for (const OptTensor* t : {&z, &wu, &bg, &bu, &residual}) wants |= *t && (*t)->requires_grad();
+    if (at::GradMode::is_enabled() && wants) return c10::nullopt;
+    at::NoGradGuard no_grad;
+    return padded(x, z, wg, wu, bg, bu, bg0, bu0, residual, act, up_relu, err);
+  }
   if (K % 8 || N % 8 || K == 0 || N == 0 || H == 0 || !weight(wg, wg) || (wu && !weight(*wu, wg))) return c10::nullopt;
   auto input = [&](const at::Tensor& t) {
     if (!operand(t, wg) || t.dim() < 1 || t.size(-1) != K || t.numel() == 0) return false;

@@ -20,4 +20,7 @@ std::vector<at::Tensor> ff_backward(const at::Tensor& dy, const at::Tensor& x, c
                                     const std::vector<at::Tensor>& held, int64_t act, bool up_relu, int64_t keep,
                                     int64_t want, const at::Tensor& err);
 
+// t [B, R, C] of 16-bit values, the last dimension contiguous, grown to [B, R8, C8] by zeros (C8 a multiple of 8).
+at::Tensor ff_pad(const at::Tensor& t, int64_t R8, int64_t C8);
+
 }  // namespace bd
