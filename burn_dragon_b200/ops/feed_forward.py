@@ -89,7 +89,7 @@ def _ref(x, z, wg, wu, bg, bu, residual, act, up, keep):
     g = project(x, wg, bg)
     u = None if wu is None else project(x if z is None else z, wu, bu)
     y = finish(g, u)
-    if keep in ("16bit", "8bit") and torch.is_grad_enabled() and not (wu is None and act == "none"):
+    if keep in ("16bit", "8bit") and torch.is_grad_enabled() and y.numel() and not (wu is None and act == "none"):
         seen = finish(_held(g, keep, x.dtype), None if u is None else _held(u, keep, x.dtype))
         y = _Forward.apply(y.detach(), seen)
     if residual is not None:
